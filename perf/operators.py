@@ -241,12 +241,12 @@ def prepare(case, seed):
 
 # ── plain forms ──────────────────────────────────────────────────────────────────
 def _quantise(x, group):
-    """Groups of `group` numbers → whole numbers −7..7 and one bf16 scale each: scale = bf16(max|x| / 7), 1 for a group of zeros; the
-    number is x times the scale's f32 reciprocal, rounded half away from zero."""
+    """Groups of `group` numbers → whole numbers −7..7 and one bf16 scale each: scale = bf16(max|x| / 7), 1 where that is below the
+    smallest normal number (a group of zeros); the number is x times the scale's f32 reciprocal, rounded half away from zero."""
     g = x.float().unflatten(-1, (-1, group))
     top = g.abs().amax(-1)
     scale = (top / 7.0).bfloat16()
-    scale = torch.where(scale == 0, torch.ones_like(scale), scale)
+    scale = torch.where(scale < 2.0 ** -126, torch.ones_like(scale), scale)
     y = (g * (1.0 / scale.float())[..., None]).double()
     n = (torch.sign(y) * torch.floor(y.abs() + 0.5)).clamp(-7, 7)
     return n.to(torch.int8).flatten(-2), scale
@@ -360,7 +360,7 @@ def _held_values(x, group):
     t, h, hd = x.shape
     g = x.to(torch.float32).reshape(t, h, hd // group, group)
     s = torch.div(g.abs().max(dim=3, keepdim=True).values, 7.0).to(torch.bfloat16).to(torch.float32)
-    s[s == 0] = 1.0
+    s[s < 2.0 ** -126] = 1.0
     y = torch.mul(g, torch.reciprocal(s)).to(torch.float64)
     m = torch.where(y >= 0, torch.floor(y + 0.5), torch.ceil(y - 0.5))
     return (m.clamp(min=-7.0, max=7.0) * s.to(torch.float64)).reshape(t, h, hd)
