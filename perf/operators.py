@@ -347,7 +347,7 @@ def run(s):
             return s["out"]
         return _decode_plain(s)
     if own:
-        s["ab"].prompt_attention(s["q"], s["k"], s["v"], s["out"], s["cu_q"], s["cu_k"], max_q=s["max_q"], scale=1.0 / math.sqrt(c["hd"]),
+        s["ab"].prompt_attention(s["q"], s["k"], s["v"], s["out"], s["cu_q"], s["cu_k"], scale=1.0 / math.sqrt(c["hd"]),
                                  window_size=c["window"], ctx=s["ctx"])
         return s["out"]
     return _prompt_plain(s)
