@@ -51,7 +51,7 @@ LAYER_HOOK = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.POINTER(C.c_float), C.c
 
 _lib = None
 
-vp, sz, u64, ci, cf = C.c_void_p, C.c_size_t, C.c_uint64, C.c_int, C.c_float
+vp, sz, u64, ci, cf, ll = C.c_void_p, C.c_size_t, C.c_uint64, C.c_int, C.c_float, C.c_longlong
 pvp = C.POINTER(C.c_void_p)
 pi = C.POINTER(C.c_int)
 
@@ -127,6 +127,15 @@ SIGNATURES = {
     "atlasx_decode_attention": (ci, [vp, vp, vp, vp, ci, vp, cf, ci]),
     "atlasx_decode_attention_bytes": (sz, [vp, ci, vp, ci]),
     "atlasx_decode_attention_static": (ci, [vp, ci, vp, vp, ci, ci, ci, ci, vp, vp, ci, vp, cf, ci]),
+    "atlasx_page_plan": (ci, [vp, vp, vp, ci, vp, ci, ci, ci, vp, ci, vp, vp, vp, vp, ci, vp]),
+    "atlasx_pagedkv_create": (ci, [vp, ci, ci, ci, ci, ci, pvp]),
+    "atlasx_pagedkv_free": (ci, [vp]),
+    "atlasx_pagedkv_bytes": (sz, [ci, ci, ci, ci, ci]),
+    "atlasx_pagedkv_ptrs": (ci, [vp, pvp, C.POINTER(sz), C.POINTER(sz)]),
+    "atlasx_pagedkv_append": (ci, [vp, vp, ci, vp, ll, ll, vp, ll, ll, vp, ci]),
+    "atlasx_pagedkv_read": (ci, [vp, vp, vp, ci, ci, vp, vp]),
+    "atlasx_pagedkv_decode_attention": (ci, [vp, vp, vp, vp, ci, vp, ci, vp, ci, cf, ci, vp, sz]),
+    "atlasx_prompt_attention": (ci, [vp, ci, vp, ll, ll, vp, ll, ll, vp, ll, ll, vp, ll, ll, vp, vp, ci, ci, ci, ci, ci, ci, cf, ci]),
     "atlasx_model_create": (ci, [vp, C.POINTER(ModelConfigC), vp, pvp]),
     "atlasx_model_free": (ci, [vp]),
     "atlasx_model_set_tensor": (ci, [vp, ci, ci, vp, ci, ci]),

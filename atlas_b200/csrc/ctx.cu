@@ -11,6 +11,7 @@
 #include "elementwise.cuh"
 #include "gemv.cuh"
 #include "objects.h"
+#include "paged.cuh"
 #include "sampling.cuh"
 
 // ── error text ───────────────────────────────────────────────────────────────────
@@ -122,6 +123,8 @@ extern "C" int atlasx_ctx_poll_device_error(atlasx_ctx* c, int* code_out) {
         if (c->attn_tickets) AX_CUDA(cudaMemsetAsync(c->attn_tickets, 0, c->attn_tickets_cap * sizeof(unsigned), c->stream));
     }
     if (code_out) *code_out = code;
+    if (code == AX_DEVERR_PAGE) return atlasx_fail(ATLASX_ERR_ARG, "a block table named a page outside the pool; its rows were left out");
+    if (code == AX_DEVERR_SLOT) return atlasx_fail(ATLASX_ERR_ARG, "a slot lay behind the pool; its row was left out");
     return code ? atlasx_fail(ATLASX_ERR_TIMEOUT, "a bounded device-side wait expired (code %d)", code) : ATLASX_OK;
 }
 

@@ -1,0 +1,408 @@
+// paged.cu — bookkeeping of a packed serving step and the four-bit paged KV cache: block tables, slots and positions from request
+// lengths (ax_page_plan_kernel), rows rounded to four bits into their slots (ax_p4_append_kernel) and back (ax_p4_read_kernel).
+// The reference keeps one linear f32 cache per sequence (GpuKvCache, crates/atlas-tensor/src/lib.rs:701-785); the number format is
+// that of its Int4Tensor (crates/atlas-quant/src/lib.rs:113-145) with the scale held as bf16.
+#include <new>
+
+#include "paged.cuh"
+
+namespace {
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanItems = 1024;      // tokens (and pages taken) per CTA
+
+struct PlanArgs {
+    const int *cached, *fresh, *free;
+    int batch, n_free, page_size, n_pages, table_width, n_tokens;
+    int *table, *cu, *lens, *slots, *pos, *status;
+};
+
+// largest b with start[b] <= x, start[0] = 0
+__device__ __forceinline__ int find_start(const int* start, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (start[m] <= x) lo = m; else hi = m; }
+    return lo;
+}
+
+// One launch, no second pass: every CTA scans the request lengths itself (at most 4096, from L2) and then serves its own range
+// of tokens and of pages taken.  What bounds it is the latency of one dependent chain — lengths → scan → search → table entry —
+// and the launch, not bandwidth.  Page j of the plan is free[j]; it belongs to the request in whose range of the scan over
+// (pages needed − pages held) j falls, so the result does not depend on the order of CTAs.
+__global__ void __launch_bounds__(kPlanThreads) ax_page_plan_kernel(const PlanArgs a) {
+    extern __shared__ int sh[];
+    int* s_cu = sh;                               // [batch + 1] first token of each request
+    int* s_first = sh + a.batch + 1;              // [batch + 1] first page taken
+    __shared__ unsigned long long s_tok[kPlanThreads / 32], s_pg[kPlanThreads / 32];
+    __shared__ int s_bad;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+    const int per = (a.batch + kPlanThreads - 1) / kPlanThreads;
+    const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+    unsigned long long tok = 0, pg = 0;
+    int bad = 0;
+    for (int b = b0; b < b1; b++) {
+        const int c = a.cached[b], n = a.fresh[b];
+        const long long need = ((long long)c + n + a.page_size - 1) / a.page_size;
+        if (c < 0 || n < 0 || need > a.table_width) { bad++; continue; }
+        tok += n;
+        pg += need - (c + (long long)a.page_size - 1) / a.page_size;
+    }
+    if (bad) atomicAdd(&s_bad, bad);
+    unsigned long long it = tok, ip = pg;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const unsigned long long xt = __shfl_up_sync(AX_FULL, it, d), xp = __shfl_up_sync(AX_FULL, ip, d);
+        if (lane >= d) { it += xt; ip += xp; }
+    }
+    if (lane == 31) { s_tok[warp] = it; s_pg[warp] = ip; }
+    __syncthreads();
+    unsigned long long bt = 0, bp = 0, all_t = 0, all_p = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; w++) {
+        if (w < warp) { bt += s_tok[w]; bp += s_pg[w]; }
+        all_t += s_tok[w]; all_p += s_pg[w];
+    }
+    const int n_bad = s_bad + (all_t > (unsigned long long)a.n_tokens ? 1 : 0);
+    const bool short_of = all_p > (unsigned long long)a.n_free;
+    const bool refused = n_bad > 0 || short_of;
+    if (blockIdx.x == 0 && tid == 0) {
+        a.status[0] = refused ? 0 : (int)all_p;
+        const unsigned long long miss = all_p - (unsigned long long)a.n_free;
+        a.status[1] = !n_bad && short_of ? (int)(miss > 0x7FFFFFFFull ? 0x7FFFFFFFull : miss) : 0;
+        a.status[2] = n_bad;
+    }
+    if (refused) {                                // nothing is planned: the calls that follow see empty requests and absent rows
+        for (int i = blockIdx.x * kPlanThreads + tid; i < max(a.batch + 1, a.n_tokens); i += gridDim.x * kPlanThreads) {
+            if (i < a.batch + 1) a.cu[i] = 0;
+            if (i < a.batch) a.lens[i] = 0;
+            if (i < a.n_tokens) { a.slots[i] = -1; a.pos[i] = -1; }
+        }
+        return;
+    }
+    int t = (int)(bt + it - tok), p = (int)(bp + ip - pg);
+    for (int b = b0; b < b1; b++) {
+        const int c = a.cached[b], n = a.fresh[b];
+        s_cu[b] = t; s_first[b] = p;
+        if (blockIdx.x == 0) { a.cu[b] = t; a.lens[b] = c + n; }
+        t += n;
+        p += (int)(((long long)c + n + a.page_size - 1) / a.page_size - (c + (long long)a.page_size - 1) / a.page_size);
+    }
+    if (tid == 0) {
+        s_cu[a.batch] = (int)all_t; s_first[a.batch] = (int)all_p;
+        if (blockIdx.x == 0) a.cu[a.batch] = (int)all_t;
+    }
+    __syncthreads();
+    const int n_tok = (int)all_t, n_pg = (int)all_p;
+    const int base = blockIdx.x * kPlanItems, end = min(base + kPlanItems, max(a.n_tokens, n_pg));
+    for (int i = base + tid; i < end; i += kPlanThreads) {
+        if (i < n_pg) {
+            const int b = find_start(s_first, a.batch + 1, i);
+            const int had = (int)((a.cached[b] + (long long)a.page_size - 1) / a.page_size);
+            a.table[(size_t)b * a.table_width + had + (i - s_first[b])] = a.free[i];
+        }
+        if (i < n_tok) {
+            const int b = find_start(s_cu, a.batch + 1, i);
+            const int c = a.cached[b], at = c + (i - s_cu[b]);
+            const int had = (int)((c + (long long)a.page_size - 1) / a.page_size), col = at / a.page_size;
+            const int page = col < had ? a.table[(size_t)b * a.table_width + col] : a.free[s_first[b] + (col - had)];
+            a.slots[i] = page >= 0 && page < a.n_pages ? page * a.page_size + at % a.page_size : -1;
+            a.pos[i] = at;
+        } else if (i < a.n_tokens) {              // rows behind the last request
+            a.slots[i] = -1; a.pos[i] = -1;
+        }
+    }
+}
+
+// ── rows to four bits ────────────────────────────────────────────────────────────
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]);
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <> __device__ __forceinline__ void load8<uint16_t>(const uint16_t* p, float (&x)[8]) {      // bf16 bits
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = { a.x, a.y, a.z, a.w };
+#pragma unroll
+    for (int i = 0; i < 4; i++) { x[2 * i] = ax_bf16_lo(w[i]); x[2 * i + 1] = ax_bf16_hi(w[i]); }
+}
+template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = { a.x, a.y, a.z, a.w };
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x; x[2 * i + 1] = f.y;
+    }
+}
+
+struct RowArgs {
+    AxP4Shape s;
+    uint8_t* pool;
+    const void *k, *v;            // append: [token][head][hd], token and head strides in elements
+    long long k_tok, k_head, v_tok, v_head;
+    void *k_out, *v_out;          // read: contiguous [token][head][hd]
+    const int* slots;
+    int n;
+    int* err;
+};
+
+// A lane holds eight consecutive numbers of one row of K or V; 4 or 8 lanes make a group and find its largest magnitude with
+// shuffles.  scale = bf16(max / 7); the number is x · (1 / scale) rounded half away from zero, at most 7 in magnitude — the f32
+// arithmetic of Int4Tensor::quantize with a scale of 16 bits: the numbers are rounded against the scale that is stored, so its
+// own rounding (2^-9 of itself) costs nothing beyond the half step of the number.  A group with a NaN or an infinity gets the scale NaN.
+// Bytes: the rows once, 4.25 or 4.5 bits per number out.
+template <typename T>
+__global__ void __launch_bounds__(256) ax_p4_append_kernel(const RowArgs a) {
+    const int lanes = a.s.hd / 8, gl = a.s.group / 8;                 // lanes per row, lanes per group
+    const long long jobs = (long long)a.n * a.s.n_kv * 2 * lanes;     // K of a (token, head), then its V
+    const long long job = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    const bool live = job < jobs;
+    const int li = (int)(job % lanes);
+    const long long row = job / lanes;
+    const int which = (int)(row & 1), head = (int)((row >> 1) % a.s.n_kv), tok = live ? (int)((row >> 1) / a.s.n_kv) : 0;
+    float x[8];
+    float top = 0.f;
+    int slot = -1;
+    if (live) {
+        slot = a.slots[tok];
+        const T* src = which ? (const T*)a.v + tok * a.v_tok + head * a.v_head : (const T*)a.k + tok * a.k_tok + head * a.k_head;
+        load8<T>(src + 8 * li, x);
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) { const float m = fabsf(x[i]); odd |= !(m <= 3.402823466e38f); top = fmaxf(top, m); }
+        if (odd) top = __int_as_float(0x7F800000);
+    }
+    for (int d = 1; d < gl; d <<= 1) top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, d));
+    if (!live || slot < 0) return;                                   // a negative slot marks an absent row
+    if (slot >= a.s.n_pages * a.s.page_size) { if (li == 0) atomicExch(a.err, AX_DEVERR_SLOT); return; }
+    const bool odd = top > 3.402823466e38f;
+    uint16_t sb = ax_f32_to_bf16_rne(__fdiv_rn(top, 7.0f));
+    float sc = ax_bf16_to_f32(sb);
+    if (sc < 1.17549435e-38f) { sc = 1.0f; sb = 0x3F80; }
+    if (odd) sb = 0x7FC0;
+    const float inv = __frcp_rn(sc);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float q = odd ? 0.f : roundf(__fmul_rn(x[i], inv));
+        q = fminf(fmaxf(q, -7.f), 7.f);
+        w |= (uint32_t)((int)q + 8) << (4 * i);
+    }
+    const int page = slot / a.s.page_size, off = slot % a.s.page_size, r = off % AX_P4_TILE;
+    uint8_t* tile = a.pool + ax_p4_tile_at(a.s, page, head, off);
+    const int plane = ax_p4_plane_bytes(a.s);
+    if (which == 0) {
+        reinterpret_cast<uint32_t*>(tile)[ax_p4_k_word(a.s, r, 8 * li)] = ax_p4_rot(w);
+    } else {
+        uint16_t* vp = reinterpret_cast<uint16_t*>(tile + plane);
+        vp[ax_p4_v_half(a.s, r, 8 * li)] = (uint16_t)(w & 0xFFFFu);
+        vp[ax_p4_v_half(a.s, r, 8 * li + 4)] = (uint16_t)(w >> 16);
+    }
+    if (li % gl == 0) {
+        uint16_t* sp = reinterpret_cast<uint16_t*>(tile + 2 * plane + which * ax_p4_scale_bytes(a.s));
+        sp[ax_p4_scale(a.s, r, li / gl)] = sb;
+    }
+}
+
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]);
+template <> __device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <> __device__ __forceinline__ void store8<uint16_t>(uint16_t* p, const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = ax_f32_to_bf16_rne(x[2 * i]) | ((uint32_t)ax_f32_to_bf16_rne(x[2 * i + 1]) << 16);
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <> __device__ __forceinline__ void store8<__half>(__half* p, const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&h); }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The values a slot holds: number · scale, exact in f32 (4 + 8 bits), one rounding for the 16-bit types.  Absent rows read as zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) ax_p4_read_kernel(const RowArgs a) {
+    const int lanes = a.s.hd / 8, gl = a.s.group / 8;
+    const long long jobs = (long long)a.n * a.s.n_kv * lanes;
+    const long long job = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (job >= jobs) return;
+    const int li = (int)(job % lanes);
+    const long long row = job / lanes;
+    const int head = (int)(row % a.s.n_kv), tok = (int)(row / a.s.n_kv);
+    const int slot = a.slots[tok];
+    float k[8], v[8];
+    if (slot >= 0 && slot < a.s.n_pages * a.s.page_size) {
+        const int page = slot / a.s.page_size, off = slot % a.s.page_size, r = off % AX_P4_TILE;
+        const uint8_t* tile = a.pool + ax_p4_tile_at(a.s, page, head, off);
+        const int plane = ax_p4_plane_bytes(a.s);
+        const uint32_t kw = ax_p4_unrot(reinterpret_cast<const uint32_t*>(tile)[ax_p4_k_word(a.s, r, 8 * li)]);
+        const uint16_t* vp = reinterpret_cast<const uint16_t*>(tile + plane);
+        const uint32_t vw = vp[ax_p4_v_half(a.s, r, 8 * li)] | ((uint32_t)vp[ax_p4_v_half(a.s, r, 8 * li + 4)] << 16);
+        const uint16_t* sp = reinterpret_cast<const uint16_t*>(tile + 2 * plane);
+        const float ks = ax_bf16_to_f32(sp[ax_p4_scale(a.s, r, li / gl)]);
+        const float vs = ax_bf16_to_f32(sp[AX_P4_TILE * ax_p4_groups(a.s) + ax_p4_scale(a.s, r, li / gl)]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            k[i] = (float)((int)((kw >> (4 * i)) & 15u) - 8) * ks;
+            v[i] = (float)((int)((vw >> (4 * i)) & 15u) - 8) * vs;
+        }
+    } else {
+        if (slot >= 0) atomicExch(a.err, AX_DEVERR_SLOT);
+#pragma unroll
+        for (int i = 0; i < 8; i++) { k[i] = 0.f; v[i] = 0.f; }
+    }
+    const size_t o = ((size_t)tok * a.s.n_kv + head) * a.s.hd + 8 * li;
+    store8<T>((T*)a.k_out + o, k);
+    store8<T>((T*)a.v_out + o, v);
+}
+
+int elem_bytes(int dtype) { return dtype == ATLASX_F32 ? 4 : 2; }
+
+}  // namespace
+
+extern "C" int atlasx_page_plan(atlasx_ctx* c, const int* cached, const int* fresh, int batch, const int* free_pages, int n_free,
+                                int page_size, int n_pages, int* table, int table_width, int* cu, int* lens, int* slots, int* pos,
+                                int n_tokens, int* status) {
+    AX_ARG(cached && fresh && table && cu && lens && status, "null argument");
+    AX_ARG(batch >= 1 && batch <= AX_PAGED_MAX_BATCH, "batch must be in 1..4096");
+    AX_ARG(page_size >= 1 && n_pages >= 1 && (long long)page_size * n_pages <= 0x7FFFFFFFll, "page_size · n_pages must be in 1..2^31 - 1");
+    AX_ARG(table_width >= 1, "the block table needs a column");
+    AX_ARG(n_tokens >= 0 && n_free >= 0, "counts must not be negative");
+    AX_ARG((free_pages || !n_free) && ((slots && pos) || !n_tokens), "null argument");
+    AX_ARG(c, "ctx is null");
+    AX_ON_DEVICE(c);
+    PlanArgs a = { cached, fresh, free_pages, batch, n_free, page_size, n_pages, table_width, n_tokens, table, cu, lens, slots, pos, status };
+    const int grid = n_tokens ? (n_tokens + kPlanItems - 1) / kPlanItems : 1;      // a page is taken for a new token: never more pages than tokens
+    ax_page_plan_kernel<<<grid, kPlanThreads, (size_t)2 * (batch + 1) * sizeof(int), c->stream>>>(a);
+    AX_CHECK_LAUNCH("ax_page_plan_kernel");
+    return ATLASX_OK;
+}
+
+static int check_shape(int n_pages, int page_size, int n_kv, int hd, int group) {
+    AX_ARG(n_pages >= 1 && n_kv >= 1, "n_pages and n_kv_heads must be positive");
+    AX_ARG(page_size >= AX_P4_TILE && page_size % AX_P4_TILE == 0, "page_size must be a multiple of 16");
+    AX_ARG((long long)n_pages * page_size <= 0x7FFFFFFFll, "n_pages · page_size must be below 2^31: slots are 32-bit");
+    AX_ARG(hd == 64 || hd == 128, "head_dim must be 64 or 128");
+    AX_ARG(group == 32 || group == 64, "group must be 32 or 64");
+    AX_ARG(n_kv <= 65535, "too many KV heads");
+    return ATLASX_OK;
+}
+extern "C" size_t atlasx_pagedkv_bytes(int n_pages, int page_size, int n_kv, int hd, int group) {
+    if (check_shape(n_pages, page_size, n_kv, hd, group)) return 0;
+    const AxP4Shape s = { n_pages, page_size, n_kv, hd, group };
+    return ax_p4_pool_bytes(s);
+}
+extern "C" int atlasx_pagedkv_create(atlasx_ctx* c, int n_pages, int page_size, int n_kv, int hd, int group, atlasx_pagedkv** out) {
+    AX_ARG(out, "null argument");
+    int rc = check_shape(n_pages, page_size, n_kv, hd, group);
+    if (rc) return rc;
+    AX_ARG(c, "ctx is null");
+    AX_ON_DEVICE(c);
+    atlasx_pagedkv* kv = new (std::nothrow) atlasx_pagedkv();
+    if (!kv) return atlasx_fail(ATLASX_ERR_STATE, "out of host memory");
+    kv->ctx = c;
+    kv->s = { n_pages, page_size, n_kv, hd, group };
+    kv->workspace_bytes = ax_paged_attn_workspace_bytes(c, kv->s);
+    const size_t bytes = ax_p4_pool_bytes(kv->s);
+    cudaError_t e = cudaMalloc((void**)&kv->pool, bytes);
+    if (e == cudaSuccess) e = cudaMalloc(&kv->workspace, kv->workspace_bytes);
+    if (e == cudaSuccess) e = cudaMemsetAsync(kv->pool, 0, bytes, c->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(kv->workspace, 0, kv->workspace_bytes, c->stream);
+    if (e != cudaSuccess) {
+        cudaFree(kv->pool); cudaFree(kv->workspace); delete kv;
+        cudaGetLastError();
+        return atlasx_fail(ATLASX_ERR_CUDA, "paged cache of %zu bytes: %s", bytes, cudaGetErrorString(e));
+    }
+    *out = kv;
+    return ATLASX_OK;
+}
+extern "C" int atlasx_pagedkv_free(atlasx_pagedkv* kv) {
+    if (!kv) return ATLASX_OK;
+    AX_ON_DEVICE(kv->ctx);
+    cudaStreamSynchronize(kv->ctx->stream);
+    cudaFree(kv->pool); cudaFree(kv->workspace);
+    delete kv;
+    return ATLASX_OK;
+}
+extern "C" int atlasx_pagedkv_ptrs(atlasx_pagedkv* kv, void** pool, size_t* bytes, size_t* workspace_bytes) {
+    AX_ARG(kv, "kv is null");
+    if (pool) *pool = kv->pool;
+    if (bytes) *bytes = ax_p4_pool_bytes(kv->s);
+    if (workspace_bytes) *workspace_bytes = kv->workspace_bytes;
+    return ATLASX_OK;
+}
+
+extern "C" int atlasx_pagedkv_append(atlasx_ctx* c, atlasx_pagedkv* kv, int dtype, const void* k, long long k_token_stride,
+                                     long long k_head_stride, const void* v, long long v_token_stride, long long v_head_stride,
+                                     const int* slots, int n) {
+    AX_ARG(dtype == ATLASX_F32 || dtype == ATLASX_BF16 || dtype == ATLASX_F16, "dtype must be f32, bf16 or f16");
+    AX_ARG(n >= 0, "the number of rows must not be negative");
+    if (n == 0) return ATLASX_OK;
+    AX_ARG(k && v && slots, "null argument");
+    const long long step = 16 / elem_bytes(dtype);
+    AX_ARG(((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_token_stride % step == 0 && k_head_stride % step == 0 &&
+           v_token_stride % step == 0 && v_head_stride % step == 0, "rows must start on 16-byte boundaries");
+    AX_ARG(c && kv, "ctx or cache is null");
+    AX_ARG(kv->ctx == c, "the cache belongs to another context");
+    AX_ON_DEVICE(c);
+    RowArgs a = {};
+    a.s = kv->s; a.pool = kv->pool; a.k = k; a.v = v;
+    a.k_tok = k_token_stride; a.k_head = k_head_stride; a.v_tok = v_token_stride; a.v_head = v_head_stride;
+    a.slots = slots; a.n = n; a.err = c->dev_error;
+    const long long jobs = (long long)n * kv->s.n_kv * 2 * (kv->s.hd / 8);
+    AX_ARG((jobs + 255) / 256 <= 0x7FFFFFFFll, "too many rows for one call");
+    const unsigned grid = (unsigned)((jobs + 255) / 256);
+    if (dtype == ATLASX_F32) ax_p4_append_kernel<float><<<grid, 256, 0, c->stream>>>(a);
+    else if (dtype == ATLASX_BF16) ax_p4_append_kernel<uint16_t><<<grid, 256, 0, c->stream>>>(a);
+    else ax_p4_append_kernel<__half><<<grid, 256, 0, c->stream>>>(a);
+    AX_CHECK_LAUNCH("ax_p4_append_kernel");
+    return ATLASX_OK;
+}
+extern "C" int atlasx_pagedkv_read(atlasx_ctx* c, const atlasx_pagedkv* kv, const int* slots, int n, int dtype, void* k_out, void* v_out) {
+    AX_ARG(dtype == ATLASX_F32 || dtype == ATLASX_BF16 || dtype == ATLASX_F16, "dtype must be f32, bf16 or f16");
+    AX_ARG(n >= 0, "the number of rows must not be negative");
+    if (n == 0) return ATLASX_OK;
+    AX_ARG(k_out && v_out && slots, "null argument");
+    AX_ARG(((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0, "outputs must be 16-byte aligned");
+    AX_ARG(c && kv, "ctx or cache is null");
+    AX_ARG(kv->ctx == c, "the cache belongs to another context");
+    AX_ON_DEVICE(c);
+    RowArgs a = {};
+    a.s = kv->s; a.pool = kv->pool; a.k_out = k_out; a.v_out = v_out; a.slots = slots; a.n = n; a.err = c->dev_error;
+    const long long jobs = (long long)n * kv->s.n_kv * (kv->s.hd / 8);
+    AX_ARG((jobs + 255) / 256 <= 0x7FFFFFFFll, "too many rows for one call");
+    const unsigned grid = (unsigned)((jobs + 255) / 256);
+    if (dtype == ATLASX_F32) ax_p4_read_kernel<float><<<grid, 256, 0, c->stream>>>(a);
+    else if (dtype == ATLASX_BF16) ax_p4_read_kernel<uint16_t><<<grid, 256, 0, c->stream>>>(a);
+    else ax_p4_read_kernel<__half><<<grid, 256, 0, c->stream>>>(a);
+    AX_CHECK_LAUNCH("ax_p4_read_kernel");
+    return ATLASX_OK;
+}
+
+extern "C" int atlasx_pagedkv_decode_attention(atlasx_ctx* c, const atlasx_pagedkv* kv, const float* q, float* out, int n_heads,
+                                               const int* table, int table_width, const int* lens, int batch, float scale,
+                                               int window, void* workspace, size_t workspace_bytes) {
+    AX_ARG(q && out && table && lens, "null argument");
+    AX_ARG(batch >= 1 && batch <= AX_PAGED_MAX_BATCH, "batch must be in 1..4096");
+    AX_ARG(n_heads >= 1, "n_heads must be positive");
+    AX_ARG(table_width >= 1, "the block table needs a column");
+    AX_ARG(window >= 0, "window must be non-negative");
+    AX_ARG(scale - scale == 0.f, "scale must be finite");
+    AX_ARG(((uintptr_t)q | (uintptr_t)out) % 16 == 0, "q and out must be 16-byte aligned");
+    AX_ARG(c && kv, "ctx or cache is null");
+    AX_ARG(kv->ctx == c, "the cache belongs to another context");
+    AX_ARG(n_heads % kv->s.n_kv == 0, "n_heads must be a multiple of n_kv_heads");
+    const long long rows = (long long)table_width * kv->s.page_size;
+    AX_ARG(rows <= 0x7FFFFFFFll && (rows / AX_P4_TILE) * batch <= 0x7FFFFFFFll, "the block table spans too many rows");
+    AX_ARG(!workspace || (workspace_bytes >= kv->workspace_bytes && (uintptr_t)workspace % 16 == 0),
+           "the workspace is too small or not 16-byte aligned");
+    AX_ON_DEVICE(c);
+    AxPagedAttnArgs a;
+    a.q = q; a.out = out; a.table = table; a.lens = lens; a.table_width = table_width; a.batch = batch; a.n_heads = n_heads;
+    a.window = window; a.scale = scale; a.workspace = workspace ? workspace : kv->workspace;
+    return ax_paged_attn_launch(c, kv, a);
+}

@@ -1,0 +1,46 @@
+// paged.cuh — object and launch declarations of the packed serving step: four-bit paged cache and prompt attention.
+#pragma once
+#include "common.cuh"
+#include "paged_index.h"
+
+#define AX_PAGED_MAX_BATCH 4096
+
+// codes of the device error word beside those of the bounded waits: what an index array holds, not a wait, was wrong
+#define AX_DEVERR_PAGE 801      // a block table names a page outside the pool
+#define AX_DEVERR_SLOT 802      // a slot lies behind the pool
+
+struct atlasx_pagedkv {
+    atlasx_ctx* ctx = nullptr;
+    AxP4Shape s = {};
+    uint8_t* pool = nullptr;
+    void* workspace = nullptr;       // of the calls that bring none
+    size_t workspace_bytes = 0;
+};
+
+// Makes the context's device current for the duration of a call and puts the caller's back.
+struct AxDeviceGuard {
+    int prev = -1;
+    cudaError_t err = cudaSuccess;
+    explicit AxDeviceGuard(int device) {
+        err = cudaGetDevice(&prev);
+        if (err == cudaSuccess && prev != device) err = cudaSetDevice(device);
+        else prev = -1;
+    }
+    ~AxDeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
+};
+#define AX_ON_DEVICE(ctx)                                                                  \
+    AxDeviceGuard _guard((ctx)->device);                                                   \
+    if (_guard.err != cudaSuccess)                                                         \
+        return atlasx_fail(ATLASX_ERR_CUDA, "device %d: %s", (ctx)->device, cudaGetErrorString(_guard.err))
+
+struct AxPagedAttnArgs {
+    const float* q;                  // [batch][n_heads][hd]
+    float* out;
+    const int* table;                // [batch][table_width] page numbers
+    const int* lens;                 // [batch] cached rows
+    int table_width, batch, n_heads, window;
+    float scale;
+    void* workspace;                 // of ax_paged_attn_workspace_bytes()
+};
+size_t ax_paged_attn_workspace_bytes(const atlasx_ctx* ctx, const AxP4Shape& s);
+int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPagedAttnArgs& a);

@@ -1,0 +1,220 @@
+"""A packed serving step over the C ABI: block tables and slots from request lengths (page_plan), the four-bit paged KV cache
+(PagedKvCache) and the causal attention of whole packed prompts (prompt_attention).
+
+The calls take device arrays: a DeviceArray of this module, or anything with data_ptr(), shape, stride(), dtype and device as a
+PyTorch tensor has them (PyTorch itself is not imported).  They run on the context's stream and return at once; arrays that another
+stream fills have to be ordered before them (`Context.stream`), and arrays must live until the stream has passed the call.
+"""
+import ctypes as C
+import math
+
+import numpy as np
+
+from . import _ffi
+from ._ffi import AtlasError, BF16, F16, F32, check
+from .tensor import Context
+
+I32 = "int32"
+_NAMES = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.float16": F16, "torch.int32": I32}
+_NUMPY = {F32: np.float32, BF16: np.uint16, F16: np.float16, I32: np.int32}     # bf16 as its bit patterns
+_SHOWN = {F32: "f32", BF16: "bf16", F16: "f16", I32: "int32"}
+
+
+class DeviceArray:
+    """A typed array in HBM; strides in elements (None: contiguous).  dtype F32, BF16 (uint16 bit patterns on the host), F16 or I32."""
+
+    def __init__(self, ctx, ptr, shape, dtype, strides=None, owner=False, base=None):
+        self.ctx, self.ptr, self.shape, self.dtype = ctx, int(ptr), tuple(int(n) for n in shape), dtype
+        if strides is None:
+            strides, n = [], 1
+            for m in reversed(self.shape):
+                strides.insert(0, n)
+                n *= m
+        self.strides, self._owner, self._base = tuple(int(n) for n in strides), owner, base
+
+    @classmethod
+    def empty(cls, shape, dtype, ctx=None):
+        ctx = ctx or Context.default()
+        n = int(np.prod(shape, dtype=np.int64)) * np.dtype(_NUMPY[dtype]).itemsize
+        return cls(ctx, ctx.malloc(max(n, 16)), shape, dtype, owner=True)
+
+    @classmethod
+    def from_host(cls, data, dtype, ctx=None):
+        a = np.ascontiguousarray(data, dtype=_NUMPY[dtype])
+        out = cls.empty(a.shape, dtype, ctx)
+        if a.size:
+            out.ctx.upload(out.ptr, a)
+        return out
+
+    def download(self):
+        """The values of a contiguous array."""
+        n, strides = 1, []
+        for m in reversed(self.shape):
+            strides.insert(0, n)
+            n *= m
+        if n and any(m > 1 and s != t for m, s, t in zip(self.shape, self.strides, strides)):
+            raise AtlasError("download needs a contiguous array")
+        return self.ctx.download(self.ptr, self.shape, _NUMPY[self.dtype])
+
+    def columns(self, first, shape, strides):
+        """A view that starts `first` elements in, with a shape and strides of its own."""
+        return DeviceArray(self.ctx, self.ptr + first * np.dtype(_NUMPY[self.dtype]).itemsize, shape, self.dtype, strides, base=self)
+
+    def __del__(self):
+        try:
+            if self._owner and self.ptr and self.ctx.handle:
+                self.ctx.free(self.ptr)
+        except Exception:
+            pass
+        self.ptr = 0
+
+
+def _view(x, name, dtypes, ndim, device):
+    """(ptr, shape, strides, dtype) of a device array, checked."""
+    if type(x) is DeviceArray:
+        ptr, shape, strides, dtype, at = x.ptr, x.shape, x.strides, x.dtype, x.ctx.device
+    else:
+        try:
+            ptr, shape, strides, dtype, at = x.data_ptr(), x.shape, x.stride(), _NAMES.get(str(x.dtype)), x.device
+            at = at.index if at.type == "cuda" else -1
+        except AttributeError:
+            raise AtlasError("%s is not a device array" % name) from None
+    if dtype not in dtypes:
+        raise AtlasError("%s must be %s" % (name, " or ".join(_SHOWN[d] for d in dtypes)))
+    if len(shape) != ndim:
+        raise AtlasError("%s must have %d dimensions, not %d" % (name, ndim, len(shape)))
+    if at != device:
+        raise AtlasError("%s is not on device %d" % (name, device))
+    return ptr, shape, strides, dtype
+
+
+def _ints(x, name, shape, device):
+    """Pointer of a contiguous int32 array; None in `shape` stands for any extent."""
+    ptr, got, strides, _ = _view(x, name, (I32,), len(shape), device)
+    n = 1
+    for i in range(len(shape) - 1, -1, -1):
+        if shape[i] is not None and got[i] != shape[i]:
+            raise AtlasError("%s must have shape %s, not %s" % (name, tuple(shape), tuple(got)))
+        if got[i] > 1 and strides[i] != n:
+            raise AtlasError("%s must be contiguous" % name)
+        n *= got[i]
+    return ptr
+
+
+def _rows(x, name, dtypes, device, heads=None, head_dim=None):
+    """(ptr, rows, token stride, head stride, dtype, heads, head_dim) of [rows, heads, head_dim] with unit stride along a row."""
+    ptr, shape, strides, dtype = _view(x, name, dtypes, 3, device)
+    if (heads is not None and shape[1] != heads) or (head_dim is not None and shape[2] != head_dim):
+        raise AtlasError("%s must be [rows, %s, %s], not %s" % (name, heads, head_dim, tuple(shape)))
+    if shape[2] > 1 and strides[2] != 1:
+        raise AtlasError("%s must have unit stride along head_dim" % name)
+    return ptr, shape[0], strides[0], strides[1], dtype, shape[1], shape[2]
+
+
+def _contiguous(view, name):
+    _, rows, tok, head, _, heads, hd = view
+    if (heads > 1 and head != hd) or (rows > 1 and tok != heads * hd):
+        raise AtlasError("%s must be contiguous" % name)
+    return view
+
+
+def _device(ctx, x):
+    """Device of the call: the context's, or — before there is one — the first array's."""
+    return ctx.device if ctx is not None else (x.ctx.device if type(x) is DeviceArray else 0)
+
+
+def page_plan(cached, fresh, free_pages, table, cu, lens, slots, pos, status, page_size, n_pages, ctx=None):
+    """Block tables, slots and positions of a step from request lengths: see atlasx_page_plan.  int32 device arrays: cached, fresh,
+    lens [batch]; free_pages [any]; table [batch, width], extended in place; cu [batch + 1]; slots, pos [rows]; status [3]."""
+    dev = _device(ctx, cached)
+    p_cached, shape, _, _ = _view(cached, "cached", (I32,), 1, dev)
+    b, rows = shape[0], slots.shape[0]
+    p_cached = _ints(cached, "cached", (b,), dev)
+    p = (_ints(fresh, "fresh", (b,), dev), _ints(free_pages, "free_pages", (None,), dev), _ints(table, "table", (b, None), dev),
+         _ints(cu, "cu", (b + 1,), dev), _ints(lens, "lens", (b,), dev), _ints(slots, "slots", (rows,), dev), _ints(pos, "pos", (rows,), dev),
+         _ints(status, "status", (3,), dev))
+    ctx = ctx or Context.default()
+    check(_ffi.lib().atlasx_page_plan(ctx.handle, p_cached, p[0], b, p[1], free_pages.shape[0], page_size, n_pages, p[2], table.shape[1],
+                                      p[3], p[4], p[5], p[6], rows, p[7]))
+
+
+class PagedKvCache:
+    """Keys and values of many requests in pages of four-bit numbers with a bf16 scale per `group` of them (GpuKvCache with pages
+    and the Int4Tensor number format): 4.25 or 4.5 bits per number instead of 16 or 32."""
+
+    def __init__(self, n_pages, page_size, n_kv_heads, head_dim, group=32, ctx=None):
+        self.ctx = ctx or Context.default()
+        self._h = None
+        h = C.c_void_p()
+        check(_ffi.lib().atlasx_pagedkv_create(self.ctx.handle, n_pages, page_size, n_kv_heads, head_dim, group, C.byref(h)))
+        self._h = h
+        self.n_pages, self.page_size, self.n_kv_heads, self.head_dim, self.group = n_pages, page_size, n_kv_heads, head_dim, group
+        pool, n, w = C.c_void_p(), C.c_size_t(), C.c_size_t()
+        check(_ffi.lib().atlasx_pagedkv_ptrs(h, C.byref(pool), C.byref(n), C.byref(w)))
+        self.bytes, self.workspace_bytes = n.value, w.value
+
+    def workspace(self):
+        """A zeroed workspace for decode_attention calls that may run beside others of this cache."""
+        p = DeviceArray.empty((self.workspace_bytes + 3) // 4 * np.ones(1, np.int64), I32, self.ctx)
+        check(_ffi.lib().atlasx_memset(self.ctx.handle, C.c_void_p(p.ptr), 0, self.workspace_bytes))
+        return p
+
+    def append(self, k, v, slots):
+        """Rows of k and v [rows, n_kv_heads, head_dim] (f32, bf16 or f16, any strides of whole 16 bytes) into their slots;
+        a negative slot marks a row that is not there."""
+        dev, types = self.ctx.device, (F32, BF16, F16)
+        kp, n, kt, kh, dt, _, _ = _rows(k, "k", types, dev, self.n_kv_heads, self.head_dim)
+        vp, m, vt, vh, dv, _, _ = _rows(v, "v", types, dev, self.n_kv_heads, self.head_dim)
+        if n != m or dt != dv:
+            raise AtlasError("k and v must have the same rows and type")
+        check(_ffi.lib().atlasx_pagedkv_append(self.ctx.handle, self._h, dt, kp, kt, kh, vp, vt, vh, _ints(slots, "slots", (n,), dev), n))
+
+    def read(self, slots, k_out, v_out):
+        """The values that the slots hold into contiguous [rows, n_kv_heads, head_dim] arrays (f32, bf16 or f16)."""
+        dev, types = self.ctx.device, (F32, BF16, F16)
+        kp, n, _, _, dt, _, _ = _contiguous(_rows(k_out, "k_out", types, dev, self.n_kv_heads, self.head_dim), "k_out")
+        vp, m, _, _, dv, _, _ = _contiguous(_rows(v_out, "v_out", types, dev, self.n_kv_heads, self.head_dim), "v_out")
+        if n != m or dt != dv:
+            raise AtlasError("k_out and v_out must have the same rows and type")
+        check(_ffi.lib().atlasx_pagedkv_read(self.ctx.handle, self._h, _ints(slots, "slots", (n,), dev), n, dt, kp, vp))
+
+    def decode_attention(self, q, out, table, lens, scale, window_size=0, workspace=None):
+        """Attention of one token per request: q, out [batch, n_heads, head_dim] f32, table [batch, width] page numbers, lens [batch]
+        cached rows (the new token's own among them)."""
+        dev = self.ctx.device
+        qp, b, _, _, _, nh, _ = _contiguous(_rows(q, "q", (F32,), dev, None, self.head_dim), "q")
+        op = _contiguous(_rows(out, "out", (F32,), dev, nh, self.head_dim), "out")
+        if op[1] != b:
+            raise AtlasError("out must have the rows of q")
+        wp, wn = (None, 0) if workspace is None else (_ints(workspace, "workspace", (None,), dev), 4 * workspace.shape[0])
+        check(_ffi.lib().atlasx_pagedkv_decode_attention(self.ctx.handle, self._h, qp, op[0], nh, _ints(table, "table", (b, None), dev),
+                                                         table.shape[1], _ints(lens, "lens", (b,), dev), b, scale, window_size, wp, wn))
+
+    def __del__(self):
+        try:
+            if self._h and self.ctx.handle:
+                _ffi.lib().atlasx_pagedkv_free(self._h)
+        except Exception:
+            pass
+        self._h = None
+
+
+def prompt_attention(q, k, v, out, cu_q, cu_k, scale=None, window_size=0, ctx=None):
+    """Causal attention of packed prompts: q, out [rows, n_heads, head_dim], k, v [key rows, n_kv_heads, head_dim], bf16 or f16; sequence
+    b owns rows cu_q[b]..cu_q[b + 1] of q and cu_k[b]..cu_k[b + 1] of k and v, its last query at its last key.  scale None: 1/√head_dim."""
+    dev, types = _device(ctx, q), (BF16, F16)
+    qp, n, qt, qh, dt, nh, hd = _rows(q, "q", types, dev)
+    kp, m, kt, kh, dk, nk, _ = _rows(k, "k", types, dev, None, hd)
+    vp, mv, vt, vh, dv, _, _ = _rows(v, "v", types, dev, nk, hd)
+    op, on, ot, oh, do, _, _ = _rows(out, "out", types, dev, nh, hd)
+    if m != mv or on != n:
+        raise AtlasError("k and v, and q and out, must have the same rows")
+    if not dt == dk == dv == do:
+        raise AtlasError("q, k, v and out must have the same type")
+    cp, shape, _, _ = _view(cu_q, "cu_q", (I32,), 1, dev)
+    b = shape[0] - 1
+    cp = _ints(cu_q, "cu_q", (b + 1,), dev)
+    cq = _ints(cu_k, "cu_k", (b + 1,), dev)
+    ctx = ctx or Context.default()
+    check(_ffi.lib().atlasx_prompt_attention(ctx.handle, dt, qp, qt, qh, kp, kt, kh, vp, vt, vh, op, ot, oh, cp, cq, b, n, m, nh, nk, hd,
+                                             1.0 / math.sqrt(hd) if scale is None else scale, window_size))

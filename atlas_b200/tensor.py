@@ -35,6 +35,12 @@ class Context:
     def handle(self):
         return self._h
 
+    @property
+    def stream(self):
+        """The context's cudaStream_t as an integer: work of other libraries that the calls read or overwrite runs on it or is
+        ordered before them."""
+        return _ffi.lib().atlasx_ctx_stream(self._h) or 0
+
     def sync(self):
         check(_ffi.lib().atlasx_ctx_sync(self._h))
 

@@ -196,6 +196,64 @@ int atlasx_decode_attention_static(void* stream, int kv_dtype, const void* k_dev
                                    const float* q_dev, float* out_dev, int n_heads,
                                    const int* pos_host, float scale, int window);
 
+/* ── a packed serving step: requests of different lengths one behind the other ─────────
+ * page_plan → pagedkv_append → prompt_attention (prompts) or pagedkv_decode_attention (one token per request).
+ * All arrays are on the device, nothing is read back and nothing allocated by a call, so the calls can be captured into a graph.
+ * The reference serves one sequence over one linear f32 cache (GpuKvCache, crates/atlas-tensor/src/lib.rs:701-785). */
+
+/* Block tables, slots and positions from request lengths.  Request b (1 ≤ batch ≤ 4096) holds cached[b] rows in the first
+ * ceil(cached[b] / page_size) entries of table[b][0 .. table_width) and brings fresh[b] more.  The pages that are missing are taken
+ * from the front of free_pages (n_free page numbers below n_pages) in the order of the requests and written behind the entries that
+ * are there.  Out: cu[batch + 1] first new row of each request (exclusive sums of fresh), lens[b] = cached[b] + fresh[b];
+ * for new row i of the pack slots[i] = page · page_size + row within the page (−1 where the page is outside the pool) and pos[i],
+ * its position in the request; rows from cu[batch] to n_tokens get −1 in both.  status[3]: pages taken, pages missing, requests
+ * with lengths that are negative or wider than the table (one more if the new rows are more than n_tokens).  Where either of the
+ * last two is not zero nothing is planned: the table stays, cu and lens are 0, slots and pos −1. */
+int atlasx_page_plan(atlasx_ctx* ctx, const int* cached_dev, const int* fresh_dev, int batch, const int* free_pages_dev, int n_free,
+                     int page_size, int n_pages, int* table_dev, int table_width, int* cu_dev, int* lens_dev, int* slots_dev,
+                     int* pos_dev, int n_tokens, int* status_dev);
+
+/* Paged KV cache in four bits: n_pages pages of page_size rows (a multiple of 16), head_dim 64 or 128.  `group` (32 or 64)
+ * consecutive numbers of a row of a head share a bf16 scale = bf16(max|x| / 7), 1.0 below the smallest normal number; the number is
+ * x · (1 / scale) in f32, rounded half away from zero, −7..7 (Int4Tensor::quantize, crates/atlas-quant/src/lib.rs:113-145, with a
+ * 16-bit scale).  A group with a NaN or an infinity reads as NaN.  The layout within a page is the library's own. */
+typedef struct atlasx_pagedkv atlasx_pagedkv;
+int atlasx_pagedkv_create(atlasx_ctx* ctx, int n_pages, int page_size, int n_kv_heads, int head_dim, int group, atlasx_pagedkv** out);
+int atlasx_pagedkv_free(atlasx_pagedkv* kv);
+/* bytes of such a cache (0: the shape is refused) */
+size_t atlasx_pagedkv_bytes(int n_pages, int page_size, int n_kv_heads, int head_dim, int group);
+int atlasx_pagedkv_ptrs(atlasx_pagedkv* kv, void** pool_dev, size_t* bytes, size_t* workspace_bytes);
+/* Rows of K and V [n][n_kv_heads][head_dim], f32, bf16 or f16, strides in elements, every row on a 16-byte boundary, into their
+ * slots.  A negative slot marks a row that is not there; one behind the pool is left out and raises the device error word
+ * (atlasx_ctx_poll_device_error).  Slots of one call are distinct. */
+int atlasx_pagedkv_append(atlasx_ctx* ctx, atlasx_pagedkv* kv, int dtype, const void* k_dev, long long k_token_stride,
+                          long long k_head_stride, const void* v_dev, long long v_token_stride, long long v_head_stride,
+                          const int* slots_dev, int n);
+/* The values that the slots hold, contiguous [n][n_kv_heads][head_dim] in f32 (exact), bf16 or f16 (rounded once); zeros for slots
+ * that are negative or behind the pool.  Gives a cached prefix back to atlasx_prompt_attention. */
+int atlasx_pagedkv_read(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const int* slots_dev, int n, int dtype, void* k_out_dev, void* v_out_dev);
+/* One new token per request: q and out [batch][n_heads][head_dim] f32, rows max(0, lens[b] − window) .. lens[b] − 1 of request b
+ * (window 0: all) through its block table; lens beyond the table are cut to it, a request of no rows gets zeros.  Rows of a page
+ * number outside the pool are left out and raise the device error word.  workspace: NULL for the cache's own, else
+ * workspace_bytes (atlasx_pagedkv_ptrs) zeroed once before its first use; calls that may run at the same time — graphs replayed on
+ * different streams — need workspaces of their own. */
+int atlasx_pagedkv_decode_attention(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const float* q_dev, float* out_dev, int n_heads,
+                                    const int* table_dev, int table_width, const int* lens_dev, int batch, float scale, int window,
+                                    void* workspace_dev, size_t workspace_bytes);
+
+/* Causal attention of whole packed prompts, bf16 or f16 in and out, f32 inside; head_dim 64 or 128.  Sequence b owns rows
+ * cu_q[b] .. cu_q[b + 1] − 1 of q and out [n_q][n_heads][head_dim] and rows cu_k[b] .. cu_k[b + 1] − 1 of k and v
+ * [n_k][n_kv_heads][head_dim] (1 ≤ batch ≤ 4096, prefix arrays on the device).  Its last query sits at its last key: query i of lq
+ * sees keys j ≤ i + lk − lq, with a window only those with i + lk − lq − j < window; a query that sees none gets zeros.  What a
+ * query does not see — NaN and infinities too — does not reach it.  Strides in elements, every row on a 16-byte boundary; rows of
+ * out in no sequence are left as they are.  out may not overlap q, k or v. */
+int atlasx_prompt_attention(atlasx_ctx* ctx, int dtype, const void* q_dev, long long q_token_stride, long long q_head_stride,
+                            const void* k_dev, long long k_token_stride, long long k_head_stride,
+                            const void* v_dev, long long v_token_stride, long long v_head_stride,
+                            void* out_dev, long long out_token_stride, long long out_head_stride,
+                            const int* cu_q_dev, const int* cu_k_dev, int batch, int n_q, int n_k, int n_heads, int n_kv_heads,
+                            int head_dim, float scale, int window);
+
 /* ── SamplingConfig and the sampling pipeline (crates/atlas-model/src/lib.rs:1223-1294, 2581-2717) ── */
 typedef struct {
     float temperature;          /* <= 0 (or < 1e-6): greedy                      */

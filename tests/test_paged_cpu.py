@@ -1,0 +1,217 @@
+"""CPU: the index arithmetic of the four-bit paged cache (csrc/paged_index.h compiled with the host compiler) and the refusals of the
+packed serving calls — arguments are checked before a device is looked for, so every refusal can be seen without one."""
+import ctypes as C
+import itertools
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+import atlas_b200 as ab
+from atlas_b200 import _ffi
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+SHIM = """
+#include "paged_index.h"
+extern "C" {
+long long tile_bytes(int n, int p, int k, int hd, int g) { AxP4Shape s = { n, p, k, hd, g }; return ax_p4_tile_bytes(s); }
+long long pool_bytes(int n, int p, int k, int hd, int g) { AxP4Shape s = { n, p, k, hd, g }; return (long long)ax_p4_pool_bytes(s); }
+long long tile_at(int n, int p, int k, int hd, int g, int page, int head, int off) { AxP4Shape s = { n, p, k, hd, g }; return (long long)ax_p4_tile_at(s, page, head, off); }
+int plane(int hd, int g) { AxP4Shape s = { 1, 16, 1, hd, g }; return ax_p4_plane_bytes(s); }
+int k_word(int hd, int g, int r, int d) { AxP4Shape s = { 1, 16, 1, hd, g }; return ax_p4_k_word(s, r, d); }
+int v_half(int hd, int g, int r, int d) { AxP4Shape s = { 1, 16, 1, hd, g }; return ax_p4_v_half(s, r, d); }
+int scale_at(int hd, int g, int r, int gr) { AxP4Shape s = { 1, 16, 1, hd, g }; return ax_p4_scale(s, r, gr); }
+int col(int r) { return ax_p4_col(r); }
+unsigned rot(unsigned w) { return ax_p4_rot(w); }
+unsigned unrot(unsigned w) { return ax_p4_unrot(w); }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def idx(tmp_path_factory):
+    d = tmp_path_factory.mktemp("idx")
+    (d / "shim.cpp").write_text(SHIM)
+    so = str(d / "shim.so")
+    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-I", os.path.join(ROOT, "atlas_b200", "csrc"), str(d / "shim.cpp"), "-o", so], check=True)
+    L = C.CDLL(so)
+    for f in ("tile_bytes", "pool_bytes", "tile_at"):
+        getattr(L, f).restype = C.c_longlong
+    L.rot.restype = L.unrot.restype = C.c_uint
+    return L
+
+
+@pytest.mark.parametrize("hd,group", [(64, 32), (64, 64), (128, 32), (128, 64)])
+def test_every_number_of_a_tile_has_a_place_of_its_own(idx, hd, group):
+    plane = idx.plane(hd, group)
+    assert plane == 16 * hd // 2
+    words = {idx.k_word(hd, group, r, d) for r in range(16) for d in range(0, hd, 8)}
+    assert words == set(range(plane // 4))
+    halves = {idx.v_half(hd, group, r, d) for r in range(16) for d in range(0, hd, 4)}
+    assert halves == set(range(plane // 2))
+    scales = {idx.scale_at(hd, group, r, g) for r in range(16) for g in range(hd // group)}
+    assert scales == set(range(16 * (hd // group)))
+    assert idx.tile_bytes(1, 16, 1, hd, group) == 2 * plane + 2 * 2 * len(scales)
+    assert idx.tile_bytes(1, 16, 1, hd, group) % 16 == 0          # a tile is one bulk copy
+
+
+@pytest.mark.parametrize("hd,group", [(64, 32), (64, 64), (128, 32), (128, 64)])
+def test_lanes_find_their_operands(idx, hd, group):
+    """What the product's lanes assume: lane 4g + t reads hd / 32 consecutive K words of column 8nt + g whose groups follow one another,
+    and V words whose halves are rows 8nt + t and 8nt + 4 + t."""
+    w = hd // 32
+    for r in range(16):
+        col = idx.col(r)
+        nt, g, t = r // 8, (r // 4) % 2, r % 4
+        assert col == 8 * nt + 2 * t + g                                   # column 2t + b of block nt is row 8nt + 4b + t
+        for d in range(0, hd, 8):
+            word = idx.k_word(hd, group, r, d)
+            assert word // (4 * w) == col
+            lane_t, i = (word // w) % 4, word % w
+            assert i // (group // 32) == d // group and lane_t == (d % group) // (group // 4)
+        for d in range(0, hd, 4):
+            half = idx.v_half(hd, group, r, d)
+            assert half % 2 == g and (half // 2 // w) % 4 == t and half // 2 // (32 * w) == nt
+            assert (half // 2) % w == (d // group) * (group // 32) + ((d % group) % (group // 8)) // 4
+
+
+def test_tiles_stay_inside_the_pool(idx):
+    for n, p, k, hd, g in itertools.product((1, 3), (16, 48, 128), (1, 5), (64, 128), (32, 64)):
+        size, total = idx.tile_bytes(n, p, k, hd, g), idx.pool_bytes(n, p, k, hd, g)
+        at = sorted({idx.tile_at(n, p, k, hd, g, page, h, off) for page in range(n) for h in range(k) for off in range(p)})
+        assert at == list(range(0, total, size))
+    # a pool of 300 GB: offsets beyond 32 bits
+    n, p, k = 8_000_000, 16, 16
+    assert idx.tile_at(n, p, k, 128, 32, n - 1, k - 1, 15) == idx.pool_bytes(n, p, k, 128, 32) - 2304 == n * k * 2304 - 2304
+
+
+def test_rotation_is_undone(idx):
+    for w in (0, 1, 0x80000000, 0xFEDCBA98, 0xFFFFFFFF):
+        assert idx.unrot(idx.rot(w)) == w
+
+
+# ── refusals ─────────────────────────────────────────────────────────────────────
+P = 1 << 20      # a pointer that is never followed: every call below is refused before it runs
+
+
+def refused(rc, text):
+    msg = _ffi.lib().atlasx_last_error().decode()
+    assert rc == -1 and text in msg, (rc, msg)
+
+
+PLAN = dict(ctx=None, cached=P, fresh=P, batch=4, free=P, n_free=8, page_size=16, n_pages=8, table=P, width=4, cu=P, lens=P, slots=P, pos=P,
+            n_tokens=4, status=P)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(cached=None), "null argument"), (dict(status=None), "null argument"), (dict(slots=None), "null argument"),
+    (dict(free=None), "null argument"), (dict(batch=0), "batch"), (dict(batch=4097), "batch"), (dict(page_size=0), "page_size"),
+    (dict(n_pages=1 << 30, page_size=16), "2^31"), (dict(width=0), "column"), (dict(n_tokens=-1), "negative"),
+    (dict(n_free=-1), "negative"), ({}, "ctx is null")])
+def test_plan_refusals(change, text):
+    refused(_ffi.lib().atlasx_page_plan(*dict(PLAN, **change).values()), text)
+
+
+@pytest.mark.parametrize("shape,text", [
+    ((0, 16, 1, 64, 32), "positive"), ((4, 16, 0, 64, 32), "positive"), ((4, 8, 1, 64, 32), "multiple of 16"),
+    ((4, 24, 1, 64, 32), "multiple of 16"), ((1 << 27, 16, 1, 64, 32), "2^31"), ((4, 16, 1, 96, 32), "head_dim"),
+    ((4, 16, 1, 128, 16), "group"), ((4, 16, 1, 128, 128), "group"), ((4, 16, 1, 128, 32), "ctx is null")])
+def test_cache_refusals(shape, text):
+    h = C.c_void_p()
+    refused(_ffi.lib().atlasx_pagedkv_create(None, *shape, C.byref(h)), text)
+    if "ctx" not in text:
+        assert _ffi.lib().atlasx_pagedkv_bytes(*shape) == 0
+    else:
+        assert _ffi.lib().atlasx_pagedkv_bytes(*shape) == 4 * 2304
+
+
+ROWS = dict(ctx=None, kv=None, dtype=1, k=P, kt=128, kh=128, v=P, vt=128, vh=128, slots=P, n=3)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=2), "dtype"), (dict(n=-1), "negative"), (dict(k=None), "null"), (dict(slots=None), "null"), (dict(k=P + 2), "16-byte"),
+    (dict(kt=129), "16-byte"), (dict(vh=4), "16-byte"), (dict(dtype=0, kt=130), "16-byte"), ({}, "ctx or cache is null")])
+def test_append_refusals(change, text):
+    refused(_ffi.lib().atlasx_pagedkv_append(*dict(ROWS, **change).values()), text)
+
+
+READ = dict(ctx=None, kv=None, slots=P, n=3, dtype=0, k=P, v=P)
+
+
+@pytest.mark.parametrize("change,text", [(dict(dtype=3), "dtype"), (dict(n=-2), "negative"), (dict(v=None), "null"), (dict(v=P + 4), "16-byte"),
+                                         ({}, "ctx or cache is null")])
+def test_read_refusals(change, text):
+    refused(_ffi.lib().atlasx_pagedkv_read(*dict(READ, **change).values()), text)
+
+
+DEC = dict(ctx=None, kv=None, q=P, out=P, n_heads=8, table=P, width=4, lens=P, batch=2, scale=0.1, window=0, ws=None, wsn=0)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(q=None), "null"), (dict(lens=None), "null"), (dict(batch=0), "batch"), (dict(batch=5000), "batch"), (dict(n_heads=0), "n_heads"),
+    (dict(width=0), "column"), (dict(window=-1), "window"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
+    (dict(q=P + 8), "16-byte"), ({}, "ctx or cache is null")])
+def test_decode_refusals(change, text):
+    refused(_ffi.lib().atlasx_pagedkv_decode_attention(*dict(DEC, **change).values()), text)
+
+
+PROMPT = dict(ctx=None, dtype=1, q=P, qt=512, qh=128, k=P, kt=256, kh=128, v=P, vt=256, vh=128, out=P, ot=512, oh=128, cu_q=P, cu_k=P, batch=2,
+              n_q=10, n_k=10, n_heads=4, n_kv=2, hd=128, scale=0.1, window=0)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=0), "dtype"), (dict(batch=0), "batch"), (dict(batch=4097), "batch"), (dict(n_q=-1), "negative"), (dict(n_heads=3), "multiple"),
+    (dict(n_kv=0), "multiple"), (dict(hd=96), "head_dim"), (dict(window=-5), "window"), (dict(scale=float("nan")), "finite"),
+    (dict(q=None), "null"), (dict(k=None), "null"), (dict(cu_k=None), "null"), (dict(q=P + 2), "16-byte"), (dict(kt=257), "16-byte"),
+    (dict(vt=-256), "negative"), (dict(oh=64), "overlap"), (dict(ot=0), "overlap"), ({}, "ctx is null")])
+def test_prompt_refusals(change, text):
+    refused(_ffi.lib().atlasx_prompt_attention(*dict(PROMPT, **change).values()), text)
+
+
+class FakeContext:
+    device, handle = 0, None
+
+
+def arr(shape, dtype, strides=None, device=0):
+    c = FakeContext()
+    c.device = device
+    return ab.DeviceArray(c, P, shape, dtype, strides)
+
+
+def test_python_refuses_arrays_that_do_not_fit():
+    q, k = arr((5, 4, 64), ab.BF16), arr((7, 2, 64), ab.BF16)
+    cu = arr((3,), ab.I32)
+    good = dict(q=q, k=k, v=k, out=q, cu_q=cu, cu_k=cu)
+    for change, text in [(dict(q=arr((5, 4, 64), ab.F32)), "bf16 or f16"), (dict(k=arr((7, 2, 128), ab.BF16)), r"k must be"),
+                         (dict(v=arr((6, 2, 64), ab.BF16)), "same rows"), (dict(v=arr((7, 2, 64), ab.F16)), "same type"),
+                         (dict(out=arr((5, 4, 64), ab.BF16, (512, 64, 2))), "unit stride"), (dict(cu_k=arr((4,), ab.I32)), "shape"),
+                         (dict(cu_q=arr((3,), ab.F32)), "int32"), (dict(q=arr((20, 64), ab.BF16)), "dimensions"),
+                         (dict(k=arr((7, 2, 64), ab.BF16, device=1)), "device"), (dict(q=7), "not a device array"),
+                         (dict(cu_q=arr((3,), ab.I32, (2,))), "contiguous")]:
+        with pytest.raises(ab.AtlasError, match=text):
+            ab.prompt_attention(**dict(good, **change))
+    b = arr((4,), ab.I32)
+    plan = dict(cached=b, fresh=b, free_pages=b, table=arr((4, 3), ab.I32), cu=arr((5,), ab.I32), lens=b, slots=b, pos=b, status=arr((3,), ab.I32),
+                page_size=16, n_pages=4)
+    for change, text in [(dict(cu=b), "cu must have shape"), (dict(table=arr((3, 3), ab.I32)), "table must"), (dict(status=b), "status"),
+                         (dict(table=arr((4, 3), ab.I32, (1, 4))), "contiguous"), (dict(pos=arr((5,), ab.I32)), "pos"),
+                         (dict(lens=arr((4,), ab.F32)), "int32")]:
+        with pytest.raises(ab.AtlasError, match=text):
+            ab.page_plan(**dict(plan, **change))
+
+
+def test_torch_tensors_on_the_host_are_refused():
+    torch = pytest.importorskip("torch")
+    x = torch.zeros(5, 4, 64, dtype=torch.bfloat16)
+    cu = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ab.AtlasError, match="not on device 0"):
+        ab.prompt_attention(x, x, x, x, cu, cu)
+
+
+def test_device_array_strides():
+    a = arr((3, 4, 8), ab.F32)
+    assert a.strides == (32, 8, 1)
+    assert a.columns(8, (3, 2, 8), (32, 8, 1)).ptr == P + 32
+    assert np.dtype(np.uint16).itemsize * 8 == 16
