@@ -1,74 +1,493 @@
 // attention_paged.cu — attention of one new token per request over the four-bit paged cache.
+//
+// What has to move is rows · n_kv · 2 · (hd / 2 + 2 · hd / group) bytes; at the copy bandwidth a tile (16 rows of one KV head,
+// 2304 bytes at hd 128, group 32) leaves an SM about 100 clocks.  Unpacking 4096 nibbles, two products with four-times-replicated
+// work for f32 accuracy and a softmax in that time is what the kernel is shaped by:
+//   * Work is cut evenly: the tiles of all (request, KV head) segments form one sequence, every warp takes a contiguous piece of
+//     it, whatever the lengths are.  Nothing of it is decided on the host, so a captured call follows the lengths.
+//   * A tile is one bulk copy into the warp's own ring of stages; no barrier of the CTA in the loop.
+//   * S = Q·Kᵀ and O = P·V run as mma.m16n8k16 with the (up to eight) query heads of a KV head as rows: rows 0..7 hold the bf16
+//     hi parts, rows 8..15 the lo parts of the same f32 values, so one instruction gives both and the sum of two accumulators
+//     is good to 2^-16 of each value.  The score accumulators are already the operand layout of the second product.
+//   * K nibbles become bf16 by one mask-and-or (16 + u, u = number + 8); −24 · Σq of the group enters as the accumulator's start
+//     value.  The scale of (row, group) multiplies the group's finished sum.  V nibbles are made exact (128 + u − 136): over
+//     a long context the sum of the numbers is far smaller than that of their offsets.  The scale of V goes into P.
+//   * Segments that end inside a warp's piece are written from registers; the others meet in shared memory, and where they
+//     reach over CTAs in the workspace, added up by the last CTA to arrive, in the order of the pieces: no result depends on timing.
 #include "paged.cuh"
 
 namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStages = 4;
+constexpr int kCtasPerSm = 3;
+constexpr int kMinTiles = 2;                    // tiles of a warp below which fewer CTAs share the work
+constexpr int kHeads = 8;                       // query heads of one segment
+constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr int kErrWait = 711;
 
 struct PagedDev {
     AxP4Shape s;
     const uint8_t* pool;
     AxPagedAttnArgs a;
+    int group_heads, head_tiles, nh;            // query heads per KV head, segments per KV head, segments per request
+    int hpt;                                    // heads per segment: min(8, group_heads)
+    unsigned* tickets;                          // [gridDim] zero between launches
+    float* part_ml;                             // [2 · gridDim][hpt][2]
+    float* part_o;                              // [2 · gridDim][hpt][hd]
     int* err;
 };
 
-// One CTA per (query head, request): every warp takes every fourth row, lanes hold hd / 32 numbers each, online softmax.
-template <int HD>
-__global__ void __launch_bounds__(128) ax_paged_attn_simple_kernel(const PagedDev dv) {
-    constexpr int N = HD / 32;
-    __shared__ float s_m[4], s_l[4], s_o[4][HD];
-    const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const AxP4Shape& s = dv.s;
-    const int kh = h / (dv.a.n_heads / s.n_kv);
-    const int len = max(0, (int)min((long long)dv.a.lens[b], (long long)dv.a.table_width * s.page_size));
-    const int lo = dv.a.window > 0 && len > dv.a.window ? len - dv.a.window : 0;
-    float q[N], o[N], m = -INFINITY, l = 0.f;
+struct TileInfo { int seg, tile, ok, pad; };
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// bounded: false after two seconds
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+    if (mbar_try(bar, parity)) return true;
+    unsigned long long t0 = ax_globaltimer();
+    while (!mbar_try(bar, parity))
+        if (ax_globaltimer() - t0 > kWaitNs) return false;
+    return true;
+}
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {        // round to nearest
+    uint32_t r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r;
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t r; asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits)); return r;
+}
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r; asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r;
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+template <int N> __device__ __forceinline__ void lds(uint32_t (&r)[N], const void* p) {
+    if constexpr (N == 4) { const uint4 v = *(const uint4*)p; r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
+    else if constexpr (N == 2) { const uint2 v = *(const uint2*)p; r[0] = v.x; r[1] = v.y; }
+    else r[0] = *(const uint32_t*)p;
+}
+
+// visible rows of a request: [lo, len)
+__device__ __forceinline__ void row_range(const PagedDev& dv, int b, int& lo, int& len) {
+    len = max(0, (int)min((long long)dv.a.lens[b], (long long)dv.a.table_width * dv.s.page_size));
+    lo = dv.a.window > 0 && len > dv.a.window ? len - dv.a.window : 0;
+}
+__device__ __forceinline__ unsigned tiles_of(int lo, int len) {
+    return len > lo ? (unsigned)((len + AX_P4_TILE - 1) / AX_P4_TILE - lo / AX_P4_TILE) : 0u;
+}
+
+template <int HD, int GS>
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(const PagedDev dv) {
+    constexpr int W = HD / 32;                  // 32-bit words per lane, row block and plane
+    constexpr int NG = HD / GS;                 // groups of a row
+    constexpr int WG = GS / 32;                 // words per group
+    constexpr int PLANE = AX_P4_TILE * HD / 2, SC = AX_P4_TILE * NG * 2, TILE = 2 * (PLANE + SC);
+    constexpr int NT = HD / 8;                  // column blocks of the output
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) uint64_t s_bar[kWarps][kStages];
+    __shared__ __align__(16) TileInfo s_info[kWarps][kStages];
+    __shared__ unsigned s_scan[kWarps];
+    __shared__ int s_seg[kWarps * 2];
+    __shared__ float s_ml[kWarps * 2][kHeads][2];
+    __shared__ int s_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int batch = dv.a.batch, hpt = dv.hpt;
+    uint8_t* ring = smem + warp * kStages * TILE;
+    float* s_o = reinterpret_cast<float*>(smem + kWarps * kStages * TILE);                 // [2 · warps][hpt][HD]
+    unsigned* s_pre = reinterpret_cast<unsigned*>(s_o + (size_t)kWarps * 2 * hpt * HD);    // [batch + 1] tiles before each request
+
+    if (tid < kWarps * kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(smem_u32(&s_bar[tid / kStages][tid % kStages])) : "memory");
+    if (tid < kWarps * 2) s_seg[tid] = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    {   // exclusive sums of the requests' tiles
+        const int per = (batch + kWarps * 32 - 1) / (kWarps * 32), b0 = min(tid * per, batch), b1 = min(b0 + per, batch);
+        unsigned own = 0;
+        for (int b = b0; b < b1; b++) { int lo, len; row_range(dv, b, lo, len); own += tiles_of(lo, len); }
+        unsigned inc = own;
 #pragma unroll
-    for (int i = 0; i < N; i++) { q[i] = dv.a.q[((size_t)b * dv.a.n_heads + h) * HD + lane * N + i] * dv.a.scale; o[i] = 0.f; }
-    for (int t = lo + warp; t < len; t += 4) {
-        const int page = dv.a.table[(size_t)b * dv.a.table_width + t / s.page_size], off = t % s.page_size, r = off % AX_P4_TILE;
-        if (page < 0 || page >= s.n_pages) { if (lane == 0) atomicExch(dv.err, AX_DEVERR_PAGE); continue; }
-        const uint8_t* tile = dv.pool + ax_p4_tile_at(s, page, kh, off);
-        const int plane = ax_p4_plane_bytes(s);
-        const uint16_t* sp = reinterpret_cast<const uint16_t*>(tile + 2 * plane);
-        float d = 0.f, v[N];
+        for (int d = 1; d < 32; d <<= 1) { const unsigned x = __shfl_up_sync(AX_FULL, inc, d); if (lane >= d) inc += x; }
+        if (lane == 31) s_scan[warp] = inc;
+        __syncthreads();
+        unsigned at = inc - own;
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int e = lane * N + i, gr = e / s.group;
-            const uint32_t kw = ax_p4_unrot(reinterpret_cast<const uint32_t*>(tile)[ax_p4_k_word(s, r, e & ~7)]);
-            const uint32_t vw = reinterpret_cast<const uint16_t*>(tile + plane)[ax_p4_v_half(s, r, e & ~3)];
-            d += q[i] * ((float)((int)((kw >> (4 * (e & 7))) & 15u) - 8) * ax_bf16_to_f32(sp[ax_p4_scale(s, r, gr)]));
-            v[i] = (float)((int)((vw >> (4 * (e & 3))) & 15u) - 8) * ax_bf16_to_f32(sp[AX_P4_TILE * ax_p4_groups(s) + ax_p4_scale(s, r, gr)]);
+        for (int w = 0; w < kWarps; w++) if (w < warp) at += s_scan[w];
+        for (int b = b0; b < b1; b++) {
+            int lo, len; row_range(dv, b, lo, len);
+            s_pre[b] = at; at += tiles_of(lo, len);
+            if (b == batch - 1) s_pre[batch] = at;
         }
-        d = ax_warp_sum(d);
-        const float mn = fmaxf(m, d);
-        const float c = m == mn ? 1.f : expf(m - mn), p = d == mn ? 1.f : expf(d - mn);
-        l = l * c + p; m = mn;
-#pragma unroll
-        for (int i = 0; i < N; i++) o[i] = o[i] * c + p * v[i];
+        __syncthreads();
     }
-    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-#pragma unroll
-    for (int i = 0; i < N; i++) s_o[warp][lane * N + i] = o[i];
-    __syncthreads();
-    if (threadIdx.x < HD) {
-        float M = -INFINITY, L = 0.f, A = 0.f;
-        for (int w = 0; w < 4; w++) M = fmaxf(M, s_m[w]);
-        for (int w = 0; w < 4; w++) {
-            const float c = s_l[w] == 0.f ? 0.f : expf(s_m[w] - M);
-            L += c * s_l[w]; A += c == 0.f && s_l[w] == 0.f ? 0.f : c * s_o[w][threadIdx.x];
+    for (int b = blockIdx.x; b < batch; b += gridDim.x)                       // requests without rows
+        if (s_pre[b] == s_pre[b + 1])
+            for (int i = tid; i < dv.a.n_heads * HD; i += kWarps * 32) dv.a.out[(size_t)b * dv.a.n_heads * HD + i] = 0.f;
+    const long long total = (long long)s_pre[batch] * dv.nh;
+    const long long want = (total + kWarps * kMinTiles - 1) / (kWarps * kMinTiles);
+    const long long C = want < (long long)gridDim.x ? want : (long long)gridDim.x;        // CTAs that share the work
+    const long long c = blockIdx.x;
+    if (c >= C) return;
+    const long long X0 = total * c / C, X1 = total * (c + 1) / C;
+    const long long x0 = X0 + (X1 - X0) * warp / kWarps, x1 = X0 + (X1 - X0) * (warp + 1) / kWarps;
+
+    // ── the warp's stream of tiles: 32 positions are resolved at a time, one per lane, and lane i copies tile i of them ──
+    long long base = x0 - 32;
+    const uint8_t* src = nullptr;
+    TileInfo mine = {};
+    auto fill = [&](long long x) {                                            // x uniform over the warp, rising by one
+        if (x >= x1) return;
+        if (x - base >= 32) {
+            base = x;
+            const long long y = x + lane;
+            mine.seg = -1; mine.tile = 0; mine.ok = 0;
+            if (y < x1) {
+                int lo = 0, hi = batch;                                       // last b with s_pre[b] · nh <= y (skipping requests without rows)
+                while (hi - lo > 1) { const int m = (lo + hi) >> 1; if ((long long)s_pre[m] * dv.nh <= y) lo = m; else hi = m; }
+                const unsigned n = s_pre[lo + 1] - s_pre[lo];
+                const long long rem = y - (long long)s_pre[lo] * dv.nh;
+                int hh, ti;
+                if (total <= 0x7FFFFFFFll) { hh = (int)((unsigned)rem / n); ti = (int)((unsigned)rem % n); }
+                else { hh = (int)(rem / n); ti = (int)(rem % n); }
+                int first, len; row_range(dv, lo, first, len);
+                mine.seg = lo * dv.nh + hh;
+                mine.tile = first / AX_P4_TILE + ti;
+                const int row = mine.tile * AX_P4_TILE, page = dv.a.table[(size_t)lo * dv.a.table_width + row / dv.s.page_size];
+                mine.ok = page >= 0 && page < dv.s.n_pages;
+                if (mine.ok) src = dv.pool + ax_p4_tile_at(dv.s, page, hh / dv.head_tiles, row % dv.s.page_size);
+                else atomicExch(dv.err, AX_DEVERR_PAGE);
+            }
         }
-        dv.a.out[((size_t)b * dv.a.n_heads + h) * HD + threadIdx.x] = len > lo && L != 0.f ? A / L : 0.f;
+        if (lane == (int)(x - base)) {
+            const int st = (int)((x - x0) % kStages);
+            const uint32_t bar = smem_u32(&s_bar[warp][st]);
+            s_info[warp][st] = mine;
+            if (mine.ok) {
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(TILE) : "memory");
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                             :: "r"(smem_u32(ring + st * TILE)), "l"(src), "r"(TILE), "r"(bar) : "memory");
+            } else {
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+            }
+        }
+    };
+    for (int i = 0; i < kStages; i++) fill(x0 + i);
+    __syncwarp();
+
+    // ── state of the segment at hand ──
+    uint32_t qa[W * 2][4];                      // operand of the scores: step 2·w + h of word w
+    float qoff[NG];                             // −24 · Σ q of a group
+    float o[NT][4], m = -INFINITY, l = 0.f;
+    int seg = -1, seg_lo = 0, seg_len = 0;
+    auto start = [&](int s) {
+        seg = s;
+        const int b = s / dv.nh, hh = s % dv.nh, kh = hh / dv.head_tiles, h0 = (hh % dv.head_tiles) * kHeads;
+        row_range(dv, b, seg_lo, seg_len);
+        const bool live = h0 + g < dv.group_heads;
+        const float* q = dv.a.q + ((size_t)b * dv.a.n_heads + (size_t)kh * dv.group_heads + h0 + g) * HD;
+        const float f = dv.a.scale * 1.4426950408889634f;
+#pragma unroll
+        for (int i = 0; i < NG; i++) qoff[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = 0.f;
+            if (live) {
+                const float4 u = *(const float4*)(q + (w / WG) * GS + t * (GS / 4) + (w % WG) * 8);
+                const float4 v = *(const float4*)(q + (w / WG) * GS + t * (GS / 4) + (w % WG) * 8 + 4);
+                x[0] = u.x * f; x[1] = u.y * f; x[2] = u.z * f; x[3] = u.w * f; x[4] = v.x * f; x[5] = v.y * f; x[6] = v.z * f; x[7] = v.w * f;
+            }
+#pragma unroll
+            for (int p = 0; p < 4; p++) {                                      // pair (p, p + 4) of the word
+                const uint32_t hi = pack_bf16(x[p], x[p + 4]);
+                const float r0 = x[p] - ax_bf16_lo(hi), r1 = x[p + 4] - ax_bf16_hi(hi);
+                const uint32_t lo = pack_bf16(r0, r1);
+                qa[2 * w + p / 2][(p & 1) * 2] = hi;
+                qa[2 * w + p / 2][(p & 1) * 2 + 1] = lo;
+                qoff[w / WG] += (ax_bf16_lo(hi) + ax_bf16_lo(lo)) + (ax_bf16_hi(hi) + ax_bf16_hi(lo));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NG; i++) {
+            qoff[i] += __shfl_xor_sync(AX_FULL, qoff[i], 1);
+            qoff[i] += __shfl_xor_sync(AX_FULL, qoff[i], 2);
+            qoff[i] *= -24.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NT; i++) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
+        m = -INFINITY; l = 0.f;
+    };
+    // Column n = 2t, 2t + 1 of column block gr · (GS / 8) + i is number gr · GS + n · (GS / 8) + i: a lane holds GS / 4 consecutive numbers
+    // of every group.
+    auto put = [&](float* dst, float f) {
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < GS / 8; i += 4) {
+                    float4 v;
+                    v.x = (o[gr * (GS / 8) + i][n] + o[gr * (GS / 8) + i][n + 2]) * f;
+                    v.y = (o[gr * (GS / 8) + i + 1][n] + o[gr * (GS / 8) + i + 1][n + 2]) * f;
+                    v.z = (o[gr * (GS / 8) + i + 2][n] + o[gr * (GS / 8) + i + 2][n + 2]) * f;
+                    v.w = (o[gr * (GS / 8) + i + 3][n] + o[gr * (GS / 8) + i + 3][n + 2]) * f;
+                    *(float4*)(dst + gr * GS + (2 * t + n) * (GS / 8) + i) = v;
+                }
+    };
+    auto flush = [&]() {
+        const int b = seg / dv.nh, hh = seg % dv.nh, kh = hh / dv.head_tiles, h0 = (hh % dv.head_tiles) * kHeads;
+        const unsigned n = s_pre[b + 1] - s_pre[b];
+        const long long s0 = (long long)s_pre[b] * dv.nh + (long long)hh * n;
+        l += __shfl_xor_sync(AX_FULL, l, 1);
+        l += __shfl_xor_sync(AX_FULL, l, 2);
+        const bool live = h0 + g < dv.group_heads;
+        if (s0 >= x0 && s0 + n <= x1) {
+            if (live) put(dv.a.out + ((size_t)b * dv.a.n_heads + (size_t)kh * dv.group_heads + h0 + g) * HD, l == 0.f ? 0.f : 1.f / l);
+        } else {
+            const int slot = warp * 2 + (s0 < x0 ? 0 : 1);
+            if (lane == 0) s_seg[slot] = seg;
+            if (t == 0) { s_ml[slot][g][0] = m; s_ml[slot][g][1] = l; }
+            if (live) put(s_o + ((size_t)slot * hpt + g) * HD, 1.f);
+        }
+    };
+
+    for (long long x = x0; x < x1; x++) {
+        const int st = (int)((x - x0) % kStages);
+        if (!mbar_wait(smem_u32(&s_bar[warp][st]), (uint32_t)((x - x0) / kStages) & 1u)) {
+            if (lane == 0) atomicExch(dv.err, kErrWait);
+            for (long long y = x; y < x1 && y < x + kStages; y++)             // what is in flight lands before the CTA goes
+                mbar_wait(smem_u32(&s_bar[warp][(int)((y - x0) % kStages)]), (uint32_t)((y - x0) / kStages) & 1u);
+            break;
+        }
+        const TileInfo info = s_info[warp][st];
+        if (info.seg != seg) { if (seg >= 0) flush(); start(info.seg); }
+        if (info.ok) {
+            const uint8_t* tile = ring + st * TILE;
+            float s[4];                                                       // (block 0: columns 2t, 2t + 1), (block 1: …)
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) {
+                uint32_t kw[W], sw[NG];
+                lds<W>(kw, tile + nt * (PLANE / 2) + lane * W * 4);
+                lds<NG>(sw, tile + 2 * PLANE + (8 * nt + 2 * t) * NG * 2);
+                float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) {
+                    float d[4];
+#pragma unroll
+                    for (int i = 0; i < WG; i++) {
+                        const uint32_t w = kw[gr * WG + i];
+                        const uint32_t b0 = and_or(w, 0x00780078u, 0x41804180u), b1 = and_or(w >> 4, 0x00780078u, 0x41804180u);
+                        const uint32_t b2 = and_or(w >> 8, 0x00780078u, 0x41804180u);
+                        const uint32_t b3 = and_or(__funnelshift_r(w, w, 12), 0x00780078u, 0x41804180u);
+                        if (i == 0) mma(d, qa[2 * (gr * WG + i)], b0, b1, qoff[gr], qoff[gr], 0.f, 0.f);
+                        else mma(d, qa[2 * (gr * WG + i)], b0, b1, d[0], d[1], d[2], d[3]);
+                        mma(d, qa[2 * (gr * WG + i) + 1], b2, b3, d[0], d[1], d[2], d[3]);
+                    }
+                    // scales of columns 2t and 2t + 1, NG numbers each
+                    const float k0 = gr & 1 ? ax_bf16_hi(sw[gr / 2]) : ax_bf16_lo(sw[gr / 2]);
+                    const float k1 = (NG + gr) & 1 ? ax_bf16_hi(sw[(NG + gr) / 2]) : ax_bf16_lo(sw[(NG + gr) / 2]);
+                    s0 = fmaf(k0, d[0] + d[2], s0);
+                    s1 = fmaf(k1, d[1] + d[3], s1);
+                }
+                s[2 * nt] = s0; s[2 * nt + 1] = s1;
+            }
+            const int row = info.tile * AX_P4_TILE;
+            const bool edge = row < seg_lo || row + AX_P4_TILE > seg_len;
+            bool seen[4] = { true, true, true, true };
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {                                  // column 8·nt + 2t + b is row 8·nt + 4b + t
+                    const int r = row + (i >> 1) * 8 + (i & 1) * 4 + t;
+                    seen[i] = r >= seg_lo && r < seg_len;
+                    if (!seen[i]) s[i] = -INFINITY;
+                }
+            }
+            float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 2));
+            // the maximum is followed only where a probability would pass 2^8: sums and outputs are f32, any reference will do
+            if (__any_sync(AX_FULL, top > m + 8.f)) {
+                const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2(m - mn);
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < NT; i++) { o[i][0] *= f; o[i][1] *= f; o[i][2] *= f; o[i][3] *= f; }
+                m = mn;
+            }
+            const float mr = m == -INFINITY ? 0.f : m;
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { p[i] = ex2(s[i] - mr); l += p[i]; }
+            uint32_t vw[2][W], sw[2][NG];
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) {
+                lds<W>(vw[nt], tile + PLANE + nt * (PLANE / 2) + lane * W * 4);
+                lds<NG>(sw[nt], tile + 2 * PLANE + SC + (8 * nt + 2 * t) * NG * 2);
+            }
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+                uint32_t a[4];
+#pragma unroll
+                for (int nt = 0; nt < 2; nt++) {
+                    float v0 = gr & 1 ? ax_bf16_hi(sw[nt][gr / 2]) : ax_bf16_lo(sw[nt][gr / 2]);
+                    float v1 = (NG + gr) & 1 ? ax_bf16_hi(sw[nt][(NG + gr) / 2]) : ax_bf16_lo(sw[nt][(NG + gr) / 2]);
+                    if (edge) { if (!seen[2 * nt]) v0 = 0.f; if (!seen[2 * nt + 1]) v1 = 0.f; }
+                    const float y0 = p[2 * nt] * v0, y1 = p[2 * nt + 1] * v1;
+                    const uint32_t hi = pack_bf16(y0, y1);
+                    a[2 * nt] = hi;
+                    a[2 * nt + 1] = pack_bf16(y0 - ax_bf16_lo(hi), y1 - ax_bf16_hi(hi));
+                }
+#pragma unroll
+                for (int i = 0; i < WG; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t b0 = sub_bf16x2(and_or(vw[0][gr * WG + i] >> (4 * j), 0x000F000Fu, 0x43004300u), 0x43084308u);
+                        const uint32_t b1 = sub_bf16x2(and_or(vw[1][gr * WG + i] >> (4 * j), 0x000F000Fu, 0x43004300u), 0x43084308u);
+                        float (&d)[4] = o[(gr * WG + i) * 4 + j];
+                        mma(d, a, b0, b1, d[0], d[1], d[2], d[3]);
+                    }
+            }
+        }
+        __syncwarp();                                                          // every lane has read the stage
+        fill(x + kStages);
+        __syncwarp();
+    }
+    if (seg >= 0) flush();
+    __syncthreads();
+
+    // ── segments that no warp holds alone ──
+    for (int i = 0; i < kWarps * 2;) {
+        const int sg = s_seg[i];
+        int j = i + 1;
+        if (sg < 0) { i = j; continue; }
+        while (j < kWarps * 2 && (s_seg[j] == sg || s_seg[j] < 0)) j++;
+        const int b = sg / dv.nh, hh = sg % dv.nh, kh = hh / dv.head_tiles, h0 = (hh % dv.head_tiles) * kHeads;
+        const int heads = min(kHeads, dv.group_heads - h0);
+        const unsigned n = s_pre[b + 1] - s_pre[b];
+        const long long s0 = (long long)s_pre[b] * dv.nh + (long long)hh * n;
+        const bool whole = s0 >= X0 && s0 + n <= X1;
+        float* out = dv.a.out + ((size_t)b * dv.a.n_heads + (size_t)kh * dv.group_heads + h0) * HD;
+        const size_t slot = 2 * (size_t)c + (s0 < X0 ? 0 : 1);
+        for (int e = tid; e < heads * (HD / 4); e += kWarps * 32) {
+            const int h = e / (HD / 4), d = (e % (HD / 4)) * 4;
+            float M = -INFINITY, L = 0.f;
+            for (int k = i; k < j; k++) if (s_seg[k] == sg) M = fmaxf(M, s_ml[k][h][0]);
+            float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = i; k < j; k++)
+                if (s_seg[k] == sg && s_ml[k][h][1] != 0.f) {
+                    const float f = s_ml[k][h][0] == M ? 1.f : ex2(s_ml[k][h][0] - M);
+                    const float4 v = *(const float4*)(s_o + ((size_t)k * hpt + h) * HD + d);
+                    L = fmaf(f, s_ml[k][h][1], L);
+                    A.x = fmaf(f, v.x, A.x); A.y = fmaf(f, v.y, A.y); A.z = fmaf(f, v.z, A.z); A.w = fmaf(f, v.w, A.w);
+                }
+            if (whole) {
+                const float f = L == 0.f ? 0.f : 1.f / L;
+                *(float4*)(out + (size_t)h * HD + d) = make_float4(A.x * f, A.y * f, A.z * f, A.w * f);
+            } else {
+                __stcg((float4*)(dv.part_o + (slot * hpt + h) * HD + d), A);
+                if (d == 0) __stcg((float2*)(dv.part_ml + (slot * hpt + h) * 2), make_float2(M, L));
+            }
+        }
+        if (!whole) {
+            const long long cf = ((s0 + 1) * C - 1) / total, cl = ((s0 + n) * C - 1) / total;     // first and last CTA of the segment
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) s_last = atomicAdd(dv.tickets + cf, 1u) == (unsigned)(cl - cf);
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                const int cnt = (int)(cl - cf) + 1;
+                float* wt = reinterpret_cast<float*>(smem);                                       // the ring is free: weights of the parts
+                const int cap = kWarps * kStages * TILE / 4;
+                float L = 0.f;
+                const bool fits = cnt * heads <= cap;
+                for (int h = warp; h < heads; h += kWarps) {
+                    float M = -INFINITY;
+                    for (int k = lane; k < cnt; k += 32)
+                        M = fmaxf(M, __ldcg(dv.part_ml + ((2 * (size_t)(cf + k) + (k == 0)) * hpt + h) * 2));
+                    M = ax_warp_max(M);
+                    L = 0.f;
+                    for (int k = lane; k < cnt; k += 32) {
+                        const float2 ml = __ldcg((const float2*)(dv.part_ml + ((2 * (size_t)(cf + k) + (k == 0)) * hpt + h) * 2));
+                        const float f = ml.y == 0.f ? 0.f : ml.x == M ? 1.f : ex2(ml.x - M);
+                        L += ml.y == 0.f ? 0.f : f * ml.y;
+                        if (fits) wt[h * cnt + k] = f;
+                    }
+                    L = ax_warp_sum(L);
+                    if (lane == 0) { s_ml[0][h][0] = M; s_ml[0][h][1] = L; }
+                }
+                __syncthreads();
+                for (int e = tid; e < heads * (HD / 4); e += kWarps * 32) {
+                    const int h = e / (HD / 4), d = (e % (HD / 4)) * 4;
+                    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                    for (int k = 0; k < cnt; k++) {
+                        const size_t at = (2 * (size_t)(cf + k) + (k == 0)) * hpt + h;
+                        float f;
+                        if (fits) f = wt[h * cnt + k];
+                        else { const float2 ml = __ldcg((const float2*)(dv.part_ml + at * 2)); f = ml.y == 0.f ? 0.f : ml.x == s_ml[0][h][0] ? 1.f : ex2(ml.x - s_ml[0][h][0]); }
+                        const float4 v = __ldcg((const float4*)(dv.part_o + at * HD + d));
+                        if (f != 0.f) { A.x = fmaf(f, v.x, A.x); A.y = fmaf(f, v.y, A.y); A.z = fmaf(f, v.z, A.z); A.w = fmaf(f, v.w, A.w); }
+                    }
+                    const float f = s_ml[0][h][1] == 0.f ? 0.f : 1.f / s_ml[0][h][1];
+                    *(float4*)(out + (size_t)h * HD + d) = make_float4(A.x * f, A.y * f, A.z * f, A.w * f);
+                }
+                if (tid == 0) dv.tickets[cf] = 0u;                                                // ready for the next launch
+            }
+            __syncthreads();
+        }
+        i = j;
     }
 }
 
+constexpr int kMaxGrid = 1024;
+
+template <int HD, int GS>
+int launch(atlasx_ctx* ctx, const PagedDev& dv, int grid, size_t smem) {
+    static bool ready[64] = {};
+    if (ctx->device < 64 && !ready[ctx->device]) {                            // the limit is per device; asking twice does no harm
+        AX_CUDA(cudaFuncSetAttribute(ax_paged_attn_kernel<HD, GS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        ready[ctx->device] = true;
+    }
+    ax_paged_attn_kernel<HD, GS><<<grid, kWarps * 32, smem, ctx->stream>>>(dv);
+    AX_CHECK_LAUNCH("ax_paged_attn_kernel");
+    return ATLASX_OK;
+}
+
+int grid_of(const atlasx_ctx* ctx) { return min(ctx->sm_count * kCtasPerSm, kMaxGrid); }
+size_t ticket_bytes(int grid) { return ((size_t)grid * 4 + 15) / 16 * 16; }
+
 }  // namespace
 
-size_t ax_paged_attn_workspace_bytes(const atlasx_ctx* ctx, const AxP4Shape& s) { (void)ctx; (void)s; return 16; }
+size_t ax_paged_attn_workspace_bytes(const atlasx_ctx* ctx, const AxP4Shape& s) {
+    const int grid = grid_of(ctx);
+    return ticket_bytes(grid) + (size_t)2 * grid * kHeads * (s.hd + 2) * 4;
+}
 
 int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPagedAttnArgs& a) {
-    PagedDev dv = { kv->s, kv->pool, a, ctx->dev_error };
-    const dim3 grid((unsigned)a.n_heads, (unsigned)a.batch);
-    if (kv->s.hd == 128) ax_paged_attn_simple_kernel<128><<<grid, 128, 0, ctx->stream>>>(dv);
-    else ax_paged_attn_simple_kernel<64><<<grid, 128, 0, ctx->stream>>>(dv);
-    AX_CHECK_LAUNCH("ax_paged_attn_simple_kernel");
-    return ATLASX_OK;
+    PagedDev dv = {};
+    dv.s = kv->s; dv.pool = kv->pool; dv.a = a; dv.err = ctx->dev_error;
+    dv.group_heads = a.n_heads / kv->s.n_kv;
+    dv.head_tiles = (dv.group_heads + kHeads - 1) / kHeads;
+    dv.hpt = min(kHeads, dv.group_heads);
+    if ((long long)kv->s.n_kv * dv.head_tiles * a.batch > 0x7FFFFFFFll)
+        return atlasx_fail(ATLASX_ERR_ARG, "batch · heads is too large");
+    dv.nh = kv->s.n_kv * dv.head_tiles;
+    const int grid = grid_of(ctx);
+    uint8_t* w = (uint8_t*)a.workspace;
+    dv.tickets = (unsigned*)w;
+    dv.part_ml = (float*)(w + ticket_bytes(grid));
+    dv.part_o = dv.part_ml + (size_t)2 * grid * kHeads * 2;
+    const int tile = ax_p4_tile_bytes(kv->s);
+    const size_t smem = (size_t)kWarps * kStages * tile + (size_t)kWarps * 2 * dv.hpt * kv->s.hd * 4 + (size_t)(a.batch + 1) * 4;
+    if (kv->s.hd == 128) return kv->s.group == 32 ? launch<128, 32>(ctx, dv, grid, smem) : launch<128, 64>(ctx, dv, grid, smem);
+    return kv->s.group == 32 ? launch<64, 32>(ctx, dv, grid, smem) : launch<64, 64>(ctx, dv, grid, smem);
 }
