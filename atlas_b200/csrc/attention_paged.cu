@@ -6,12 +6,15 @@
 //   * Work is cut evenly: the tiles of all (request, KV head) segments form one sequence, every warp takes a contiguous piece of
 //     it, whatever the lengths are.  Nothing of it is decided on the host, so a captured call follows the lengths.
 //   * A tile is one bulk copy into the warp's own ring of stages; no barrier of the CTA in the loop.
-//   * S = Q·Kᵀ and O = P·V run as mma.m16n8k16 with the (up to eight) query heads of a KV head as rows: rows 0..7 hold the bf16
+//   * S = Q·Kᵀ and O = P·V run as mma.m16n8k16 with the (up to eight) query heads of a KV head as rows: rows 0..7 hold the f16
 //     hi parts, rows 8..15 the lo parts of the same f32 values, so one instruction gives both and the sum of two accumulators
-//     is good to 2^-16 of each value.  The score accumulators are already the operand layout of the second product.
-//   * K nibbles become bf16 by one mask-and-or (16 + u, u = number + 8); −24 · Σq of the group enters as the accumulator's start
-//     value.  The scale of (row, group) multiplies the group's finished sum.  V nibbles are made exact (128 + u − 136): over
-//     a long context the sum of the numbers is far smaller than that of their offsets.  The scale of V goes into P.
+//     is good to 2^-22 of each value (bf16 halves left 4e-6 of the output, 2^-16 of each value).  The score accumulators are
+//     already the operand layout of the second product.  f16 has little range, so a head's query is brought to 2^14 by a power
+//     of two, and the softmax reference follows the largest p · scale of V instead of the largest p.
+//   * K nibbles become f16 by one mask-and-or (16 + u, u = number + 8); −24 · Σq of the group enters as the accumulator's start
+//     value.  The scale of (row, group) multiplies the group's finished sum.  V nibbles are made exact (1024 + u − 1032, or
+//     (1024 + 16u) / 16 − 72 without a shift): over a long context the sum of the numbers is far smaller than that of their
+//     offsets.  The scale of V goes into P.
 //   * Segments that end inside a warp's piece are written from registers; the others meet in shared memory, and where they
 //     reach over CTAs in the workspace, added up by the last CTA to arrive, in the order of the pieces: no result depends on timing.
 #include "paged.cuh"
@@ -56,17 +59,25 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     return true;
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {        // round to nearest
-    uint32_t r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r;
+__device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {         // round to nearest
+    uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r;
 }
+__device__ __forceinline__ float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
     uint32_t r; asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits)); return r;
 }
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r; asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r;
+// numbers of two V nibbles in the low bits (sub) or four bits up of their halves
+__device__ __forceinline__ uint32_t v_low(uint32_t w) {
+    uint32_t r; asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(and_or(w, 0x000F000Fu, 0x64006400u)), "r"(0x64086408u)); return r;
+}
+__device__ __forceinline__ uint32_t v_high(uint32_t w) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(and_or(w, 0x00F000F0u, 0x64006400u)), "r"(0x2C002C00u), "r"(0xD480D480u));
+    return r;
 }
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
@@ -185,6 +196,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     // ── state of the segment at hand ──
     uint32_t qa[W * 2][4];                      // operand of the scores: step 2·w + h of word w
     float qoff[NG];                             // −24 · Σ q of a group
+    float qback = 1.f;                          // the power of two that the query was divided by
     float o[NT][4], m = -INFINITY, l = 0.f;
     int seg = -1, seg_lo = 0, seg_len = 0;
     auto start = [&](int s) {
@@ -196,26 +208,39 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         const float f = dv.a.scale * 1.4426950408889634f;
 #pragma unroll
         for (int i = 0; i < NG; i++) qoff[i] = 0.f;
+        float x[W][8], big = 0.f;
 #pragma unroll
         for (int w = 0; w < W; w++) {
-            float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = 0.f;
+            for (int i = 0; i < 8; i++) x[w][i] = 0.f;
             if (live) {
                 const float4 u = *(const float4*)(q + (w / WG) * GS + t * (GS / 4) + (w % WG) * 8);
                 const float4 v = *(const float4*)(q + (w / WG) * GS + t * (GS / 4) + (w % WG) * 8 + 4);
-                x[0] = u.x * f; x[1] = u.y * f; x[2] = u.z * f; x[3] = u.w * f; x[4] = v.x * f; x[5] = v.y * f; x[6] = v.z * f; x[7] = v.w * f;
+                x[w][0] = u.x * f; x[w][1] = u.y * f; x[w][2] = u.z * f; x[w][3] = u.w * f;
+                x[w][4] = v.x * f; x[w][5] = v.y * f; x[w][6] = v.z * f; x[w][7] = v.w * f;
             }
 #pragma unroll
+            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[w][i]));
+        }
+        big = fmaxf(big, __shfl_xor_sync(AX_FULL, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(AX_FULL, big, 2));
+        // 2^e brings the largest number into [2^14, 2^15); e stays where 2^e and 2^-e are normal numbers
+        const int e = big > 0.f && big <= 3.402823466e38f ? min(max(14 - ((__float_as_int(big) >> 23) - 127), -126), 126) : 0;
+        const float up = __int_as_float((e + 127) << 23);
+        qback = __int_as_float((127 - e) << 23);
+#pragma unroll
+        for (int w = 0; w < W; w++)
+#pragma unroll
             for (int p = 0; p < 4; p++) {                                      // pair (p, p + 4) of the word
-                const uint32_t hi = pack_bf16(x[p], x[p + 4]);
-                const float r0 = x[p] - ax_bf16_lo(hi), r1 = x[p + 4] - ax_bf16_hi(hi);
-                const uint32_t lo = pack_bf16(r0, r1);
+                const float y0 = x[w][p] * up, y1 = x[w][p + 4] * up;
+                const uint32_t hi = pack_f16(y0, y1);
+                const float2 h = unpack_f16(hi);
+                const uint32_t lo = pack_f16(y0 - h.x, y1 - h.y);
+                const float2 r = unpack_f16(lo);
                 qa[2 * w + p / 2][(p & 1) * 2] = hi;
                 qa[2 * w + p / 2][(p & 1) * 2 + 1] = lo;
-                qoff[w / WG] += (ax_bf16_lo(hi) + ax_bf16_lo(lo)) + (ax_bf16_hi(hi) + ax_bf16_hi(lo));
+                qoff[w / WG] += (h.x + r.x) + (h.y + r.y);
             }
-        }
 #pragma unroll
         for (int i = 0; i < NG; i++) {
             qoff[i] += __shfl_xor_sync(AX_FULL, qoff[i], 1);
@@ -285,9 +310,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
 #pragma unroll
                     for (int i = 0; i < WG; i++) {
                         const uint32_t w = kw[gr * WG + i];
-                        const uint32_t b0 = and_or(w, 0x00780078u, 0x41804180u), b1 = and_or(w >> 4, 0x00780078u, 0x41804180u);
-                        const uint32_t b2 = and_or(w >> 8, 0x00780078u, 0x41804180u);
-                        const uint32_t b3 = and_or(__funnelshift_r(w, w, 12), 0x00780078u, 0x41804180u);
+                        const uint32_t b0 = and_or(w, 0x03C003C0u, 0x4C004C00u), b1 = and_or(w >> 4, 0x03C003C0u, 0x4C004C00u);
+                        const uint32_t b2 = and_or(__funnelshift_r(w, w, 8), 0x03C003C0u, 0x4C004C00u);
+                        const uint32_t b3 = and_or(__funnelshift_r(w, w, 12), 0x03C003C0u, 0x4C004C00u);
                         if (i == 0) mma(d, qa[2 * (gr * WG + i)], b0, b1, qoff[gr], qoff[gr], 0.f, 0.f);
                         else mma(d, qa[2 * (gr * WG + i)], b0, b1, d[0], d[1], d[2], d[3]);
                         mma(d, qa[2 * (gr * WG + i) + 1], b2, b3, d[0], d[1], d[2], d[3]);
@@ -311,12 +336,38 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                     if (!seen[i]) s[i] = -INFINITY;
                 }
             }
-            float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            // scales of V of the lane's four rows; an absent row has none
+            float vs[4][NG], z[4];
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) {
+                uint32_t sw[NG];
+                lds<NG>(sw, tile + 2 * PLANE + SC + (8 * nt + 2 * t) * NG * 2);
+#pragma unroll
+                for (int i = 0; i < 2 * NG; i++) vs[2 * nt + i / NG][i % NG] = i & 1 ? ax_bf16_hi(sw[i / 2]) : ax_bf16_lo(sw[i / 2]);
+            }
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (!seen[i]) {
+#pragma unroll
+                        for (int gr = 0; gr < NG; gr++) vs[i][gr] = 0.f;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[i] *= qback;
+                float big = vs[i][0];
+#pragma unroll
+                for (int gr = 1; gr < NG; gr++) big = fmaxf(big, vs[i][gr]);
+                z[i] = s[i] + fmaxf(lg2(big), -100.f);
+            }
+            float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
             top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 1));
             top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 2));
-            // the maximum is followed only where a probability would pass 2^8: sums and outputs are f32, any reference will do
-            if (__any_sync(AX_FULL, top > m + 8.f)) {
-                const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2(m - mn);
+            // The reference is moved only where a p · scale would pass 2^15; then the largest becomes 2^7, so what is lost of the small
+            // ones (half a step of f16's subnormals, 2^-25) is at most 2^-32 of the largest.
+            if (__any_sync(AX_FULL, top > m + 15.f)) {
+                const float mn = fmaxf(m, top - 7.f), f = m == -INFINITY ? 0.f : ex2(m - mn);
                 l *= f;
 #pragma unroll
                 for (int i = 0; i < NT; i++) { o[i][0] *= f; o[i][1] *= f; o[i][2] *= f; o[i][3] *= f; }
@@ -326,34 +377,30 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             float p[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) { p[i] = ex2(s[i] - mr); l += p[i]; }
-            uint32_t vw[2][W], sw[2][NG];
+            uint32_t vw[2][W];
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                lds<W>(vw[nt], tile + PLANE + nt * (PLANE / 2) + lane * W * 4);
-                lds<NG>(sw[nt], tile + 2 * PLANE + SC + (8 * nt + 2 * t) * NG * 2);
-            }
+            for (int nt = 0; nt < 2; nt++) lds<W>(vw[nt], tile + PLANE + nt * (PLANE / 2) + lane * W * 4);
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) {
                 uint32_t a[4];
 #pragma unroll
                 for (int nt = 0; nt < 2; nt++) {
-                    float v0 = gr & 1 ? ax_bf16_hi(sw[nt][gr / 2]) : ax_bf16_lo(sw[nt][gr / 2]);
-                    float v1 = (NG + gr) & 1 ? ax_bf16_hi(sw[nt][(NG + gr) / 2]) : ax_bf16_lo(sw[nt][(NG + gr) / 2]);
-                    if (edge) { if (!seen[2 * nt]) v0 = 0.f; if (!seen[2 * nt + 1]) v1 = 0.f; }
-                    const float y0 = p[2 * nt] * v0, y1 = p[2 * nt + 1] * v1;
-                    const uint32_t hi = pack_bf16(y0, y1);
+                    const float y0 = p[2 * nt] * vs[2 * nt][gr], y1 = p[2 * nt + 1] * vs[2 * nt + 1][gr];
+                    const uint32_t hi = pack_f16(y0, y1);
+                    const float2 h = unpack_f16(hi);
                     a[2 * nt] = hi;
-                    a[2 * nt + 1] = pack_bf16(y0 - ax_bf16_lo(hi), y1 - ax_bf16_hi(hi));
+                    a[2 * nt + 1] = pack_f16(y0 - h.x, y1 - h.y);
                 }
 #pragma unroll
-                for (int i = 0; i < WG; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t b0 = sub_bf16x2(and_or(vw[0][gr * WG + i] >> (4 * j), 0x000F000Fu, 0x43004300u), 0x43084308u);
-                        const uint32_t b1 = sub_bf16x2(and_or(vw[1][gr * WG + i] >> (4 * j), 0x000F000Fu, 0x43004300u), 0x43084308u);
-                        float (&d)[4] = o[(gr * WG + i) * 4 + j];
-                        mma(d, a, b0, b1, d[0], d[1], d[2], d[3]);
-                    }
+                for (int i = 0; i < WG; i++) {
+                    const int cw = gr * WG + i;
+                    const uint32_t u0 = vw[0][cw], u1 = vw[1][cw];
+                    float (&d0)[4] = o[cw * 4], (&d1)[4] = o[cw * 4 + 1], (&d2)[4] = o[cw * 4 + 2], (&d3)[4] = o[cw * 4 + 3];
+                    mma(d0, a, v_low(u0), v_low(u1), d0[0], d0[1], d0[2], d0[3]);
+                    mma(d1, a, v_high(u0), v_high(u1), d1[0], d1[1], d1[2], d1[3]);
+                    mma(d2, a, v_low(u0 >> 8), v_low(u1 >> 8), d2[0], d2[1], d2[2], d2[3]);
+                    mma(d3, a, v_high(u0 >> 8), v_high(u1 >> 8), d3[0], d3[1], d3[2], d3[3]);
+                }
             }
         }
         __syncwarp();                                                          // every lane has read the stage

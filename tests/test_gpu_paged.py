@@ -3,9 +3,12 @@ plain implementations in 64 bits.
 
 Tolerances, from the arithmetic (u16 = half a step of the 16-bit type: 2^-8 bf16, 2^-11 f16):
   * plan, four-bit values: equal.
-  * decode attention: queries and probabilities are split into bf16 hi + lo (error 2^-16 of the value each), sums are f32.  A score is
+  * decode attention: queries and probabilities are split into 16-bit hi + lo parts (error at most 2^-16 of the value each), sums are f32.  A score is
     off by at most e = (2^-16 + 2^-18)·scale·Σ|q·k|, a probability by 2e of itself (its own and the normaliser's), the product by
-    2^-16 more, f32 sums by 2^-18 at these lengths:  |Δo| ≤ (2·max e + 2^-15)·Σ p|v|.
+    2^-16 more, f32 sums by 2^-18 at these lengths:  |Δo| ≤ (2·max e + 2^-15)·Σ p|v|.  The parts of p·(scale of V) are f16 numbers whose
+    smallest step is 2^-24 where the row's largest is at least 2^7, so every row may be off by 2^-32 of the largest, times a number of
+    at most 7; the largest number of a group is 7 (a scale rounded up leaves it at least 6.97), so 7·scale ≤ 1.01·max|v|:
+    |Δo| ≤ … + rows·2^-32·1.01·max_j (p_j·max|v_j|).
   * prompt attention: products of 16-bit numbers are exact in f32, so a score is off by e = 2^-18·scale·Σ|q·k|; a probability is
     rounded to the 16-bit type (u16 of itself; in f16 at least 2^-25 of the row's largest) and the output once more:
     |Δo| ≤ u16·|o| + (u16 + 2·max e + 2^-16)·Σ p|v| + 2^-25·Σ|v| / l for f16, l ≥ 1 the normaliser.
@@ -276,7 +279,7 @@ def decode_by_hand(c, q, scale, window, lens):
             p = np.exp(a - a.max())
             p /= p.sum()
             out[i, h] = p @ v[:, kh]
-            tol[i, h] = (2 * e + 2.0 ** -15) * (p @ np.abs(v[:, kh]))
+            tol[i, h] = (2 * e + 2.0 ** -15) * (p @ np.abs(v[:, kh])) + (n - lo) * 2.0 ** -32 * 1.01 * (p * np.abs(v[:, kh]).max(1)).max()
     return out, tol + 1e-30
 
 
