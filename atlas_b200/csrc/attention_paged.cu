@@ -11,10 +11,11 @@
 //     is good to 2^-22 of each value (bf16 halves left 4e-6 of the output, 2^-16 of each value).  The score accumulators are
 //     already the operand layout of the second product.  f16 has little range, so a head's query is brought to 2^14 by a power
 //     of two, and the softmax reference follows the largest p · scale of V instead of the largest p.
-//   * K nibbles become f16 by one mask-and-or (16 + u, u = number + 8); −24 · Σq of the group enters as the accumulator's start
-//     value.  The scale of (row, group) multiplies the group's finished sum.  V nibbles are made exact (1024 + u − 1032, or
-//     (1024 + 16u) / 16 − 72 without a shift): over a long context the sum of the numbers is far smaller than that of their
-//     offsets.  The scale of V goes into P.
+//   * A nibble u (the number plus eight) becomes an f16 number by mask-and-or and one exact operation: 1024 + u − 1032, or, four
+//     bits up, (1024 + 16u) / 16 − 72: nine instructions for eight numbers.  (Leaving the offset in and subtracting −24 · Σq from
+//     the scores costs as much in register moves and five times the rounding; for V the sum of the numbers over a long context is
+//     far smaller than that of their offsets.)  The scale of (row, group) multiplies the group's finished score; the scale of V
+//     goes into P.
 //   * Segments that end inside a warp's piece are written from registers; the others meet in shared memory, and where they
 //     reach over CTAs in the workspace, added up by the last CTA to arrive, in the order of the pieces: no result depends on timing.
 #include "paged.cuh"
@@ -67,19 +68,19 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t x) { return __half22float2
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
     uint32_t r; asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits)); return r;
 }
-// numbers of two V nibbles in the low bits (sub) or four bits up of their halves
-__device__ __forceinline__ uint32_t v_low(uint32_t w) {
+// the two numbers whose nibbles lie in the low bits of the halves of a word, or four bits up
+__device__ __forceinline__ uint32_t n_low(uint32_t w) {
     uint32_t r; asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(and_or(w, 0x000F000Fu, 0x64006400u)), "r"(0x64086408u)); return r;
 }
-__device__ __forceinline__ uint32_t v_high(uint32_t w) {
+__device__ __forceinline__ uint32_t n_high(uint32_t w) {
     uint32_t r;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(and_or(w, 0x00F000F0u, 0x64006400u)), "r"(0x2C002C00u), "r"(0xD480D480u));
     return r;
 }
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <int N> __device__ __forceinline__ void lds(uint32_t (&r)[N], const void* p) {
     if constexpr (N == 4) { const uint4 v = *(const uint4*)p; r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
@@ -151,14 +152,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     const long long x0 = X0 + (X1 - X0) * warp / kWarps, x1 = X0 + (X1 - X0) * (warp + 1) / kWarps;
 
     // ── the warp's stream of tiles: 32 positions are resolved at a time, one per lane, and lane i copies tile i of them ──
-    long long base = x0 - 32;
+    const int count = (int)(x1 - x0);
     const uint8_t* src = nullptr;
     TileInfo mine = {};
-    auto fill = [&](long long x) {                                            // x uniform over the warp, rising by one
-        if (x >= x1) return;
-        if (x - base >= 32) {
-            base = x;
-            const long long y = x + lane;
+    auto fill = [&](int i) {                                                  // i uniform over the warp, rising by one
+        if (i >= count) return;
+        if ((i & 31) == 0) {
+            const long long y = x0 + i + lane;
             mine.seg = -1; mine.tile = 0; mine.ok = 0;
             if (y < x1) {
                 int lo = 0, hi = batch;                                       // last b with s_pre[b] · nh <= y (skipping requests without rows)
@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 else atomicExch(dv.err, AX_DEVERR_PAGE);
             }
         }
-        if (lane == (int)(x - base)) {
-            const int st = (int)((x - x0) % kStages);
+        if (lane == (i & 31)) {
+            const int st = i & (kStages - 1);
             const uint32_t bar = smem_u32(&s_bar[warp][st]);
             s_info[warp][st] = mine;
             if (mine.ok) {
@@ -190,12 +190,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             }
         }
     };
-    for (int i = 0; i < kStages; i++) fill(x0 + i);
+    for (int i = 0; i < kStages; i++) fill(i);
     __syncwarp();
 
     // ── state of the segment at hand ──
     uint32_t qa[W * 2][4];                      // operand of the scores: step 2·w + h of word w
-    float qoff[NG];                             // −24 · Σ q of a group
     float qback = 1.f;                          // the power of two that the query was divided by
     float o[NT][4], m = -INFINITY, l = 0.f;
     int seg = -1, seg_lo = 0, seg_len = 0;
@@ -206,8 +205,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         const bool live = h0 + g < dv.group_heads;
         const float* q = dv.a.q + ((size_t)b * dv.a.n_heads + (size_t)kh * dv.group_heads + h0 + g) * HD;
         const float f = dv.a.scale * 1.4426950408889634f;
-#pragma unroll
-        for (int i = 0; i < NG; i++) qoff[i] = 0.f;
         float x[W][8], big = 0.f;
 #pragma unroll
         for (int w = 0; w < W; w++) {
@@ -236,17 +233,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 const uint32_t hi = pack_f16(y0, y1);
                 const float2 h = unpack_f16(hi);
                 const uint32_t lo = pack_f16(y0 - h.x, y1 - h.y);
-                const float2 r = unpack_f16(lo);
                 qa[2 * w + p / 2][(p & 1) * 2] = hi;
                 qa[2 * w + p / 2][(p & 1) * 2 + 1] = lo;
-                qoff[w / WG] += (h.x + r.x) + (h.y + r.y);
             }
-#pragma unroll
-        for (int i = 0; i < NG; i++) {
-            qoff[i] += __shfl_xor_sync(AX_FULL, qoff[i], 1);
-            qoff[i] += __shfl_xor_sync(AX_FULL, qoff[i], 2);
-            qoff[i] *= -24.f;
-        }
 #pragma unroll
         for (int i = 0; i < NT; i++) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
         m = -INFINITY; l = 0.f;
@@ -285,12 +274,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         }
     };
 
-    for (long long x = x0; x < x1; x++) {
-        const int st = (int)((x - x0) % kStages);
-        if (!mbar_wait(smem_u32(&s_bar[warp][st]), (uint32_t)((x - x0) / kStages) & 1u)) {
+    for (int it = 0; it < count; it++) {
+        const int st = it & (kStages - 1);
+        if (!mbar_wait(smem_u32(&s_bar[warp][st]), (uint32_t)(it / kStages) & 1u)) {
             if (lane == 0) atomicExch(dv.err, kErrWait);
-            for (long long y = x; y < x1 && y < x + kStages; y++)             // what is in flight lands before the CTA goes
-                mbar_wait(smem_u32(&s_bar[warp][(int)((y - x0) % kStages)]), (uint32_t)((y - x0) / kStages) & 1u);
+            for (int y = it; y < count && y < it + kStages; y++)              // what is in flight lands before the CTA goes
+                mbar_wait(smem_u32(&s_bar[warp][y & (kStages - 1)]), (uint32_t)(y / kStages) & 1u);
             break;
         }
         const TileInfo info = s_info[warp][st];
@@ -306,16 +295,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 float s0 = 0.f, s1 = 0.f;
 #pragma unroll
                 for (int gr = 0; gr < NG; gr++) {
-                    float d[4];
+                    float d[4] = { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
                     for (int i = 0; i < WG; i++) {
-                        const uint32_t w = kw[gr * WG + i];
-                        const uint32_t b0 = and_or(w, 0x03C003C0u, 0x4C004C00u), b1 = and_or(w >> 4, 0x03C003C0u, 0x4C004C00u);
-                        const uint32_t b2 = and_or(__funnelshift_r(w, w, 8), 0x03C003C0u, 0x4C004C00u);
-                        const uint32_t b3 = and_or(__funnelshift_r(w, w, 12), 0x03C003C0u, 0x4C004C00u);
-                        if (i == 0) mma(d, qa[2 * (gr * WG + i)], b0, b1, qoff[gr], qoff[gr], 0.f, 0.f);
-                        else mma(d, qa[2 * (gr * WG + i)], b0, b1, d[0], d[1], d[2], d[3]);
-                        mma(d, qa[2 * (gr * WG + i) + 1], b2, b3, d[0], d[1], d[2], d[3]);
+                        const uint32_t w = kw[gr * WG + i], v = w >> 8;
+                        mma(d, qa[2 * (gr * WG + i)], n_low(w), n_high(w));
+                        mma(d, qa[2 * (gr * WG + i) + 1], n_low(v), n_high(v));
                     }
                     // scales of columns 2t and 2t + 1, NG numbers each
                     const float k0 = gr & 1 ? ax_bf16_hi(sw[gr / 2]) : ax_bf16_lo(sw[gr / 2]);
@@ -396,15 +381,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                     const int cw = gr * WG + i;
                     const uint32_t u0 = vw[0][cw], u1 = vw[1][cw];
                     float (&d0)[4] = o[cw * 4], (&d1)[4] = o[cw * 4 + 1], (&d2)[4] = o[cw * 4 + 2], (&d3)[4] = o[cw * 4 + 3];
-                    mma(d0, a, v_low(u0), v_low(u1), d0[0], d0[1], d0[2], d0[3]);
-                    mma(d1, a, v_high(u0), v_high(u1), d1[0], d1[1], d1[2], d1[3]);
-                    mma(d2, a, v_low(u0 >> 8), v_low(u1 >> 8), d2[0], d2[1], d2[2], d2[3]);
-                    mma(d3, a, v_high(u0 >> 8), v_high(u1 >> 8), d3[0], d3[1], d3[2], d3[3]);
+                    mma(d0, a, n_low(u0), n_low(u1));
+                    mma(d1, a, n_high(u0), n_high(u1));
+                    mma(d2, a, n_low(u0 >> 8), n_low(u1 >> 8));
+                    mma(d3, a, n_high(u0 >> 8), n_high(u1 >> 8));
                 }
             }
         }
         __syncwarp();                                                          // every lane has read the stage
-        fill(x + kStages);
+        fill(it + kStages);
         __syncwarp();
     }
     if (seg >= 0) flush();

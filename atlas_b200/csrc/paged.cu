@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(256) ax_p4_append_kernel(const RowArgs a) {
     uint8_t* tile = a.pool + ax_p4_tile_at(a.s, page, head, off);
     const int plane = ax_p4_plane_bytes(a.s);
     if (which == 0) {
-        reinterpret_cast<uint32_t*>(tile)[ax_p4_k_word(a.s, r, 8 * li)] = ax_p4_rot(w);
+        reinterpret_cast<uint32_t*>(tile)[ax_p4_k_word(a.s, r, 8 * li)] = w;
     } else {
         uint16_t* vp = reinterpret_cast<uint16_t*>(tile + plane);
         vp[ax_p4_v_half(a.s, r, 8 * li)] = (uint16_t)(w & 0xFFFFu);
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256) ax_p4_read_kernel(const RowArgs a) {
         const int page = slot / a.s.page_size, off = slot % a.s.page_size, r = off % AX_P4_TILE;
         const uint8_t* tile = a.pool + ax_p4_tile_at(a.s, page, head, off);
         const int plane = ax_p4_plane_bytes(a.s);
-        const uint32_t kw = ax_p4_unrot(reinterpret_cast<const uint32_t*>(tile)[ax_p4_k_word(a.s, r, 8 * li)]);
+        const uint32_t kw = reinterpret_cast<const uint32_t*>(tile)[ax_p4_k_word(a.s, r, 8 * li)];
         const uint16_t* vp = reinterpret_cast<const uint16_t*>(tile + plane);
         const uint32_t vw = vp[ax_p4_v_half(a.s, r, 8 * li)] | ((uint32_t)vp[ax_p4_v_half(a.s, r, 8 * li + 4)] << 16);
         const uint16_t* sp = reinterpret_cast<const uint16_t*>(tile + 2 * plane);

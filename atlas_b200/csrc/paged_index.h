@@ -9,8 +9,7 @@
 // Inside a tile the nibbles lie in the order in which the lanes of mma.m16n8k16 want them (attention_paged.cu): lane 4·g + t
 // reads its share of eight rows as one 16-byte word group (hd / 32 words of 32 bits), no bank conflicts and no shuffles.
 //   K: the B operand of S = Q·Kᵀ.  Column g of row block nt is row 8·nt + 4·(g & 1) + (g >> 1); thread t owns GS / 4
-//      consecutive numbers of every group of GS numbers.  The word is rotated left by six bits: a nibble then meets the top four
-//      mantissa bits of an f16 (16 + nibble) after a rotation by a multiple of four.
+//      consecutive numbers of every group of GS numbers.
 //   V: the B operand of O = P·V.  A 32-bit word holds four numbers of row 8·nt + t in its low half and the same four of row
 //      8·nt + 4 + t in its high half (the k pair 2t, 2t + 1 of the product), column g owning GS / 8 consecutive numbers of a group.
 // A nibble is the number plus eight.
@@ -42,13 +41,11 @@ AX_HD size_t ax_p4_tile_at(const AxP4Shape& s, int page, int head, int off) {
 }
 // row r (0..15) of a tile → the column index that the product gives it (8·nt + g)
 AX_HD int ax_p4_col(int r) { return (r & 8) | ((r & 3) << 1) | ((r >> 2) & 1); }
-// K: 32-bit word (within the K plane) of the eight numbers d8 = 8·i .. 8·i + 7 of row r; number j of them is nibble j before the rotation
+// K: 32-bit word (within the K plane) of the eight numbers d8 = 8·i .. 8·i + 7 of row r; number j of them is nibble j
 AX_HD int ax_p4_k_word(const AxP4Shape& s, int r, int d8) {
     const int dg = d8 % s.group, t = dg / (s.group / 4), sub = (dg % (s.group / 4)) / 8;
     return (ax_p4_col(r) * 4 + t) * (s.hd / 32) + (d8 / s.group) * (s.group / 32) + sub;
 }
-AX_HD uint32_t ax_p4_rot(uint32_t w) { return (w << 6) | (w >> 26); }
-AX_HD uint32_t ax_p4_unrot(uint32_t w) { return (w >> 6) | (w << 26); }
 // V: 16-bit half word (within the V plane) of the four numbers d4 = 4·i .. 4·i + 3 of row r; number j of them is nibble j
 AX_HD int ax_p4_v_half(const AxP4Shape& s, int r, int d4) {
     const int dg = d4 % s.group, g = dg / (s.group / 8), c = (d4 / s.group) * (s.group / 32) + (dg % (s.group / 8)) / 4;

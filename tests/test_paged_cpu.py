@@ -24,8 +24,6 @@ int k_word(int hd, int g, int r, int d) { AxP4Shape s = { 1, 16, 1, hd, g }; ret
 int v_half(int hd, int g, int r, int d) { AxP4Shape s = { 1, 16, 1, hd, g }; return ax_p4_v_half(s, r, d); }
 int scale_at(int hd, int g, int r, int gr) { AxP4Shape s = { 1, 16, 1, hd, g }; return ax_p4_scale(s, r, gr); }
 int col(int r) { return ax_p4_col(r); }
-unsigned rot(unsigned w) { return ax_p4_rot(w); }
-unsigned unrot(unsigned w) { return ax_p4_unrot(w); }
 }
 """
 
@@ -39,7 +37,6 @@ def idx(tmp_path_factory):
     L = C.CDLL(so)
     for f in ("tile_bytes", "pool_bytes", "tile_at"):
         getattr(L, f).restype = C.c_longlong
-    L.rot.restype = L.unrot.restype = C.c_uint
     return L
 
 
@@ -85,11 +82,6 @@ def test_tiles_stay_inside_the_pool(idx):
     # a pool of 300 GB: offsets beyond 32 bits
     n, p, k = 8_000_000, 16, 16
     assert idx.tile_at(n, p, k, 128, 32, n - 1, k - 1, 15) == idx.pool_bytes(n, p, k, 128, 32) - 2304 == n * k * 2304 - 2304
-
-
-def test_rotation_is_undone(idx):
-    for w in (0, 1, 0x80000000, 0xFEDCBA98, 0xFFFFFFFF):
-        assert idx.unrot(idx.rot(w)) == w
 
 
 # ── refusals ─────────────────────────────────────────────────────────────────────
