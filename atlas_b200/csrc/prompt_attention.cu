@@ -1,16 +1,488 @@
-// prompt_attention.cu — causal attention of whole packed prompts.
+// prompt_attention.cu — causal attention of whole packed prompts on the fifth-generation tensor cores.
+//
+// 4 · hd flops and one exponential per visible (query, key) pair and head: at hd 128 a tile of 128 × 128 pairs is 1024 clocks of
+// tcgen05.mma and 1024 clocks of the SM's 16 exponentials a clock, so neither may wait for the other.
+//   * A CTA works on two query tiles of 128 rows with the same keys: the same rows of two heads that share a KV head, or — where the
+//     heads do not pair up — 256 consecutive rows of one head.  While four warps take the softmax of one tile the tensor core runs the
+//     products of the other.
+//   * S = Q·Kᵀ (128 × 128 f32) and O (128 × hd f32) live in tensor memory; the probabilities go back over the scores as 16-bit numbers
+//     and are the A operand of O += P·V straight from there.  V is the B operand as it lies in memory (rows of keys).
+//   * A thread owns a row: its maximum and sum need no exchange between lanes.  O is rescaled only when the running maximum has grown by
+//     more than 2^8 — sums are f32 and any reference between is exact — so the rescaling almost never runs.
+//   * K and V tiles come by tiled bulk copies through one ring of shared-memory stages: K0 V0 K1 V1 …
+//   * Which sequence and rows a CTA owns it finds in the prefix array itself, late (long) row tiles first: nothing depends on host-side
+//     lengths, and a captured call follows the arrays.
+//   * A product of 0 and a NaN or infinity in a value row that the query does not see would be NaN: value rows behind the sequence are
+//     zeroed in shared memory, and an output row that is not finite is taken again by ax_prompt_row, which reads visible rows only.
+//   * Every wait is bounded (two seconds of %globaltimer): on expiry the CTA raises the context's error word, all roles leave, copies
+//     in flight are waited for and tensor memory is released.
+#include <cuda.h>
+#include <type_traits>
+
 #include "prompt_attention.cuh"
 
 namespace {
 
+constexpr int kRows = 128;                        // rows of a query tile, keys of a K / V tile
+constexpr int kBoxBytes = kRows * 128;            // one box: 128 rows of 128 bytes
+constexpr int kThreads = 320;                     // warps 0..3, 4..7: softmax of tile 0, 1; 8: products; 9: copies
+constexpr int kMaxStages = 6;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+
+struct PromptDev {
+    AxPromptArgs a;
+    int pair_heads;                               // 1: two heads of a KV head, 0: 256 rows of one head
+    float sc;                                     // |scale| · log2 e
+    int negate;                                   // scale < 0
+    int* err;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded wait.  false: gave up (this thread's deadline passed, or another role raised the abort flag).
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+    if (mbar_try(bar, parity)) return true;
+    unsigned spins = 0;
+    unsigned long long t0 = 0;
+    while (!mbar_try(bar, parity)) {
+        if (*abort_flag) return false;
+        if ((++spins & 255u) == 0) {
+            const unsigned long long t = ax_globaltimer();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > kWaitNs) { *abort_flag = 1; atomicExch(err, code); return false; }
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// Shared-memory matrix descriptors, 128-byte swizzle (layout code 2, version 1), groups of eight rows of 128 bytes 1024 bytes apart.
+// K-major (rows hold the contracted index): the contracted index advances 32 bytes per step inside the row.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// MN-major (rows are the contracted index, 64 columns each): the next 64 columns lie one box further.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(kBoxBytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+}
+#define AX_R32(m) m(0), m(1), m(2), m(3), m(4), m(5), m(6), m(7), m(8), m(9), m(10), m(11), m(12), m(13), m(14), m(15), \
+                  m(16), m(17), m(18), m(19), m(20), m(21), m(22), m(23), m(24), m(25), m(26), m(27), m(28), m(29), m(30), m(31)
+// 32 columns of the warp's lane quarter; the values may be used after tmem_wait_ld
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+#define AX_O(i) "=r"(r[i])
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : AX_R32(AX_O) : "r"(addr));
+#undef AX_O
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
+#define AX_O(i) "+r"(r[i])
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : AX_R32(AX_O) :: "memory");
+#undef AX_O
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+#define AX_I(i) "r"(r[i])
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+                 :: AX_R32(AX_I), "r"(addr) : "memory");
+#undef AX_I
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\t"
+        "mov.b64 {%0, %1}, w;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+template <bool F16> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) ax_prompt_row_kernel(const AxPromptArgs a) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    int lo = 0, hi = a.batch;                                     // the last sequence that starts at or before the row
-    while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (a.cu_q[m] <= row) lo = m; else hi = m; }
-    const AxPromptSeq s = ax_prompt_seq(a, lo);
-    if (row < s.q0 || row >= s.q0 + s.lq) return;                 // rows outside every sequence are left as they are
-    ax_prompt_row<T, HD>(a, s, (int)blockIdx.y, row - s.q0, lane);
+__device__ __noinline__ void row_again(const AxPromptArgs& a, const AxPromptSeq& s, int h, int i, int lane) {
+    ax_prompt_row<T, HD>(a, s, h, i, lane);
+}
+
+template <bool F16, int HD>
+__global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __grid_constant__ CUtensorMap map_q,
+                                                                     const __grid_constant__ CUtensorMap map_k,
+                                                                     const __grid_constant__ CUtensorMap map_v, const PromptDev dv) {
+    using T = typename std::conditional<F16, __half, uint16_t>::type;
+    constexpr int BOXES = HD / 64, TILE = BOXES * kBoxBytes, NS = HD == 128 ? 5 : 6;
+    constexpr uint32_t kS = 0, kO = 256;                                      // columns: scores of tile t at 128 t, output at 256 + HD t
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_ready[2], o_done[2], kv_full[kMaxStages], kv_empty[kMaxStages];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort, s_issued, s_seq, s_tile, s_scan[kThreads / 32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const AxPromptArgs& a = dv.a;
+    volatile int* abort_flag = &s_abort;
+    const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t ring = smem0 + 2 * TILE;
+
+    // ── which rows: tile x of the pack counted from its end ──
+    const int tb = dv.pair_heads ? kRows : 2 * kRows;
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_u32(&q_full[i]), 1); mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&p_ready[i]), kRows); mbar_init(smem_u32(&o_done[i]), 1);
+        }
+        for (int i = 0; i < NS; i++) { mbar_init(smem_u32(&kv_full[i]), 1); mbar_init(smem_u32(&kv_empty[i]), 1); }
+        s_abort = 0; s_issued = 0; s_seq = -1; s_tile = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    {
+        const int per = (a.batch + kThreads - 1) / kThreads, b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+        int own = 0;
+        for (int b = b0; b < b1; b++) own += (ax_prompt_seq(a, b).lq + tb - 1) / tb;
+        int inc = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const int x = __shfl_up_sync(AX_FULL, inc, d); if (lane >= d) inc += x; }
+        if (lane == 31) s_scan[warp] = inc;
+        __syncthreads();
+        int at = inc - own, all = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; w++) { if (w < warp) at += s_scan[w]; all += s_scan[w]; }
+        const int x = all - 1 - (int)blockIdx.x;
+        if (x < 0) return;
+        if (x >= at && x < at + own)
+            for (int b = b0; b < b1; b++) {
+                const int n = (ax_prompt_seq(a, b).lq + tb - 1) / tb;
+                if (x < at + n) { s_seq = b; s_tile = x - at; break; }
+                at += n;
+            }
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    const AxPromptSeq s = ax_prompt_seq(a, s_seq);
+    const int off = s.lk - s.lq;
+    const int h0 = dv.pair_heads ? 2 * (int)blockIdx.y : (int)blockIdx.y, kh = h0 / (a.n_heads / a.n_kv);
+    int base[2], lo[2], hi[2];                                                // first row and K / V tiles [lo, hi] of both query tiles
+    base[0] = s_tile * tb; base[1] = dv.pair_heads ? base[0] : base[0] + kRows;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int last = min(base[t] + kRows, s.lq) - 1 + off, first = base[t] + off;
+        lo[t] = 0; hi[t] = -1;
+        if (base[t] < s.lq && last >= 0 && s.lk > 0) {
+            lo[t] = a.window > 0 && first - a.window + 1 > 0 ? (first - a.window + 1) / kRows : 0;
+            hi[t] = last / kRows;
+        }
+    }
+    const bool on0 = hi[0] >= lo[0], on1 = hi[1] >= lo[1];
+    const int j0 = on0 ? (on1 ? min(lo[0], lo[1]) : lo[0]) : lo[1], j1 = max(hi[0], hi[1]);      // j1 < j0: no tile at all
+
+    if (warp == 9) {
+        if (lane == 0) {
+            for (int t = 0; t < 2; t++)
+                if (t ? on1 : on0) {
+                    const uint32_t bar = smem_u32(&q_full[t]);
+                    mbar_expect_tx(bar, TILE);
+                    for (int b = 0; b < BOXES; b++)
+                        tma_load_3d(smem0 + t * TILE + b * kBoxBytes, &map_q, b * 64, dv.pair_heads ? h0 + t : h0, s.q0 + base[t], bar);
+                }
+            const int n = j1 >= j0 ? 2 * (j1 - j0 + 1) : 0;
+            for (int i = 0; i < n; i++) {
+                const int st = i % NS;
+                if (i >= NS && !mbar_wait(smem_u32(&kv_empty[st]), (uint32_t)(i / NS - 1) & 1u, abort_flag, dv.err, 721)) break;
+                const uint32_t bar = smem_u32(&kv_full[st]);
+                mbar_expect_tx(bar, TILE);
+                const CUtensorMap* map = i & 1 ? &map_v : &map_k;
+                for (int b = 0; b < BOXES; b++) tma_load_3d(ring + st * TILE + b * kBoxBytes, map, b * 64, kh, s.k0 + (j0 + i / 2) * kRows, bar);
+                s_issued = i + 1;
+            }
+        }
+    } else if (warp == 8) {
+        constexpr uint32_t fmt = F16 ? 0u : 1u;                               // accumulator f32, A and B f16 or bf16; B of P·V is MN-major
+        constexpr uint32_t id_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kRows >> 3) << 17) | ((kRows >> 4) << 24);
+        constexpr uint32_t id_pv = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((HD >> 3) << 17) | ((kRows >> 4) << 24);
+        int np[2] = { 0, 0 };                                                 // P tiles taken
+        bool ok = true;
+        auto qk = [&](int t, int j) {                                         // scores of query tile t with K tile j
+            const uint32_t k = ring + (uint32_t)((2 * (j - j0)) % NS) * TILE, q = smem0 + t * TILE;
+            if (lane == 0) {
+#pragma unroll
+                for (int i = 0; i < HD / 16; i++)
+                    umma_ss(tmem + kS + t * 128, desc_k(q + (i / 4) * kBoxBytes + (i % 4) * 32), desc_k(k + (i / 4) * kBoxBytes + (i % 4) * 32), id_qk, i != 0);
+                umma_commit(smem_u32(&s_full[t]));
+            }
+        };
+        auto full = [&](int i) { return mbar_wait(smem_u32(&kv_full[i % NS]), (uint32_t)(i / NS) & 1u, abort_flag, dv.err, 722); };
+        auto release = [&](int i) { if (lane == 0) umma_commit(smem_u32(&kv_empty[i % NS])); };
+        if (j1 >= j0) {
+            ok = full(0);
+            for (int t = 0; t < 2 && ok; t++)
+                if ((t ? on1 : on0)) {
+                    ok = mbar_wait(smem_u32(&q_full[t]), 0, abort_flag, dv.err, 723);
+                    if (ok && lo[t] == j0) qk(t, j0);
+                }
+            if (ok) release(0);
+        }
+        for (int j = j0; j <= j1 && ok; j++) {
+            const int vi = 2 * (j - j0) + 1, ki = vi + 1;
+            const uint32_t v = ring + (uint32_t)(vi % NS) * TILE;
+            ok = full(vi);
+            if (!ok) break;
+            const int valid = s.lk - j * kRows;
+            if (valid < kRows) {                                              // value rows behind the sequence: zeros
+                for (int i = lane; i < (kRows - valid) * 8 * BOXES; i += 32) {
+                    const int b = i / ((kRows - valid) * 8), r = i % ((kRows - valid) * 8);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(v + b * kBoxBytes + valid * 128 + r * 16), "r"(0) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
+            if (j < j1) { ok = full(ki); if (!ok) break; }
+            for (int t = 0; t < 2; t++) {
+                if (j >= lo[t] && j <= hi[t]) {
+                    ok = mbar_wait(smem_u32(&p_ready[t]), (uint32_t)np[t] & 1u, abort_flag, dv.err, 724);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (lane == 0) {
+#pragma unroll
+                        for (int i = 0; i < kRows / 16; i++)
+                            umma_ts(tmem + kO + t * HD, tmem + kS + t * 128 + i * 8, desc_mn(v + i * 2048), id_pv, (np[t] | i) != 0);
+                        umma_commit(smem_u32(&o_done[t]));
+                    }
+                    np[t]++;
+                }
+                if (j + 1 >= lo[t] && j + 1 <= hi[t]) qk(t, j + 1);
+            }
+            if (!ok) break;
+            release(vi);
+            if (j < j1) release(ki);
+        }
+    } else {
+        const int t = warp >> 2;
+        const int r = (warp & 3) * 32 + lane, row = base[t] + r, pos = row + off;         // row of the sequence, key at its own position
+        const int h = dv.pair_heads ? h0 + t : h0;
+        const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t ts = quarter + kS + t * 128, to = quarter + kO + t * HD;
+        const float sc = dv.sc;
+        const int j_lo = lo[t], j_hi = hi[t];
+        const int key_hi = pos, key_lo = a.window > 0 ? pos - a.window : -1;               // visible: key_lo < j <= key_hi
+        const int first = base[t] + off, lastp = min(base[t] + kRows, s.lq) - 1 + off;     // positions of the tile's first and last row
+        float m = -INFINITY;
+        float2 l0 = make_float2(0.f, 0.f), l1 = l0;
+        bool ok = true;
+        for (int j = j_lo, it = 0; j <= j_hi; j++, it++) {
+            ok = mbar_wait(smem_u32(&s_full[t]), (uint32_t)it & 1u, abort_flag, dv.err, 725);
+            if (!__all_sync(AX_FULL, ok)) { ok = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            uint32_t u[128];
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, u + 32 * c);
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_wait_ld(u + 32 * c);
+            float* x = reinterpret_cast<float*>(u);
+            if (dv.negate) {
+#pragma unroll
+                for (int c = 0; c < 128; c++) x[c] = -x[c];
+            }
+            const int k0 = j * kRows;
+            if (k0 + kRows - 1 > first || (a.window > 0 && k0 <= lastp - a.window)) {      // some row of the tile does not see all keys
+#pragma unroll
+                for (int c = 0; c < 128; c++) if (k0 + c > key_hi || k0 + c <= key_lo) x[c] = -INFINITY;
+            }
+            float mx[4] = { x[0], x[1], x[2], x[3] };
+#pragma unroll
+            for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const bool grow = top > m && (m == -INFINITY || (top - m) * sc > 8.f);
+            if (__any_sync(AX_FULL, grow)) {
+                const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * sc);
+                if (grow) m = top;
+                l0.x *= f; l0.y *= f; l1.x *= f; l1.y *= f;
+                if (it > 0) {
+                    ok = mbar_wait(smem_u32(&o_done[t]), (uint32_t)(it - 1) & 1u, abort_flag, dv.err, 726);
+                    if (!__all_sync(AX_FULL, ok)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(to + c, o);
+                        tmem_wait_ld(o);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(to + c, o);
+                    }
+                    tmem_wait_st();
+                }
+            }
+            const float neg = m == -INFINITY ? 0.f : -m * sc;
+            const float2 sc2 = make_float2(sc, sc), neg2 = make_float2(neg, neg);
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                uint32_t p[32];
+#pragma unroll
+                for (int c = 0; c < 32; c++) {
+                    float2 y = fma2(make_float2(x[64 * half + 2 * c], x[64 * half + 2 * c + 1]), sc2, neg2);
+                    y.x = ex2(y.x); y.y = ex2(y.y);
+                    if (c & 1) l1 = add2(l1, y); else l0 = add2(l0, y);
+                    p[c] = pack<F16>(y.x, y.y);
+                }
+                tmem_st32(ts + 32 * half, p);
+            }
+            tmem_wait_st();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            mbar_arrive(smem_u32(&p_ready[t]));
+        }
+        // ── output ──
+        const int tiles = j_hi - j_lo + 1;
+        if (ok && tiles > 0) {
+            ok = mbar_wait(smem_u32(&o_done[t]), (uint32_t)(tiles - 1) & 1u, abort_flag, dv.err, 727);
+            ok = __all_sync(AX_FULL, ok);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        if (ok) {
+            const bool live = row < s.lq;
+            const float l = (l0.x + l0.y) + (l1.x + l1.y);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            float odd = 0.f;                                                  // becomes NaN with the first output that is not finite
+            T* out = (T*)a.out + (long long)(s.q0 + row) * a.o_tok + (long long)h * a.o_head;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                if (tiles > 0) {
+                    tmem_ld32(to + c, o);
+                    tmem_wait_ld(o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0u;
+                }
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float x0 = __uint_as_float(o[2 * e]) * inv, x1 = __uint_as_float(o[2 * e + 1]) * inv;
+                    odd = fmaf(x0, 0.f, fmaf(x1, 0.f, odd));
+                    w[e] = pack<F16>(x0, x1);
+                }
+                if (live) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) *reinterpret_cast<uint4*>(out + c + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                }
+            }
+            const bool sees = key_hi >= 0 && s.lk > 0;
+            unsigned again = __ballot_sync(AX_FULL, live && (odd != odd || (l == 0.f && sees)));
+            __syncwarp();
+            while (again) {
+                const int i = __ffs(again) - 1;
+                again &= again - 1;
+                row_again<T, HD>(a, s, h, base[t] + (warp & 3) * 32 + i, lane);
+            }
+        }
+    }
+
+    // ── tail: nothing of this CTA may still be in flight when its shared and tensor memory go away ──
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (s_abort) {
+        if (tid == 0) {                                                       // copies issued into stages nobody consumed any more
+            const int issued = s_issued;
+            for (int i = issued > NS ? issued - NS : 0; i < issued; i++) {
+                const unsigned long long t0 = ax_globaltimer();
+                while (!mbar_try(smem_u32(&kv_full[i % NS]), (uint32_t)(i / NS) & 1u) && ax_globaltimer() - t0 < kWaitNs) { }
+            }
+            for (int t = 0; t < 2; t++) {
+                const unsigned long long t0 = ax_globaltimer();
+                while ((t ? on1 : on0) && !mbar_try(smem_u32(&q_full[t]), 0) && ax_globaltimer() - t0 < kWaitNs) { }
+            }
+        }
+        if (tid == 32) {                                                      // products issued before the failure: time to drain
+            const unsigned long long t0 = ax_globaltimer();
+            while (ax_globaltimer() - t0 < 2000000ull) { }
+        }
+        __syncthreads();
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess) p = nullptr;
+        return (EncodeTiledFn)p;
+    }();
+    return fn;
+}
+// [rows][heads][hd] seen as boxes of 64 numbers × one head × 128 rows; reads behind the last row give zeros
+int make_map(CUtensorMap* map, bool f16, const void* data, int rows, int heads, int hd, long long tok, long long head) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return atlasx_fail(ATLASX_ERR_CUDA, "the driver does not export cuTensorMapEncodeTiled");
+    const cuuint64_t dims[3] = { (cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows };
+    // a stride that is never used may be anything the caller had; the map wants a multiple of 16 above zero
+    const cuuint64_t strides[2] = { (cuuint64_t)(heads > 1 ? head : hd) * 2, (cuuint64_t)(rows > 1 ? tok : (long long)heads * hd) * 2 };
+    const cuuint32_t box[3] = { 64, 1, kRows }, step[3] = { 1, 1, 1 };
+    const CUresult r = fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(data), dims, strides,
+                          box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return atlasx_fail(ATLASX_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+    return ATLASX_OK;
+}
+
+template <bool F16, int HD>
+int launch(atlasx_ctx* ctx, const PromptDev& dv, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v) {
+    constexpr int smem = (2 + (HD == 128 ? 5 : 6)) * (HD / 64) * kBoxBytes + 1024;
+    static bool ready[64] = {};
+    if (ctx->device >= 64 || !ready[ctx->device]) {                           // the limit is per device; asking twice does no harm
+        AX_CUDA(cudaFuncSetAttribute(ax_prompt_umma_kernel<F16, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        if (ctx->device < 64) ready[ctx->device] = true;
+    }
+    const int tb = dv.pair_heads ? kRows : 2 * kRows;
+    // at most one unfilled tile per sequence, and no more sequences with rows than rows
+    const long long tiles = (long long)dv.a.n_q / tb + (dv.a.batch < dv.a.n_q ? dv.a.batch : dv.a.n_q);
+    ax_prompt_umma_kernel<F16, HD><<<dim3((unsigned)tiles, (unsigned)(dv.pair_heads ? dv.a.n_heads / 2 : dv.a.n_heads)), kThreads, smem, ctx->stream>>>(q, k, v, dv);
+    AX_CHECK_LAUNCH("ax_prompt_umma_kernel");
+    return ATLASX_OK;
 }
 
 }  // namespace
@@ -22,6 +494,7 @@ extern "C" int atlasx_prompt_attention(atlasx_ctx* c, int dtype, const void* q, 
     AX_ARG(dtype == ATLASX_BF16 || dtype == ATLASX_F16, "dtype must be bf16 or f16");
     AX_ARG(batch >= 1 && batch <= AX_PAGED_MAX_BATCH, "batch must be in 1..4096");
     AX_ARG(n_q >= 0 && n_k >= 0, "row counts must not be negative");
+    AX_ARG(n_q <= 0x3FFFFFFF && n_k <= 0x3FFFFFFF, "too many rows");
     AX_ARG(n_heads >= 1 && n_kv >= 1 && n_heads % n_kv == 0, "n_heads must be a multiple of n_kv_heads");
     AX_ARG(n_heads <= 65535, "too many heads");
     AX_ARG(hd == 64 || hd == 128, "head_dim must be 64 or 128");
@@ -32,19 +505,27 @@ extern "C" int atlasx_prompt_attention(atlasx_ctx* c, int dtype, const void* q, 
     AX_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 == 0 &&
            (q_tok | q_head | k_tok | k_head | v_tok | v_head | o_tok | o_head) % 8 == 0, "rows must start on 16-byte boundaries");
     AX_ARG(q_tok >= 0 && q_head >= 0 && k_tok >= 0 && k_head >= 0 && v_tok >= 0 && v_head >= 0, "strides must not be negative");
+    AX_ARG((q_head > 0 || n_heads == 1) && ((k_head > 0 && v_head > 0) || n_kv == 1 || n_k == 0) &&
+           (q_tok > 0 || n_q == 1) && ((k_tok > 0 && v_tok > 0) || n_k <= 1), "strides must not be zero");
     AX_ARG((o_head >= hd || n_heads == 1) && (o_tok >= hd || n_q == 1), "rows of out overlap");
+    AX_ARG(q_tok < (1ll << 38) && q_head < (1ll << 38) && k_tok < (1ll << 38) && k_head < (1ll << 38) && v_tok < (1ll << 38) && v_head < (1ll << 38),
+           "strides must be below 2^38");
     AX_ARG(c, "ctx is null");
     AX_ON_DEVICE(c);
-    AxPromptArgs a = { q, k, v, out, q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head, cu_q, cu_k, batch, n_q, n_k,
-                       n_heads, n_kv, hd, window, scale };
-    const dim3 grid((unsigned)((n_q + 3) / 4), (unsigned)n_heads);
-    if (dtype == ATLASX_BF16) {
-        if (hd == 128) ax_prompt_row_kernel<uint16_t, 128><<<grid, 128, 0, c->stream>>>(a);
-        else ax_prompt_row_kernel<uint16_t, 64><<<grid, 128, 0, c->stream>>>(a);
-    } else {
-        if (hd == 128) ax_prompt_row_kernel<__half, 128><<<grid, 128, 0, c->stream>>>(a);
-        else ax_prompt_row_kernel<__half, 64><<<grid, 128, 0, c->stream>>>(a);
-    }
-    AX_CHECK_LAUNCH("ax_prompt_row_kernel");
-    return ATLASX_OK;
+    PromptDev dv = {};
+    dv.a = { q, k, v, out, q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head, cu_q, cu_k, batch, n_q, n_k, n_heads, n_kv, hd, window, scale };
+    dv.pair_heads = (n_heads / n_kv) % 2 == 0;
+    dv.negate = scale < 0.f;
+    // a hidden key's score is −inf · sc: a scale of zero must not make it NaN.  Scores below 2^126 / 1e37 of it are still all alike.
+    dv.sc = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-37f);
+    dv.err = c->dev_error;
+    const bool f16 = dtype == ATLASX_F16;
+    CUtensorMap mq, mk, mv;
+    int rc = make_map(&mq, f16, q, n_q, n_heads, hd, q_tok, q_head);
+    if (!rc && n_k > 0) rc = make_map(&mk, f16, k, n_k, n_kv, hd, k_tok, k_head);
+    if (!rc && n_k > 0) rc = make_map(&mv, f16, v, n_k, n_kv, hd, v_tok, v_head);
+    if (rc) return rc;
+    if (n_k == 0) mk = mv = mq;                                               // never read: no sequence has keys
+    if (f16) return hd == 128 ? launch<true, 128>(c, dv, mq, mk, mv) : launch<true, 64>(c, dv, mq, mk, mv);
+    return hd == 128 ? launch<false, 128>(c, dv, mq, mk, mv) : launch<false, 64>(c, dv, mq, mk, mv);
 }

@@ -506,20 +506,22 @@ def test_prompt_scores_that_grow_along_the_row(ab):
 
 
 def poisoned(ab, hd, lens, total, bad, window, value):
-    """Outputs with `value` in K and V at the rows `bad`, next to the outputs without; rows from lens' sum to total are padding."""
+    """Outputs with `value` in K and V at the rows `bad`; what they would be without, in 64 bits, and how far off the format lets them
+    be (a row that is taken again because its tile held the value rounds differently, within the same bound).  Rows from lens' sum
+    to total are padding."""
     rng = np.random.default_rng(5)
     nh = 2
     q, k, v = (bf16(rng.standard_normal((total, nh, hd)).astype(np.float32)) for _ in range(3))
-    cu = ab.DeviceArray.from_host(np.concatenate([[0], np.cumsum(lens)]), ab.I32)
-    got = []
-    for x in (None, value):
-        if x is not None:
-            k[bad] = x
-            v[bad] = x
-        out = up(ab, np.full(q.shape, 7.0), ab.BF16)
-        ab.prompt_attention(*(up(ab, t, ab.BF16) for t in (q, k, v)), out, cu, cu, 0.1, window)
-        got.append(down(ab, out))
-    return got
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    want, tol = prompt_by_hand(q, k, v, cu, cu, 0.1, window, False)
+    k[bad] = value
+    v[bad] = value
+    out = up(ab, np.full(q.shape, 7.0), ab.BF16)
+    cu = ab.DeviceArray.from_host(cu, ab.I32)
+    ab.prompt_attention(*(up(ab, t, ab.BF16) for t in (q, k, v)), out, cu, cu, 0.1, window)
+    got = down(ab, out)
+    with np.errstate(invalid="ignore"):
+        return got, np.abs(got - want) <= tol
 
 
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
@@ -527,18 +529,16 @@ def poisoned(ab, hd, lens, total, bad, window, value):
 def test_prompt_hidden_rows_do_not_reach_a_query(ab, hd, value):
     # a row in the middle of the second sequence: the queries before it, and the other sequences, do not see it
     lens, first = [130, 300, 40], 130
-    a, b = poisoned(ab, hd, lens, 470, [first + 150], 0, value)
-    assert np.array_equal(a[:first + 150], b[:first + 150]) and np.array_equal(a[430:], b[430:])
-    assert not np.isfinite(b[first + 150:430]).any() or value == -np.inf
-    if value != -np.inf:
-        assert np.isnan(b[first + 150:430]).all()
+    got, fine = poisoned(ab, hd, lens, 470, [first + 150], 0, value)
+    assert fine[:first + 150].all() and fine[430:].all()
+    # a query that sees it: NaN as soon as a score is NaN or +inf (inf · q has either sign: q·k is NaN for mixed signs)
+    assert np.isnan(got[first + 150:430]).all()
     # with a window the queries far behind it do not see it either
-    a, b = poisoned(ab, hd, lens, 470, [first + 20], 30, value)
-    keep = np.r_[0:first + 20, first + 50:470]
-    assert np.array_equal(a[keep], b[keep])
+    got, fine = poisoned(ab, hd, lens, 470, [first + 20], 30, value)
+    assert fine[np.r_[0:first + 20, first + 50:470]].all() and np.isnan(got[first + 20:first + 50]).all()
     # padding behind the last sequence, never written
-    a, b = poisoned(ab, hd, lens, 500, list(range(470, 500)), 0, value)
-    assert np.array_equal(a, b) and np.isfinite(b).all() and (b[470:] == 7).all()
+    got, fine = poisoned(ab, hd, lens, 500, list(range(470, 500)), 0, value)
+    assert fine[:470].all() and (got[470:] == 7).all()
 
 
 def test_prompt_outputs_may_be_strided(ab):
