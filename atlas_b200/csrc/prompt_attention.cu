@@ -3,13 +3,14 @@
 // 4 · hd flops and one exponential per visible (query, key) pair and head: at hd 128 a tile of 128 × 128 pairs is 1024 clocks of
 // tcgen05.mma and 1024 clocks of the SM's 16 exponentials a clock, so neither may wait for the other.
 //   * A CTA works on two query tiles of 128 rows with the same keys: the same rows of two heads that share a KV head, or — where the
-//     heads do not pair up — 256 consecutive rows of one head.  While four warps take the softmax of one tile the tensor core runs the
-//     products of the other.
-//   * S = Q·Kᵀ (128 × 128 f32) and O (128 × hd f32) live in tensor memory; the probabilities go back over the scores as 16-bit numbers
-//     and are the A operand of O += P·V straight from there.  V is the B operand as it lies in memory (rows of keys).
+//     heads do not pair up — 256 consecutive rows of one head.
+//   * S = Q·Kᵀ (f32) and O (128 × hd f32) live in tensor memory; the probabilities go back over the scores as 16-bit numbers and are
+//     the A operand of O += P·V straight from there.  V is the B operand as it lies in memory (rows of keys).
 //   * A thread owns a row: its maximum and sum need no exchange between lanes.  O is rescaled only when the running maximum has grown by
 //     more than 2^8 — sums are f32 and any reference between is exact — so the rescaling almost never runs.
-//   * K and V tiles come by tiled bulk copies through one ring of shared-memory stages: K0 V0 K1 V1 …
+//   * While the softmax of one query tile runs, the tensor core has the other's products.
+//   * A quarter of the exponentials goes to the FMA pipe (ex2_fma).
+//   * K and V tiles of 128 keys come by tiled bulk copies through one ring of shared-memory stages: K0 V0 K1 V1 …
 //   * Which sequence and rows a CTA owns it finds in the prefix array itself, late (long) row tiles first: nothing depends on host-side
 //     lengths, and a captured call follows the arrays.
 //   * A product of 0 and a NaN or infinity in a value row that the query does not see would be NaN: value rows behind the sequence are
@@ -24,8 +25,11 @@
 namespace {
 
 constexpr int kRows = 128;                        // rows of a query tile, keys of a K / V tile
+constexpr int kPart = 64;                         // keys whose probabilities are handed over at a time
 constexpr int kBoxBytes = kRows * 128;            // one box: 128 rows of 128 bytes
-constexpr int kThreads = 320;                     // warps 0..3, 4..7: softmax of tile 0, 1; 8: products; 9: copies
+constexpr int kThreads = 384;                     // warps 0..3, 4..7: softmax of tile 0, 1; 8: products; 9: copies; 10, 11 complete the
+                                                  // warpgroup that hands registers over
+constexpr int kProduct = 8, kCopy = 9;
 constexpr int kMaxStages = 6;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
@@ -56,56 +60,88 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 // Bounded wait.  false: gave up (this thread's deadline passed, or another role raised the abort flag).
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
     if (mbar_try(bar, parity)) return true;
-    unsigned spins = 0;
     unsigned long long t0 = 0;
-    while (!mbar_try(bar, parity)) {
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 256; i++)                                         // as few instructions as can be: waiting warps share the issue slots
+            if (mbar_try(bar, parity)) return true;
         if (*abort_flag) return false;
-        if ((++spins & 255u) == 0) {
-            const unsigned long long t = ax_globaltimer();
-            if (t0 == 0) t0 = t;
-            else if (t - t0 > kWaitNs) { *abort_flag = 1; atomicExch(err, code); return false; }
-        }
+        const unsigned long long t = ax_globaltimer();
+        if (t0 == 0) t0 = t;
+        else if (t - t0 > kWaitNs) { *abort_flag = 1; atomicExch(err, code); return false; }
     }
-    return true;
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
-// Shared-memory matrix descriptors, 128-byte swizzle (layout code 2, version 1), groups of eight rows of 128 bytes 1024 bytes apart.
-// K-major (rows hold the contracted index): the contracted index advances 32 bytes per step inside the row.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// Shared-memory matrix descriptors, 128-byte swizzle (layout code 2, version 1), groups of eight rows of 128 bytes 1024 bytes apart: the high
+// word is always the same, the low word holds the address and, for MN-major operands, how far the next 64 columns lie (one box).
+// Advancing is an addition to the low word — the thread that issues the products spent more time on descriptors than the tensor core
+// on the products when each was built from its address.
+//   K-major (rows hold the contracted index): 16 numbers further are 32 bytes inside the row.
+//   MN-major (rows are the contracted index, 64 columns each): 16 numbers further are 16 rows.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return (addr >> 4) | ((uint32_t)(kBoxBytes >> 4) << 16); }
+template <bool ACC> __device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "r"(b), "r"(idesc), "n"(ACC ? 1 : 0), "n"(kDescHigh) : "memory");
 }
-// MN-major (rows are the contracted index, 64 columns each): the next 64 columns lie one box further.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(kBoxBytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHigh) : "memory");
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
-}
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+// One lane of a converged warp.  The products are issued under this predicate, not under lane == 0: their descriptors live in uniform
+// registers, and only here does the compiler know that one thread runs (eight products: 600 clocks instead of 1000).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
 }
 #define AX_R32(m) m(0), m(1), m(2), m(3), m(4), m(5), m(6), m(7), m(8), m(9), m(10), m(11), m(12), m(13), m(14), m(15), \
                   m(16), m(17), m(18), m(19), m(20), m(21), m(22), m(23), m(24), m(25), m(26), m(27), m(28), m(29), m(30), m(31)
-// 32 columns of the warp's lane quarter; the values may be used after tmem_wait_ld
+// Columns of the warp's lane quarter.  The wait is part of the statement: the registers are written asynchronously, and a register that
+// the compiler moved or spilled between the load and its wait would be moved too early.
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
 #define AX_O(i) "=r"(r[i])
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : AX_R32(AX_O) : "r"(addr));
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;" : AX_R32(AX_O) : "r"(addr) : "memory");
 #undef AX_O
 }
-__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
-#define AX_O(i) "+r"(r[i])
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : AX_R32(AX_O) :: "memory");
+__device__ __forceinline__ void tmem_ld128(uint32_t addr, uint32_t* r) {
+#define AX_O(i) "=r"(r[i])
+#define AX_P(i) "=r"(r[32 + i])
+#define AX_Q(i) "=r"(r[64 + i])
+#define AX_S(i) "=r"(r[96 + i])
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, "
+                 "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
+                 "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;" : AX_R32(AX_O), AX_R32(AX_P), AX_R32(AX_Q), AX_R32(AX_S) : "r"(addr) : "memory");
 #undef AX_O
+#undef AX_P
+#undef AX_Q
+#undef AX_S
+}
+#define AX_R16(m) m(0), m(1), m(2), m(3), m(4), m(5), m(6), m(7), m(8), m(9), m(10), m(11), m(12), m(13), m(14), m(15)
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+#define AX_O(i) "=r"(r[i])
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;" : AX_R16(AX_O) : "r"(addr) : "memory");
+#undef AX_O
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+#define AX_I(i) "r"(r[i])
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+                 :: AX_R16(AX_I), "r"(addr) : "memory");
+#undef AX_I
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
 #define AX_I(i) "r"(r[i])
@@ -128,6 +164,30 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+// largest of three; NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+// 2^y for y ≤ 126 on the FMA pipe: y = n + f with |f| ≤ 1/2 by adding 1.5 · 2^23, a polynomial for 2^f, n added to the exponent.  The
+// coefficients are the minimax fit of the relative error over [−1/2, 1/2] (Lawson's iteration): 7.5e-5 with degree 3, 2.6e-6 with degree 4 —
+// a fiftieth of the half step of a bf16 number, a two-hundredth of an f16 number's.  Below 2^-126 it stays there.
+template <bool F16> __device__ __forceinline__ float2 ex2_fma(float2 y) {
+    y.x = fmaxf(y.x, -126.f); y.y = fmaxf(y.y, -126.f);
+    const float2 r = add2(y, make_float2(12582912.f, 12582912.f));
+    const float2 f = fma2(add2(r, make_float2(-12582912.f, -12582912.f)), make_float2(-1.f, -1.f), y);
+    float2 p;
+    if (F16) {
+        p = fma2(f, make_float2(0.009570102207f, 0.009570102207f), make_float2(0.05591786280f, 0.05591786280f));
+        p = fma2(p, f, make_float2(0.2402474433f, 0.2402474433f));
+        p = fma2(p, f, make_float2(0.6931217909f, 0.6931217909f));
+        p = fma2(p, f, make_float2(0.9999992847f, 0.9999992847f));
+    } else {
+        p = fma2(f, make_float2(0.05517166853f, 0.05517166853f), make_float2(0.2426111251f, 0.2426111251f));
+        p = fma2(p, f, make_float2(0.6932609677f, 0.6932609677f));
+        p = fma2(p, f, make_float2(0.9999280572f, 0.9999280572f));
+    }
+    p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23));
+    p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23));
+    return p;
+}
 template <bool F16> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     uint32_t r;
     if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -146,12 +206,12 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                                                                      const __grid_constant__ CUtensorMap map_v, const PromptDev dv) {
     using T = typename std::conditional<F16, __half, uint16_t>::type;
     constexpr int BOXES = HD / 64, TILE = BOXES * kBoxBytes, NS = HD == 128 ? 5 : 6;
-    constexpr uint32_t kS = 0, kO = 256;                                      // columns: scores of tile t at 128 t, output at 256 + HD t
+    constexpr uint32_t kS = 0, kO = 256;                                      // columns: scores of tile t at 128 t (its probabilities over the first half), output at 256 + HD t
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_ready[2], o_done[2], kv_full[kMaxStages], kv_empty[kMaxStages];
+    __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_ready[2][kRows / kPart], o_done[2], kv_full[kMaxStages], kv_empty[kMaxStages];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_issued, s_seq, s_tile, s_scan[kThreads / 32];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(AX_FULL, tid >> 5, 0), lane = tid & 31;
     const AxPromptArgs& a = dv.a;
     volatile int* abort_flag = &s_abort;
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -161,8 +221,8 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     const int tb = dv.pair_heads ? kRows : 2 * kRows;
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(smem_u32(&q_full[i]), 1); mbar_init(smem_u32(&s_full[i]), 1);
-            mbar_init(smem_u32(&p_ready[i]), kRows); mbar_init(smem_u32(&o_done[i]), 1);
+            mbar_init(smem_u32(&q_full[i]), 1); mbar_init(smem_u32(&s_full[i]), 1); mbar_init(smem_u32(&o_done[i]), 1);
+            for (int b = 0; b < kRows / kPart; b++) mbar_init(smem_u32(&p_ready[i][b]), kRows);
         }
         for (int i = 0; i < NS; i++) { mbar_init(smem_u32(&kv_full[i]), 1); mbar_init(smem_u32(&kv_empty[i]), 1); }
         s_abort = 0; s_issued = 0; s_seq = -1; s_tile = 0;
@@ -181,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         int at = inc - own, all = 0;
 #pragma unroll
         for (int w = 0; w < kThreads / 32; w++) { if (w < warp) at += s_scan[w]; all += s_scan[w]; }
-        const int x = all - 1 - (int)blockIdx.x;
+        const int x = all - 1 - (int)blockIdx.y;
         if (x < 0) return;
         if (x >= at && x < at + own)
             for (int b = b0; b < b1; b++) {
@@ -190,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 at += n;
             }
     }
-    if (warp == 8) {
+    if (warp == kProduct) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -200,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     const uint32_t tmem = s_tmem;
     const AxPromptSeq s = ax_prompt_seq(a, s_seq);
     const int off = s.lk - s.lq;
-    const int h0 = dv.pair_heads ? 2 * (int)blockIdx.y : (int)blockIdx.y, kh = h0 / (a.n_heads / a.n_kv);
+    const int h0 = dv.pair_heads ? 2 * (int)blockIdx.x : (int)blockIdx.x, kh = h0 / (a.n_heads / a.n_kv);
     int base[2], lo[2], hi[2];                                                // first row and K / V tiles [lo, hi] of both query tiles
     base[0] = s_tile * tb; base[1] = dv.pair_heads ? base[0] : base[0] + kRows;
 #pragma unroll
@@ -215,7 +275,10 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     const bool on0 = hi[0] >= lo[0], on1 = hi[1] >= lo[1];
     const int j0 = on0 ? (on1 ? min(lo[0], lo[1]) : lo[0]) : lo[1], j1 = max(hi[0], hi[1]);      // j1 < j0: no tile at all
 
-    if (warp == 9) {
+    // 384 threads start with 168 registers each (64512 in all); a row of scores is 128 of them.  256 · 208 + 128 · 80 = 63488.
+    if (warp >= kProduct) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == kCopy) {
         if (lane == 0) {
             for (int t = 0; t < 2; t++)
                 if (t ? on1 : on0) {
@@ -235,27 +298,28 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 s_issued = i + 1;
             }
         }
-    } else if (warp == 8) {
+    } else if (warp == kProduct) {
         constexpr uint32_t fmt = F16 ? 0u : 1u;                               // accumulator f32, A and B f16 or bf16; B of P·V is MN-major
         constexpr uint32_t id_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kRows >> 3) << 17) | ((kRows >> 4) << 24);
         constexpr uint32_t id_pv = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((HD >> 3) << 17) | ((kRows >> 4) << 24);
         int np[2] = { 0, 0 };                                                 // P tiles taken
         bool ok = true;
         auto qk = [&](int t, int j) {                                         // scores of query tile t with K tile j
-            const uint32_t k = ring + (uint32_t)((2 * (j - j0)) % NS) * TILE, q = smem0 + t * TILE;
-            if (lane == 0) {
+            const uint32_t k = desc_k(ring + (uint32_t)((2 * (j - j0)) % NS) * TILE), q = desc_k(smem0 + t * TILE), d = tmem + kS + t * 128;
+            if (elect_one()) {
+                umma_ss<false>(d, q, k, id_qk);
 #pragma unroll
-                for (int i = 0; i < HD / 16; i++)
-                    umma_ss(tmem + kS + t * 128, desc_k(q + (i / 4) * kBoxBytes + (i % 4) * 32), desc_k(k + (i / 4) * kBoxBytes + (i % 4) * 32), id_qk, i != 0);
+                for (int i = 1; i < HD / 16; i++)
+                    umma_ss<true>(d, q + (i / 4) * (kBoxBytes >> 4) + (i % 4) * 2, k + (i / 4) * (kBoxBytes >> 4) + (i % 4) * 2, id_qk);
                 umma_commit(smem_u32(&s_full[t]));
             }
         };
         auto full = [&](int i) { return mbar_wait(smem_u32(&kv_full[i % NS]), (uint32_t)(i / NS) & 1u, abort_flag, dv.err, 722); };
-        auto release = [&](int i) { if (lane == 0) umma_commit(smem_u32(&kv_empty[i % NS])); };
+        auto release = [&](int i) { if (elect_one()) umma_commit(smem_u32(&kv_empty[i % NS])); };
         if (j1 >= j0) {
             ok = full(0);
             for (int t = 0; t < 2 && ok; t++)
-                if ((t ? on1 : on0)) {
+                if (t ? on1 : on0) {
                     ok = mbar_wait(smem_u32(&q_full[t]), 0, abort_flag, dv.err, 723);
                     if (ok && lo[t] == j0) qk(t, j0);
                 }
@@ -263,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         }
         for (int j = j0; j <= j1 && ok; j++) {
             const int vi = 2 * (j - j0) + 1, ki = vi + 1;
-            const uint32_t v = ring + (uint32_t)(vi % NS) * TILE;
+            const uint32_t v = ring + (uint32_t)(vi % NS) * TILE, vd = desc_mn(v);
             ok = full(vi);
             if (!ok) break;
             const int valid = s.lk - j * kRows;
@@ -275,27 +339,38 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
-            if (j < j1) { ok = full(ki); if (!ok) break; }
             for (int t = 0; t < 2; t++) {
                 if (j >= lo[t] && j <= hi[t]) {
-                    ok = mbar_wait(smem_u32(&p_ready[t]), (uint32_t)np[t] & 1u, abort_flag, dv.err, 724);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (lane == 0) {
 #pragma unroll
-                        for (int i = 0; i < kRows / 16; i++)
-                            umma_ts(tmem + kO + t * HD, tmem + kS + t * 128 + i * 8, desc_mn(v + i * 2048), id_pv, (np[t] | i) != 0);
-                        umma_commit(smem_u32(&o_done[t]));
+                    for (int part = 0; part < kRows / kPart && ok; part++) {  // the product starts with the first probabilities
+                        ok = mbar_wait(smem_u32(&p_ready[t][part]), (uint32_t)np[t] & 1u, abort_flag, dv.err, 724);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (elect_one()) {
+#pragma unroll
+                            for (int e = 0; e < kPart / 16; e++) {
+                                const int i = part * (kPart / 16) + e;
+                                umma_ts(tmem + kO + t * HD, tmem + kS + t * 128 + i * 8, vd + i * (2048 >> 4), id_pv, i ? 1u : (uint32_t)(np[t] != 0));
+                            }
+                            if (part == kRows / kPart - 1) umma_commit(smem_u32(&o_done[t]));
+                        }
                     }
+                    if (!ok) break;
                     np[t]++;
                 }
-                if (j + 1 >= lo[t] && j + 1 <= hi[t]) qk(t, j + 1);
+                if (j + 1 >= lo[t] && j + 1 <= hi[t]) {
+                    ok = full(ki);
+                    if (!ok) break;
+                    qk(t, j + 1);
+                }           // over the scores and probabilities just used
             }
             if (!ok) break;
             release(vi);
             if (j < j1) release(ki);
         }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int t = warp >> 2;
         const int r = (warp & 3) * 32 + lane, row = base[t] + r, pos = row + off;         // row of the sequence, key at its own position
         const int h = dv.pair_heads ? h0 + t : h0;
@@ -312,25 +387,27 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             ok = mbar_wait(smem_u32(&s_full[t]), (uint32_t)it & 1u, abort_flag, dv.err, 725);
             if (!__all_sync(AX_FULL, ok)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t u[128];
-#pragma unroll
-            for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, u + 32 * c);
-#pragma unroll
-            for (int c = 0; c < 4; c++) tmem_wait_ld(u + 32 * c);
+            uint32_t u[kRows];
+            tmem_ld128(ts, u);
             float* x = reinterpret_cast<float*>(u);
             if (dv.negate) {
 #pragma unroll
-                for (int c = 0; c < 128; c++) x[c] = -x[c];
+                for (int c = 0; c < kRows; c++) x[c] = -x[c];
             }
             const int k0 = j * kRows;
-            if (k0 + kRows - 1 > first || (a.window > 0 && k0 <= lastp - a.window)) {      // some row of the tile does not see all keys
+            const bool edge = k0 + kRows - 1 > first || (a.window > 0 && k0 <= lastp - a.window);      // some row of the tile does not see all keys
+            if (edge) {
 #pragma unroll
-                for (int c = 0; c < 128; c++) if (k0 + c > key_hi || k0 + c <= key_lo) x[c] = -INFINITY;
+                for (int c = 0; c < kRows; c++) if (k0 + c > key_hi || k0 + c <= key_lo) x[c] = -INFINITY;
             }
-            float mx[4] = { x[0], x[1], x[2], x[3] };
+            float mx[8];
 #pragma unroll
-            for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            for (int c = 0; c < 8; c++) mx[c] = x[c];
+#pragma unroll
+            for (int c = 8; c < 120; c += 2) mx[(c >> 1) & 7] = max3(mx[(c >> 1) & 7], x[c], x[c + 1]);
+            const float top = max3(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], x[120])),
+                                   max3(x[121], x[122], x[123]), max3(max3(x[124], x[125], x[126]), x[127], x[127]));
+            if (top != top) m = top;                                          // the row is taken again
             const bool grow = top > m && (m == -INFINITY || (top - m) * sc > 8.f);
             if (__any_sync(AX_FULL, grow)) {
                 const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * sc);
@@ -341,34 +418,37 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                     if (!__all_sync(AX_FULL, ok)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(to + c, o);
-                        tmem_wait_ld(o);
+                    for (int c = 0; c < HD; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(to + c, o);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st32(to + c, o);
+                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st16(to + c, o);
                     }
-                    tmem_wait_st();
                 }
             }
             const float neg = m == -INFINITY ? 0.f : -m * sc;
             const float2 sc2 = make_float2(sc, sc), neg2 = make_float2(neg, neg);
+            // Where keys are hidden every exponential is exact, so that what is hidden is zero.
+            auto probs = [&](bool all) {
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                uint32_t p[32];
+                for (int part = 0; part < kRows / kPart; part++) {
+                    uint32_t p[kPart / 2];
 #pragma unroll
-                for (int c = 0; c < 32; c++) {
-                    float2 y = fma2(make_float2(x[64 * half + 2 * c], x[64 * half + 2 * c + 1]), sc2, neg2);
-                    y.x = ex2(y.x); y.y = ex2(y.y);
-                    if (c & 1) l1 = add2(l1, y); else l0 = add2(l0, y);
-                    p[c] = pack<F16>(y.x, y.y);
+                    for (int c = 0; c < kPart / 2; c++) {
+                        float2 y = fma2(make_float2(x[kPart * part + 2 * c], x[kPart * part + 2 * c + 1]), sc2, neg2);
+                        if (!all && (c & 3) >= 4) y = ex2_fma<F16>(y);
+                        else { y.x = ex2(y.x); y.y = ex2(y.y); }
+                        if (c & 1) l1 = add2(l1, y); else l0 = add2(l0, y);
+                        p[c] = pack<F16>(y.x, y.y);
+                    }
+                    tmem_st32(ts + (kPart / 2) * part, p);
+                    tmem_wait_st();
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    mbar_arrive(smem_u32(&p_ready[t][part]));
                 }
-                tmem_st32(ts + 32 * half, p);
-            }
-            tmem_wait_st();
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            mbar_arrive(smem_u32(&p_ready[t]));
+            };
+            if (edge) probs(true); else probs(false);
         }
         // ── output ──
         const int tiles = j_hi - j_lo + 1;
@@ -388,7 +468,6 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 uint32_t o[32];
                 if (tiles > 0) {
                     tmem_ld32(to + c, o);
-                    tmem_wait_ld(o);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = 0u;
@@ -406,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 }
             }
             const bool sees = key_hi >= 0 && s.lk > 0;
-            unsigned again = __ballot_sync(AX_FULL, live && (odd != odd || (l == 0.f && sees)));
+            unsigned again = __ballot_sync(AX_FULL, live && (odd != odd || (sees && !(fabsf(m) <= 3.402823466e38f))));
             __syncwarp();
             while (again) {
                 const int i = __ffs(again) - 1;
@@ -437,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         }
         __syncthreads();
     }
-    if (warp == 8) {
+    if (warp == kProduct) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
     }
@@ -480,7 +559,7 @@ int launch(atlasx_ctx* ctx, const PromptDev& dv, const CUtensorMap& q, const CUt
     const int tb = dv.pair_heads ? kRows : 2 * kRows;
     // at most one unfilled tile per sequence, and no more sequences with rows than rows
     const long long tiles = (long long)dv.a.n_q / tb + (dv.a.batch < dv.a.n_q ? dv.a.batch : dv.a.n_q);
-    ax_prompt_umma_kernel<F16, HD><<<dim3((unsigned)tiles, (unsigned)(dv.pair_heads ? dv.a.n_heads / 2 : dv.a.n_heads)), kThreads, smem, ctx->stream>>>(q, k, v, dv);
+    ax_prompt_umma_kernel<F16, HD><<<dim3((unsigned)(dv.pair_heads ? dv.a.n_heads / 2 : dv.a.n_heads), (unsigned)tiles), kThreads, smem, ctx->stream>>>(q, k, v, dv);
     AX_CHECK_LAUNCH("ax_prompt_umma_kernel");
     return ATLASX_OK;
 }
