@@ -6,6 +6,7 @@ fallback — if the library is missing or no CUDA device is present, calls raise
 """
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libatlas_kernels.so")
@@ -49,9 +50,15 @@ class LoadStatsC(C.Structure):
 TOKEN_CALLBACK = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint32)
 LAYER_HOOK = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.POINTER(C.c_float), C.c_int, C.POINTER(C.c_float))
 
+# argument structs of the packed serving calls, packed to bytes (the same layout as in include/atlas_kernels.h)
+PAGE_PLAN = struct.Struct("@9P6i")
+PAGED_ROWS = struct.Struct("@3P4q2i")
+PAGED_ATTN = struct.Struct("@5PN4if")
+PROMPT = struct.Struct("@4P8q2P8if")
+
 _lib = None
 
-vp, sz, u64, ci, cf, ll = C.c_void_p, C.c_size_t, C.c_uint64, C.c_int, C.c_float, C.c_longlong
+vp, sz, u64, ci, cf, cp = C.c_void_p, C.c_size_t, C.c_uint64, C.c_int, C.c_float, C.c_char_p
 pvp = C.POINTER(C.c_void_p)
 pi = C.POINTER(C.c_int)
 
@@ -127,15 +134,15 @@ SIGNATURES = {
     "atlasx_decode_attention": (ci, [vp, vp, vp, vp, ci, vp, cf, ci]),
     "atlasx_decode_attention_bytes": (sz, [vp, ci, vp, ci]),
     "atlasx_decode_attention_static": (ci, [vp, ci, vp, vp, ci, ci, ci, ci, vp, vp, ci, vp, cf, ci]),
-    "atlasx_page_plan": (ci, [vp, vp, vp, ci, vp, ci, ci, ci, vp, ci, vp, vp, vp, vp, ci, vp]),
+    "atlasx_page_plan": (ci, [vp, cp]),
     "atlasx_pagedkv_create": (ci, [vp, ci, ci, ci, ci, ci, pvp]),
     "atlasx_pagedkv_free": (ci, [vp]),
     "atlasx_pagedkv_bytes": (sz, [ci, ci, ci, ci, ci]),
     "atlasx_pagedkv_ptrs": (ci, [vp, pvp, C.POINTER(sz), C.POINTER(sz)]),
-    "atlasx_pagedkv_append": (ci, [vp, vp, ci, vp, ll, ll, vp, ll, ll, vp, ci]),
+    "atlasx_pagedkv_append": (ci, [vp, vp, cp]),
     "atlasx_pagedkv_read": (ci, [vp, vp, vp, ci, ci, vp, vp]),
-    "atlasx_pagedkv_decode_attention": (ci, [vp, vp, vp, vp, ci, vp, ci, vp, ci, cf, ci, vp, sz]),
-    "atlasx_prompt_attention": (ci, [vp, ci, vp, ll, ll, vp, ll, ll, vp, ll, ll, vp, ll, ll, vp, vp, ci, ci, ci, ci, ci, ci, cf, ci]),
+    "atlasx_pagedkv_decode_attention": (ci, [vp, vp, cp]),
+    "atlasx_prompt_attention": (ci, [vp, cp]),
     "atlasx_model_create": (ci, [vp, C.POINTER(ModelConfigC), vp, pvp]),
     "atlasx_model_free": (ci, [vp]),
     "atlasx_model_set_tensor": (ci, [vp, ci, ci, vp, ci, ci]),

@@ -264,9 +264,11 @@ int elem_bytes(int dtype) { return dtype == ATLASX_F32 ? 4 : 2; }
 
 }  // namespace
 
-extern "C" int atlasx_page_plan(atlasx_ctx* c, const int* cached, const int* fresh, int batch, const int* free_pages, int n_free,
-                                int page_size, int n_pages, int* table, int table_width, int* cu, int* lens, int* slots, int* pos,
-                                int n_tokens, int* status) {
+extern "C" int atlasx_page_plan(atlasx_ctx* c, const atlasx_page_plan_args* p) {
+    AX_ARG(p, "null argument");
+    const int *cached = p->cached, *fresh = p->fresh, *free_pages = p->free_pages;
+    int *table = p->table, *cu = p->cu, *lens = p->lens, *slots = p->slots, *pos = p->pos, *status = p->status;
+    const int batch = p->batch, n_free = p->n_free, page_size = p->page_size, n_pages = p->n_pages, table_width = p->table_width, n_tokens = p->n_tokens;
     AX_ARG(cached && fresh && table && cu && lens && status, "null argument");
     AX_ARG(batch >= 1 && batch <= AX_PAGED_MAX_BATCH, "batch must be in 1..4096");
     AX_ARG(page_size >= 1 && n_pages >= 1 && (long long)page_size * n_pages <= 0x7FFFFFFFll, "page_size · n_pages must be in 1..2^31 - 1");
@@ -336,9 +338,11 @@ extern "C" int atlasx_pagedkv_ptrs(atlasx_pagedkv* kv, void** pool, size_t* byte
     return ATLASX_OK;
 }
 
-extern "C" int atlasx_pagedkv_append(atlasx_ctx* c, atlasx_pagedkv* kv, int dtype, const void* k, long long k_token_stride,
-                                     long long k_head_stride, const void* v, long long v_token_stride, long long v_head_stride,
-                                     const int* slots, int n) {
+extern "C" int atlasx_pagedkv_append(atlasx_ctx* c, atlasx_pagedkv* kv, const atlasx_pagedkv_rows* p) {
+    AX_ARG(p, "null argument");
+    const int dtype = p->dtype, n = p->n, *slots = p->slots;
+    const void *k = p->k, *v = p->v;
+    const long long k_token_stride = p->k_token_stride, k_head_stride = p->k_head_stride, v_token_stride = p->v_token_stride, v_head_stride = p->v_head_stride;
     AX_ARG(dtype == ATLASX_F32 || dtype == ATLASX_BF16 || dtype == ATLASX_F16, "dtype must be f32, bf16 or f16");
     AX_ARG(n >= 0, "the number of rows must not be negative");
     if (n == 0) return ATLASX_OK;
@@ -383,9 +387,14 @@ extern "C" int atlasx_pagedkv_read(atlasx_ctx* c, const atlasx_pagedkv* kv, cons
     return ATLASX_OK;
 }
 
-extern "C" int atlasx_pagedkv_decode_attention(atlasx_ctx* c, const atlasx_pagedkv* kv, const float* q, float* out, int n_heads,
-                                               const int* table, int table_width, const int* lens, int batch, float scale,
-                                               int window, void* workspace, size_t workspace_bytes) {
+extern "C" int atlasx_pagedkv_decode_attention(atlasx_ctx* c, const atlasx_pagedkv* kv, const atlasx_pagedkv_attn_args* p) {
+    AX_ARG(p, "null argument");
+    const float* q = p->q;
+    float* out = p->out;
+    const int *table = p->table, *lens = p->lens, n_heads = p->n_heads, table_width = p->table_width, batch = p->batch, window = p->window;
+    const float scale = p->scale;
+    void* workspace = p->workspace;
+    const size_t workspace_bytes = p->workspace_bytes;
     AX_ARG(q && out && table && lens, "null argument");
     AX_ARG(batch >= 1 && batch <= AX_PAGED_MAX_BATCH, "batch must be in 1..4096");
     AX_ARG(n_heads >= 1, "n_heads must be positive");

@@ -552,10 +552,15 @@ int launch(atlasx_ctx* ctx, const PromptDev& dv, const CUtensorMap& q, const CUt
 
 }  // namespace
 
-extern "C" int atlasx_prompt_attention(atlasx_ctx* c, int dtype, const void* q, long long q_tok, long long q_head,
-                                       const void* k, long long k_tok, long long k_head, const void* v, long long v_tok, long long v_head,
-                                       void* out, long long o_tok, long long o_head, const int* cu_q, const int* cu_k, int batch,
-                                       int n_q, int n_k, int n_heads, int n_kv, int hd, float scale, int window) {
+extern "C" int atlasx_prompt_attention(atlasx_ctx* c, const atlasx_prompt_args* p) {
+    AX_ARG(p, "null argument");
+    const void *q = p->q, *k = p->k, *v = p->v;
+    void* out = p->out;
+    const long long q_tok = p->q_token_stride, q_head = p->q_head_stride, k_tok = p->k_token_stride, k_head = p->k_head_stride,
+                    v_tok = p->v_token_stride, v_head = p->v_head_stride, o_tok = p->out_token_stride, o_head = p->out_head_stride;
+    const int *cu_q = p->cu_q, *cu_k = p->cu_k, dtype = p->dtype, batch = p->batch, n_q = p->n_q, n_k = p->n_k, n_heads = p->n_heads,
+              n_kv = p->n_kv_heads, hd = p->head_dim, window = p->window;
+    const float scale = p->scale;
     AX_ARG(dtype == ATLASX_BF16 || dtype == ATLASX_F16, "dtype must be bf16 or f16");
     AX_ARG(batch >= 1 && batch <= AX_PAGED_MAX_BATCH, "batch must be in 1..4096");
     AX_ARG(n_q >= 0 && n_k >= 0, "row counts must not be negative");

@@ -1,8 +1,8 @@
 """A packed serving step over the C ABI: block tables and slots from request lengths (page_plan), the four-bit paged KV cache
 (PagedKvCache) and the causal attention of whole packed prompts (prompt_attention).
 
-The calls take device arrays: a DeviceArray of this module, or anything with data_ptr(), shape, stride(), dtype and device as a
-PyTorch tensor has them (PyTorch itself is not imported).  They run on the context's stream and return at once; arrays that another
+The calls take device arrays: a DeviceArray of this module, or anything with data_ptr(), shape, stride(),
+is_contiguous(), dtype and get_device() as a PyTorch tensor has them (PyTorch itself is not imported).  They run on the context's stream and return at once; arrays that another
 stream fills have to be ordered before them (`Context.stream`), and arrays must live until the stream has passed the call.
 """
 import ctypes as C
@@ -46,13 +46,17 @@ class DeviceArray:
             out.ctx.upload(out.ptr, a)
         return out
 
+    def is_contiguous(self):
+        n = 1
+        for m, s in zip(reversed(self.shape), reversed(self.strides)):
+            if m > 1 and s != n:
+                return False
+            n *= m
+        return True
+
     def download(self):
         """The values of a contiguous array."""
-        n, strides = 1, []
-        for m in reversed(self.shape):
-            strides.insert(0, n)
-            n *= m
-        if n and any(m > 1 and s != t for m, s, t in zip(self.shape, self.strides, strides)):
+        if not self.is_contiguous():
             raise AtlasError("download needs a contiguous array")
         return self.ctx.download(self.ptr, self.shape, _NUMPY[self.dtype])
 
@@ -69,14 +73,25 @@ class DeviceArray:
         self.ptr = 0
 
 
-def _view(x, name, dtypes, ndim, device):
-    """(ptr, shape, strides, dtype) of a device array, checked."""
+_CODES = {}      # dtype objects of other libraries seen so far → codes
+
+
+def _code(dtype):
+    c = _CODES.get(dtype)
+    if c is None:
+        c = _NAMES.get(str(dtype), -1)
+        _CODES[dtype] = c
+    return c
+
+
+def _refuse(x, name, dtypes, ndim, device):
+    """Says what is wrong with an array that did not pass."""
     if type(x) is DeviceArray:
-        ptr, shape, strides, dtype, at = x.ptr, x.shape, x.strides, x.dtype, x.ctx.device
+        shape, dtype, at = x.shape, x.dtype, x.ctx.device
     else:
         try:
-            ptr, shape, strides, dtype, at = x.data_ptr(), x.shape, x.stride(), _NAMES.get(str(x.dtype)), x.device
-            at = at.index if at.type == "cuda" else -1
+            shape, dtype, at = x.shape, _code(x.dtype), x.get_device()
+            x.data_ptr, x.stride
         except AttributeError:
             raise AtlasError("%s is not a device array" % name) from None
     if dtype not in dtypes:
@@ -85,30 +100,46 @@ def _view(x, name, dtypes, ndim, device):
         raise AtlasError("%s must have %d dimensions, not %d" % (name, ndim, len(shape)))
     if at != device:
         raise AtlasError("%s is not on device %d" % (name, device))
-    return ptr, shape, strides, dtype
 
 
 def _ints(x, name, shape, device):
     """Pointer of a contiguous int32 array; None in `shape` stands for any extent."""
-    ptr, got, strides, _ = _view(x, name, (I32,), len(shape), device)
-    n = 1
-    for i in range(len(shape) - 1, -1, -1):
-        if shape[i] is not None and got[i] != shape[i]:
+    try:
+        if type(x) is DeviceArray:
+            ptr, got, fine = x.ptr, x.shape, x.dtype is I32 and x.ctx.device == device
+            whole = x.is_contiguous()
+        else:
+            ptr, got, whole, fine = x.data_ptr(), x.shape, x.is_contiguous(), _code(x.dtype) is I32 and x.get_device() == device
+    except AttributeError:
+        fine = False
+    if not fine or len(got) != len(shape):
+        _refuse(x, name, (I32,), len(shape), device)
+    for m, n in zip(shape, got):
+        if m is not None and m != n:
             raise AtlasError("%s must have shape %s, not %s" % (name, tuple(shape), tuple(got)))
-        if got[i] > 1 and strides[i] != n:
-            raise AtlasError("%s must be contiguous" % name)
-        n *= got[i]
+    if not whole:
+        raise AtlasError("%s must be contiguous" % name)
     return ptr
 
 
 def _rows(x, name, dtypes, device, heads=None, head_dim=None):
     """(ptr, rows, token stride, head stride, dtype, heads, head_dim) of [rows, heads, head_dim] with unit stride along a row."""
-    ptr, shape, strides, dtype = _view(x, name, dtypes, 3, device)
-    if (heads is not None and shape[1] != heads) or (head_dim is not None and shape[2] != head_dim):
+    try:
+        if type(x) is DeviceArray:
+            ptr, shape, strides, dtype, at = x.ptr, x.shape, x.strides, x.dtype, x.ctx.device
+        else:
+            ptr, shape, strides, dtype, at = x.data_ptr(), x.shape, x.stride(), _code(x.dtype), x.get_device()
+        fine = dtype in dtypes and len(shape) == 3 and at == device
+    except AttributeError:
+        fine = False
+    if not fine:
+        _refuse(x, name, dtypes, 3, device)
+    n, h, d = shape
+    if (heads is not None and h != heads) or (head_dim is not None and d != head_dim):
         raise AtlasError("%s must be [rows, %s, %s], not %s" % (name, heads, head_dim, tuple(shape)))
-    if shape[2] > 1 and strides[2] != 1:
+    if d > 1 and strides[2] != 1:
         raise AtlasError("%s must have unit stride along head_dim" % name)
-    return ptr, shape[0], strides[0], strides[1], dtype, shape[1], shape[2]
+    return ptr, n, strides[0], strides[1], dtype, h, d
 
 
 def _contiguous(view, name):
@@ -123,19 +154,26 @@ def _device(ctx, x):
     return ctx.device if ctx is not None else (x.ctx.device if type(x) is DeviceArray else 0)
 
 
+def _whole(x, name, limit=0x7FFFFFFF):
+    """An int argument that a C int can hold."""
+    if not -limit - 1 <= x <= limit:
+        raise AtlasError("%s is out of range" % name)
+    return x
+
+
 def page_plan(cached, fresh, free_pages, table, cu, lens, slots, pos, status, page_size, n_pages, ctx=None):
     """Block tables, slots and positions of a step from request lengths: see atlasx_page_plan.  int32 device arrays: cached, fresh,
     lens [batch]; free_pages [any]; table [batch, width], extended in place; cu [batch + 1]; slots, pos [rows]; status [3]."""
     dev = _device(ctx, cached)
-    p_cached, shape, _, _ = _view(cached, "cached", (I32,), 1, dev)
-    b, rows = shape[0], slots.shape[0]
-    p_cached = _ints(cached, "cached", (b,), dev)
-    p = (_ints(fresh, "fresh", (b,), dev), _ints(free_pages, "free_pages", (None,), dev), _ints(table, "table", (b, None), dev),
-         _ints(cu, "cu", (b + 1,), dev), _ints(lens, "lens", (b,), dev), _ints(slots, "slots", (rows,), dev), _ints(pos, "pos", (rows,), dev),
-         _ints(status, "status", (3,), dev))
-    ctx = ctx or Context.default()
-    check(_ffi.lib().atlasx_page_plan(ctx.handle, p_cached, p[0], b, p[1], free_pages.shape[0], page_size, n_pages, p[2], table.shape[1],
-                                      p[3], p[4], p[5], p[6], rows, p[7]))
+    p_cached = _ints(cached, "cached", (None,), dev)
+    b = cached.shape[0]
+    p_slots = _ints(slots, "slots", (None,), dev)
+    rows = slots.shape[0]
+    args = _ffi.PAGE_PLAN.pack(
+        p_cached, _ints(fresh, "fresh", (b,), dev), _ints(free_pages, "free_pages", (None,), dev), _ints(table, "table", (b, None), dev),
+        _ints(cu, "cu", (b + 1,), dev), _ints(lens, "lens", (b,), dev), p_slots, _ints(pos, "pos", (rows,), dev),
+        _ints(status, "status", (3,), dev), b, free_pages.shape[0], _whole(page_size, "page_size"), _whole(n_pages, "n_pages"), table.shape[1], rows)
+    check(_ffi.lib().atlasx_page_plan((ctx or Context.default()).handle, args))
 
 
 class PagedKvCache:
@@ -167,7 +205,8 @@ class PagedKvCache:
         vp, m, vt, vh, dv, _, _ = _rows(v, "v", types, dev, self.n_kv_heads, self.head_dim)
         if n != m or dt != dv:
             raise AtlasError("k and v must have the same rows and type")
-        check(_ffi.lib().atlasx_pagedkv_append(self.ctx.handle, self._h, dt, kp, kt, kh, vp, vt, vh, _ints(slots, "slots", (n,), dev), n))
+        check(_ffi.lib().atlasx_pagedkv_append(self.ctx.handle, self._h,
+                                               _ffi.PAGED_ROWS.pack(kp, vp, _ints(slots, "slots", (n,), dev), kt, kh, vt, vh, dt, n)))
 
     def read(self, slots, k_out, v_out):
         """The values that the slots hold into contiguous [rows, n_kv_heads, head_dim] arrays (f32, bf16 or f16)."""
@@ -186,9 +225,11 @@ class PagedKvCache:
         op = _contiguous(_rows(out, "out", (F32,), dev, nh, self.head_dim), "out")
         if op[1] != b:
             raise AtlasError("out must have the rows of q")
-        wp, wn = (None, 0) if workspace is None else (_ints(workspace, "workspace", (None,), dev), 4 * workspace.shape[0])
-        check(_ffi.lib().atlasx_pagedkv_decode_attention(self.ctx.handle, self._h, qp, op[0], nh, _ints(table, "table", (b, None), dev),
-                                                         table.shape[1], _ints(lens, "lens", (b,), dev), b, scale, window_size, wp, wn))
+        wp, wn = (0, 0) if workspace is None else (_ints(workspace, "workspace", (None,), dev), 4 * workspace.shape[0])
+        p_table = _ints(table, "table", (b, None), dev)
+        check(_ffi.lib().atlasx_pagedkv_decode_attention(
+            self.ctx.handle, self._h, _ffi.PAGED_ATTN.pack(qp, op[0], p_table, _ints(lens, "lens", (b,), dev), wp, wn, nh, table.shape[1], b,
+                                                           _whole(window_size, "window_size"), scale)))
 
     def __del__(self):
         try:
@@ -211,10 +252,8 @@ def prompt_attention(q, k, v, out, cu_q, cu_k, scale=None, window_size=0, ctx=No
         raise AtlasError("k and v, and q and out, must have the same rows")
     if not dt == dk == dv == do:
         raise AtlasError("q, k, v and out must have the same type")
-    cp, shape, _, _ = _view(cu_q, "cu_q", (I32,), 1, dev)
-    b = shape[0] - 1
-    cp = _ints(cu_q, "cu_q", (b + 1,), dev)
-    cq = _ints(cu_k, "cu_k", (b + 1,), dev)
-    ctx = ctx or Context.default()
-    check(_ffi.lib().atlasx_prompt_attention(ctx.handle, dt, qp, qt, qh, kp, kt, kh, vp, vt, vh, op, ot, oh, cp, cq, b, n, m, nh, nk, hd,
-                                             1.0 / math.sqrt(hd) if scale is None else scale, window_size))
+    p_cu_q = _ints(cu_q, "cu_q", (None,), dev)
+    b = cu_q.shape[0] - 1
+    args = _ffi.PROMPT.pack(qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, p_cu_q, _ints(cu_k, "cu_k", (b + 1,), dev), dt, b, n, m, nh, nk, hd,
+                            _whole(window_size, "window_size"), 1.0 / math.sqrt(hd) if scale is None else scale)
+    check(_ffi.lib().atlasx_prompt_attention((ctx or Context.default()).handle, args))

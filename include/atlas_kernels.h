@@ -209,9 +209,14 @@ int atlasx_decode_attention_static(void* stream, int kv_dtype, const void* k_dev
  * its position in the request; rows from cu[batch] to n_tokens get −1 in both.  status[3]: pages taken, pages missing, requests
  * with lengths that are negative or wider than the table (one more if the new rows are more than n_tokens).  Where either of the
  * last two is not zero nothing is planned: the table stays, cu and lens are 0, slots and pos −1. */
-int atlasx_page_plan(atlasx_ctx* ctx, const int* cached_dev, const int* fresh_dev, int batch, const int* free_pages_dev, int n_free,
-                     int page_size, int n_pages, int* table_dev, int table_width, int* cu_dev, int* lens_dev, int* slots_dev,
-                     int* pos_dev, int n_tokens, int* status_dev);
+typedef struct {
+    const int *cached, *fresh;                    /* [batch] */
+    const int* free_pages;                        /* [n_free] */
+    int* table;                                   /* [batch][table_width] */
+    int *cu, *lens, *slots, *pos, *status;        /* [batch + 1], [batch], [n_tokens], [n_tokens], [3] */
+    int batch, n_free, page_size, n_pages, table_width, n_tokens;
+} atlasx_page_plan_args;
+int atlasx_page_plan(atlasx_ctx* ctx, const atlasx_page_plan_args* args);
 
 /* Paged KV cache in four bits: n_pages pages of page_size rows (a multiple of 16), head_dim 64 or 128.  `group` (32 or 64)
  * consecutive numbers of a row of a head share a bf16 scale = bf16(max|x| / 7), 1.0 below the smallest normal number; the number is
@@ -226,9 +231,13 @@ int atlasx_pagedkv_ptrs(atlasx_pagedkv* kv, void** pool_dev, size_t* bytes, size
 /* Rows of K and V [n][n_kv_heads][head_dim], f32, bf16 or f16, strides in elements, every row on a 16-byte boundary, into their
  * slots.  A negative slot marks a row that is not there; one behind the pool is left out and raises the device error word
  * (atlasx_ctx_poll_device_error).  Slots of one call are distinct. */
-int atlasx_pagedkv_append(atlasx_ctx* ctx, atlasx_pagedkv* kv, int dtype, const void* k_dev, long long k_token_stride,
-                          long long k_head_stride, const void* v_dev, long long v_token_stride, long long v_head_stride,
-                          const int* slots_dev, int n);
+typedef struct {
+    const void *k, *v;
+    const int* slots;                             /* [n] */
+    long long k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int dtype, n;
+} atlasx_pagedkv_rows;
+int atlasx_pagedkv_append(atlasx_ctx* ctx, atlasx_pagedkv* kv, const atlasx_pagedkv_rows* rows);
 /* The values that the slots hold, contiguous [n][n_kv_heads][head_dim] in f32 (exact), bf16 or f16 (rounded once); zeros for slots
  * that are negative or behind the pool.  Gives a cached prefix back to atlasx_prompt_attention. */
 int atlasx_pagedkv_read(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const int* slots_dev, int n, int dtype, void* k_out_dev, void* v_out_dev);
@@ -237,9 +246,16 @@ int atlasx_pagedkv_read(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const int* sl
  * number outside the pool are left out and raise the device error word.  workspace: NULL for the cache's own, else
  * workspace_bytes (atlasx_pagedkv_ptrs) zeroed once before its first use; calls that may run at the same time — graphs replayed on
  * different streams — need workspaces of their own. */
-int atlasx_pagedkv_decode_attention(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const float* q_dev, float* out_dev, int n_heads,
-                                    const int* table_dev, int table_width, const int* lens_dev, int batch, float scale, int window,
-                                    void* workspace_dev, size_t workspace_bytes);
+typedef struct {
+    const float* q;
+    float* out;
+    const int *table, *lens;                      /* [batch][table_width], [batch] */
+    void* workspace;
+    size_t workspace_bytes;
+    int n_heads, table_width, batch, window;
+    float scale;
+} atlasx_pagedkv_attn_args;
+int atlasx_pagedkv_decode_attention(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const atlasx_pagedkv_attn_args* args);
 
 /* Causal attention of whole packed prompts, bf16 or f16 in and out, f32 inside; head_dim 64 or 128.  Sequence b owns rows
  * cu_q[b] .. cu_q[b + 1] − 1 of q and out [n_q][n_heads][head_dim] and rows cu_k[b] .. cu_k[b + 1] − 1 of k and v
@@ -247,12 +263,15 @@ int atlasx_pagedkv_decode_attention(atlasx_ctx* ctx, const atlasx_pagedkv* kv, c
  * sees keys j ≤ i + lk − lq, with a window only those with i + lk − lq − j < window; a query that sees none gets zeros.  What a
  * query does not see — NaN and infinities too — does not reach it.  Strides in elements, every row on a 16-byte boundary; rows of
  * out in no sequence are left as they are.  out may not overlap q, k or v. */
-int atlasx_prompt_attention(atlasx_ctx* ctx, int dtype, const void* q_dev, long long q_token_stride, long long q_head_stride,
-                            const void* k_dev, long long k_token_stride, long long k_head_stride,
-                            const void* v_dev, long long v_token_stride, long long v_head_stride,
-                            void* out_dev, long long out_token_stride, long long out_head_stride,
-                            const int* cu_q_dev, const int* cu_k_dev, int batch, int n_q, int n_k, int n_heads, int n_kv_heads,
-                            int head_dim, float scale, int window);
+typedef struct {
+    const void *q, *k, *v;
+    void* out;
+    long long q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+    const int *cu_q, *cu_k;                       /* [batch + 1] */
+    int dtype, batch, n_q, n_k, n_heads, n_kv_heads, head_dim, window;
+    float scale;
+} atlasx_prompt_args;
+int atlasx_prompt_attention(atlasx_ctx* ctx, const atlasx_prompt_args* args);
 
 /* ── SamplingConfig and the sampling pipeline (crates/atlas-model/src/lib.rs:1223-1294, 2581-2717) ── */
 typedef struct {

@@ -711,13 +711,13 @@ def test_two_contexts_do_not_meet(ab):
     from atlas_b200 import _ffi
     d = ab.DeviceArray.from_host(np.zeros(64), ab.F32)
     i = ab.DeviceArray.from_host([0], ab.I32)
-    rc = _ffi.lib().atlasx_pagedkv_decode_attention(other.handle, kv._h, d.ptr, d.ptr, 1, i.ptr, 1, i.ptr, 1, 0.1, 0, None, 0)
+    attn = lambda w, n: _ffi.PAGED_ATTN.pack(d.ptr, d.ptr, i.ptr, i.ptr, w, n, 1, 1, 1, 0, 0.1)      # noqa: E731
+    rc = _ffi.lib().atlasx_pagedkv_decode_attention(other.handle, kv._h, attn(0, 0))
     assert rc == -1 and b"another context" in _ffi.lib().atlasx_last_error()
-    rc = _ffi.lib().atlasx_pagedkv_append(other.handle, kv._h, 0, d.ptr, 64, 64, d.ptr, 64, 64, i.ptr, 1)
+    rc = _ffi.lib().atlasx_pagedkv_append(other.handle, kv._h, _ffi.PAGED_ROWS.pack(d.ptr, d.ptr, i.ptr, 64, 64, 64, 64, 0, 1))
     assert rc == -1 and b"another context" in _ffi.lib().atlasx_last_error()
-    rc = _ffi.lib().atlasx_pagedkv_decode_attention(kv.ctx.handle, kv._h, d.ptr, d.ptr, 1, i.ptr, 1, i.ptr, 1, 0.1, 0, d.ptr, 8)
-    if kv.workspace_bytes > 8:
-        assert rc == -1 and b"workspace" in _ffi.lib().atlasx_last_error()
+    rc = _ffi.lib().atlasx_pagedkv_decode_attention(kv.ctx.handle, kv._h, attn(d.ptr, 8))
+    assert rc == -1 and b"workspace" in _ffi.lib().atlasx_last_error()
     with pytest.raises(ab.AtlasError, match="multiple"):
         ab.PagedKvCache(2, 16, 2, 64).decode_attention(ab.DeviceArray.empty((1, 3, 64), ab.F32), ab.DeviceArray.empty((1, 3, 64), ab.F32),
                                                        ab.DeviceArray.from_host([[0]], ab.I32), i, 0.1)

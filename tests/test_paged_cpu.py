@@ -84,6 +84,20 @@ def test_tiles_stay_inside_the_pool(idx):
     assert idx.tile_at(n, p, k, 128, 32, n - 1, k - 1, 15) == idx.pool_bytes(n, p, k, 128, 32) - 2304 == n * k * 2304 - 2304
 
 
+def test_argument_structs_have_the_c_layout(tmp_path):
+    """Sizes and the offset of the last member, from the header with the host compiler."""
+    src = tmp_path / "sizes.c"
+    src.write_text('#include "atlas_kernels.h"\n#include <stdio.h>\nint main(void) {'
+                   'printf("%zu %zu %zu %zu %zu %zu %zu %zu", sizeof(atlasx_page_plan_args), offsetof(atlasx_page_plan_args, n_tokens),'
+                   'sizeof(atlasx_pagedkv_rows), offsetof(atlasx_pagedkv_rows, n), sizeof(atlasx_pagedkv_attn_args), offsetof(atlasx_pagedkv_attn_args, scale),'
+                   'sizeof(atlasx_prompt_args), offsetof(atlasx_prompt_args, scale)); return 0; }')
+    exe = str(tmp_path / "sizes")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", exe], check=True)
+    got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    for i, f in enumerate((_ffi.PAGE_PLAN, _ffi.PAGED_ROWS, _ffi.PAGED_ATTN, _ffi.PROMPT)):
+        assert f.size - 4 == got[2 * i + 1] and f.size <= got[2 * i] < f.size + 8
+
+
 # ── refusals ─────────────────────────────────────────────────────────────────────
 P = 1 << 20      # a pointer that is never followed: every call below is refused before it runs
 
@@ -93,8 +107,13 @@ def refused(rc, text):
     assert rc == -1 and text in msg, (rc, msg)
 
 
-PLAN = dict(ctx=None, cached=P, fresh=P, batch=4, free=P, n_free=8, page_size=16, n_pages=8, table=P, width=4, cu=P, lens=P, slots=P, pos=P,
-            n_tokens=4, status=P)
+def packed(layout, args):
+    """The argument struct as the library gets it (None: a null pointer)."""
+    return layout.pack(*(0 if v is None else v for v in args.values()))
+
+
+PLAN = dict(cached=P, fresh=P, free=P, table=P, cu=P, lens=P, slots=P, pos=P, status=P, batch=4, n_free=8, page_size=16, n_pages=8, width=4,
+            n_tokens=4)
 
 
 @pytest.mark.parametrize("change,text", [
@@ -103,7 +122,7 @@ PLAN = dict(ctx=None, cached=P, fresh=P, batch=4, free=P, n_free=8, page_size=16
     (dict(n_pages=1 << 30, page_size=16), "2^31"), (dict(width=0), "column"), (dict(n_tokens=-1), "negative"),
     (dict(n_free=-1), "negative"), ({}, "ctx is null")])
 def test_plan_refusals(change, text):
-    refused(_ffi.lib().atlasx_page_plan(*dict(PLAN, **change).values()), text)
+    refused(_ffi.lib().atlasx_page_plan(None, packed(_ffi.PAGE_PLAN, dict(PLAN, **change))), text)
 
 
 @pytest.mark.parametrize("shape,text", [
@@ -119,14 +138,14 @@ def test_cache_refusals(shape, text):
         assert _ffi.lib().atlasx_pagedkv_bytes(*shape) == 4 * 2304
 
 
-ROWS = dict(ctx=None, kv=None, dtype=1, k=P, kt=128, kh=128, v=P, vt=128, vh=128, slots=P, n=3)
+ROWS = dict(k=P, v=P, slots=P, kt=128, kh=128, vt=128, vh=128, dtype=1, n=3)
 
 
 @pytest.mark.parametrize("change,text", [
     (dict(dtype=2), "dtype"), (dict(n=-1), "negative"), (dict(k=None), "null"), (dict(slots=None), "null"), (dict(k=P + 2), "16-byte"),
     (dict(kt=129), "16-byte"), (dict(vh=4), "16-byte"), (dict(dtype=0, kt=130), "16-byte"), ({}, "ctx or cache is null")])
 def test_append_refusals(change, text):
-    refused(_ffi.lib().atlasx_pagedkv_append(*dict(ROWS, **change).values()), text)
+    refused(_ffi.lib().atlasx_pagedkv_append(None, None, packed(_ffi.PAGED_ROWS, dict(ROWS, **change))), text)
 
 
 READ = dict(ctx=None, kv=None, slots=P, n=3, dtype=0, k=P, v=P)
@@ -138,7 +157,7 @@ def test_read_refusals(change, text):
     refused(_ffi.lib().atlasx_pagedkv_read(*dict(READ, **change).values()), text)
 
 
-DEC = dict(ctx=None, kv=None, q=P, out=P, n_heads=8, table=P, width=4, lens=P, batch=2, scale=0.1, window=0, ws=None, wsn=0)
+DEC = dict(q=P, out=P, table=P, lens=P, ws=None, wsn=0, n_heads=8, width=4, batch=2, window=0, scale=0.1)
 
 
 @pytest.mark.parametrize("change,text", [
@@ -146,11 +165,11 @@ DEC = dict(ctx=None, kv=None, q=P, out=P, n_heads=8, table=P, width=4, lens=P, b
     (dict(width=0), "column"), (dict(window=-1), "window"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
     (dict(q=P + 8), "16-byte"), ({}, "ctx or cache is null")])
 def test_decode_refusals(change, text):
-    refused(_ffi.lib().atlasx_pagedkv_decode_attention(*dict(DEC, **change).values()), text)
+    refused(_ffi.lib().atlasx_pagedkv_decode_attention(None, None, packed(_ffi.PAGED_ATTN, dict(DEC, **change))), text)
 
 
-PROMPT = dict(ctx=None, dtype=1, q=P, qt=512, qh=128, k=P, kt=256, kh=128, v=P, vt=256, vh=128, out=P, ot=512, oh=128, cu_q=P, cu_k=P, batch=2,
-              n_q=10, n_k=10, n_heads=4, n_kv=2, hd=128, scale=0.1, window=0)
+PROMPT = dict(q=P, k=P, v=P, out=P, qt=512, qh=128, kt=256, kh=128, vt=256, vh=128, ot=512, oh=128, cu_q=P, cu_k=P, dtype=1, batch=2,
+              n_q=10, n_k=10, n_heads=4, n_kv=2, hd=128, window=0, scale=0.1)
 
 
 @pytest.mark.parametrize("change,text", [
@@ -159,7 +178,7 @@ PROMPT = dict(ctx=None, dtype=1, q=P, qt=512, qh=128, k=P, kt=256, kh=128, v=P, 
     (dict(q=None), "null"), (dict(k=None), "null"), (dict(cu_k=None), "null"), (dict(q=P + 2), "16-byte"), (dict(kt=257), "16-byte"),
     (dict(vt=-256), "negative"), (dict(oh=64), "overlap"), (dict(ot=0), "overlap"), ({}, "ctx is null")])
 def test_prompt_refusals(change, text):
-    refused(_ffi.lib().atlasx_prompt_attention(*dict(PROMPT, **change).values()), text)
+    refused(_ffi.lib().atlasx_prompt_attention(None, packed(_ffi.PROMPT, dict(PROMPT, **change))), text)
 
 
 class FakeContext:
@@ -181,7 +200,7 @@ def test_python_refuses_arrays_that_do_not_fit():
                          (dict(out=arr((5, 4, 64), ab.BF16, (512, 64, 2))), "unit stride"), (dict(cu_k=arr((4,), ab.I32)), "shape"),
                          (dict(cu_q=arr((3,), ab.F32)), "int32"), (dict(q=arr((20, 64), ab.BF16)), "dimensions"),
                          (dict(k=arr((7, 2, 64), ab.BF16, device=1)), "device"), (dict(q=7), "not a device array"),
-                         (dict(cu_q=arr((3,), ab.I32, (2,))), "contiguous")]:
+                         (dict(cu_q=arr((3,), ab.I32, (2,))), "contiguous"), (dict(window_size=1 << 40), "out of range")]:
         with pytest.raises(ab.AtlasError, match=text):
             ab.prompt_attention(**dict(good, **change))
     b = arr((4,), ab.I32)
