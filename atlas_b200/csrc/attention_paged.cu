@@ -27,6 +27,7 @@ constexpr int kStages = 4;
 constexpr int kCtasPerSm = 3;
 constexpr int kMinTiles = 2;                    // tiles of a warp below which fewer CTAs share the work
 constexpr int kHeads = 8;                       // query heads of one segment
+constexpr int kChunk = 128;                     // parts of a segment whose weights are in shared memory at a time
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr int kErrWait = 711;
 
@@ -436,41 +437,62 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             __syncthreads();
             if (s_last) {
                 __threadfence();
+                // part k is the tail of CTA cf (k = 0) or the head of CTA cf + k
                 const int cnt = (int)(cl - cf) + 1;
-                float* wt = reinterpret_cast<float*>(smem);                                       // the ring is free: weights of the parts
-                const int cap = kWarps * kStages * TILE / 4;
-                float L = 0.f;
-                const bool fits = cnt * heads <= cap;
+                const float* ml = dv.part_ml + 2 * (size_t)cf * hpt * 2;
+                const float* po = dv.part_o + 2 * (size_t)cf * hpt * HD;
+                auto part = [&](int k) { return (size_t)(2 * k + (k == 0)) * hpt; };
+                float* wt = reinterpret_cast<float*>(smem);                                       // the ring is free: weights of kChunk parts, per head
                 for (int h = warp; h < heads; h += kWarps) {
                     float M = -INFINITY;
-                    for (int k = lane; k < cnt; k += 32)
-                        M = fmaxf(M, __ldcg(dv.part_ml + ((2 * (size_t)(cf + k) + (k == 0)) * hpt + h) * 2));
+                    for (int k = lane; k < cnt; k += 32) M = fmaxf(M, __ldcg(ml + (part(k) + h) * 2));
                     M = ax_warp_max(M);
-                    L = 0.f;
-                    for (int k = lane; k < cnt; k += 32) {
-                        const float2 ml = __ldcg((const float2*)(dv.part_ml + ((2 * (size_t)(cf + k) + (k == 0)) * hpt + h) * 2));
-                        const float f = ml.y == 0.f ? 0.f : ml.x == M ? 1.f : ex2(ml.x - M);
-                        L += ml.y == 0.f ? 0.f : f * ml.y;
-                        if (fits) wt[h * cnt + k] = f;
-                    }
-                    L = ax_warp_sum(L);
-                    if (lane == 0) { s_ml[0][h][0] = M; s_ml[0][h][1] = L; }
+                    if (lane == 0) s_ml[0][h][0] = M;
                 }
-                __syncthreads();
-                for (int e = tid; e < heads * (HD / 4); e += kWarps * 32) {
-                    const int h = e / (HD / 4), d = (e % (HD / 4)) * 4;
-                    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (int k = 0; k < cnt; k++) {
-                        const size_t at = (2 * (size_t)(cf + k) + (k == 0)) * hpt + h;
-                        float f;
-                        if (fits) f = wt[h * cnt + k];
-                        else { const float2 ml = __ldcg((const float2*)(dv.part_ml + at * 2)); f = ml.y == 0.f ? 0.f : ml.x == s_ml[0][h][0] ? 1.f : ex2(ml.x - s_ml[0][h][0]); }
-                        const float4 v = __ldcg((const float4*)(dv.part_o + at * HD + d));
-                        if (f != 0.f) { A.x = fmaf(f, v.x, A.x); A.y = fmaf(f, v.y, A.y); A.z = fmaf(f, v.z, A.z); A.w = fmaf(f, v.w, A.w); }
+                constexpr int E = (kHeads * HD / 4 + kWarps * 32 - 1) / (kWarps * 32);            // float4 outputs of a thread
+                float4 A[E];
+#pragma unroll
+                for (int e = 0; e < E; e++) A[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                float L = 0.f;                                                                    // of head `warp`, then `warp + kWarps`
+                float L2 = 0.f;
+                for (int k0 = 0; k0 < cnt; k0 += kChunk) {
+                    const int kn = min(kChunk, cnt - k0);
+                    __syncthreads();
+                    for (int h = warp; h < heads; h += kWarps) {
+                        const float M = s_ml[0][h][0];
+                        float sum = 0.f;
+                        for (int k = lane; k < kn; k += 32) {
+                            const float2 v = __ldcg((const float2*)(ml + (part(k0 + k) + h) * 2));
+                            const float f = v.y == 0.f ? 0.f : v.x == M ? 1.f : ex2(v.x - M);
+                            wt[h * kChunk + k] = f;
+                            sum += f * v.y;
+                        }
+                        sum = ax_warp_sum(sum);
+                        if (h < kWarps) L += sum; else L2 += sum;
                     }
-                    const float f = s_ml[0][h][1] == 0.f ? 0.f : 1.f / s_ml[0][h][1];
-                    *(float4*)(out + (size_t)h * HD + d) = make_float4(A.x * f, A.y * f, A.z * f, A.w * f);
+                    __syncthreads();
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const int at = tid + e * kWarps * 32, h = at / (HD / 4), d = (at % (HD / 4)) * 4;
+                        if (h < heads) {
+#pragma unroll 8
+                            for (int k = 0; k < kn; k++) {                                        // loads of eight parts under way
+                                const float4 v = __ldcg((const float4*)(po + (part(k0 + k) + h) * HD + d));
+                                const float f = wt[h * kChunk + k];
+                                A[e].x = fmaf(f, v.x, A[e].x); A[e].y = fmaf(f, v.y, A[e].y); A[e].z = fmaf(f, v.z, A[e].z); A[e].w = fmaf(f, v.w, A[e].w);
+                            }
+                        }
+                    }
+                }
+                if (lane == 0) { if (warp < heads) s_ml[0][warp][1] = L; if (warp + kWarps < heads) s_ml[0][warp + kWarps][1] = L2; }
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const int at = tid + e * kWarps * 32, h = at / (HD / 4), d = (at % (HD / 4)) * 4;
+                    if (h < heads) {
+                        const float f = s_ml[0][h][1] == 0.f ? 0.f : 1.f / s_ml[0][h][1];
+                        *(float4*)(out + (size_t)h * HD + d) = make_float4(A[e].x * f, A[e].y * f, A[e].z * f, A[e].w * f);
+                    }
                 }
                 if (tid == 0) dv.tickets[cf] = 0u;                                                // ready for the next launch
             }
