@@ -138,6 +138,7 @@ template <> __device__ __forceinline__ void load8<__half>(const __half* p, float
 
 struct RowArgs {
     AxP4Shape s;
+    unsigned long long inv_page;  // ceil(2^36 / (page_size / 16)): slot / page_size without a division
     uint8_t* pool;
     const void *k, *v;            // append: [token][head][hd], token and head strides in elements
     long long k_tok, k_head, v_tok, v_head;
@@ -147,61 +148,74 @@ struct RowArgs {
     int* err;
 };
 
+// A slot's page and row within it.  slot / 16 < 2^27 and page_size / 16 ≤ 2^9, so the rounded-up reciprocal with 36 bits is exact.
+__device__ __forceinline__ void slot_place(const RowArgs& a, int slot, int& page, int& off) {
+    page = (int)(((unsigned long long)(unsigned)(slot >> 4) * a.inv_page) >> 36);
+    off = slot - page * a.s.page_size;
+}
+template <int HD, int GS> __device__ __forceinline__ AxP4Shape fixed_shape(const AxP4Shape& s) { return AxP4Shape{ s.n_pages, s.page_size, s.n_kv, HD, GS }; }
+
 // A lane holds eight consecutive numbers of one row of K or V; 4 or 8 lanes make a group and find its largest magnitude with
 // shuffles.  scale = bf16(max / 7); the number is x · (1 / scale) rounded half away from zero, at most 7 in magnitude — the f32
 // arithmetic of Int4Tensor::quantize with a scale of 16 bits: the numbers are rounded against the scale that is stored, so its
-// own rounding (2^-9 of itself) costs nothing beyond the half step of the number.  A group with a NaN or an infinity gets the scale NaN.
-// Bytes: the rows once, 4.25 or 4.5 bits per number out.
-template <typename T>
+// own rounding (2^-8 of itself) costs nothing beyond the half step of the number.  A group with a NaN or an infinity gets the scale NaN.
+// Bytes: the rows once, 4.25 or 4.5 bits per number out.  A CTA takes 16 (hd 128) or 32 consecutive rows of one head: as a rule one or two
+// tiles of the pool.  What bounds it after the memory is instructions (83 % of the issue slots when shapes were run-time values and
+// rows were found by division: 8191 rows × 32 heads × 128 took 181 µs).
+template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(256) ax_p4_append_kernel(const RowArgs a) {
-    const int lanes = a.s.hd / 8, gl = a.s.group / 8;                 // lanes per row, lanes per group
-    const long long jobs = (long long)a.n * a.s.n_kv * 2 * lanes;     // K of a (token, head), then its V
-    const long long job = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const bool live = job < jobs;
-    const int li = (int)(job % lanes);
-    const long long row = job / lanes;
-    const int which = (int)(row & 1), head = (int)((row >> 1) % a.s.n_kv), tok = live ? (int)((row >> 1) / a.s.n_kv) : 0;
-    float x[8];
+    constexpr int LANES = HD / 8, GL = GS / 8, TOKENS = 256 / LANES;          // lanes per row, lanes per group, rows per CTA
+    const int li = threadIdx.x % LANES, tok = blockIdx.x * TOKENS + threadIdx.x / LANES, head = blockIdx.y, which = blockIdx.z;
+    const AxP4Shape sh = fixed_shape<HD, GS>(a.s);
+    const bool live = tok < a.n;
+    float x[8] = {};
     float top = 0.f;
     int slot = -1;
+    bool odd = false;
     if (live) {
         slot = a.slots[tok];
         const T* src = which ? (const T*)a.v + tok * a.v_tok + head * a.v_head : (const T*)a.k + tok * a.k_tok + head * a.k_head;
         load8<T>(src + 8 * li, x);
-        bool odd = false;
+        float all = 0.f;                                             // NaN as soon as one number is not finite
 #pragma unroll
-        for (int i = 0; i < 8; i++) { const float m = fabsf(x[i]); odd |= !(m <= 3.402823466e38f); top = fmaxf(top, m); }
-        if (odd) top = __int_as_float(0x7F800000);
+        for (int i = 0; i < 8; i++) { top = fmaxf(top, fabsf(x[i])); all = fmaf(x[i], 0.f, all); }
+        if (all != all) top = __int_as_float(0x7F800000);
     }
-    for (int d = 1; d < gl; d <<= 1) top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, d));
+#pragma unroll
+    for (int d = 1; d < GL; d <<= 1) top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, d));
     if (!live || slot < 0) return;                                   // a negative slot marks an absent row
-    if (slot >= a.s.n_pages * a.s.page_size) { if (li == 0) atomicExch(a.err, AX_DEVERR_SLOT); return; }
-    const bool odd = top > 3.402823466e38f;
+    if (slot >= sh.n_pages * sh.page_size) { if (li == 0) atomicExch(a.err, AX_DEVERR_SLOT); return; }
+    odd = top > 3.402823466e38f;
     uint16_t sb = ax_f32_to_bf16_rne(__fdiv_rn(top, 7.0f));
     float sc = ax_bf16_to_f32(sb);
     if (sc < 1.17549435e-38f) { sc = 1.0f; sb = 0x3F80; }
-    if (odd) sb = 0x7FC0;
+    if (odd) { sc = 1.0f; sb = 0x7FC0; }
     const float inv = __frcp_rn(sc);
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        float q = odd ? 0.f : roundf(__fmul_rn(x[i], inv));
-        q = fminf(fmaxf(q, -7.f), 7.f);
-        w |= (uint32_t)((int)q + 8) << (4 * i);
+        // |y| + (1/2 − 2^-25), cut off: rounds half away from zero for |y| < 8.  Added to 2^23 with rounding toward zero the whole part is
+        // the low bits of the sum.
+        const float y = __fmul_rn(x[i], inv);
+        const int m = __float_as_int(__fadd_rz(fminf(fabsf(y) + 0.49999997f, 7.5f), 8388608.f)) & 15;
+        w |= (uint32_t)(8 + (y < 0.f ? -m : m)) << (4 * i);
     }
-    const int page = slot / a.s.page_size, off = slot % a.s.page_size, r = off % AX_P4_TILE;
-    uint8_t* tile = a.pool + ax_p4_tile_at(a.s, page, head, off);
-    const int plane = ax_p4_plane_bytes(a.s);
+    if (odd) w = 0x88888888u;
+    int page, off;
+    slot_place(a, slot, page, off);
+    const int r = off % AX_P4_TILE;
+    uint8_t* tile = a.pool + ax_p4_tile_at(sh, page, head, off);
+    const int plane = ax_p4_plane_bytes(sh);
     if (which == 0) {
-        reinterpret_cast<uint32_t*>(tile)[ax_p4_k_word(a.s, r, 8 * li)] = w;
+        reinterpret_cast<uint32_t*>(tile)[ax_p4_k_word(sh, r, 8 * li)] = w;
     } else {
         uint16_t* vp = reinterpret_cast<uint16_t*>(tile + plane);
-        vp[ax_p4_v_half(a.s, r, 8 * li)] = (uint16_t)(w & 0xFFFFu);
-        vp[ax_p4_v_half(a.s, r, 8 * li + 4)] = (uint16_t)(w >> 16);
+        vp[ax_p4_v_half(sh, r, 8 * li)] = (uint16_t)(w & 0xFFFFu);
+        vp[ax_p4_v_half(sh, r, 8 * li + 4)] = (uint16_t)(w >> 16);
     }
-    if (li % gl == 0) {
-        uint16_t* sp = reinterpret_cast<uint16_t*>(tile + 2 * plane + which * ax_p4_scale_bytes(a.s));
-        sp[ax_p4_scale(a.s, r, li / gl)] = sb;
+    if (li % GL == 0) {
+        uint16_t* sp = reinterpret_cast<uint16_t*>(tile + 2 * plane + which * ax_p4_scale_bytes(sh));
+        sp[ax_p4_scale(sh, r, li / GL)] = sb;
     }
 }
 
@@ -224,42 +238,62 @@ template <> __device__ __forceinline__ void store8<__half>(__half* p, const floa
 }
 
 // The values a slot holds: number · scale, exact in f32 (4 + 8 bits), one rounding for the 16-bit types.  Absent rows read as zeros.
-template <typename T>
+template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(256) ax_p4_read_kernel(const RowArgs a) {
-    const int lanes = a.s.hd / 8, gl = a.s.group / 8;
-    const long long jobs = (long long)a.n * a.s.n_kv * lanes;
-    const long long job = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (job >= jobs) return;
-    const int li = (int)(job % lanes);
-    const long long row = job / lanes;
-    const int head = (int)(row % a.s.n_kv), tok = (int)(row / a.s.n_kv);
+    constexpr int LANES = HD / 8, GL = GS / 8, TOKENS = 256 / LANES;
+    const int li = threadIdx.x % LANES, tok = blockIdx.x * TOKENS + threadIdx.x / LANES, head = blockIdx.y;
+    if (tok >= a.n) return;
+    const AxP4Shape sh = fixed_shape<HD, GS>(a.s);
     const int slot = a.slots[tok];
     float k[8], v[8];
-    if (slot >= 0 && slot < a.s.n_pages * a.s.page_size) {
-        const int page = slot / a.s.page_size, off = slot % a.s.page_size, r = off % AX_P4_TILE;
-        const uint8_t* tile = a.pool + ax_p4_tile_at(a.s, page, head, off);
-        const int plane = ax_p4_plane_bytes(a.s);
-        const uint32_t kw = reinterpret_cast<const uint32_t*>(tile)[ax_p4_k_word(a.s, r, 8 * li)];
+    if (slot >= 0 && slot < sh.n_pages * sh.page_size) {
+        int page, off;
+        slot_place(a, slot, page, off);
+        const int r = off % AX_P4_TILE;
+        const uint8_t* tile = a.pool + ax_p4_tile_at(sh, page, head, off);
+        const int plane = ax_p4_plane_bytes(sh);
+        const uint32_t kw = reinterpret_cast<const uint32_t*>(tile)[ax_p4_k_word(sh, r, 8 * li)];
         const uint16_t* vp = reinterpret_cast<const uint16_t*>(tile + plane);
-        const uint32_t vw = vp[ax_p4_v_half(a.s, r, 8 * li)] | ((uint32_t)vp[ax_p4_v_half(a.s, r, 8 * li + 4)] << 16);
+        const uint32_t vw = vp[ax_p4_v_half(sh, r, 8 * li)] | ((uint32_t)vp[ax_p4_v_half(sh, r, 8 * li + 4)] << 16);
         const uint16_t* sp = reinterpret_cast<const uint16_t*>(tile + 2 * plane);
-        const float ks = ax_bf16_to_f32(sp[ax_p4_scale(a.s, r, li / gl)]);
-        const float vs = ax_bf16_to_f32(sp[AX_P4_TILE * ax_p4_groups(a.s) + ax_p4_scale(a.s, r, li / gl)]);
+        const float ks = ax_bf16_to_f32(sp[ax_p4_scale(sh, r, li / GL)]);
+        const float vs = ax_bf16_to_f32(sp[AX_P4_TILE * (HD / GS) + ax_p4_scale(sh, r, li / GL)]);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            k[i] = (float)((int)((kw >> (4 * i)) & 15u) - 8) * ks;
-            v[i] = (float)((int)((vw >> (4 * i)) & 15u) - 8) * vs;
+        for (int i = 0; i < 8; i++) {                                // 2^23 + nibble − (2^23 + 8): no conversion instruction
+            k[i] = (__int_as_float(0x4B000000 | ((kw >> (4 * i)) & 15u)) - 8388616.f) * ks;
+            v[i] = (__int_as_float(0x4B000000 | ((vw >> (4 * i)) & 15u)) - 8388616.f) * vs;
         }
     } else {
         if (slot >= 0) atomicExch(a.err, AX_DEVERR_SLOT);
 #pragma unroll
         for (int i = 0; i < 8; i++) { k[i] = 0.f; v[i] = 0.f; }
     }
-    const size_t o = ((size_t)tok * a.s.n_kv + head) * a.s.hd + 8 * li;
+    const size_t o = ((size_t)tok * sh.n_kv + head) * HD + 8 * li;
     store8<T>((T*)a.k_out + o, k);
     store8<T>((T*)a.v_out + o, v);
 }
 
+template <typename T, bool READ>
+void launch_rows(const RowArgs& a, cudaStream_t stream) {
+    const int tokens = 256 / (a.s.hd / 8);
+    const dim3 grid((unsigned)((a.n + (long long)tokens - 1) / tokens), (unsigned)a.s.n_kv, READ ? 1u : 2u);
+#define AX_ROWS(HD, GS) do { if (READ) ax_p4_read_kernel<T, HD, GS><<<grid, 256, 0, stream>>>(a); \
+                             else ax_p4_append_kernel<T, HD, GS><<<grid, 256, 0, stream>>>(a); } while (0)
+    if (a.s.hd == 128) { if (a.s.group == 32) AX_ROWS(128, 32); else AX_ROWS(128, 64); }
+    else { if (a.s.group == 32) AX_ROWS(64, 32); else AX_ROWS(64, 64); }
+#undef AX_ROWS
+}
+template <bool READ>
+void launch_rows(int dtype, const RowArgs& a, cudaStream_t stream) {
+    if (dtype == ATLASX_F32) launch_rows<float, READ>(a, stream);
+    else if (dtype == ATLASX_BF16) launch_rows<uint16_t, READ>(a, stream);
+    else launch_rows<__half, READ>(a, stream);
+}
+
+unsigned long long page_inverse(int page_size) {
+    const unsigned long long d = (unsigned long long)page_size / AX_P4_TILE;
+    return ((1ull << 36) + d - 1) / d;
+}
 int elem_bytes(int dtype) { return dtype == ATLASX_F32 ? 4 : 2; }
 
 }  // namespace
@@ -286,7 +320,7 @@ extern "C" int atlasx_page_plan(atlasx_ctx* c, const atlasx_page_plan_args* p) {
 
 static int check_shape(int n_pages, int page_size, int n_kv, int hd, int group) {
     AX_ARG(n_pages >= 1 && n_kv >= 1, "n_pages and n_kv_heads must be positive");
-    AX_ARG(page_size >= AX_P4_TILE && page_size % AX_P4_TILE == 0, "page_size must be a multiple of 16");
+    AX_ARG(page_size >= AX_P4_TILE && page_size <= 8192 && page_size % AX_P4_TILE == 0, "page_size must be a multiple of 16, at most 8192");
     AX_ARG((long long)n_pages * page_size <= 0x7FFFFFFFll, "n_pages · page_size must be below 2^31: slots are 32-bit");
     AX_ARG(hd == 64 || hd == 128, "head_dim must be 64 or 128");
     AX_ARG(group == 32 || group == 64, "group must be 32 or 64");
@@ -357,12 +391,8 @@ extern "C" int atlasx_pagedkv_append(atlasx_ctx* c, atlasx_pagedkv* kv, const at
     a.s = kv->s; a.pool = kv->pool; a.k = k; a.v = v;
     a.k_tok = k_token_stride; a.k_head = k_head_stride; a.v_tok = v_token_stride; a.v_head = v_head_stride;
     a.slots = slots; a.n = n; a.err = c->dev_error;
-    const long long jobs = (long long)n * kv->s.n_kv * 2 * (kv->s.hd / 8);
-    AX_ARG((jobs + 255) / 256 <= 0x7FFFFFFFll, "too many rows for one call");
-    const unsigned grid = (unsigned)((jobs + 255) / 256);
-    if (dtype == ATLASX_F32) ax_p4_append_kernel<float><<<grid, 256, 0, c->stream>>>(a);
-    else if (dtype == ATLASX_BF16) ax_p4_append_kernel<uint16_t><<<grid, 256, 0, c->stream>>>(a);
-    else ax_p4_append_kernel<__half><<<grid, 256, 0, c->stream>>>(a);
+    a.inv_page = page_inverse(kv->s.page_size);
+    launch_rows<false>(dtype, a, c->stream);
     AX_CHECK_LAUNCH("ax_p4_append_kernel");
     return ATLASX_OK;
 }
@@ -377,12 +407,8 @@ extern "C" int atlasx_pagedkv_read(atlasx_ctx* c, const atlasx_pagedkv* kv, cons
     AX_ON_DEVICE(c);
     RowArgs a = {};
     a.s = kv->s; a.pool = kv->pool; a.k_out = k_out; a.v_out = v_out; a.slots = slots; a.n = n; a.err = c->dev_error;
-    const long long jobs = (long long)n * kv->s.n_kv * (kv->s.hd / 8);
-    AX_ARG((jobs + 255) / 256 <= 0x7FFFFFFFll, "too many rows for one call");
-    const unsigned grid = (unsigned)((jobs + 255) / 256);
-    if (dtype == ATLASX_F32) ax_p4_read_kernel<float><<<grid, 256, 0, c->stream>>>(a);
-    else if (dtype == ATLASX_BF16) ax_p4_read_kernel<uint16_t><<<grid, 256, 0, c->stream>>>(a);
-    else ax_p4_read_kernel<__half><<<grid, 256, 0, c->stream>>>(a);
+    a.inv_page = page_inverse(kv->s.page_size);
+    launch_rows<true>(dtype, a, c->stream);
     AX_CHECK_LAUNCH("ax_p4_read_kernel");
     return ATLASX_OK;
 }

@@ -84,6 +84,17 @@ def test_tiles_stay_inside_the_pool(idx):
     assert idx.tile_at(n, p, k, 128, 32, n - 1, k - 1, 15) == idx.pool_bytes(n, p, k, 128, 32) - 2304 == n * k * 2304 - 2304
 
 
+def test_reciprocal_of_the_page_size_is_exact():
+    """slot / page_size as the kernels take it: (slot / 16) · ceil(2^36 / (page_size / 16)) >> 36, at the borders of every page size."""
+    for d in range(1, 513):
+        inv = -(-(1 << 36) // d)
+        top = (1 << 27) - 1
+        q = np.unique(np.concatenate([np.arange(0, 50), np.arange(top // d - 50, top // d + 1)]))
+        for n in np.concatenate([q * d, q * d + d - 1, [top]]):
+            n = int(min(max(n, 0), top))
+            assert (n * inv) >> 36 == n // d and n * inv < 1 << 64
+
+
 def test_argument_structs_have_the_c_layout(tmp_path):
     """Sizes and the offset of the last member, from the header with the host compiler."""
     src = tmp_path / "sizes.c"
@@ -127,7 +138,7 @@ def test_plan_refusals(change, text):
 
 @pytest.mark.parametrize("shape,text", [
     ((0, 16, 1, 64, 32), "positive"), ((4, 16, 0, 64, 32), "positive"), ((4, 8, 1, 64, 32), "multiple of 16"),
-    ((4, 24, 1, 64, 32), "multiple of 16"), ((1 << 27, 16, 1, 64, 32), "2^31"), ((4, 16, 1, 96, 32), "head_dim"),
+    ((4, 24, 1, 64, 32), "multiple of 16"), ((4, 8208, 1, 64, 32), "8192"), ((1 << 27, 16, 1, 64, 32), "2^31"), ((4, 16, 1, 96, 32), "head_dim"),
     ((4, 16, 1, 128, 16), "group"), ((4, 16, 1, 128, 128), "group"), ((4, 16, 1, 128, 32), "ctx is null")])
 def test_cache_refusals(shape, text):
     h = C.c_void_p()
