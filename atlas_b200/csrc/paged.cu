@@ -155,63 +155,73 @@ __device__ __forceinline__ void slot_place(const RowArgs& a, int slot, int& page
 }
 template <int HD, int GS> __device__ __forceinline__ AxP4Shape fixed_shape(const AxP4Shape& s) { return AxP4Shape{ s.n_pages, s.page_size, s.n_kv, HD, GS }; }
 
-// A lane holds eight consecutive numbers of one row of K or V; 4 or 8 lanes make a group and find its largest magnitude with
-// shuffles.  scale = bf16(max / 7); the number is x · (1 / scale) rounded half away from zero, at most 7 in magnitude — the f32
-// arithmetic of Int4Tensor::quantize with a scale of 16 bits: the numbers are rounded against the scale that is stored, so its
-// own rounding (2^-8 of itself) costs nothing beyond the half step of the number.  A group with a NaN or an infinity gets the scale NaN.
-// Bytes: the rows once, 4.25 or 4.5 bits per number out.  A CTA takes 16 (hd 128) or 32 consecutive rows of one head: as a rule one or two
-// tiles of the pool.  What bounds it after the memory is instructions (83 % of the issue slots when shapes were run-time values and
-// rows were found by division: 8191 rows × 32 heads × 128 took 181 µs).
+__device__ __forceinline__ float max3(float x, float y, float z) {      // NaN if one is
+    float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z)); return d;
+}
+
+// A lane holds sixteen consecutive numbers of one row of K or V; 2 or 4 lanes make a group and find its largest magnitude with
+// shuffles.  scale = bf16(max / 7); the number is x · (1 / scale) rounded half away from zero — the f32 arithmetic of
+// Int4Tensor::quantize with a scale of 16 bits: the numbers are rounded against the scale that is stored, so its own rounding (2^-8 of
+// itself) costs nothing beyond the half step of the number, and no number passes 7 · (1 + 2^-7) before it is rounded: 7 is the largest.
+// A group with a NaN or an infinity gets the scale NaN.
+// Bytes: the rows once, 4.25 or 4.5 bits per number out.  A CTA takes 32 (hd 128) or 64 consecutive rows of one head: as a rule a few whole
+// tiles of the pool.  What bounds it beside the memory is instructions: with run-time shapes and rows found by division 8191 rows × 32
+// heads × 128 took 181 µs, with eight numbers a lane and integer packing 76 µs.
 template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(256) ax_p4_append_kernel(const RowArgs a) {
-    constexpr int LANES = HD / 8, GL = GS / 8, TOKENS = 256 / LANES;          // lanes per row, lanes per group, rows per CTA
+    constexpr int LANES = HD / 16, GL = GS / 16, TOKENS = 256 / LANES;        // lanes per row, lanes per group, rows per CTA
     const int li = threadIdx.x % LANES, tok = blockIdx.x * TOKENS + threadIdx.x / LANES, head = blockIdx.y, which = blockIdx.z;
     const AxP4Shape sh = fixed_shape<HD, GS>(a.s);
     const bool live = tok < a.n;
-    float x[8] = {};
+    float x[16] = {};
     float top = 0.f;
     int slot = -1;
-    bool odd = false;
     if (live) {
         slot = a.slots[tok];
         const T* src = which ? (const T*)a.v + tok * a.v_tok + head * a.v_head : (const T*)a.k + tok * a.k_tok + head * a.k_head;
-        load8<T>(src + 8 * li, x);
-        float all = 0.f;                                             // NaN as soon as one number is not finite
+        load8<T>(src + 16 * li, reinterpret_cast<float (&)[8]>(x[0]));
+        load8<T>(src + 16 * li + 8, reinterpret_cast<float (&)[8]>(x[8]));
 #pragma unroll
-        for (int i = 0; i < 8; i++) { top = fmaxf(top, fabsf(x[i])); all = fmaf(x[i], 0.f, all); }
-        if (all != all) top = __int_as_float(0x7F800000);
+        for (int i = 0; i < 16; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
     }
 #pragma unroll
-    for (int d = 1; d < GL; d <<= 1) top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, d));
+    for (int d = 1; d < GL; d <<= 1) { const float o = __shfl_xor_sync(AX_FULL, top, d); top = max3(top, o, o); }
     if (!live || slot < 0) return;                                   // a negative slot marks an absent row
     if (slot >= sh.n_pages * sh.page_size) { if (li == 0) atomicExch(a.err, AX_DEVERR_SLOT); return; }
-    odd = top > 3.402823466e38f;
+    const bool odd = !(top <= 3.402823466e38f);
     uint16_t sb = ax_f32_to_bf16_rne(__fdiv_rn(top, 7.0f));
     float sc = ax_bf16_to_f32(sb);
     if (sc < 1.17549435e-38f) { sc = 1.0f; sb = 0x3F80; }
     if (odd) { sc = 1.0f; sb = 0x7FC0; }
     const float inv = __frcp_rn(sc);
-    uint32_t w = 0;
+    uint32_t half[4];                                                // four numbers each
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        // |y| + (1/2 − 2^-25), cut off: rounds half away from zero for |y| < 8.  Added to 2^23 with rounding toward zero the whole part is
-        // the low bits of the sum.
-        const float y = __fmul_rn(x[i], inv);
-        const int m = __float_as_int(__fadd_rz(fminf(fabsf(y) + 0.49999997f, 7.5f), 8388608.f)) & 15;
-        w |= (uint32_t)(8 + (y < 0.f ? -m : m)) << (4 * i);
+    for (int i = 0; i < 4; i++) {
+        // |y| + (1/2 − 2^-25) + 2^23, the second sum cut off: rounds half away from zero for |y| < 8.  Σ number · 16^j is exact in f32, and so
+        // is the sum with 1.5 · 2^23 + 0x8888, whose low bits are the four nibbles.
+        float w = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float y = __fmul_rn(x[4 * i + j], inv);
+            const float m = __fadd_rz(fabsf(y) + 0.49999997f, 8388608.f) - 8388608.f;
+            w = fmaf(copysignf(m, y), (float)(1 << (4 * j)), w);
+        }
+        half[i] = odd ? 0x8888u : (uint32_t)__float_as_int(w + (12582912.f + 34952.f)) & 0xFFFFu;
     }
-    if (odd) w = 0x88888888u;
     int page, off;
     slot_place(a, slot, page, off);
     const int r = off % AX_P4_TILE;
     uint8_t* tile = a.pool + ax_p4_tile_at(sh, page, head, off);
     const int plane = ax_p4_plane_bytes(sh);
     if (which == 0) {
-        reinterpret_cast<uint32_t*>(tile)[ax_p4_k_word(sh, r, 8 * li)] = w;
+        uint32_t* kp = reinterpret_cast<uint32_t*>(tile);
+        const uint32_t w0 = half[0] | (half[1] << 16), w1 = half[2] | (half[3] << 16);
+        if (GS == 64) *reinterpret_cast<uint2*>(kp + ax_p4_k_word(sh, r, 16 * li)) = make_uint2(w0, w1);      // one thread's pair of words
+        else { kp[ax_p4_k_word(sh, r, 16 * li)] = w0; kp[ax_p4_k_word(sh, r, 16 * li + 8)] = w1; }
     } else {
         uint16_t* vp = reinterpret_cast<uint16_t*>(tile + plane);
-        vp[ax_p4_v_half(sh, r, 8 * li)] = (uint16_t)(w & 0xFFFFu);
-        vp[ax_p4_v_half(sh, r, 8 * li + 4)] = (uint16_t)(w >> 16);
+#pragma unroll
+        for (int i = 0; i < 4; i++) vp[ax_p4_v_half(sh, r, 16 * li + 4 * i)] = (uint16_t)half[i];
     }
     if (li % GL == 0) {
         uint16_t* sp = reinterpret_cast<uint16_t*>(tile + 2 * plane + which * ax_p4_scale_bytes(sh));
@@ -275,7 +285,7 @@ __global__ void __launch_bounds__(256) ax_p4_read_kernel(const RowArgs a) {
 
 template <typename T, bool READ>
 void launch_rows(const RowArgs& a, cudaStream_t stream) {
-    const int tokens = 256 / (a.s.hd / 8);
+    const int tokens = 256 / (a.s.hd / (READ ? 8 : 16));
     const dim3 grid((unsigned)((a.n + (long long)tokens - 1) / tokens), (unsigned)a.s.n_kv, READ ? 1u : 2u);
 #define AX_ROWS(HD, GS) do { if (READ) ax_p4_read_kernel<T, HD, GS><<<grid, 256, 0, stream>>>(a); \
                              else ax_p4_append_kernel<T, HD, GS><<<grid, 256, 0, stream>>>(a); } while (0)

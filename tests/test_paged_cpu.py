@@ -74,6 +74,30 @@ def test_lanes_find_their_operands(idx, hd, group):
             assert (half // 2) % w == (d // group) * (group // 32) + ((d % group) % (group // 8)) // 4
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_groups_of_64_keep_a_threads_two_k_words_together(idx, hd):
+    """The pair that is written as one 8-byte word."""
+    for r in range(16):
+        for d in range(0, hd, 16):
+            w = idx.k_word(hd, 64, r, d)
+            assert w % 2 == 0 and idx.k_word(hd, 64, r, d + 8) == w + 1
+
+
+def test_numbers_are_rounded_half_away_from_zero():
+    """|y| + (1/2 − 2^-25) + 2^23 with the second sum cut off, in f32, next to every border below 8."""
+    f = np.float32
+    for k in range(8):
+        for c in (f(k), f(k + 0.5)):
+            y = c
+            for _ in range(4):
+                y = np.nextafter(y, f(-1))
+            for _ in range(9):
+                if 0 <= y < 7.5:
+                    s = f(y) + f(0.49999997)
+                    assert np.floor(np.float64(s)) == np.floor(np.float64(y) + 0.5), y
+                y = np.nextafter(y, f(100))
+
+
 def test_tiles_stay_inside_the_pool(idx):
     for n, p, k, hd, g in itertools.product((1, 3), (16, 48, 128), (1, 5), (64, 128), (32, 64)):
         size, total = idx.tile_bytes(n, p, k, hd, g), idx.pool_bytes(n, p, k, hd, g)
