@@ -229,63 +229,53 @@ __global__ void __launch_bounds__(256) ax_p4_append_kernel(const RowArgs a) {
     }
 }
 
-template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]);
-template <> __device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+template <typename T> __device__ __forceinline__ void store4(T* p, const float (&x)[4]);
+template <> __device__ __forceinline__ void store4<float>(float* p, const float (&x)[4]) { __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3])); }
+template <> __device__ __forceinline__ void store4<uint16_t>(uint16_t* p, const float (&x)[4]) {
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(ax_f32_to_bf16_rne(x[0]) | ((uint32_t)ax_f32_to_bf16_rne(x[1]) << 16),
+                                                   ax_f32_to_bf16_rne(x[2]) | ((uint32_t)ax_f32_to_bf16_rne(x[3]) << 16)));
 }
-template <> __device__ __forceinline__ void store8<uint16_t>(uint16_t* p, const float (&x)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = ax_f32_to_bf16_rne(x[2 * i]) | ((uint32_t)ax_f32_to_bf16_rne(x[2 * i + 1]) << 16);
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <> __device__ __forceinline__ void store8<__half>(__half* p, const float (&x)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) { const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&h); }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+template <> __device__ __forceinline__ void store4<__half>(__half* p, const float (&x)[4]) {
+    const __half2 h0 = __floats2half2_rn(x[0], x[1]), h1 = __floats2half2_rn(x[2], x[3]);
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1)));
 }
 
 // The values a slot holds: number · scale, exact in f32 (4 + 8 bits), one rounding for the 16-bit types.  Absent rows read as zeros.
+// A lane makes four numbers of K and of V, so that a warp's store is one run of bytes (with eight a lane, 32 bytes apart, 8191 rows × 32
+// heads × 128 took 75 µs in f32).
 template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(256) ax_p4_read_kernel(const RowArgs a) {
-    constexpr int LANES = HD / 8, GL = GS / 8, TOKENS = 256 / LANES;
+    constexpr int LANES = HD / 4, TOKENS = 256 / LANES;
     const int li = threadIdx.x % LANES, tok = blockIdx.x * TOKENS + threadIdx.x / LANES, head = blockIdx.y;
     if (tok >= a.n) return;
     const AxP4Shape sh = fixed_shape<HD, GS>(a.s);
     const int slot = a.slots[tok];
-    float k[8], v[8];
+    float k[4] = {}, v[4] = {};
     if (slot >= 0 && slot < sh.n_pages * sh.page_size) {
         int page, off;
         slot_place(a, slot, page, off);
-        const int r = off % AX_P4_TILE;
+        const int r = off % AX_P4_TILE, gr = 4 * li / GS;
         const uint8_t* tile = a.pool + ax_p4_tile_at(sh, page, head, off);
         const int plane = ax_p4_plane_bytes(sh);
-        const uint32_t kw = reinterpret_cast<const uint32_t*>(tile)[ax_p4_k_word(sh, r, 8 * li)];
-        const uint16_t* vp = reinterpret_cast<const uint16_t*>(tile + plane);
-        const uint32_t vw = vp[ax_p4_v_half(sh, r, 8 * li)] | ((uint32_t)vp[ax_p4_v_half(sh, r, 8 * li + 4)] << 16);
-        const uint16_t* sp = reinterpret_cast<const uint16_t*>(tile + 2 * plane);
-        const float ks = ax_bf16_to_f32(sp[ax_p4_scale(sh, r, li / GL)]);
-        const float vs = ax_bf16_to_f32(sp[AX_P4_TILE * (HD / GS) + ax_p4_scale(sh, r, li / GL)]);
+        // numbers 4 · li .. + 3: the low or high half of a K word, a half word of V
+        const uint32_t kw = reinterpret_cast<const uint16_t*>(tile)[2 * ax_p4_k_word(sh, r, 4 * li & ~7) + (li & 1)];
+        const uint32_t vw = reinterpret_cast<const uint16_t*>(tile + plane)[ax_p4_v_half(sh, r, 4 * li)];
+        const uint16_t* sp = reinterpret_cast<const uint16_t*>(tile + 2 * plane) + ax_p4_scale(sh, r, gr);
+        const float ks = ax_bf16_to_f32(sp[0]), vs = ax_bf16_to_f32(sp[AX_P4_TILE * (HD / GS)]);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {                                // 2^23 + nibble − (2^23 + 8): no conversion instruction
+        for (int i = 0; i < 4; i++) {                                // 2^23 + nibble − (2^23 + 8): no conversion instruction
             k[i] = (__int_as_float(0x4B000000 | ((kw >> (4 * i)) & 15u)) - 8388616.f) * ks;
             v[i] = (__int_as_float(0x4B000000 | ((vw >> (4 * i)) & 15u)) - 8388616.f) * vs;
         }
-    } else {
-        if (slot >= 0) atomicExch(a.err, AX_DEVERR_SLOT);
-#pragma unroll
-        for (int i = 0; i < 8; i++) { k[i] = 0.f; v[i] = 0.f; }
-    }
-    const size_t o = ((size_t)tok * sh.n_kv + head) * HD + 8 * li;
-    store8<T>((T*)a.k_out + o, k);
-    store8<T>((T*)a.v_out + o, v);
+    } else if (slot >= 0) atomicExch(a.err, AX_DEVERR_SLOT);
+    const size_t o = ((size_t)tok * sh.n_kv + head) * HD + 4 * li;
+    store4<T>((T*)a.k_out + o, k);
+    store4<T>((T*)a.v_out + o, v);
 }
 
 template <typename T, bool READ>
 void launch_rows(const RowArgs& a, cudaStream_t stream) {
-    const int tokens = 256 / (a.s.hd / (READ ? 8 : 16));
+    const int tokens = 256 / (a.s.hd / (READ ? 4 : 16));
     const dim3 grid((unsigned)((a.n + (long long)tokens - 1) / tokens), (unsigned)a.s.n_kv, READ ? 1u : 2u);
 #define AX_ROWS(HD, GS) do { if (READ) ax_p4_read_kernel<T, HD, GS><<<grid, 256, 0, stream>>>(a); \
                              else ax_p4_append_kernel<T, HD, GS><<<grid, 256, 0, stream>>>(a); } while (0)
