@@ -27,7 +27,7 @@ constexpr int kStages = 4;
 constexpr int kCtasPerSm = 3;
 constexpr int kMinTiles = 2;                    // tiles of a warp below which fewer CTAs share the work
 constexpr int kHeads = 8;                       // query heads of one segment
-constexpr int kChunk = 128;                     // parts of a segment whose weights are in shared memory at a time
+constexpr int kChunk = 64;                      // parts of a segment whose weights are in shared memory at a time
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr int kErrWait = 711;
 
@@ -78,10 +78,10 @@ __device__ __forceinline__ uint32_t n_high(uint32_t w) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(and_or(w, 0x00F000F0u, 0x64006400u)), "r"(0x2C002C00u), "r"(0xD480D480u));
     return r;
 }
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 template <int N> __device__ __forceinline__ void lds(uint32_t (&r)[N], const void* p) {
     if constexpr (N == 4) { const uint4 v = *(const uint4*)p; r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
@@ -114,9 +114,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     __shared__ int s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int batch = dv.a.batch, hpt = dv.hpt;
-    uint8_t* ring = smem + warp * kStages * TILE;
-    float* s_o = reinterpret_cast<float*>(smem + kWarps * kStages * TILE);                 // [2 · warps][hpt][HD]
-    unsigned* s_pre = reinterpret_cast<unsigned*>(s_o + (size_t)kWarps * 2 * hpt * HD);    // [batch + 1] tiles before each request
+    // Shared memory: per warp its ring, its query operand, and the output of a first segment that ends within its piece; the output of the
+    // last segment goes over the ring, which is empty by then.  Then [batch + 1] tiles before each request.
+    constexpr int RING = kStages * TILE, QBYTES = W * 2 * 32 * 16;
+    const int own = RING + QBYTES + hpt * HD * 4;
+    uint8_t* ring = smem + warp * own;
+    uint4* s_q = reinterpret_cast<uint4*>(ring + RING);                                     // [step][lane]
+    auto s_o = [&](int slot) { return reinterpret_cast<float*>(smem + (slot >> 1) * own + (slot & 1 ? 0 : RING + QBYTES)); };
+    unsigned* s_pre = reinterpret_cast<unsigned*>(smem + kWarps * own);
 
     if (tid < kWarps * kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(smem_u32(&s_bar[tid / kStages][tid % kStages])) : "memory");
     if (tid < kWarps * 2) s_seg[tid] = -1;
@@ -156,7 +161,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     const int count = (int)(x1 - x0);
     const uint8_t* src = nullptr;
     TileInfo mine = {};
-    auto fill = [&](int i) {                                                  // i uniform over the warp, rising by one
+    auto fill = [&](int i, int st) {                                          // i uniform over the warp, rising by one; st: its stage
         if (i >= count) return;
         if ((i & 31) == 0) {
             const long long y = x0 + i + lane;
@@ -179,7 +184,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             }
         }
         if (lane == (i & 31)) {
-            const int st = i & (kStages - 1);
             const uint32_t bar = smem_u32(&s_bar[warp][st]);
             s_info[warp][st] = mine;
             if (mine.ok) {
@@ -191,11 +195,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             }
         }
     };
-    for (int i = 0; i < kStages; i++) fill(i);
+    for (int i = 0; i < kStages; i++) fill(i, i);
     __syncwarp();
 
     // ── state of the segment at hand ──
-    uint32_t qa[W * 2][4];                      // operand of the scores: step 2·w + h of word w
     float qback = 1.f;                          // the power of two that the query was divided by
     float o[NT][4], m = -INFINITY, l = 0.f;
     int seg = -1, seg_lo = 0, seg_len = 0;
@@ -229,13 +232,16 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
 #pragma unroll
         for (int w = 0; w < W; w++)
 #pragma unroll
-            for (int p = 0; p < 4; p++) {                                      // pair (p, p + 4) of the word
-                const float y0 = x[w][p] * up, y1 = x[w][p + 4] * up;
-                const uint32_t hi = pack_f16(y0, y1);
-                const float2 h = unpack_f16(hi);
-                const uint32_t lo = pack_f16(y0 - h.x, y1 - h.y);
-                qa[2 * w + p / 2][(p & 1) * 2] = hi;
-                qa[2 * w + p / 2][(p & 1) * 2 + 1] = lo;
+            for (int h = 0; h < 2; h++) {                                      // step 2 · w + h: pairs (p, p + 4) of the word for p = 2h, 2h + 1
+                uint32_t q4[4];
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    const float y0 = x[w][2 * h + p] * up, y1 = x[w][2 * h + p + 4] * up;
+                    q4[2 * p] = pack_f16(y0, y1);
+                    const float2 r = unpack_f16(q4[2 * p]);
+                    q4[2 * p + 1] = pack_f16(y0 - r.x, y1 - r.y);
+                }
+                s_q[(2 * w + h) * 32 + lane] = make_uint4(q4[0], q4[1], q4[2], q4[3]);      // read by this lane alone
             }
 #pragma unroll
         for (int i = 0; i < NT; i++) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
@@ -271,45 +277,50 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             const int slot = warp * 2 + (s0 < x0 ? 0 : 1);
             if (lane == 0) s_seg[slot] = seg;
             if (t == 0) { s_ml[slot][g][0] = m; s_ml[slot][g][1] = l; }
-            if (live) put(s_o + ((size_t)slot * hpt + g) * HD, 1.f);
+            if (live) put(s_o(slot) + g * HD, 1.f);
         }
     };
 
+    int st = 0;
+    uint32_t phase = 0;
     for (int it = 0; it < count; it++) {
-        const int st = it & (kStages - 1);
-        if (!mbar_wait(smem_u32(&s_bar[warp][st]), (uint32_t)(it / kStages) & 1u)) {
+        if (!mbar_wait(smem_u32(&s_bar[warp][st]), phase)) {
             if (lane == 0) atomicExch(dv.err, kErrWait);
             for (int y = it; y < count && y < it + kStages; y++)              // what is in flight lands before the CTA goes
-                mbar_wait(smem_u32(&s_bar[warp][y & (kStages - 1)]), (uint32_t)(y / kStages) & 1u);
+                mbar_wait(smem_u32(&s_bar[warp][y % kStages]), (uint32_t)(y / kStages) & 1u);
             break;
         }
         const TileInfo info = s_info[warp][st];
         if (info.seg != seg) { if (seg >= 0) flush(); start(info.seg); }
         if (info.ok) {
             const uint8_t* tile = ring + st * TILE;
-            float s[4];                                                       // (block 0: columns 2t, 2t + 1), (block 1: …)
+            float s[4] = { 0.f, 0.f, 0.f, 0.f };                              // (block 0: columns 2t, 2t + 1), (block 1: …)
+            uint32_t kw[2][W], ks[2][NG];
 #pragma unroll
             for (int nt = 0; nt < 2; nt++) {
-                uint32_t kw[W], sw[NG];
-                lds<W>(kw, tile + nt * (PLANE / 2) + lane * W * 4);
-                lds<NG>(sw, tile + 2 * PLANE + (8 * nt + 2 * t) * NG * 2);
-                float s0 = 0.f, s1 = 0.f;
+                lds<W>(kw[nt], tile + nt * (PLANE / 2) + lane * W * 4);
+                lds<NG>(ks[nt], tile + 2 * PLANE + (8 * nt + 2 * t) * NG * 2);
+            }
 #pragma unroll
-                for (int gr = 0; gr < NG; gr++) {
-                    float d[4] = { 0.f, 0.f, 0.f, 0.f };
+            for (int gr = 0; gr < NG; gr++) {
+                float d[2][4] = {};
 #pragma unroll
-                    for (int i = 0; i < WG; i++) {
-                        const uint32_t w = kw[gr * WG + i], v = w >> 8;
-                        mma(d, qa[2 * (gr * WG + i)], n_low(w), n_high(w));
-                        mma(d, qa[2 * (gr * WG + i) + 1], n_low(v), n_high(v));
+                for (int i = 0; i < WG; i++) {
+                    const uint4 q0 = s_q[(2 * (gr * WG + i)) * 32 + lane], q1 = s_q[(2 * (gr * WG + i) + 1) * 32 + lane];
+#pragma unroll
+                    for (int nt = 0; nt < 2; nt++) {
+                        const uint32_t w = kw[nt][gr * WG + i], v = w >> 8;
+                        mma(d[nt], q0, n_low(w), n_high(w));
+                        mma(d[nt], q1, n_low(v), n_high(v));
                     }
-                    // scales of columns 2t and 2t + 1, NG numbers each
-                    const float k0 = gr & 1 ? ax_bf16_hi(sw[gr / 2]) : ax_bf16_lo(sw[gr / 2]);
-                    const float k1 = (NG + gr) & 1 ? ax_bf16_hi(sw[(NG + gr) / 2]) : ax_bf16_lo(sw[(NG + gr) / 2]);
-                    s0 = fmaf(k0, d[0] + d[2], s0);
-                    s1 = fmaf(k1, d[1] + d[3], s1);
                 }
-                s[2 * nt] = s0; s[2 * nt + 1] = s1;
+#pragma unroll
+                for (int nt = 0; nt < 2; nt++) {                               // scales of columns 2t and 2t + 1, NG numbers each
+                    const float k0 = gr & 1 ? ax_bf16_hi(ks[nt][gr / 2]) : ax_bf16_lo(ks[nt][gr / 2]);
+                    const float k1 = (NG + gr) & 1 ? ax_bf16_hi(ks[nt][(NG + gr) / 2]) : ax_bf16_lo(ks[nt][(NG + gr) / 2]);
+                    s[2 * nt] = fmaf(k0, d[nt][0] + d[nt][2], s[2 * nt]);
+                    s[2 * nt + 1] = fmaf(k1, d[nt][1] + d[nt][3], s[2 * nt + 1]);
+                }
             }
             const int row = info.tile * AX_P4_TILE;
             const bool edge = row < seg_lo || row + AX_P4_TILE > seg_len;
@@ -368,15 +379,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             for (int nt = 0; nt < 2; nt++) lds<W>(vw[nt], tile + PLANE + nt * (PLANE / 2) + lane * W * 4);
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) {
-                uint32_t a[4];
+                uint32_t hl[4];
 #pragma unroll
                 for (int nt = 0; nt < 2; nt++) {
                     const float y0 = p[2 * nt] * vs[2 * nt][gr], y1 = p[2 * nt + 1] * vs[2 * nt + 1][gr];
-                    const uint32_t hi = pack_f16(y0, y1);
-                    const float2 h = unpack_f16(hi);
-                    a[2 * nt] = hi;
-                    a[2 * nt + 1] = pack_f16(y0 - h.x, y1 - h.y);
+                    hl[2 * nt] = pack_f16(y0, y1);
+                    const float2 h = unpack_f16(hl[2 * nt]);
+                    hl[2 * nt + 1] = pack_f16(y0 - h.x, y1 - h.y);
                 }
+                const uint4 a = make_uint4(hl[0], hl[1], hl[2], hl[3]);
 #pragma unroll
                 for (int i = 0; i < WG; i++) {
                     const int cw = gr * WG + i;
@@ -390,9 +401,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             }
         }
         __syncwarp();                                                          // every lane has read the stage
-        fill(it + kStages);
+        fill(it + kStages, st);
         __syncwarp();
+        if (++st == kStages) { st = 0; phase ^= 1u; }
     }
+    __syncwarp();                                                              // the ring is read by all lanes before the last output goes over it
     if (seg >= 0) flush();
     __syncthreads();
 
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             for (int k = i; k < j; k++)
                 if (s_seg[k] == sg && s_ml[k][h][1] != 0.f) {
                     const float f = s_ml[k][h][0] == M ? 1.f : ex2(s_ml[k][h][0] - M);
-                    const float4 v = *(const float4*)(s_o + ((size_t)k * hpt + h) * HD + d);
+                    const float4 v = *(const float4*)(s_o(k) + h * HD + d);
                     L = fmaf(f, s_ml[k][h][1], L);
                     A.x = fmaf(f, v.x, A.x); A.y = fmaf(f, v.y, A.y); A.z = fmaf(f, v.z, A.z); A.w = fmaf(f, v.w, A.w);
                 }
@@ -442,7 +455,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 const float* ml = dv.part_ml + 2 * (size_t)cf * hpt * 2;
                 const float* po = dv.part_o + 2 * (size_t)cf * hpt * HD;
                 auto part = [&](int k) { return (size_t)(2 * k + (k == 0)) * hpt; };
-                float* wt = reinterpret_cast<float*>(smem);                                       // the ring is free: weights of kChunk parts, per head
+                float* wt = reinterpret_cast<float*>(smem + RING);                                // weights of kChunk parts per head, over the first warp's query
+                static_assert(kHeads * kChunk * 4 <= QBYTES, "weights do not fit");
                 for (int h = warp; h < heads; h += kWarps) {
                     float M = -INFINITY;
                     for (int k = lane; k < cnt; k += 32) M = fmaxf(M, __ldcg(ml + (part(k) + h) * 2));
@@ -541,7 +555,7 @@ int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPage
     dv.part_ml = (float*)(w + ticket_bytes(grid));
     dv.part_o = dv.part_ml + (size_t)2 * grid * kHeads * 2;
     const int tile = ax_p4_tile_bytes(kv->s);
-    const size_t smem = (size_t)kWarps * kStages * tile + (size_t)kWarps * 2 * dv.hpt * kv->s.hd * 4 + (size_t)(a.batch + 1) * 4;
+    const size_t smem = (size_t)kWarps * (kStages * tile + kv->s.hd / 32 * 2 * 32 * 16 + dv.hpt * kv->s.hd * 4) + (size_t)(a.batch + 1) * 4;
     if (kv->s.hd == 128) return kv->s.group == 32 ? launch<128, 32>(ctx, dv, grid, smem) : launch<128, 64>(ctx, dv, grid, smem);
     return kv->s.group == 32 ? launch<64, 32>(ctx, dv, grid, smem) : launch<64, 64>(ctx, dv, grid, smem);
 }
