@@ -12,11 +12,13 @@
 //     more than 2^8 — sums are f32 and any reference between is exact — so the rescaling almost never runs.
 //   * While the softmax of one query tile runs, the tensor core has the other's products.
 //   * K and V tiles of 128 keys come by tiled bulk copies through one ring of shared-memory stages: K0 V0 K1 V1 …
-//   * Which sequence and rows a CTA owns it finds in the prefix array itself, late (long) row tiles first: nothing depends on host-side
-//     lengths, and a captured call follows the arrays.
+//   * An item is one pair of query tiles; there is a CTA for each, late (long) row tiles of all heads first.  A CTA that runs takes over the
+//     items of CTAs that have not started (clusterlaunchcontrol: the hardware hands them out, no counter in memory): its copies and
+//     first scores of the next item run under the end of the one before (a CTA per item spent 5 to 7 µs starting and ending).  A warp of its
+//     own finds sequence and rows in the prefix arrays: nothing depends on host-side lengths, and a captured call follows the arrays.
 //   * A product of 0 and a NaN or infinity in a value row that the query does not see would be NaN: value rows behind the sequence are
 //     zeroed in shared memory, and an output row that is not finite is taken again by ax_prompt_row, which reads visible rows only.
-//   * Every wait is bounded (two seconds of %globaltimer): on expiry the CTA raises the context's error word, all roles leave, copies
+//   * Every wait is bounded (ten seconds of %globaltimer): on expiry the CTA raises the context's error word, all roles leave, copies
 //     in flight are waited for and tensor memory is released.
 #include <cuda.h>
 #include <type_traits>
@@ -29,10 +31,14 @@ constexpr int kRows = 128;                        // rows of a query tile, keys 
 constexpr int kFirst = 64;                        // keys whose probabilities are handed over first; the rest ends the tile's chain
 constexpr int kBoxBytes = kRows * 128;            // one box: 128 rows of 128 bytes
 constexpr int kThreads = 384;                     // warps 0..3, 4..7: softmax of tile 0, 1; 8: products; 9: copies; 10: the end of a
-                                                  // sequence's last V tile; 11 completes the warpgroup that hands registers over
-constexpr int kProduct = 8, kCopy = 9, kCut = 10;
+                                                  // sequence's last V tile; 11: items
+constexpr int kProduct = 8, kCopy = 9, kItems = 11;
+constexpr int kSlots = 2;                         // items known ahead
+constexpr int kReaders = 11;                      // arrivals that free an item's slot: eight softmax warps, products, copies, cut
 constexpr int kMaxStages = 6;
-constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr unsigned long long kWaitNs = 10000000000ull;      // rows that are taken again one by one may hold the others up
+
+constexpr unsigned long long kAbortNs = 5000000ull;          // after a failure: what is in flight lands within microseconds
 
 struct PromptDev {
     AxPromptArgs a;
@@ -172,6 +178,37 @@ __device__ __noinline__ void row_again(const AxPromptArgs& a, const AxPromptSeq&
     ax_prompt_row<T, HD>(a, s, h, i, lane);
 }
 
+// A pair of query tiles: rows [q0, q0 + lq) and keys [k0, k0 + lk) of its sequence, first row of the pair, first head.  lq < 0: no more.
+struct Item { int q0, lq, k0, lk, base, h0; };
+// What every role derives from it.
+struct Work {
+    AxPromptSeq s;
+    int off, h0, base0, base1;                    // key at a query's own position = row + off
+    int lo0, hi0, lo1, hi1, j0, j1;               // K / V tiles [lo, hi] of both query tiles, and of the pair; hi < lo: none
+    bool on0, on1, cut;                           // cut: the last V tile reaches behind the sequence
+};
+__device__ __forceinline__ Work work_of(const PromptDev& dv, const Item& it) {
+    Work w;
+    w.s.q0 = it.q0; w.s.lq = it.lq; w.s.k0 = it.k0; w.s.lk = it.lk;
+    w.off = it.lk - it.lq; w.h0 = it.h0;
+    w.base0 = it.base; w.base1 = dv.pair_heads ? it.base : it.base + kRows;
+    auto range = [&](int base, int& lo, int& hi) {
+        const int last = min(base + kRows, it.lq) - 1 + w.off, first = base + w.off;
+        lo = 0; hi = -1;
+        if (base < it.lq && last >= 0 && it.lk > 0) {
+            lo = dv.a.window > 0 && first - dv.a.window + 1 > 0 ? (first - dv.a.window + 1) / kRows : 0;
+            hi = last / kRows;
+        }
+    };
+    range(w.base0, w.lo0, w.hi0); range(w.base1, w.lo1, w.hi1);
+    w.on0 = w.hi0 >= w.lo0; w.on1 = w.hi1 >= w.lo1;
+    w.j0 = w.on0 ? (w.on1 ? min(w.lo0, w.lo1) : w.lo0) : w.lo1;
+    w.j1 = max(w.hi0, w.hi1);
+    if (w.j1 < w.j0) w.j1 = w.j0 - 1;
+    w.cut = w.j1 >= w.j0 && (w.j1 + 1) * kRows > it.lk;
+    return w;
+}
+
 template <bool F16, int HD>
 __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                      const __grid_constant__ CUtensorMap map_k,
@@ -180,48 +217,30 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     constexpr int BOXES = HD / 64, TILE = BOXES * kBoxBytes, NS = HD == 128 ? 5 : 6;
     constexpr uint32_t kS = 0, kO = 256;                                      // columns: scores of tile t at 128 t (its probabilities over the first half), output at 256 + HD t
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_ready[2][2], o_done[2], kv_full[kMaxStages], kv_empty[kMaxStages], v_here, v_cut;
+    __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2][2], o_done[2], o_free[2], kv_full[kMaxStages], kv_empty[kMaxStages],
+        v_here, v_cut, i_full[kSlots], i_empty[kSlots], clc_bar;
+    __shared__ __align__(16) uint4 s_clc;
+    __shared__ __align__(16) Item s_item[kSlots];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_issued, s_seq, s_tile, s_scan[kThreads / 32];
+    __shared__ int s_abort, s_issued;
     const int tid = threadIdx.x, warp = __shfl_sync(AX_FULL, tid >> 5, 0), lane = tid & 31;
     const AxPromptArgs& a = dv.a;
     volatile int* abort_flag = &s_abort;
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t ring = smem0 + 2 * TILE;
 
-    // ── which rows: tile x of the pack counted from its end ──
-    const int tb = dv.pair_heads ? kRows : 2 * kRows;
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(smem_u32(&q_full[i]), 1); mbar_init(smem_u32(&s_full[i]), 1); mbar_init(smem_u32(&o_done[i]), 1);
+            mbar_init(smem_u32(&q_full[i]), 1); mbar_init(smem_u32(&q_empty[i]), 1); mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&o_done[i]), 1); mbar_init(smem_u32(&o_free[i]), kRows);
             for (int b = 0; b < 2; b++) mbar_init(smem_u32(&p_ready[i][b]), kRows);
         }
         for (int i = 0; i < NS; i++) { mbar_init(smem_u32(&kv_full[i]), 1); mbar_init(smem_u32(&kv_empty[i]), 1); }
-        mbar_init(smem_u32(&v_here), 1); mbar_init(smem_u32(&v_cut), 1);
-        s_abort = 0; s_issued = 0; s_seq = -1; s_tile = 0;
+        for (int i = 0; i < kSlots; i++) { mbar_init(smem_u32(&i_full[i]), 1); mbar_init(smem_u32(&i_empty[i]), kReaders); }
+        mbar_init(smem_u32(&v_here), 1); mbar_init(smem_u32(&v_cut), 1); mbar_init(smem_u32(&clc_bar), 1);
+        s_abort = 0; s_issued = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    {
-        const int per = (a.batch + kThreads - 1) / kThreads, b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-        int own = 0;
-        for (int b = b0; b < b1; b++) own += (ax_prompt_seq(a, b).lq + tb - 1) / tb;
-        int inc = own;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) { const int x = __shfl_up_sync(AX_FULL, inc, d); if (lane >= d) inc += x; }
-        if (lane == 31) s_scan[warp] = inc;
-        __syncthreads();
-        int at = inc - own, all = 0;
-#pragma unroll
-        for (int w = 0; w < kThreads / 32; w++) { if (w < warp) at += s_scan[w]; all += s_scan[w]; }
-        const int x = all - 1 - (int)blockIdx.y;
-        if (x < 0) return;
-        if (x >= at && x < at + own)
-            for (int b = b0; b < b1; b++) {
-                const int n = (ax_prompt_seq(a, b).lq + tb - 1) / tb;
-                if (x < at + n) { s_seq = b; s_tile = x - at; break; }
-                at += n;
-            }
     }
     if (warp == kProduct) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&s_tmem)) : "memory");
@@ -231,57 +250,130 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
-    const AxPromptSeq s = ax_prompt_seq(a, s_seq);
-    const int off = s.lk - s.lq;
-    const int h0 = dv.pair_heads ? 2 * (int)blockIdx.x : (int)blockIdx.x, kh = h0 / (a.n_heads / a.n_kv);
-    int base[2], lo[2], hi[2];                                                // first row and K / V tiles [lo, hi] of both query tiles
-    base[0] = s_tile * tb; base[1] = dv.pair_heads ? base[0] : base[0] + kRows;
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const int last = min(base[t] + kRows, s.lq) - 1 + off, first = base[t] + off;
-        lo[t] = 0; hi[t] = -1;
-        if (base[t] < s.lq && last >= 0 && s.lk > 0) {
-            lo[t] = a.window > 0 && first - a.window + 1 > 0 ? (first - a.window + 1) / kRows : 0;
-            hi[t] = last / kRows;
-        }
-    }
-    const bool on0 = hi[0] >= lo[0], on1 = hi[1] >= lo[1];
-    const int j0 = on0 ? (on1 ? min(lo[0], lo[1]) : lo[0]) : lo[1], j1 = max(hi[0], hi[1]);      // j1 < j0: no tile at all
-    const bool cut = j1 >= j0 && (j1 + 1) * kRows > s.lk;                     // the last V tile reaches behind the sequence
+    // the n-th item of this CTA, for every reader in turn; false: no more
+    auto item_at = [&](int n, Item& it) {
+        const int slot = n % kSlots;
+        if (!mbar_wait(smem_u32(&i_full[slot]), (uint32_t)(n / kSlots) & 1u, abort_flag, dv.err, 731)) return false;
+        it = *const_cast<const Item*>(&s_item[slot]);
+        return it.lq >= 0;
+    };
+    auto item_read = [&](int n) { mbar_arrive(smem_u32(&i_empty[n % kSlots])); };
 
     // 384 threads start with 168 registers each (64512 in all); a row of scores is 128 of them.  256 · 208 + 128 · 80 = 63488.
     if (warp >= kProduct) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == kCopy) {
+    if (warp == kItems) {
+        // Tiles of the sequences before each lane's share of them; then item after item: its tile counted from the pack's end.
+        const int tb = dv.pair_heads ? kRows : 2 * kRows, hx = dv.pair_heads ? a.n_heads / 2 : a.n_heads;
+        const int per = (a.batch + 31) / 32, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
+        int own = 0;
+        for (int b = b0; b < b1; b++) own += (ax_prompt_seq(a, b).lq + tb - 1) / tb;
+        int inc = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const int x = __shfl_up_sync(AX_FULL, inc, d); if (lane >= d) inc += x; }
+        const int before = inc - own, all = __shfl_sync(AX_FULL, inc, 31);
+        long long block = blockIdx.x;                                         // the CTA whose item is next
+        int n = 0;
+        uint32_t clc_phase = 0;
+        bool ok = true, more = true;
+        while (ok && more) {
+            // ask for the next CTA's place while this one's item is looked up
+            if (lane == 0) {
+                mbar_expect_tx(smem_u32(&clc_bar), 16);
+                asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                             :: "r"(smem_u32(&s_clc)), "r"(smem_u32(&clc_bar)) : "memory");
+            }
+            __syncwarp();
+            const int x = all - 1 - (int)(block / hx);
+            if (x >= 0) {
+                const int g = 31 - __clz((int)__ballot_sync(AX_FULL, x >= before && own > 0));       // the lane in whose share the tile lies
+                int at = __shfl_sync(AX_FULL, before, g);
+                const int c0 = min(g * per, a.batch), c1 = min(c0 + per, a.batch);
+                Item it = {};
+                for (int c = c0; c < c1; c += 32) {
+                    const int b = c + lane;
+                    AxPromptSeq q = {};
+                    if (b < c1) q = ax_prompt_seq(a, b);
+                    const int mine = (q.lq + tb - 1) / tb;
+                    int up = mine;
+#pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) { const int y = __shfl_up_sync(AX_FULL, up, d); if (lane >= d) up += y; }
+                    const unsigned hit = __ballot_sync(AX_FULL, x >= at + up - mine && x < at + up);
+                    if (hit) {
+                        const int l = __ffs(hit) - 1;
+                        it.q0 = __shfl_sync(AX_FULL, q.q0, l); it.lq = __shfl_sync(AX_FULL, q.lq, l);
+                        it.k0 = __shfl_sync(AX_FULL, q.k0, l); it.lk = __shfl_sync(AX_FULL, q.lk, l);
+                        it.base = (x - __shfl_sync(AX_FULL, at + up - mine, l)) * tb;
+                        break;
+                    }
+                    at += __shfl_sync(AX_FULL, up, 31);
+                }
+                it.h0 = (int)(block % hx) * (dv.pair_heads ? 2 : 1);
+                if (n >= kSlots) ok = mbar_wait(smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, abort_flag, dv.err, 732);
+                ok = __all_sync(AX_FULL, ok);
+                if (ok && lane == 0) { s_item[n % kSlots] = it; mbar_arrive(smem_u32(&i_full[n % kSlots])); }
+                n++;
+            }
+            bool got = mbar_wait(smem_u32(&clc_bar), clc_phase, abort_flag, dv.err, 733);
+            if (!__all_sync(AX_FULL, got)) { ok = false; break; }
+            clc_phase ^= 1u;
+            uint32_t took, next;
+            asm volatile("{\n\t.reg .b128 r;\n\t.reg .pred p;\n\tld.shared.b128 r, [%2];\n\t"
+                         "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                         "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+                         : "=r"(took), "=r"(next) : "r"(smem_u32(&s_clc)) : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // read before the next answer is written
+            __syncwarp();
+            more = took != 0;
+            block = next;
+        }
+        if (ok) {
+            if (n >= kSlots) ok = mbar_wait(smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, abort_flag, dv.err, 732);
+            if (__all_sync(AX_FULL, ok) && lane == 0) { s_item[n % kSlots].lq = -1; mbar_arrive(smem_u32(&i_full[n % kSlots])); }
+        }
+        __syncwarp();
+    } else if (warp == kCopy) {
         if (elect_one()) {
-            for (int t = 0; t < 2; t++)
-                if (t ? on1 : on0) {
+            Item it;
+            int st = 0, nq[2] = { 0, 0 };
+            uint32_t ph = 1;                                                  // a fresh barrier counts as a phase of parity one that is over
+            bool ok = true;
+            for (int n = 0; ok && item_at(n, it); n++) {
+                item_read(n);
+                const Work w = work_of(dv, it);
+                const int kh = w.h0 / (a.n_heads / a.n_kv);
+                auto query = [&](int t) {
+                    ok = mbar_wait(smem_u32(&q_empty[t]), (uint32_t)(nq[t] + 1) & 1u, abort_flag, dv.err, 734);
+                    if (!ok) return;
+                    nq[t]++;
                     const uint32_t bar = smem_u32(&q_full[t]);
                     mbar_expect_tx(bar, TILE);
                     for (int b = 0; b < BOXES; b++)
-                        tma_load_3d(smem0 + t * TILE + b * kBoxBytes, &map_q, b * 64, dv.pair_heads ? h0 + t : h0, s.q0 + base[t], bar);
+                        tma_load_3d(smem0 + t * TILE + b * kBoxBytes, &map_q, b * 64, dv.pair_heads ? w.h0 + t : w.h0, w.s.q0 + (t ? w.base1 : w.base0), bar);
+                };
+                // The first K tile goes ahead of the queries: their places are free only when the item before has its last scores.
+                const int m = 2 * (w.j1 - w.j0 + 1);
+                for (int i = 0; i < m && ok; i++) {
+                    ok = mbar_wait(smem_u32(&kv_empty[st]), ph, abort_flag, dv.err, 721);
+                    if (!ok) break;
+                    const uint32_t bar = smem_u32(&kv_full[st]);
+                    mbar_expect_tx(bar, TILE);
+                    const CUtensorMap* map = i & 1 ? &map_v : &map_k;
+                    for (int b = 0; b < BOXES; b++) tma_load_3d(ring + st * TILE + b * kBoxBytes, map, b * 64, kh, w.s.k0 + (w.j0 + i / 2) * kRows, bar);
+                    s_issued++;
+                    if (++st == NS) { st = 0; ph ^= 1u; }
+                    if (i == 0) { if (w.on0) query(0); if (ok && w.on1) query(1); }
                 }
-            const int n = j1 >= j0 ? 2 * (j1 - j0 + 1) : 0;
-            int st = 0;
-            uint32_t ph = 1;                                                  // a fresh barrier counts as a phase of parity one that is over
-            for (int i = 0; i < n; i++) {
-                if (!mbar_wait(smem_u32(&kv_empty[st]), ph, abort_flag, dv.err, 721)) break;
-                const uint32_t bar = smem_u32(&kv_full[st]);
-                mbar_expect_tx(bar, TILE);
-                const CUtensorMap* map = i & 1 ? &map_v : &map_k;
-                for (int b = 0; b < BOXES; b++) tma_load_3d(ring + st * TILE + b * kBoxBytes, map, b * 64, kh, s.k0 + (j0 + i / 2) * kRows, bar);
-                s_issued = i + 1;
-                if (++st == NS) { st = 0; ph ^= 1u; }
             }
         }
+        __syncwarp();
     } else if (warp == kProduct) {
         constexpr uint32_t fmt = F16 ? 0u : 1u;                               // accumulator f32, A and B f16 or bf16; B of P·V is MN-major
         constexpr uint32_t id_qk = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kRows >> 3) << 17) | ((kRows >> 4) << 24);
         constexpr uint32_t id_pv = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((HD >> 3) << 17) | ((kRows >> 4) << 24);
-        // One thread does all of it.  Its loop counts from zero and tensor memory starts at column zero (all of it is ours), so that stages,
+        // One thread does all of it.  Its loops count from zero and tensor memory starts at column zero (all of it is ours), so that stages,
         // descriptors and columns are uniform values: with a vector register behind each, issuing a product took longer than the product.
         if (elect_one()) {
-            const int n = j1 - j0 + 1, a0 = lo[0] - j0, z0 = on0 ? hi[0] - j0 : -1, a1 = lo[1] - j0, z1 = on1 ? hi[1] - j0 : -1;   // tile t works at i in [a, z]
             bool ok = s_tmem == 0;
             if (!ok) { *abort_flag = 1; atomicExch(dv.err, 728); }
             auto qk = [&](int t, int st) {                                    // scores of query tile t with the K tile in stage st
@@ -293,58 +385,96 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 umma_commit(smem_u32(&s_full[t]));
             };
             int st = 0;                                                       // stages are taken in turn; ph: parity of their phase
-            uint32_t ph = 0;
+            uint32_t ph = 0, pq[2] = { 0, 0 }, pp[2] = { 0, 0 }, cuts = 0;    // parities of a tile's queries and probabilities, of the cuts
+            int items[2] = { 0, 0 };                                          // items a tile took part in
             auto next = [&] { if (++st == NS) { st = 0; ph ^= 1u; } };
-            if (n > 0 && ok) {
-                ok = mbar_wait(smem_u32(&kv_full[0]), 0, abort_flag, dv.err, 722);
-                if (ok && on0) { ok = mbar_wait(smem_u32(&q_full[0]), 0, abort_flag, dv.err, 723); if (ok && a0 == 0) qk(0, 0); }
-                if (ok && on1) { ok = mbar_wait(smem_u32(&q_full[1]), 0, abort_flag, dv.err, 723); if (ok && a1 == 0) qk(1, 0); }
-                if (ok) umma_commit(smem_u32(&kv_empty[0]));
-                next();
-            }
-            for (int i = 0; i < n && ok; i++) {
-                const int sv = st;
-                ok = mbar_wait(smem_u32(&kv_full[sv]), ph, abort_flag, dv.err, 722);
-                if (ok && i == n - 1 && cut) { mbar_arrive(smem_u32(&v_here)); ok = mbar_wait(smem_u32(&v_cut), 0, abort_flag, dv.err, 729); }
-                if (!ok) break;
-                next();
-                const int sk = st;
-                const bool more = i + 1 < n;
-                const uint32_t vd = desc_mn(ring) + (uint32_t)sv * (TILE >> 4);
+            Item it;
+            for (int ni = 0; ok && item_at(ni, it); ni++) {
+                item_read(ni);
+                const Work w = work_of(dv, it);
+                const int n = w.j1 - w.j0 + 1, a0 = w.lo0 - w.j0, z0 = w.on0 ? w.hi0 - w.j0 : -1, a1 = w.lo1 - w.j0, z1 = w.on1 ? w.hi1 - w.j0 : -1;
+                if (n <= 0) continue;
+                ok = mbar_wait(smem_u32(&kv_full[st]), ph, abort_flag, dv.err, 722);
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const int at = t ? a1 : a0, zt = t ? z1 : z0;
-                    if (ok && i >= at && i <= zt) {
-                        const uint32_t p = (uint32_t)(i - at) & 1u;
-#pragma unroll
-                        for (int part = 0; part < 2; part++) {                // the product starts with the first probabilities
-                            ok = ok && mbar_wait(smem_u32(&p_ready[t][part]), p, abort_flag, dv.err, 724);
-                            if (!ok) break;
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                            for (int c = part ? kFirst / 16 : 0; c < (part ? kRows : kFirst) / 16; c++)
-                                umma_ts(kO + t * HD, kS + t * 128 + c * 8, vd + c * (2048 >> 4), id_pv, c ? 1u : (uint32_t)(i != at));
+                for (int t = 0; t < 2; t++)
+                    if (ok && (t ? w.on1 : w.on0)) {
+                        ok = mbar_wait(smem_u32(&q_full[t]), pq[t], abort_flag, dv.err, 723);
+                        pq[t] ^= 1u;
+                        if (ok && (t ? a1 : a0) == 0) {
+                            qk(t, st);
+                            if ((t ? z1 : z0) == 0) umma_commit(smem_u32(&q_empty[t]));
                         }
-                        if (ok) umma_commit(smem_u32(&o_done[t]));
                     }
-                    if (ok && i + 1 >= at && i + 1 <= zt) {                   // over the scores and probabilities just used
-                        ok = mbar_wait(smem_u32(&kv_full[sk]), ph, abort_flag, dv.err, 722);
-                        if (ok) qk(t, sk);
-                    }
-                }
                 if (!ok) break;
-                umma_commit(smem_u32(&kv_empty[sv]));
-                if (more) { umma_commit(smem_u32(&kv_empty[sk])); next(); }
+                umma_commit(smem_u32(&kv_empty[st]));
+                next();
+                for (int i = 0; i < n && ok; i++) {
+                    const int sv = st;
+                    ok = mbar_wait(smem_u32(&kv_full[sv]), ph, abort_flag, dv.err, 722);
+                    if (ok && i == n - 1 && w.cut) {
+                        mbar_arrive(smem_u32(&v_here));
+                        ok = mbar_wait(smem_u32(&v_cut), cuts & 1u, abort_flag, dv.err, 729);
+                        cuts++;
+                    }
+                    if (!ok) break;
+                    next();
+                    const int sk = st;
+                    const uint32_t vd = desc_mn(ring) + (uint32_t)sv * (TILE >> 4);
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const int at = t ? a1 : a0, zt = t ? z1 : z0;
+                        if (ok && i >= at && i <= zt) {
+                            // the item before has been read out of the accumulator
+                            if (i == at && items[t] > 0) ok = mbar_wait(smem_u32(&o_free[t]), (uint32_t)(items[t] - 1) & 1u, abort_flag, dv.err, 735);
+                            if (i == at) items[t]++;
+#pragma unroll
+                            for (int part = 0; part < 2; part++) {            // the product starts with the first probabilities
+                                ok = ok && mbar_wait(smem_u32(&p_ready[t][part]), pp[t], abort_flag, dv.err, 724);
+                                if (!ok) break;
+                                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                                for (int c = part ? kFirst / 16 : 0; c < (part ? kRows : kFirst) / 16; c++)
+                                    umma_ts(kO + t * HD, kS + t * 128 + c * 8, vd + c * (2048 >> 4), id_pv, c ? 1u : (uint32_t)(i != at));
+                            }
+                            pp[t] ^= 1u;
+                            if (ok) umma_commit(smem_u32(&o_done[t]));
+                        }
+                        if (ok && i + 1 >= at && i + 1 <= zt) {               // over the scores and probabilities just used
+                            ok = mbar_wait(smem_u32(&kv_full[sk]), ph, abort_flag, dv.err, 722);
+                            if (ok) {
+                                qk(t, sk);
+                                if (i + 1 == zt) umma_commit(smem_u32(&q_empty[t]));
+                            }
+                        }
+                    }
+                    if (!ok) break;
+                    umma_commit(smem_u32(&kv_empty[sv]));
+                    if (i + 1 < n) { umma_commit(smem_u32(&kv_empty[sk])); next(); }
+                }
             }
         }
         __syncwarp();
-    } else if (warp == kCut) {
+    } else {
         // Value rows behind the sequence, in its last tile: zeros, so that whatever lies there meets a probability of zero as a number.
-        if (cut) {
-            const int vi = 2 * (j1 - j0) + 1, valid = s.lk - j1 * kRows;
-            const uint32_t v = ring + (uint32_t)(vi % NS) * TILE;
-            const bool ok = mbar_wait(smem_u32(&v_here), 0, abort_flag, dv.err, 730);      // told by the thread that saw it arrive
-            if (__all_sync(AX_FULL, ok)) {
+        Item it;
+        int st = 0;
+        uint32_t cuts = 0;
+        bool ok = true;
+        for (int n = 0; ok; n++) {
+            ok = item_at(n, it);
+            ok = __all_sync(AX_FULL, ok);
+            if (!ok) break;
+            __syncwarp();
+            if (lane == 0) item_read(n);
+            const Work w = work_of(dv, it);
+            const int m = 2 * (w.j1 - w.j0 + 1);
+            if (w.cut) {
+                const int valid = w.s.lk - w.j1 * kRows;
+                const uint32_t v = ring + (uint32_t)((st + m - 1) % NS) * TILE;
+                ok = mbar_wait(smem_u32(&v_here), cuts & 1u, abort_flag, dv.err, 730);       // told by the thread that saw it arrive
+                ok = __all_sync(AX_FULL, ok);
+                if (!ok) break;
+                cuts++;
                 for (int i = lane; i < (kRows - valid) * 8 * BOXES; i += 32) {
                     const int b = i / ((kRows - valid) * 8), r = i % ((kRows - valid) * 8);
                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(v + b * kBoxBytes + valid * 128 + r * 16), "r"(0) : "memory");
@@ -353,130 +483,148 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&v_cut));
             }
+            st = (st + m) % NS;
         }
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int t = warp >> 2;
-        const int r = (warp & 3) * 32 + lane, row = base[t] + r, pos = row + off;         // row of the sequence, key at its own position
-        const int h = dv.pair_heads ? h0 + t : h0;
         const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t ts = quarter + kS + t * 128, to = quarter + kO + t * HD;
         const float sc = dv.sc;
-        const int j_lo = lo[t], j_hi = hi[t];
-        const int key_hi = pos, key_lo = a.window > 0 ? pos - a.window : -1;               // visible: key_lo < j <= key_hi
-        const int first = base[t] + off, lastp = min(base[t] + kRows, s.lq) - 1 + off;     // positions of the tile's first and last row
-        float m = -INFINITY;
-        float2 l0 = make_float2(0.f, 0.f), l1 = l0;
+        uint32_t ps = 0, po = 0;                                              // parities of the tile's scores and of its finished products
+        Item item;
         bool ok = true;
-        for (int j = j_lo, it = 0; j <= j_hi; j++, it++) {
-            ok = mbar_wait(smem_u32(&s_full[t]), (uint32_t)it & 1u, abort_flag, dv.err, 725);
-            if (!__all_sync(AX_FULL, ok)) { ok = false; break; }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t u[kRows];
-            tmem_ld128(ts, u);
-            float* x = reinterpret_cast<float*>(u);
-            if (dv.negate) {
+        for (int ni = 0; ok; ni++) {
+            ok = item_at(ni, item);
+            ok = __all_sync(AX_FULL, ok);
+            if (!ok) break;
+            __syncwarp();
+            if (lane == 0) item_read(ni);
+            const Work w = work_of(dv, item);
+            const int base = t ? w.base1 : w.base0, h = dv.pair_heads ? w.h0 + t : w.h0;
+            const int row = base + (warp & 3) * 32 + lane, pos = row + w.off;              // row of the sequence, key at its own position
+            const int j_lo = t ? w.lo1 : w.lo0, j_hi = t ? w.hi1 : w.hi0;
+            const int key_hi = pos, key_lo = a.window > 0 ? pos - a.window : -1;           // visible: key_lo < j <= key_hi
+            const int first = base + w.off, lastp = min(base + kRows, w.s.lq) - 1 + w.off; // positions of the tile's first and last row
+            float m = -INFINITY;
+            float2 l0 = make_float2(0.f, 0.f), l1 = l0;
+            for (int j = j_lo; j <= j_hi; j++) {
+                ok = mbar_wait(smem_u32(&s_full[t]), ps, abort_flag, dv.err, 725);
+                ok = __all_sync(AX_FULL, ok);
+                if (!ok) break;
+                ps ^= 1u;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t u[kRows];
+                tmem_ld128(ts, u);
+                float* x = reinterpret_cast<float*>(u);
+                if (dv.negate) {
 #pragma unroll
-                for (int c = 0; c < kRows; c++) x[c] = -x[c];
-            }
-            const int k0 = j * kRows;
-            const bool edge = k0 + kRows - 1 > first || (a.window > 0 && k0 <= lastp - a.window);      // some row of the tile does not see all keys
-            if (edge) {
+                    for (int c = 0; c < kRows; c++) x[c] = -x[c];
+                }
+                const int k0 = j * kRows;
+                if (k0 + kRows - 1 > first || (a.window > 0 && k0 <= lastp - a.window)) {  // some row of the tile does not see all keys
 #pragma unroll
-                for (int c = 0; c < kRows; c++) if (k0 + c > key_hi || k0 + c <= key_lo) x[c] = -INFINITY;
-            }
-            float mx[8];
+                    for (int c = 0; c < kRows; c++) if (k0 + c > key_hi || k0 + c <= key_lo) x[c] = -INFINITY;
+                }
+                float mx[8];
 #pragma unroll
-            for (int c = 0; c < 8; c++) mx[c] = x[c];
+                for (int c = 0; c < 8; c++) mx[c] = x[c];
 #pragma unroll
-            for (int c = 8; c < 120; c += 2) mx[(c >> 1) & 7] = max3(mx[(c >> 1) & 7], x[c], x[c + 1]);
-            const float top = max3(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], x[120])),
-                                   max3(x[121], x[122], x[123]), max3(max3(x[124], x[125], x[126]), x[127], x[127]));
-            if (top != top) m = top;                                          // the row is taken again
-            const bool grow = top > m && (m == -INFINITY || (top - m) * sc > 8.f);
-            if (__any_sync(AX_FULL, grow)) {
-                const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * sc);
-                if (grow) m = top;
-                l0.x *= f; l0.y *= f; l1.x *= f; l1.y *= f;
-                if (it > 0) {
-                    ok = mbar_wait(smem_u32(&o_done[t]), (uint32_t)(it - 1) & 1u, abort_flag, dv.err, 726);
-                    if (!__all_sync(AX_FULL, ok)) { ok = false; break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int c = 8; c < 120; c += 2) mx[(c >> 1) & 7] = max3(mx[(c >> 1) & 7], x[c], x[c + 1]);
+                const float top = max3(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], x[120])),
+                                       max3(x[121], x[122], x[123]), max3(max3(x[124], x[125], x[126]), x[127], x[127]));
+                if (top != top) m = top;                                      // the row is taken again
+                const bool grow = top > m && (m == -INFINITY || (top - m) * sc > 8.f);
+                const bool started = j > j_lo;
+                if (__any_sync(AX_FULL, grow)) {
+                    const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * sc);
+                    if (grow) m = top;
+                    l0.x *= f; l0.y *= f; l1.x *= f; l1.y *= f;
+                    if (started) {                                            // the products of the tile before are in: po is the parity they leave
+                        ok = mbar_wait(smem_u32(&o_done[t]), po ^ 1u, abort_flag, dv.err, 726);
+                        ok = __all_sync(AX_FULL, ok);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(to + c, o);
+                        for (int c = 0; c < HD; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(to + c, o);
 #pragma unroll
-                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st16(to + c, o);
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16(to + c, o);
+                        }
                     }
                 }
-            }
-            const float neg = m == -INFINITY ? 0.f : -m * sc;
-            const float2 sc2 = make_float2(sc, sc), neg2 = make_float2(neg, neg);
-            auto probs = [&](int c0) {                                        // 32 keys
-                uint32_t p[16];
+                const float neg = m == -INFINITY ? 0.f : -m * sc;
+                const float2 sc2 = make_float2(sc, sc), neg2 = make_float2(neg, neg);
+                auto probs = [&](int c0) {                                    // 32 keys
+                    uint32_t p[16];
 #pragma unroll
-                for (int c = 0; c < 16; c++) {
-                    float2 y = fma2(make_float2(x[c0 + 2 * c], x[c0 + 2 * c + 1]), sc2, neg2);
-                    y.x = ex2(y.x); y.y = ex2(y.y);
-                    if (c & 1) l1 = add2(l1, y); else l0 = add2(l0, y);
-                    p[c] = pack<F16>(y.x, y.y);
-                }
-                tmem_st16(ts + c0 / 2, p);
-            };
-            auto hand_over = [&](int part) {
-                tmem_wait_st();
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                mbar_arrive(smem_u32(&p_ready[t][part]));
-            };
-            probs(0); probs(32);
-            hand_over(0);
-            probs(64); probs(96);
-            hand_over(1);
-        }
-        // ── output ──
-        const int tiles = j_hi - j_lo + 1;
-        if (ok && tiles > 0) {
-            ok = mbar_wait(smem_u32(&o_done[t]), (uint32_t)(tiles - 1) & 1u, abort_flag, dv.err, 727);
-            ok = __all_sync(AX_FULL, ok);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        }
-        if (ok) {
-            const bool live = row < s.lq;
+                    for (int c = 0; c < 16; c++) {
+                        float2 y = fma2(make_float2(x[c0 + 2 * c], x[c0 + 2 * c + 1]), sc2, neg2);
+                        y.x = ex2(y.x); y.y = ex2(y.y);
+                        if (c & 1) l1 = add2(l1, y); else l0 = add2(l0, y);
+                        p[c] = pack<F16>(y.x, y.y);
+                    }
+                    tmem_st16(ts + c0 / 2, p);
+                };
+                auto hand_over = [&](int part) {
+                    tmem_wait_st();
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    mbar_arrive(smem_u32(&p_ready[t][part]));
+                };
+                probs(0); probs(32);
+                hand_over(0);
+                probs(64); probs(96);
+                hand_over(1);
+                po ^= 1u;
+            }
+            // ── output ──
+            const bool any = j_hi >= j_lo;
+            if (ok && any) {
+                ok = mbar_wait(smem_u32(&o_done[t]), po ^ 1u, abort_flag, dv.err, 727);
+                ok = __all_sync(AX_FULL, ok);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
+            if (!ok) break;
+            const bool live = row < w.s.lq;
             const float l = (l0.x + l0.y) + (l1.x + l1.y);
             const float inv = l == 0.f ? 0.f : 1.f / l;
             float odd = 0.f;                                                  // becomes NaN with the first output that is not finite
-            T* out = (T*)a.out + (long long)(s.q0 + row) * a.o_tok + (long long)h * a.o_head;
+            T* out = (T*)a.out + (long long)(w.s.q0 + row) * a.o_tok + (long long)h * a.o_head;
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
-                if (tiles > 0) {
+                if (any) {
                     tmem_ld32(to + c, o);
+                    if (c + 32 == HD) {                                       // the accumulator may take the next item's products
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        mbar_arrive(smem_u32(&o_free[t]));
+                    }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = 0u;
                 }
-                uint32_t w[16];
+                uint32_t pk[16];
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const float x0 = __uint_as_float(o[2 * e]) * inv, x1 = __uint_as_float(o[2 * e + 1]) * inv;
                     odd = fmaf(x0, 0.f, fmaf(x1, 0.f, odd));
-                    w[e] = pack<F16>(x0, x1);
+                    pk[e] = pack<F16>(x0, x1);
                 }
                 if (live) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) *reinterpret_cast<uint4*>(out + c + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                    for (int e = 0; e < 4; e++) *reinterpret_cast<uint4*>(out + c + 8 * e) = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
                 }
             }
-            const bool sees = key_hi >= 0 && s.lk > 0;
+            const bool sees = key_hi >= 0 && w.s.lk > 0;
             unsigned again = __ballot_sync(AX_FULL, live && (odd != odd || (sees && !(fabsf(m) <= 3.402823466e38f))));
             __syncwarp();
             while (again) {
                 const int i = __ffs(again) - 1;
                 again &= again - 1;
-                row_again<T, HD>(a, s, h, base[t] + (warp & 3) * 32 + i, lane);
+                row_again<T, HD>(a, w.s, h, base + (warp & 3) * 32 + i, lane);
             }
         }
     }
@@ -489,16 +637,12 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             const int issued = s_issued;
             for (int i = issued > NS ? issued - NS : 0; i < issued; i++) {
                 const unsigned long long t0 = ax_globaltimer();
-                while (!mbar_try(smem_u32(&kv_full[i % NS]), (uint32_t)(i / NS) & 1u) && ax_globaltimer() - t0 < kWaitNs) { }
-            }
-            for (int t = 0; t < 2; t++) {
-                const unsigned long long t0 = ax_globaltimer();
-                while ((t ? on1 : on0) && !mbar_try(smem_u32(&q_full[t]), 0) && ax_globaltimer() - t0 < kWaitNs) { }
+                while (!mbar_try(smem_u32(&kv_full[i % NS]), (uint32_t)(i / NS) & 1u) && ax_globaltimer() - t0 < kAbortNs) { }
             }
         }
-        if (tid == 32) {                                                      // products issued before the failure: time to drain
+        if (tid == 32) {                                                      // queries, products and an answer asked for before the failure: time to land
             const unsigned long long t0 = ax_globaltimer();
-            while (ax_globaltimer() - t0 < 2000000ull) { }
+            while (ax_globaltimer() - t0 < kAbortNs) { }
         }
         __syncthreads();
     }
@@ -545,7 +689,9 @@ int launch(atlasx_ctx* ctx, const PromptDev& dv, const CUtensorMap& q, const CUt
     const int tb = dv.pair_heads ? kRows : 2 * kRows;
     // at most one unfilled tile per sequence, and no more sequences with rows than rows
     const long long tiles = (long long)dv.a.n_q / tb + (dv.a.batch < dv.a.n_q ? dv.a.batch : dv.a.n_q);
-    ax_prompt_umma_kernel<F16, HD><<<dim3((unsigned)(dv.pair_heads ? dv.a.n_heads / 2 : dv.a.n_heads), (unsigned)tiles), kThreads, smem, ctx->stream>>>(q, k, v, dv);
+    const long long items = tiles * (dv.pair_heads ? dv.a.n_heads / 2 : dv.a.n_heads);
+    AX_ARG(items <= 0x7FFFFFFFll, "too many rows and heads for one call");
+    ax_prompt_umma_kernel<F16, HD><<<(unsigned)items, kThreads, smem, ctx->stream>>>(q, k, v, dv);
     AX_CHECK_LAUNCH("ax_prompt_umma_kernel");
     return ATLASX_OK;
 }
