@@ -45,6 +45,7 @@ struct PromptDev {
     int pair_heads;                               // 1: two heads of a KV head, 0: 256 rows of one head
     float sc;                                     // |scale| · log2 e
     int negate;                                   // scale < 0
+    int wide;                                     // rows of out start on 32-byte boundaries
     int* err;
 };
 
@@ -522,10 +523,30 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
 #pragma unroll
                     for (int c = 0; c < kRows; c++) x[c] = -x[c];
                 }
+                // What hides keys is looked at in blocks of 32, for the warp's 32 rows: most blocks of a tile on the diagonal are seen by all rows
+                // or by none, and those that none sees need no exponentials.  (Two comparisons for each of 128 scores took 3000 clocks.)
                 const int k0 = j * kRows;
-                if (k0 + kRows - 1 > first || (a.window > 0 && k0 <= lastp - a.window)) {  // some row of the tile does not see all keys
+                unsigned hidden = 0u;                                         // bit q: no row of the warp sees keys 32 q .. 32 q + 31
+                if (k0 + kRows - 1 > first || (a.window > 0 && k0 <= lastp - a.window)) {
+                    const int p0 = pos - lane, p1 = p0 + 31;
 #pragma unroll
-                    for (int c = 0; c < kRows; c++) if (k0 + c > key_hi || k0 + c <= key_lo) x[c] = -INFINITY;
+                    for (int q = 0; q < 4; q++) {
+                        const int kq = k0 + 32 * q;
+                        if (kq > p1 || (a.window > 0 && kq + 31 <= p0 - a.window)) {
+                            hidden |= 1u << q;
+#pragma unroll
+                            for (int c = 0; c < 32; c++) x[32 * q + c] = -INFINITY;
+                        } else {
+                            if (kq + 31 > p0) {
+#pragma unroll
+                                for (int c = 0; c < 32; c++) if (c > key_hi - kq) x[32 * q + c] = -INFINITY;
+                            }
+                            if (a.window > 0 && kq <= p1 - a.window) {
+#pragma unroll
+                                for (int c = 0; c < 32; c++) if (c <= key_lo - kq) x[32 * q + c] = -INFINITY;
+                            }
+                        }
+                    }
                 }
                 float mx[8];
 #pragma unroll
@@ -538,10 +559,11 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 const bool grow = top > m && (m == -INFINITY || (top - m) * sc > 8.f);
                 const bool started = j > j_lo;
                 if (__any_sync(AX_FULL, grow)) {
-                    const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * sc);
+                    const bool moved = grow && m != -INFINITY;                // a row that has seen nothing has sums and outputs of zero
+                    const float f = moved ? ex2((m - top) * sc) : 1.f;
                     if (grow) m = top;
                     l0.x *= f; l0.y *= f; l1.x *= f; l1.y *= f;
-                    if (started) {                                            // the products of the tile before are in: po is the parity they leave
+                    if (started && __any_sync(AX_FULL, moved)) {              // the products of the tile before are in: po is the parity they leave
                         ok = mbar_wait(smem_u32(&o_done[t]), po ^ 1u, abort_flag, dv.err, 726);
                         ok = __all_sync(AX_FULL, ok);
                         if (!ok) break;
@@ -558,8 +580,12 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 }
                 const float neg = m == -INFINITY ? 0.f : -m * sc;
                 const float2 sc2 = make_float2(sc, sc), neg2 = make_float2(neg, neg);
-                auto probs = [&](int c0) {                                    // 32 keys
+                auto probs = [&](int c0, bool some) {                                    // 32 keys
                     uint32_t p[16];
+                    if (some && (hidden >> (c0 / 32) & 1u)) {
+#pragma unroll
+                        for (int c = 0; c < 16; c++) p[c] = 0u;
+                    } else
 #pragma unroll
                     for (int c = 0; c < 16; c++) {
                         float2 y = fma2(make_float2(x[c0 + 2 * c], x[c0 + 2 * c + 1]), sc2, neg2);
@@ -574,10 +600,17 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     mbar_arrive(smem_u32(&p_ready[t][part]));
                 };
-                probs(0); probs(32);
-                hand_over(0);
-                probs(64); probs(96);
-                hand_over(1);
+                if (hidden) {
+                    probs(0, true); probs(32, true);
+                    hand_over(0);
+                    probs(64, true); probs(96, true);
+                    hand_over(1);
+                } else {
+                    probs(0, false); probs(32, false);
+                    hand_over(0);
+                    probs(64, false); probs(96, false);
+                    hand_over(1);
+                }
                 po ^= 1u;
             }
             // ── output ──
@@ -614,8 +647,16 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                     pk[e] = pack<F16>(x0, x1);
                 }
                 if (live) {
+                    if (dv.wide) {                                            // whole sectors
 #pragma unroll
-                    for (int e = 0; e < 4; e++) *reinterpret_cast<uint4*>(out + c + 8 * e) = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+                        for (int e = 0; e < 2; e++)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                                         :: "l"(out + c + 16 * e), "r"(pk[8 * e]), "r"(pk[8 * e + 1]), "r"(pk[8 * e + 2]), "r"(pk[8 * e + 3]),
+                                            "r"(pk[8 * e + 4]), "r"(pk[8 * e + 5]), "r"(pk[8 * e + 6]), "r"(pk[8 * e + 7]) : "memory");
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) *reinterpret_cast<uint4*>(out + c + 8 * e) = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+                    }
                 }
             }
             const bool sees = key_hi >= 0 && w.s.lk > 0;
@@ -732,6 +773,7 @@ extern "C" int atlasx_prompt_attention(atlasx_ctx* c, const atlasx_prompt_args* 
     dv.a = { q, k, v, out, q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head, cu_q, cu_k, batch, n_q, n_k, n_heads, n_kv, hd, window, scale };
     dv.pair_heads = (n_heads / n_kv) % 2 == 0;
     dv.negate = scale < 0.f;
+    dv.wide = (uintptr_t)out % 32 == 0 && (n_q == 1 || o_tok % 16 == 0) && (n_heads == 1 || o_head % 16 == 0);
     // a hidden key's score is −inf · sc: a scale of zero must not make it NaN.  Scores below 2^126 / 1e37 of it are still all alike.
     dv.sc = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-37f);
     dv.err = c->dev_error;
