@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kPlanThreads) ax_page_plan_kernel(const PlanAr
     for (int b = b0; b < b1; b++) {
         const int c = a.cached[b], n = a.fresh[b];
         const long long need = ((long long)c + n + a.page_size - 1) / a.page_size;
-        if (c < 0 || n < 0 || need > a.table_width) { bad++; continue; }
+        if (c < 0 || n < 0 || need > a.table_width || (long long)c + n > 0x7FFFFFFFll) { bad++; continue; }
         tok += n;
         pg += need - (c + (long long)a.page_size - 1) / a.page_size;
     }
@@ -308,6 +308,7 @@ extern "C" int atlasx_page_plan(atlasx_ctx* c, const atlasx_page_plan_args* p) {
     AX_ARG(page_size >= 1 && n_pages >= 1 && (long long)page_size * n_pages <= 0x7FFFFFFFll, "page_size · n_pages must be in 1..2^31 - 1");
     AX_ARG(table_width >= 1, "the block table needs a column");
     AX_ARG(n_tokens >= 0 && n_free >= 0, "counts must not be negative");
+    AX_ARG(n_tokens <= 0x3FFFFFFF, "too many new rows for one call");
     AX_ARG((free_pages || !n_free) && ((slots && pos) || !n_tokens), "null argument");
     AX_ARG(c, "ctx is null");
     AX_ON_DEVICE(c);
@@ -379,6 +380,7 @@ extern "C" int atlasx_pagedkv_append(atlasx_ctx* c, atlasx_pagedkv* kv, const at
     const long long k_token_stride = p->k_token_stride, k_head_stride = p->k_head_stride, v_token_stride = p->v_token_stride, v_head_stride = p->v_head_stride;
     AX_ARG(dtype == ATLASX_F32 || dtype == ATLASX_BF16 || dtype == ATLASX_F16, "dtype must be f32, bf16 or f16");
     AX_ARG(n >= 0, "the number of rows must not be negative");
+    AX_ARG(n <= 0x3FFFFFFF, "too many rows for one call");
     if (n == 0) return ATLASX_OK;
     AX_ARG(k && v && slots, "null argument");
     const long long step = 16 / elem_bytes(dtype);
@@ -399,6 +401,7 @@ extern "C" int atlasx_pagedkv_append(atlasx_ctx* c, atlasx_pagedkv* kv, const at
 extern "C" int atlasx_pagedkv_read(atlasx_ctx* c, const atlasx_pagedkv* kv, const int* slots, int n, int dtype, void* k_out, void* v_out) {
     AX_ARG(dtype == ATLASX_F32 || dtype == ATLASX_BF16 || dtype == ATLASX_F16, "dtype must be f32, bf16 or f16");
     AX_ARG(n >= 0, "the number of rows must not be negative");
+    AX_ARG(n <= 0x3FFFFFFF, "too many rows for one call");
     if (n == 0) return ATLASX_OK;
     AX_ARG(k_out && v_out && slots, "null argument");
     AX_ARG(((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0, "outputs must be 16-byte aligned");

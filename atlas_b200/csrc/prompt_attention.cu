@@ -21,6 +21,7 @@
 //   * Every wait is bounded (ten seconds of %globaltimer): on expiry the CTA raises the context's error word, all roles leave, copies
 //     in flight are waited for and tensor memory is released.
 #include <cuda.h>
+#include <atomic>
 #include <type_traits>
 
 #include "prompt_attention.cuh"
@@ -267,12 +268,12 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         // Tiles of the sequences before each lane's share of them; then item after item: its tile counted from the pack's end.
         const int tb = dv.pair_heads ? kRows : 2 * kRows, hx = dv.pair_heads ? a.n_heads / 2 : a.n_heads;
         const int per = (a.batch + 31) / 32, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
-        int own = 0;
+        long long own = 0;                                                    // 64 bits: prefix arrays that overlap may name more rows than there are
         for (int b = b0; b < b1; b++) own += (ax_prompt_seq(a, b).lq + tb - 1) / tb;
-        int inc = own;
+        long long inc = own;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) { const int x = __shfl_up_sync(AX_FULL, inc, d); if (lane >= d) inc += x; }
-        const int before = inc - own, all = __shfl_sync(AX_FULL, inc, 31);
+        for (int d = 1; d < 32; d <<= 1) { const long long x = __shfl_up_sync(AX_FULL, inc, d); if (lane >= d) inc += x; }
+        const long long before = inc - own, all = __shfl_sync(AX_FULL, inc, 31);
         long long block = blockIdx.x;                                         // the CTA whose item is next
         int n = 0;
         uint32_t clc_phase = 0;
@@ -285,10 +286,10 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                              :: "r"(smem_u32(&s_clc)), "r"(smem_u32(&clc_bar)) : "memory");
             }
             __syncwarp();
-            const int x = all - 1 - (int)(block / hx);
+            const long long x = all - 1 - block / hx;
             if (x >= 0) {
                 const int g = 31 - __clz((int)__ballot_sync(AX_FULL, x >= before && own > 0));       // the lane in whose share the tile lies
-                int at = __shfl_sync(AX_FULL, before, g);
+                long long at = __shfl_sync(AX_FULL, before, g);
                 const int c0 = min(g * per, a.batch), c1 = min(c0 + per, a.batch);
                 Item it = {};
                 for (int c = c0; c < c1; c += 32) {
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                         const int l = __ffs(hit) - 1;
                         it.q0 = __shfl_sync(AX_FULL, q.q0, l); it.lq = __shfl_sync(AX_FULL, q.lq, l);
                         it.k0 = __shfl_sync(AX_FULL, q.k0, l); it.lk = __shfl_sync(AX_FULL, q.lk, l);
-                        it.base = (x - __shfl_sync(AX_FULL, at + up - mine, l)) * tb;
+                        it.base = (int)(x - __shfl_sync(AX_FULL, at + up - mine, l)) * tb;
                         break;
                     }
                     at += __shfl_sync(AX_FULL, up, 31);
@@ -722,7 +723,7 @@ int make_map(CUtensorMap* map, bool f16, const void* data, int rows, int heads, 
 template <bool F16, int HD>
 int launch(atlasx_ctx* ctx, const PromptDev& dv, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v) {
     constexpr int smem = (2 + (HD == 128 ? 5 : 6)) * (HD / 64) * kBoxBytes + 1024;
-    static bool ready[64] = {};
+    static std::atomic<bool> ready[64] = {};
     if (ctx->device >= 64 || !ready[ctx->device]) {                           // the limit is per device; asking twice does no harm
         AX_CUDA(cudaFuncSetAttribute(ax_prompt_umma_kernel<F16, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         if (ctx->device < 64) ready[ctx->device] = true;

@@ -102,24 +102,34 @@ def _refuse(x, name, dtypes, ndim, device):
         raise AtlasError("%s is not on device %d" % (name, device))
 
 
-def _ints(x, name, shape, device):
-    """Pointer of a contiguous int32 array; None in `shape` stands for any extent."""
+def _ints(x, name, n, device):
+    """Pointer of a contiguous int32 array of n numbers (None: any)."""
     try:
         if type(x) is DeviceArray:
-            ptr, got, fine = x.ptr, x.shape, x.dtype is I32 and x.ctx.device == device
-            whole = x.is_contiguous()
+            fine, ptr = x.dtype is I32 and x.ctx.device == device and len(x.shape) == 1 and x.is_contiguous() and (n is None or x.shape[0] == n), x.ptr
         else:
-            ptr, got, whole, fine = x.data_ptr(), x.shape, x.is_contiguous(), _code(x.dtype) is I32 and x.get_device() == device
+            fine = _CODES.get(x.dtype) is I32 and x.get_device() == device and x.ndim == 1 and x.is_contiguous() and (n is None or x.numel() == n)
+            ptr = x.data_ptr()
     except AttributeError:
         fine = False
-    if not fine or len(got) != len(shape):
-        _refuse(x, name, (I32,), len(shape), device)
-    for m, n in zip(shape, got):
-        if m is not None and m != n:
-            raise AtlasError("%s must have shape %s, not %s" % (name, tuple(shape), tuple(got)))
-    if not whole:
-        raise AtlasError("%s must be contiguous" % name)
+    if not fine:
+        ptr = _ints_slowly(x, name, (n,), device)
     return ptr
+
+
+def _ints_slowly(x, name, shape, device):
+    """The same for any number of dimensions (None in `shape` stands for any extent); says what is wrong."""
+    _refuse(x, name, (I32,), len(shape), device)
+    for m, n in zip(shape, x.shape):
+        if m is not None and m != n:
+            raise AtlasError("%s must have shape %s, not %s" % (name, tuple(shape), tuple(x.shape)))
+    if not x.is_contiguous():
+        raise AtlasError("%s must be contiguous" % name)
+    return x.ptr if type(x) is DeviceArray else x.data_ptr()
+
+
+def _length(x):
+    return x.shape[0] if type(x) is DeviceArray else x.numel()
 
 
 def _rows(x, name, dtypes, device, heads=None, head_dim=None):
@@ -165,14 +175,14 @@ def page_plan(cached, fresh, free_pages, table, cu, lens, slots, pos, status, pa
     """Block tables, slots and positions of a step from request lengths: see atlasx_page_plan.  int32 device arrays: cached, fresh,
     lens [batch]; free_pages [any]; table [batch, width], extended in place; cu [batch + 1]; slots, pos [rows]; status [3]."""
     dev = _device(ctx, cached)
-    p_cached = _ints(cached, "cached", (None,), dev)
-    b = cached.shape[0]
-    p_slots = _ints(slots, "slots", (None,), dev)
-    rows = slots.shape[0]
+    p_cached = _ints(cached, "cached", None, dev)
+    b = _length(cached)
+    p_slots = _ints(slots, "slots", None, dev)
+    rows = _length(slots)
     args = _ffi.PAGE_PLAN.pack(
-        p_cached, _ints(fresh, "fresh", (b,), dev), _ints(free_pages, "free_pages", (None,), dev), _ints(table, "table", (b, None), dev),
-        _ints(cu, "cu", (b + 1,), dev), _ints(lens, "lens", (b,), dev), p_slots, _ints(pos, "pos", (rows,), dev),
-        _ints(status, "status", (3,), dev), b, free_pages.shape[0], _whole(page_size, "page_size"), _whole(n_pages, "n_pages"), table.shape[1], rows)
+        p_cached, _ints(fresh, "fresh", b, dev), _ints(free_pages, "free_pages", None, dev), _ints_slowly(table, "table", (b, None), dev),
+        _ints(cu, "cu", b + 1, dev), _ints(lens, "lens", b, dev), p_slots, _ints(pos, "pos", rows, dev),
+        _ints(status, "status", 3, dev), b, _length(free_pages), _whole(page_size, "page_size"), _whole(n_pages, "n_pages"), table.shape[1], rows)
     check(_ffi.lib().atlasx_page_plan((ctx or Context.default()).handle, args))
 
 
@@ -206,7 +216,7 @@ class PagedKvCache:
         if n != m or dt != dv:
             raise AtlasError("k and v must have the same rows and type")
         check(_ffi.lib().atlasx_pagedkv_append(self.ctx.handle, self._h,
-                                               _ffi.PAGED_ROWS.pack(kp, vp, _ints(slots, "slots", (n,), dev), kt, kh, vt, vh, dt, n)))
+                                               _ffi.PAGED_ROWS.pack(kp, vp, _ints(slots, "slots", n, dev), kt, kh, vt, vh, dt, n)))
 
     def read(self, slots, k_out, v_out):
         """The values that the slots hold into contiguous [rows, n_kv_heads, head_dim] arrays (f32, bf16 or f16)."""
@@ -215,7 +225,7 @@ class PagedKvCache:
         vp, m, _, _, dv, _, _ = _contiguous(_rows(v_out, "v_out", types, dev, self.n_kv_heads, self.head_dim), "v_out")
         if n != m or dt != dv:
             raise AtlasError("k_out and v_out must have the same rows and type")
-        check(_ffi.lib().atlasx_pagedkv_read(self.ctx.handle, self._h, _ints(slots, "slots", (n,), dev), n, dt, kp, vp))
+        check(_ffi.lib().atlasx_pagedkv_read(self.ctx.handle, self._h, _ints(slots, "slots", n, dev), n, dt, kp, vp))
 
     def decode_attention(self, q, out, table, lens, scale, window_size=0, workspace=None):
         """Attention of one token per request: q, out [batch, n_heads, head_dim] f32, table [batch, width] page numbers, lens [batch]
@@ -225,10 +235,10 @@ class PagedKvCache:
         op = _contiguous(_rows(out, "out", (F32,), dev, nh, self.head_dim), "out")
         if op[1] != b:
             raise AtlasError("out must have the rows of q")
-        wp, wn = (0, 0) if workspace is None else (_ints(workspace, "workspace", (None,), dev), 4 * workspace.shape[0])
-        p_table = _ints(table, "table", (b, None), dev)
+        wp, wn = (0, 0) if workspace is None else (_ints(workspace, "workspace", None, dev), 4 * _length(workspace))
+        p_table = _ints_slowly(table, "table", (b, None), dev)
         check(_ffi.lib().atlasx_pagedkv_decode_attention(
-            self.ctx.handle, self._h, _ffi.PAGED_ATTN.pack(qp, op[0], p_table, _ints(lens, "lens", (b,), dev), wp, wn, nh, table.shape[1], b,
+            self.ctx.handle, self._h, _ffi.PAGED_ATTN.pack(qp, op[0], p_table, _ints(lens, "lens", b, dev), wp, wn, nh, table.shape[1], b,
                                                            _whole(window_size, "window_size"), scale)))
 
     def __del__(self):
@@ -252,8 +262,8 @@ def prompt_attention(q, k, v, out, cu_q, cu_k, scale=None, window_size=0, ctx=No
         raise AtlasError("k and v, and q and out, must have the same rows")
     if not dt == dk == dv == do:
         raise AtlasError("q, k, v and out must have the same type")
-    p_cu_q = _ints(cu_q, "cu_q", (None,), dev)
-    b = cu_q.shape[0] - 1
-    args = _ffi.PROMPT.pack(qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, p_cu_q, _ints(cu_k, "cu_k", (b + 1,), dev), dt, b, n, m, nh, nk, hd,
+    p_cu_q = _ints(cu_q, "cu_q", None, dev)
+    b = _length(cu_q) - 1
+    args = _ffi.PROMPT.pack(qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, p_cu_q, _ints(cu_k, "cu_k", b + 1, dev), dt, b, n, m, nh, nk, hd,
                             _whole(window_size, "window_size"), 1.0 / math.sqrt(hd) if scale is None else scale)
     check(_ffi.lib().atlasx_prompt_attention((ctx or Context.default()).handle, args))

@@ -117,7 +117,7 @@ def test_plan(ab, batch, cached_max, fresh_max, page, pad):
     assert got[5].tolist() == [want[5], 0, 0]
 
 
-@pytest.mark.parametrize("what", ["short", "negative", "wide", "tokens"])
+@pytest.mark.parametrize("what", ["short", "negative", "wide", "tokens", "long"])
 def test_plan_that_cannot_be_made_changes_nothing(ab, what):
     cached, fresh, free = np.array([16, 3, 0]), np.array([1, 20, 16]), np.array([5, 6, 7])
     table, n = np.array([[0, -1], [1, -1], [-1, -1]]), 37
@@ -129,6 +129,8 @@ def test_plan_that_cannot_be_made_changes_nothing(ab, what):
         fresh[0] = 17
     if what == "tokens":
         n = 36
+    if what == "long":                                                   # 2^31 rows and more
+        cached[1], fresh[1] = 1 << 30, 1 << 30
     got = call_plan(ab, cached, fresh, free, table, 16, 8, n)
     assert np.array_equal(got[0], table)
     assert not got[1].any() and not got[2].any() and (got[3] == -1).all() and (got[4] == -1).all()
@@ -319,6 +321,21 @@ def test_decode_long_and_many(ab, lens, n_kv, nh, window):
     rng = np.random.default_rng(len(lens))
     c = Cache(ab, rng, lens, n_kv, 64, 32, 32)
     check_decode(ab, c, nh, 0.2, window, rng=rng)
+
+
+def test_decode_of_the_largest_batch(ab):
+    rng = np.random.default_rng(41)
+    lens = rng.integers(0, 20, 4096).tolist()
+    c = Cache(ab, rng, lens, 1, 64, 32, 16)
+    check_decode(ab, c, 1, 0.125, 0, rng=rng)
+
+
+def test_decode_requests_may_share_pages(ab):
+    rng = np.random.default_rng(42)
+    c = Cache(ab, rng, [64, 80, 33], 2, 128, 64, 16)
+    c.table[1, :4] = c.table[0, :4]                                         # a common prefix
+    c.table[2, :2] = c.table[0, 0]                                          # the same page twice
+    check_decode(ab, c, 6, 0.1, 0, rng=rng)
 
 
 def test_decode_takes_the_lengths_as_they_are(ab):
@@ -560,6 +577,28 @@ def test_prompt_outputs_may_be_strided(ab):
     assert np.all(np.abs(down(ab, out).transpose(1, 0, 2) - want) <= tol)
 
 
+def test_prompt_of_the_largest_batch(ab):
+    rng = np.random.default_rng(43)
+    lens = rng.integers(0, 4, 4096).tolist()
+    prompt_case(ab, lens, lens, 1, 1, 64, 0, "BF16", rng)
+
+
+def test_prompt_prefix_arrays_are_cut_to_the_buffers(ab):
+    """Numbers outside the buffers and decreasing ones: no row is read or written that is not there."""
+    rng = np.random.default_rng(44)
+    q = bf16(rng.standard_normal((40, 2, 64)).astype(np.float32))
+    buf = up(ab, np.full((80, 2, 64), 7.0), ab.BF16)
+    qd, out = up(ab, q, ab.BF16), buf.columns(20 * 128, (40, 2, 64), (128, 64, 1))
+    for cu_q, cu_k in (([-5, 30, 1000], [-1000, 30, 70]), ([0, 40, 10], [0, 40, 40]), ([2147483647, -2147483648, 7], [0, 0, 0])):
+        ab.prompt_attention(qd, qd, qd, out, ab.DeviceArray.from_host(cu_q, ab.I32), ab.DeviceArray.from_host(cu_k, ab.I32), 0.1)
+        got = down(ab, buf)
+        assert (got[:20] == 7).all() and (got[60:] == 7).all()
+    assert ab.Context.default().poll_device_error() == 0
+    ab.prompt_attention(qd, qd, qd, out, ab.DeviceArray.from_host([-5, 30, 1000], ab.I32), ab.DeviceArray.from_host([-1000, 30, 70], ab.I32), 0.1)
+    want, tol = prompt_by_hand(q, q, q, [0, 30, 40], [0, 30, 40], 0.1, 0, False)
+    assert np.all(np.abs(down(ab, buf)[20:60] - want) <= tol)
+
+
 def test_prompt_rows_outside_every_sequence_stay(ab):
     rng = np.random.default_rng(7)
     q = bf16(rng.standard_normal((60, 1, 64)).astype(np.float32))
@@ -702,6 +741,38 @@ def test_a_captured_step_follows_the_lengths(ab):
         cached.copy_(i32(lens0))
         torch.cuda.synchronize()
     del graphs
+
+
+def test_a_captured_prompt_follows_the_arrays(ab):
+    """Prompt attention captured once, replayed with other rows and other sequence boundaries."""
+    torch = pytest.importorskip("torch")
+    ctx = ab.Context.default()
+    dev = torch.device("cuda", ctx.device)
+    s = torch.cuda.ExternalStream(ctx.stream, device=dev)
+    n, nh, n_kv, hd = 300, 4, 2, 128
+    q, k, v = (torch.zeros(n, m, hd, dtype=torch.bfloat16, device=dev) for m in (nh, n_kv, n_kv))
+    out = torch.zeros_like(q)
+    cu = torch.zeros(4, dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s, capture_error_mode="thread_local"):
+        ab.prompt_attention(q, k, v, out, cu, cu, 0.09)
+    rng = np.random.default_rng(51)
+    for bounds in ([0, 300, 300, 300], [0, 1, 140, 290], [0, 0, 0, 0], [0, 128, 256, 300]):
+        x = [bf16(rng.standard_normal(tuple(t.shape)).astype(np.float32)) for t in (q, k, v)]
+        for t, y in zip((q, k, v), x):
+            t.copy_(torch.from_numpy(y))
+        out.fill_(7.0)
+        cu.copy_(torch.tensor(bounds, dtype=torch.int32))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            g.replay()
+        torch.cuda.synchronize()
+        want, tol = prompt_by_hand(*x, bounds, bounds, 0.09, 0, False)
+        got = out.float().cpu().numpy()
+        assert np.all(np.abs(got - want)[:bounds[-1]] <= tol[:bounds[-1]]) and (got[bounds[-1]:] == 7).all()
+    assert ctx.poll_device_error() == 0
+    del g
 
 
 def test_two_contexts_do_not_meet(ab):

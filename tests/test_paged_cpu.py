@@ -154,7 +154,7 @@ PLAN = dict(cached=P, fresh=P, free=P, table=P, cu=P, lens=P, slots=P, pos=P, st
 @pytest.mark.parametrize("change,text", [
     (dict(cached=None), "null argument"), (dict(status=None), "null argument"), (dict(slots=None), "null argument"),
     (dict(free=None), "null argument"), (dict(batch=0), "batch"), (dict(batch=4097), "batch"), (dict(page_size=0), "page_size"),
-    (dict(n_pages=1 << 30, page_size=16), "2^31"), (dict(width=0), "column"), (dict(n_tokens=-1), "negative"),
+    (dict(n_pages=1 << 30, page_size=16), "2^31"), (dict(width=0), "column"), (dict(n_tokens=-1), "negative"), (dict(n_tokens=1 << 30), "too many"),
     (dict(n_free=-1), "negative"), ({}, "ctx is null")])
 def test_plan_refusals(change, text):
     refused(_ffi.lib().atlasx_page_plan(None, packed(_ffi.PAGE_PLAN, dict(PLAN, **change))), text)
@@ -177,7 +177,7 @@ ROWS = dict(k=P, v=P, slots=P, kt=128, kh=128, vt=128, vh=128, dtype=1, n=3)
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(dtype=2), "dtype"), (dict(n=-1), "negative"), (dict(k=None), "null"), (dict(slots=None), "null"), (dict(k=P + 2), "16-byte"),
+    (dict(dtype=2), "dtype"), (dict(n=-1), "negative"), (dict(n=1 << 30), "too many"), (dict(k=None), "null"), (dict(slots=None), "null"), (dict(k=P + 2), "16-byte"),
     (dict(kt=129), "16-byte"), (dict(vh=4), "16-byte"), (dict(dtype=0, kt=130), "16-byte"), ({}, "ctx or cache is null")])
 def test_append_refusals(change, text):
     refused(_ffi.lib().atlasx_pagedkv_append(None, None, packed(_ffi.PAGED_ROWS, dict(ROWS, **change))), text)
@@ -211,7 +211,7 @@ PROMPT = dict(q=P, k=P, v=P, out=P, qt=512, qh=128, kt=256, kh=128, vt=256, vh=1
     (dict(dtype=0), "dtype"), (dict(batch=0), "batch"), (dict(batch=4097), "batch"), (dict(n_q=-1), "negative"), (dict(n_heads=3), "multiple"),
     (dict(n_kv=0), "multiple"), (dict(hd=96), "head_dim"), (dict(window=-5), "window"), (dict(scale=float("nan")), "finite"),
     (dict(q=None), "null"), (dict(k=None), "null"), (dict(cu_k=None), "null"), (dict(q=P + 2), "16-byte"), (dict(kt=257), "16-byte"),
-    (dict(vt=-256), "negative"), (dict(oh=64), "overlap"), (dict(ot=0), "overlap"), ({}, "ctx is null")])
+    (dict(vt=-256), "negative"), (dict(kh=0), "zero"), (dict(qt=0), "zero"), (dict(n_q=1 << 30), "too many"), (dict(oh=64), "overlap"), (dict(ot=0), "overlap"), ({}, "ctx is null")])
 def test_prompt_refusals(change, text):
     refused(_ffi.lib().atlasx_prompt_attention(None, packed(_ffi.PROMPT, dict(PROMPT, **change))), text)
 
