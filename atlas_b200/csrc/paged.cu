@@ -9,7 +9,7 @@
 namespace {
 
 constexpr int kPlanThreads = 256;
-constexpr int kPlanItems = 1024;      // tokens (and pages taken) per CTA
+constexpr int kPlanItems = 512;      // tokens (and pages taken) per CTA
 
 struct PlanArgs {
     const int *cached, *fresh, *free;
@@ -94,23 +94,37 @@ __global__ void __launch_bounds__(kPlanThreads) ax_page_plan_kernel(const PlanAr
     }
     __syncthreads();
     const int n_tok = (int)all_t, n_pg = (int)all_p;
-    const int base = blockIdx.x * kPlanItems, end = min(base + kPlanItems, max(a.n_tokens, n_pg));
-    for (int i = base + tid; i < end; i += kPlanThreads) {
-        if (i < n_pg) {
-            const int b = find_start(s_first, a.batch + 1, i);
-            const int had = (int)((a.cached[b] + (long long)a.page_size - 1) / a.page_size);
-            a.table[(size_t)b * a.table_width + had + (i - s_first[b])] = a.free[i];
-        }
-        if (i < n_tok) {
-            const int b = find_start(s_cu, a.batch + 1, i);
-            const int c = a.cached[b], at = c + (i - s_cu[b]);
-            const int had = (int)((c + (long long)a.page_size - 1) / a.page_size), col = at / a.page_size;
-            const int page = col < had ? a.table[(size_t)b * a.table_width + col] : a.free[s_first[b] + (col - had)];
-            a.slots[i] = page >= 0 && page < a.n_pages ? page * a.page_size + at % a.page_size : -1;
-            a.pos[i] = at;
-        } else if (i < a.n_tokens) {              // rows behind the last request
-            a.slots[i] = -1; a.pos[i] = -1;
-        }
+    const int base = blockIdx.x * kPlanItems;
+    for (int i = base + tid; i < min(base + kPlanItems, n_pg); i += kPlanThreads) {
+        const int b = find_start(s_first, a.batch + 1, i);
+        const int had = (int)((a.cached[b] + (long long)a.page_size - 1) / a.page_size);
+        a.table[(size_t)b * a.table_width + had + (i - s_first[b])] = a.free[i];
+    }
+    // A thread's tokens side by side: the loads of one step are under way together.
+    constexpr int N = kPlanItems / kPlanThreads;
+    int b[N], at[N], page[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+        const int i = base + tid + u * kPlanThreads;
+        b[u] = i < n_tok ? find_start(s_cu, a.batch + 1, i) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < N; u++) at[u] = b[u] >= 0 ? a.cached[b[u]] : 0;
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+        page[u] = -1;
+        if (b[u] < 0) continue;
+        const int c = at[u], had = (int)(((unsigned)c + (unsigned)a.page_size - 1u) / (unsigned)a.page_size);
+        at[u] = c + (base + tid + u * kPlanThreads - s_cu[b[u]]);
+        const int col = at[u] / a.page_size;
+        page[u] = col < had ? a.table[(size_t)b[u] * a.table_width + col] : a.free[s_first[b[u]] + (col - had)];
+    }
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+        const int i = base + tid + u * kPlanThreads;
+        if (i >= a.n_tokens) continue;                                // rows behind the last request: −1 in both
+        a.slots[i] = page[u] >= 0 && page[u] < a.n_pages ? page[u] * a.page_size + at[u] % a.page_size : -1;
+        a.pos[i] = b[u] >= 0 ? at[u] : -1;
     }
 }
 
