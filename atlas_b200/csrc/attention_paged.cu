@@ -324,17 +324,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                     s[2 * nt + 1] = fmaf(k1, d[nt][1] + d[nt][3], s[2 * nt + 1]);
                 }
             }
-            const int row = info.tile * AX_P4_TILE;
-            const bool edge = row < seg_lo || row + AX_P4_TILE > seg_len;
-            bool seen[4] = { true, true, true, true };
-            if (edge) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {                                  // column 8·nt + 2t + b is row 8·nt + 4b + t
-                    const int r = row + (i >> 1) * 8 + (i & 1) * 4 + t;
-                    seen[i] = r >= seg_lo && r < seg_len;
-                    if (!seen[i]) s[i] = -INFINITY;
-                }
-            }
             // scales of V of the lane's four rows; an absent row has none
             float vs[4][NG], z[4];
 #pragma unroll
@@ -344,13 +333,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
 #pragma unroll
                 for (int i = 0; i < 2 * NG; i++) vs[2 * nt + i / NG][i % NG] = i & 1 ? ax_bf16_hi(sw[i / 2]) : ax_bf16_lo(sw[i / 2]);
             }
-            if (edge) {
+            const int row = info.tile * AX_P4_TILE;
+            if (row < seg_lo || row + AX_P4_TILE > seg_len) {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (!seen[i]) {
+                for (int i = 0; i < 4; i++) {                                  // column 8·nt + 2t + b is row 8·nt + 4b + t
+                    const int r = row + (i >> 1) * 8 + (i & 1) * 4 + t;
+                    if (r < seg_lo || r >= seg_len) {
+                        s[i] = -INFINITY;
 #pragma unroll
                         for (int gr = 0; gr < NG; gr++) vs[i][gr] = 0.f;
                     }
+                }
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
