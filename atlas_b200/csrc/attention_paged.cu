@@ -85,6 +85,25 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
+// two f32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\t"
+        "mov.b64 {%0, %1}, w;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 template <int N> __device__ __forceinline__ void lds(uint32_t (&r)[N], const void* p) {
     if constexpr (N == 4) { const uint4 v = *(const uint4*)p; r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
     else if constexpr (N == 2) { const uint2 v = *(const uint2*)p; r[0] = v.x; r[1] = v.y; }
@@ -202,7 +221,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
 
     // ── state of the segment at hand ──
     float qback = 1.f;                          // the power of two that the query was divided by
-    float o[NT][4], m = -INFINITY, l = 0.f;
+    float o[NT][4], m = -INFINITY;
+    float2 l = {};                              // sums of columns 2t and of 2t + 1
     int seg = -1, seg_lo = 0, seg_len = 0;
     auto start = [&](int s) {
         seg = s;
@@ -247,7 +267,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             }
 #pragma unroll
         for (int i = 0; i < NT; i++) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
-        m = -INFINITY; l = 0.f;
+        m = -INFINITY; l = make_float2(0.f, 0.f);
     };
     // Column n = 2t, 2t + 1 of column block gr · (GS / 8) + i is number gr · GS + n · (GS / 8) + i: a lane holds GS / 4 consecutive numbers
     // of every group.
@@ -270,15 +290,16 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         const int b = seg / dv.nh, hh = seg % dv.nh, kh = hh / dv.head_tiles, h0 = (hh % dv.head_tiles) * kHeads;
         const unsigned n = s_pre[b + 1] - s_pre[b];
         const long long s0 = (long long)s_pre[b] * dv.nh + (long long)hh * n;
-        l += __shfl_xor_sync(AX_FULL, l, 1);
-        l += __shfl_xor_sync(AX_FULL, l, 2);
+        float sum = l.x + l.y;
+        sum += __shfl_xor_sync(AX_FULL, sum, 1);
+        sum += __shfl_xor_sync(AX_FULL, sum, 2);
         const bool live = h0 + g < dv.group_heads;
         if (s0 >= x0 && s0 + n <= x1) {
-            if (live) put(dv.a.out + ((size_t)b * dv.a.n_heads + (size_t)kh * dv.group_heads + h0 + g) * HD, l == 0.f ? 0.f : 1.f / l);
+            if (live) put(dv.a.out + ((size_t)b * dv.a.n_heads + (size_t)kh * dv.group_heads + h0 + g) * HD, sum == 0.f ? 0.f : 1.f / sum);
         } else {
             const int slot = warp * 2 + (s0 < x0 ? 0 : 1);
             if (lane == 0) s_seg[slot] = seg;
-            if (t == 0) { s_ml[slot][g][0] = m; s_ml[slot][g][1] = l; }
+            if (t == 0) { s_ml[slot][g][0] = m; s_ml[slot][g][1] = sum; }
             if (live) put(s_o(slot) + g * HD, 1.f);
         }
     };
@@ -296,7 +317,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         if (info.seg != seg) { if (seg >= 0) flush(); start(info.seg); }
         if (info.ok) {
             const uint8_t* tile = ring + st * TILE;
-            float s[4] = { 0.f, 0.f, 0.f, 0.f };                              // (block 0: columns 2t, 2t + 1), (block 1: …)
+            float2 s[2] = {};                                                 // columns 2t, 2t + 1 of row block nt
             uint32_t kw[2][W], ks[2][NG];
 #pragma unroll
             for (int nt = 0; nt < 2; nt++) {
@@ -320,55 +341,67 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 for (int nt = 0; nt < 2; nt++) {                               // scales of columns 2t and 2t + 1, NG numbers each
                     const float k0 = gr & 1 ? ax_bf16_hi(ks[nt][gr / 2]) : ax_bf16_lo(ks[nt][gr / 2]);
                     const float k1 = (NG + gr) & 1 ? ax_bf16_hi(ks[nt][(NG + gr) / 2]) : ax_bf16_lo(ks[nt][(NG + gr) / 2]);
-                    s[2 * nt] = fmaf(k0, d[nt][0] + d[nt][2], s[2 * nt]);
-                    s[2 * nt + 1] = fmaf(k1, d[nt][1] + d[nt][3], s[2 * nt + 1]);
+                    s[nt] = fma2(make_float2(k0, k1), add2(make_float2(d[nt][0], d[nt][1]), make_float2(d[nt][2], d[nt][3])), s[nt]);
                 }
             }
             // scales of V of the lane's four rows; an absent row has none
-            float vs[4][NG], z[4];
+            float2 vs[2][NG];
 #pragma unroll
             for (int nt = 0; nt < 2; nt++) {
                 uint32_t sw[NG];
                 lds<NG>(sw, tile + 2 * PLANE + SC + (8 * nt + 2 * t) * NG * 2);
 #pragma unroll
-                for (int i = 0; i < 2 * NG; i++) vs[2 * nt + i / NG][i % NG] = i & 1 ? ax_bf16_hi(sw[i / 2]) : ax_bf16_lo(sw[i / 2]);
+                for (int gr = 0; gr < NG; gr++) {
+                    vs[nt][gr].x = gr & 1 ? ax_bf16_hi(sw[gr / 2]) : ax_bf16_lo(sw[gr / 2]);
+                    vs[nt][gr].y = (NG + gr) & 1 ? ax_bf16_hi(sw[(NG + gr) / 2]) : ax_bf16_lo(sw[(NG + gr) / 2]);
+                }
+                s[nt] = mul2(s[nt], make_float2(qback, qback));
             }
             const int row = info.tile * AX_P4_TILE;
             if (row < seg_lo || row + AX_P4_TILE > seg_len) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {                                  // column 8·nt + 2t + b is row 8·nt + 4b + t
-                    const int r = row + (i >> 1) * 8 + (i & 1) * 4 + t;
-                    if (r < seg_lo || r >= seg_len) {
-                        s[i] = -INFINITY;
+                for (int nt = 0; nt < 2; nt++) {                               // column 8·nt + 2t + b is row 8·nt + 4b + t
+                    const int r0 = row + nt * 8 + t, r1 = r0 + 4;
+                    if (r0 < seg_lo || r0 >= seg_len) {
+                        s[nt].x = -INFINITY;
 #pragma unroll
-                        for (int gr = 0; gr < NG; gr++) vs[i][gr] = 0.f;
+                        for (int gr = 0; gr < NG; gr++) vs[nt][gr].x = 0.f;
+                    }
+                    if (r1 < seg_lo || r1 >= seg_len) {
+                        s[nt].y = -INFINITY;
+#pragma unroll
+                        for (int gr = 0; gr < NG; gr++) vs[nt][gr].y = 0.f;
                     }
                 }
             }
+            float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                s[i] *= qback;
-                float big = vs[i][0];
+            for (int nt = 0; nt < 2; nt++) {
+                float2 big = vs[nt][0];
 #pragma unroll
-                for (int gr = 1; gr < NG; gr++) big = fmaxf(big, vs[i][gr]);
-                z[i] = s[i] + fmaxf(lg2(big), -100.f);
+                for (int gr = 1; gr < NG; gr++) { big.x = fmaxf(big.x, vs[nt][gr].x); big.y = fmaxf(big.y, vs[nt][gr].y); }
+                const float2 z = add2(s[nt], make_float2(fmaxf(lg2(big.x), -100.f), fmaxf(lg2(big.y), -100.f)));
+                top = fmaxf(top, fmaxf(z.x, z.y));
             }
-            float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
             top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 1));
             top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 2));
             // The reference is moved only where a p · scale would pass 2^15; then the largest becomes 2^7, so what is lost of the small
             // ones (half a step of f16's subnormals, 2^-25) is at most 2^-32 of the largest.
             if (__any_sync(AX_FULL, top > m + 15.f)) {
                 const float mn = fmaxf(m, top - 7.f), f = m == -INFINITY ? 0.f : ex2(m - mn);
-                l *= f;
+                l.x *= f; l.y *= f;
 #pragma unroll
                 for (int i = 0; i < NT; i++) { o[i][0] *= f; o[i][1] *= f; o[i][2] *= f; o[i][3] *= f; }
                 m = mn;
             }
-            const float mr = m == -INFINITY ? 0.f : m;
-            float p[4];
+            const float mr = m == -INFINITY ? 0.f : -m;
+            float2 p[2];
 #pragma unroll
-            for (int i = 0; i < 4; i++) { p[i] = ex2(s[i] - mr); l += p[i]; }
+            for (int nt = 0; nt < 2; nt++) {
+                p[nt] = add2(s[nt], make_float2(mr, mr));
+                p[nt].x = ex2(p[nt].x); p[nt].y = ex2(p[nt].y);
+                l = add2(l, p[nt]);
+            }
             uint32_t vw[2][W];
 #pragma unroll
             for (int nt = 0; nt < 2; nt++) lds<W>(vw[nt], tile + PLANE + nt * (PLANE / 2) + lane * W * 4);
@@ -377,10 +410,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 uint32_t hl[4];
 #pragma unroll
                 for (int nt = 0; nt < 2; nt++) {
-                    const float y0 = p[2 * nt] * vs[2 * nt][gr], y1 = p[2 * nt + 1] * vs[2 * nt + 1][gr];
-                    hl[2 * nt] = pack_f16(y0, y1);
-                    const float2 h = unpack_f16(hl[2 * nt]);
-                    hl[2 * nt + 1] = pack_f16(y0 - h.x, y1 - h.y);
+                    const float2 y = mul2(p[nt], vs[nt][gr]);
+                    hl[2 * nt] = pack_f16(y.x, y.y);
+                    const float2 r = fma2(unpack_f16(hl[2 * nt]), make_float2(-1.f, -1.f), y);
+                    hl[2 * nt + 1] = pack_f16(r.x, r.y);
                 }
                 const uint4 a = make_uint4(hl[0], hl[1], hl[2], hl[3]);
 #pragma unroll
