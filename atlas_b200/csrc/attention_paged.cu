@@ -3,9 +3,9 @@
 // What has to move is rows · n_kv · 2 · (hd / 2 + 2 · hd / group) bytes; at the copy bandwidth a tile (16 rows of one KV head,
 // 2304 bytes at hd 128, group 32) leaves an SM about 100 clocks.  Unpacking 4096 nibbles, two products with four-times-replicated
 // work for f32 accuracy and a softmax in that time is what the kernel is shaped by:
-//   * Work is cut evenly: the tiles of all (request, KV head) segments form one sequence, every warp takes a contiguous piece of
-//     it, whatever the lengths are.  Nothing of it is decided on the host, so a captured call follows the lengths.
-//   * A tile is one bulk copy into the warp's own ring of stages; no barrier of the CTA in the loop.
+//   * Work is cut evenly: the units (two tiles, 32 rows) of all (request, KV head) segments form one sequence, every warp takes a
+//     contiguous piece of it, whatever the lengths are.  Nothing of it is decided on the host, so a captured call follows the lengths.
+//   * A unit is one bulk copy (two where its tiles lie in different pages) into the warp's own ring; no barrier of the CTA in the loop.
 //   * S = Q·Kᵀ and O = P·V run as mma.m16n8k16 with the (up to eight) query heads of a KV head as rows: rows 0..7 hold the f16
 //     hi parts, rows 8..15 the lo parts of the same f32 values, so one instruction gives both and the sum of two accumulators
 //     is good to 2^-22 of each value (bf16 halves left 4e-6 of the output, 2^-16 of each value).  The score accumulators are
@@ -25,9 +25,10 @@
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
+constexpr int kStages = 2;
 constexpr int kCtasPerSm = 3;
-constexpr int kMinTiles = 1;                    // tiles of a warp below which fewer CTAs share the work (1 × 700 rows: 13.0 µs, with two tiles 15.3, four 18.3)
+constexpr int kUnit = 2;                        // tiles that a warp takes at a time (one where there are not two for each warp: 1 × 700 rows
+                                                // take 13 µs so, with two 15.7)
 constexpr int kHeads = 8;                       // query heads of one segment
 constexpr int kChunk = 64;                      // parts of a segment whose weights are in shared memory at a time
 constexpr unsigned long long kWaitNs = 2000000000ull;
@@ -45,7 +46,8 @@ struct PagedDev {
     int* err;
 };
 
-struct TileInfo { int seg, tile, ok, pad; };
+struct UnitInfo { int seg, tile, ok, pad; };     // segment, first tile, bit u: tile + u is there
+
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
@@ -128,16 +130,16 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     constexpr int NT = HD / 8;                  // column blocks of the output
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t s_bar[kWarps][kStages];
-    __shared__ __align__(16) TileInfo s_info[kWarps][kStages];
-    __shared__ unsigned s_scan[kWarps];
+    __shared__ __align__(16) UnitInfo s_info[kWarps][kStages];
+    __shared__ unsigned s_scan[2][kWarps];
     __shared__ int s_seg[kWarps * 2];
     __shared__ float s_ml[kWarps * 2][kHeads][2];
     __shared__ int s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int batch = dv.a.batch, hpt = dv.hpt;
     // Shared memory: per warp its ring, its query operand, and the output of a first segment that ends within its piece; the output of the
-    // last segment goes over the ring, which is empty by then.  Then [batch + 1] tiles before each request.
-    constexpr int RING = kStages * TILE, QBYTES = W * 2 * 32 * 16;
+    // last segment goes over the ring, which is empty by then.  Then [batch + 1] units before each request.
+    constexpr int UNIT = kUnit * TILE, RING = kStages * UNIT, QBYTES = W * 2 * 32 * 16;
     const int own = RING + QBYTES + hpt * HD * 4;
     uint8_t* ring = smem + warp * own;
     uint4* s_q = reinterpret_cast<uint4*>(ring + RING);                                     // [step][lane]
@@ -148,21 +150,35 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     if (tid < kWarps * 2) s_seg[tid] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    {   // exclusive sums of the requests' tiles
+    int us;                                                                   // tiles of a unit: two, or one where that many warps would have none
+    {   // exclusive sums of the requests' units
         const int per = (batch + kWarps * 32 - 1) / (kWarps * 32), b0 = min(tid * per, batch), b1 = min(b0 + per, batch);
         unsigned own = 0;
         for (int b = b0; b < b1; b++) { int lo, len; row_range(dv, b, lo, len); own += tiles_of(lo, len); }
+        unsigned sum = own;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(AX_FULL, sum, d);
+        if (lane == 0) s_scan[0][warp] = sum;
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) sum += s_scan[0][w];
+        us = (long long)sum * dv.nh <= (long long)gridDim.x * kWarps ? 1 : kUnit;
+        if (us > 1) {
+            own = 0;
+            for (int b = b0; b < b1; b++) { int lo, len; row_range(dv, b, lo, len); own += (tiles_of(lo, len) + kUnit - 1) / kUnit; }
+        }
         unsigned inc = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) { const unsigned x = __shfl_up_sync(AX_FULL, inc, d); if (lane >= d) inc += x; }
-        if (lane == 31) s_scan[warp] = inc;
+        if (lane == 31) s_scan[1][warp] = inc;
         __syncthreads();
         unsigned at = inc - own;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) if (w < warp) at += s_scan[w];
+        for (int w = 0; w < kWarps; w++) if (w < warp) at += s_scan[1][w];
         for (int b = b0; b < b1; b++) {
             int lo, len; row_range(dv, b, lo, len);
-            s_pre[b] = at; at += tiles_of(lo, len);
+            s_pre[b] = at; at += (tiles_of(lo, len) + us - 1) / us;
             if (b == batch - 1) s_pre[batch] = at;
         }
         __syncthreads();
@@ -171,17 +187,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         if (s_pre[b] == s_pre[b + 1])
             for (int i = tid; i < dv.a.n_heads * HD; i += kWarps * 32) dv.a.out[(size_t)b * dv.a.n_heads * HD + i] = 0.f;
     const long long total = (long long)s_pre[batch] * dv.nh;
-    const long long want = (total + kWarps * kMinTiles - 1) / (kWarps * kMinTiles);
+    const long long want = (total + kWarps - 1) / kWarps;
     const long long C = want < (long long)gridDim.x ? want : (long long)gridDim.x;        // CTAs that share the work
     const long long c = blockIdx.x;
     if (c >= C) return;
     const long long X0 = total * c / C, X1 = total * (c + 1) / C;
     const long long x0 = X0 + (X1 - X0) * warp / kWarps, x1 = X0 + (X1 - X0) * (warp + 1) / kWarps;
 
-    // ── the warp's stream of tiles: 32 positions are resolved at a time, one per lane, and lane i copies tile i of them ──
+    // ── the warp's stream of units: 32 positions are resolved at a time, one per lane, and lane i copies unit i of them ──
     const int count = (int)(x1 - x0);
-    const uint8_t* src = nullptr;
-    TileInfo mine = {};
+    const uint8_t* src[kUnit] = {};
+    UnitInfo mine = {};
     auto fill = [&](int i, int st) {                                          // i uniform over the warp, rising by one; st: its stage
         if (i >= count) return;
         if ((i & 31) == 0) {
@@ -197,22 +213,33 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 else { hh = (int)(rem / n); ti = (int)(rem % n); }
                 int first, len; row_range(dv, lo, first, len);
                 mine.seg = lo * dv.nh + hh;
-                mine.tile = first / AX_P4_TILE + ti;
-                const int row = mine.tile * AX_P4_TILE, page = dv.a.table[(size_t)lo * dv.a.table_width + row / dv.s.page_size];
-                mine.ok = page >= 0 && page < dv.s.n_pages;
-                if (mine.ok) src = dv.pool + ax_p4_tile_at(dv.s, page, hh / dv.head_tiles, row % dv.s.page_size);
-                else atomicExch(dv.err, AX_DEVERR_PAGE);
+                mine.tile = first / AX_P4_TILE + us * ti;
+#pragma unroll
+                for (int u = 0; u < kUnit; u++) {
+                    const int row = (mine.tile + u) * AX_P4_TILE;
+                    if (row >= len || u >= us) continue;
+                    const int page = dv.a.table[(size_t)lo * dv.a.table_width + row / dv.s.page_size];
+                    if (page >= 0 && page < dv.s.n_pages) {
+                        mine.ok |= 1 << u;
+                        src[u] = dv.pool + ax_p4_tile_at(dv.s, page, hh / dv.head_tiles, row % dv.s.page_size);
+                    } else atomicExch(dv.err, AX_DEVERR_PAGE);
+                }
             }
         }
         if (lane == (i & 31)) {
             const uint32_t bar = smem_u32(&s_bar[warp][st]);
             s_info[warp][st] = mine;
-            if (mine.ok) {
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(TILE) : "memory");
+            auto copy = [&](int u, uint32_t bytes) {
                 asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                             :: "r"(smem_u32(ring + st * TILE)), "l"(src), "r"(TILE), "r"(bar) : "memory");
-            } else {
-                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+                             :: "r"(smem_u32(ring + st * UNIT + u * TILE)), "l"(src[u]), "r"(bytes), "r"(bar) : "memory");
+            };
+            const bool one = mine.ok == 3 && src[1] == src[0] + TILE;          // neighbours in a page
+            if (mine.ok) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(mine.ok == 3 ? UNIT : TILE) : "memory");
+            else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+            if (one) copy(0, UNIT);
+            else {
+                if (mine.ok & 1) copy(0, TILE);
+                if (mine.ok & 2) copy(1, TILE);
             }
         }
     };
@@ -313,76 +340,95 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 mbar_wait(smem_u32(&s_bar[warp][y % kStages]), (uint32_t)(y / kStages) & 1u);
             break;
         }
-        const TileInfo info = s_info[warp][st];
+        const UnitInfo info = s_info[warp][st];
         if (info.seg != seg) { if (seg >= 0) flush(); start(info.seg); }
         if (info.ok) {
-            const uint8_t* tile = ring + st * TILE;
-            float2 s[2] = {};                                                 // columns 2t, 2t + 1 of row block nt
-            uint32_t kw[2][W], ks[2][NG];
+            // Both tiles side by side: their chains — scores, softmax, products — are each other's cover.  (One tile at a time left 54 % of the
+            // issue slots and 41 % of the busiest pipe in use.)
+            const uint8_t* unit = ring + st * UNIT;
+            float2 s[kUnit][2] = {};                                          // columns 2t, 2t + 1 of row block nt
+            float2 vs[kUnit][2][NG];                                          // scales of V of the lane's four rows
+            {
+                uint32_t kw[kUnit][2][W], ks[kUnit][2][NG];
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                lds<W>(kw[nt], tile + nt * (PLANE / 2) + lane * W * 4);
-                lds<NG>(ks[nt], tile + 2 * PLANE + (8 * nt + 2 * t) * NG * 2);
-            }
-#pragma unroll
-            for (int gr = 0; gr < NG; gr++) {
-                float d[2][4] = {};
-#pragma unroll
-                for (int i = 0; i < WG; i++) {
-                    const uint4 q0 = s_q[(2 * (gr * WG + i)) * 32 + lane], q1 = s_q[(2 * (gr * WG + i) + 1) * 32 + lane];
+                for (int u = 0; u < kUnit; u++)
 #pragma unroll
                     for (int nt = 0; nt < 2; nt++) {
-                        const uint32_t w = kw[nt][gr * WG + i], v = w >> 8;
-                        mma(d[nt], q0, n_low(w), n_high(w));
-                        mma(d[nt], q1, n_low(v), n_high(v));
+                        lds<W>(kw[u][nt], unit + u * TILE + nt * (PLANE / 2) + lane * W * 4);
+                        lds<NG>(ks[u][nt], unit + u * TILE + 2 * PLANE + (8 * nt + 2 * t) * NG * 2);
                     }
-                }
-#pragma unroll
-                for (int nt = 0; nt < 2; nt++) {                               // scales of columns 2t and 2t + 1, NG numbers each
-                    const float k0 = gr & 1 ? ax_bf16_hi(ks[nt][gr / 2]) : ax_bf16_lo(ks[nt][gr / 2]);
-                    const float k1 = (NG + gr) & 1 ? ax_bf16_hi(ks[nt][(NG + gr) / 2]) : ax_bf16_lo(ks[nt][(NG + gr) / 2]);
-                    s[nt] = fma2(make_float2(k0, k1), add2(make_float2(d[nt][0], d[nt][1]), make_float2(d[nt][2], d[nt][3])), s[nt]);
-                }
-            }
-            // scales of V of the lane's four rows; an absent row has none
-            float2 vs[2][NG];
-#pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                uint32_t sw[NG];
-                lds<NG>(sw, tile + 2 * PLANE + SC + (8 * nt + 2 * t) * NG * 2);
 #pragma unroll
                 for (int gr = 0; gr < NG; gr++) {
-                    vs[nt][gr].x = gr & 1 ? ax_bf16_hi(sw[gr / 2]) : ax_bf16_lo(sw[gr / 2]);
-                    vs[nt][gr].y = (NG + gr) & 1 ? ax_bf16_hi(sw[(NG + gr) / 2]) : ax_bf16_lo(sw[(NG + gr) / 2]);
+                    float d[kUnit][2][4] = {};
+#pragma unroll
+                    for (int i = 0; i < WG; i++) {
+                        const uint4 q0 = s_q[(2 * (gr * WG + i)) * 32 + lane], q1 = s_q[(2 * (gr * WG + i) + 1) * 32 + lane];
+#pragma unroll
+                        for (int u = 0; u < kUnit; u++)
+#pragma unroll
+                            for (int nt = 0; nt < 2; nt++) mma(d[u][nt], q0, n_low(kw[u][nt][gr * WG + i]), n_high(kw[u][nt][gr * WG + i]));
+#pragma unroll
+                        for (int u = 0; u < kUnit; u++)
+#pragma unroll
+                            for (int nt = 0; nt < 2; nt++) {
+                                const uint32_t v = kw[u][nt][gr * WG + i] >> 8;
+                                mma(d[u][nt], q1, n_low(v), n_high(v));
+                            }
+                    }
+#pragma unroll
+                    for (int u = 0; u < kUnit; u++)
+#pragma unroll
+                        for (int nt = 0; nt < 2; nt++) {                       // scales of columns 2t and 2t + 1, NG numbers each
+                            const float k0 = gr & 1 ? ax_bf16_hi(ks[u][nt][gr / 2]) : ax_bf16_lo(ks[u][nt][gr / 2]);
+                            const float k1 = (NG + gr) & 1 ? ax_bf16_hi(ks[u][nt][(NG + gr) / 2]) : ax_bf16_lo(ks[u][nt][(NG + gr) / 2]);
+                            s[u][nt] = fma2(make_float2(k0, k1), add2(make_float2(d[u][nt][0], d[u][nt][1]), make_float2(d[u][nt][2], d[u][nt][3])), s[u][nt]);
+                        }
                 }
-                s[nt] = mul2(s[nt], make_float2(qback, qback));
             }
-            const int row = info.tile * AX_P4_TILE;
-            if (row < seg_lo || row + AX_P4_TILE > seg_len) {
 #pragma unroll
-                for (int nt = 0; nt < 2; nt++) {                               // column 8·nt + 2t + b is row 8·nt + 4b + t
-                    const int r0 = row + nt * 8 + t, r1 = r0 + 4;
-                    if (r0 < seg_lo || r0 >= seg_len) {
-                        s[nt].x = -INFINITY;
+            for (int u = 0; u < kUnit; u++)
 #pragma unroll
-                        for (int gr = 0; gr < NG; gr++) vs[nt][gr].x = 0.f;
+                for (int nt = 0; nt < 2; nt++) {
+                    uint32_t sw[NG];
+                    lds<NG>(sw, unit + u * TILE + 2 * PLANE + SC + (8 * nt + 2 * t) * NG * 2);
+#pragma unroll
+                    for (int gr = 0; gr < NG; gr++) {
+                        vs[u][nt][gr].x = gr & 1 ? ax_bf16_hi(sw[gr / 2]) : ax_bf16_lo(sw[gr / 2]);
+                        vs[u][nt][gr].y = (NG + gr) & 1 ? ax_bf16_hi(sw[(NG + gr) / 2]) : ax_bf16_lo(sw[(NG + gr) / 2]);
                     }
-                    if (r1 < seg_lo || r1 >= seg_len) {
-                        s[nt].y = -INFINITY;
-#pragma unroll
-                        for (int gr = 0; gr < NG; gr++) vs[nt][gr].y = 0.f;
-                    }
+                    s[u][nt] = mul2(s[u][nt], make_float2(qback, qback));
                 }
+            const int row = info.tile * AX_P4_TILE;
+            if (row < seg_lo || row + kUnit * AX_P4_TILE > seg_len || info.ok != 3) {      // rows out of sight have no score and no scale
+#pragma unroll
+                for (int u = 0; u < kUnit; u++)
+#pragma unroll
+                    for (int nt = 0; nt < 2; nt++) {                           // column 8·nt + 2t + b is row 8·nt + 4b + t
+                        const int r0 = row + u * AX_P4_TILE + nt * 8 + t, r1 = r0 + 4;
+                        const bool here = info.ok >> u & 1;
+                        if (!here || r0 < seg_lo || r0 >= seg_len) {
+                            s[u][nt].x = -INFINITY;
+#pragma unroll
+                            for (int gr = 0; gr < NG; gr++) vs[u][nt][gr].x = 0.f;
+                        }
+                        if (!here || r1 < seg_lo || r1 >= seg_len) {
+                            s[u][nt].y = -INFINITY;
+#pragma unroll
+                            for (int gr = 0; gr < NG; gr++) vs[u][nt][gr].y = 0.f;
+                        }
+                    }
             }
             float top = -INFINITY;
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                float2 big = vs[nt][0];
+            for (int u = 0; u < kUnit; u++)
 #pragma unroll
-                for (int gr = 1; gr < NG; gr++) { big.x = fmaxf(big.x, vs[nt][gr].x); big.y = fmaxf(big.y, vs[nt][gr].y); }
-                const float2 z = add2(s[nt], make_float2(fmaxf(lg2(big.x), -100.f), fmaxf(lg2(big.y), -100.f)));
-                top = fmaxf(top, fmaxf(z.x, z.y));
-            }
+                for (int nt = 0; nt < 2; nt++) {
+                    float2 big = vs[u][nt][0];
+#pragma unroll
+                    for (int gr = 1; gr < NG; gr++) { big.x = fmaxf(big.x, vs[u][nt][gr].x); big.y = fmaxf(big.y, vs[u][nt][gr].y); }
+                    const float2 z = add2(s[u][nt], make_float2(fmaxf(lg2(big.x), -100.f), fmaxf(lg2(big.y), -100.f)));
+                    top = fmaxf(top, fmaxf(z.x, z.y));
+                }
             top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 1));
             top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 2));
             // The reference is moved only where a p · scale would pass 2^15; then the largest becomes 2^7, so what is lost of the small
@@ -395,36 +441,45 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 m = mn;
             }
             const float mr = m == -INFINITY ? 0.f : -m;
-            float2 p[2];
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-                p[nt] = add2(s[nt], make_float2(mr, mr));
-                p[nt].x = ex2(p[nt].x); p[nt].y = ex2(p[nt].y);
-                l = add2(l, p[nt]);
-            }
-            uint32_t vw[2][W];
+            for (int u = 0; u < kUnit; u++)
 #pragma unroll
-            for (int nt = 0; nt < 2; nt++) lds<W>(vw[nt], tile + PLANE + nt * (PLANE / 2) + lane * W * 4);
+                for (int nt = 0; nt < 2; nt++) {                               // scores become probabilities
+                    s[u][nt] = add2(s[u][nt], make_float2(mr, mr));
+                    s[u][nt].x = ex2(s[u][nt].x); s[u][nt].y = ex2(s[u][nt].y);
+                    l = add2(l, s[u][nt]);
+                }
+            uint32_t vw[kUnit][2][W];
+#pragma unroll
+            for (int u = 0; u < kUnit; u++)
+#pragma unroll
+                for (int nt = 0; nt < 2; nt++) lds<W>(vw[u][nt], unit + u * TILE + PLANE + nt * (PLANE / 2) + lane * W * 4);
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) {
-                uint32_t hl[4];
+                uint4 a[kUnit];
 #pragma unroll
-                for (int nt = 0; nt < 2; nt++) {
-                    const float2 y = mul2(p[nt], vs[nt][gr]);
-                    hl[2 * nt] = pack_f16(y.x, y.y);
-                    const float2 r = fma2(unpack_f16(hl[2 * nt]), make_float2(-1.f, -1.f), y);
-                    hl[2 * nt + 1] = pack_f16(r.x, r.y);
+                for (int u = 0; u < kUnit; u++) {
+                    uint32_t hl[4];
+#pragma unroll
+                    for (int nt = 0; nt < 2; nt++) {
+                        const float2 y = mul2(s[u][nt], vs[u][nt][gr]);
+                        hl[2 * nt] = pack_f16(y.x, y.y);
+                        const float2 r = fma2(unpack_f16(hl[2 * nt]), make_float2(-1.f, -1.f), y);
+                        hl[2 * nt + 1] = pack_f16(r.x, r.y);
+                    }
+                    a[u] = make_uint4(hl[0], hl[1], hl[2], hl[3]);
                 }
-                const uint4 a = make_uint4(hl[0], hl[1], hl[2], hl[3]);
 #pragma unroll
                 for (int i = 0; i < WG; i++) {
                     const int cw = gr * WG + i;
-                    const uint32_t u0 = vw[0][cw], u1 = vw[1][cw];
-                    float (&d0)[4] = o[cw * 4], (&d1)[4] = o[cw * 4 + 1], (&d2)[4] = o[cw * 4 + 2], (&d3)[4] = o[cw * 4 + 3];
-                    mma(d0, a, n_low(u0), n_low(u1));
-                    mma(d1, a, n_high(u0), n_high(u1));
-                    mma(d2, a, n_low(u0 >> 8), n_low(u1 >> 8));
-                    mma(d3, a, n_high(u0 >> 8), n_high(u1 >> 8));
+#pragma unroll
+                    for (int u = 0; u < kUnit; u++) {
+                        const uint32_t u0 = vw[u][0][cw], u1 = vw[u][1][cw];
+                        mma(o[cw * 4], a[u], n_low(u0), n_low(u1));
+                        mma(o[cw * 4 + 1], a[u], n_high(u0), n_high(u1));
+                        mma(o[cw * 4 + 2], a[u], n_low(u0 >> 8), n_low(u1 >> 8));
+                        mma(o[cw * 4 + 3], a[u], n_high(u0 >> 8), n_high(u1 >> 8));
+                    }
                 }
             }
         }
@@ -583,7 +638,7 @@ int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPage
     dv.part_ml = (float*)(w + ticket_bytes(grid));
     dv.part_o = dv.part_ml + (size_t)2 * grid * kHeads * 2;
     const int tile = ax_p4_tile_bytes(kv->s);
-    const size_t smem = (size_t)kWarps * (kStages * tile + kv->s.hd / 32 * 2 * 32 * 16 + dv.hpt * kv->s.hd * 4) + (size_t)(a.batch + 1) * 4;
+    const size_t smem = (size_t)kWarps * (kStages * kUnit * tile + kv->s.hd / 32 * 2 * 32 * 16 + dv.hpt * kv->s.hd * 4) + (size_t)(a.batch + 1) * 4;
     if (kv->s.hd == 128) return kv->s.group == 32 ? launch<128, 32>(ctx, dv, grid, smem) : launch<128, 64>(ctx, dv, grid, smem);
     return kv->s.group == 32 ? launch<64, 32>(ctx, dv, grid, smem) : launch<64, 64>(ctx, dv, grid, smem);
 }
