@@ -244,6 +244,9 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    if (tid == kCopy * 32) {
+        for (const CUtensorMap* map : { &map_q, &map_k, &map_v }) asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory");
+    }
     if (warp == kProduct) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -269,7 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         const int tb = dv.pair_heads ? kRows : 2 * kRows, hx = dv.pair_heads ? a.n_heads / 2 : a.n_heads;
         const int per = (a.batch + 31) / 32, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
         long long own = 0;                                                    // 64 bits: prefix arrays that overlap may name more rows than there are
-        for (int b = b0; b < b1; b++) own += (ax_prompt_seq(a, b).lq + tb - 1) / tb;
+        AxPromptSeq held = {};                                                // the lane's sequence where it has one at most
+        for (int b = b0; b < b1; b++) { held = ax_prompt_seq(a, b); own += (held.lq + tb - 1) / tb; }
         long long inc = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) { const long long x = __shfl_up_sync(AX_FULL, inc, d); if (lane >= d) inc += x; }
@@ -295,7 +299,8 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 for (int c = c0; c < c1; c += 32) {
                     const int b = c + lane;
                     AxPromptSeq q = {};
-                    if (b < c1) q = ax_prompt_seq(a, b);
+                    if (per == 1) { if (lane == g) q = held; }
+                    else if (b < c1) q = ax_prompt_seq(a, b);
                     const int mine = (q.lq + tb - 1) / tb;
                     int up = mine;
 #pragma unroll
@@ -477,10 +482,10 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 ok = __all_sync(AX_FULL, ok);
                 if (!ok) break;
                 cuts++;
-                for (int i = lane; i < (kRows - valid) * 8 * BOXES; i += 32) {
-                    const int b = i / ((kRows - valid) * 8), r = i % ((kRows - valid) * 8);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(v + b * kBoxBytes + valid * 128 + r * 16), "r"(0) : "memory");
-                }
+#pragma unroll
+                for (int b = 0; b < BOXES; b++)
+                    for (uint32_t at = valid * 128 + lane * 16; at < kBoxBytes; at += 512)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(v + b * kBoxBytes + at), "r"(0) : "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&v_cut));
