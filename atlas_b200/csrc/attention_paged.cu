@@ -334,14 +334,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     int st = 0;
     uint32_t phase = 0;
     for (int it = 0; it < count; it++) {
+        const UnitInfo info = s_info[warp][st];
+        // known before the unit is here: a new segment's query comes under its copy
+        if (info.seg != seg) { if (seg >= 0) flush(); start(info.seg); }
         if (!mbar_wait(smem_u32(&s_bar[warp][st]), phase)) {
             if (lane == 0) atomicExch(dv.err, kErrWait);
             for (int y = it; y < count && y < it + kStages; y++)              // what is in flight lands before the CTA goes
                 mbar_wait(smem_u32(&s_bar[warp][y % kStages]), (uint32_t)(y / kStages) & 1u);
             break;
         }
-        const UnitInfo info = s_info[warp][st];
-        if (info.seg != seg) { if (seg >= 0) flush(); start(info.seg); }
         if (info.ok) {
             // Both tiles side by side: their chains — scores, softmax, products — are each other's cover.  (One tile at a time left 54 % of the
             // issue slots and 41 % of the busiest pipe in use.)
