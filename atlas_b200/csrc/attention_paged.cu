@@ -528,12 +528,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         }
         if (!whole) {
             const long long cf = ((s0 + 1) * C - 1) / total, cl = ((s0 + n) * C - 1) / total;     // first and last CTA of the segment
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) s_last = atomicAdd(dv.tickets + cf, 1u) == (unsigned)(cl - cf);
+            __syncthreads();                                                                      // the CTA's stores come before thread 0's
+            if (tid == 0) {                                                                       // release, and through it before the count
+                unsigned before;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(dv.tickets + cf) : "memory");
+                s_last = before == (unsigned)(cl - cf);
+            }
             __syncthreads();
             if (s_last) {
-                __threadfence();
                 // part k is the tail of CTA cf (k = 0) or the head of CTA cf + k
                 const int cnt = (int)(cl - cf) + 1;
                 const float* ml = dv.part_ml + 2 * (size_t)cf * hpt * 2;
@@ -541,32 +543,46 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                 auto part = [&](int k) { return (size_t)(2 * k + (k == 0)) * hpt; };
                 float* wt = reinterpret_cast<float*>(smem + RING);                                // weights of kChunk parts per head, over the first warp's query
                 static_assert(kHeads * kChunk * 4 <= QBYTES, "weights do not fit");
-                for (int h = warp; h < heads; h += kWarps) {
-                    float M = -INFINITY;
-                    for (int k = lane; k < cnt; k += 32) M = fmaxf(M, __ldcg(ml + (part(k) + h) * 2));
-                    M = ax_warp_max(M);
-                    if (lane == 0) s_ml[0][h][0] = M;
+                // maxima of the parts; those of the first chunk stay in registers with their sums
+                constexpr int HW = kHeads / kWarps;                                               // heads of a warp: warp, warp + kWarps
+                float2 own[HW][kChunk / 32];
+                float M[HW], L[HW] = {};
+#pragma unroll
+                for (int i = 0; i < HW; i++) {
+                    const int h = warp + i * kWarps;
+                    M[i] = -INFINITY;
+                    if (h >= heads) continue;
+#pragma unroll
+                    for (int r = 0; r < kChunk / 32; r++) {
+                        const int k = lane + 32 * r;
+                        own[i][r] = k < cnt ? __ldcg((const float2*)(ml + (part(k) + h) * 2)) : make_float2(-INFINITY, 0.f);
+                        M[i] = fmaxf(M[i], own[i][r].x);
+                    }
+                    for (int k = lane + kChunk; k < cnt; k += 32) M[i] = fmaxf(M[i], __ldcg(ml + (part(k) + h) * 2));
+                    M[i] = ax_warp_max(M[i]);
                 }
                 constexpr int E = (kHeads * HD / 4 + kWarps * 32 - 1) / (kWarps * 32);            // float4 outputs of a thread
                 float4 A[E];
 #pragma unroll
                 for (int e = 0; e < E; e++) A[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-                float L = 0.f;                                                                    // of head `warp`, then `warp + kWarps`
-                float L2 = 0.f;
                 for (int k0 = 0; k0 < cnt; k0 += kChunk) {
                     const int kn = min(kChunk, cnt - k0);
-                    __syncthreads();
-                    for (int h = warp; h < heads; h += kWarps) {
-                        const float M = s_ml[0][h][0];
+                    if (k0) __syncthreads();
+#pragma unroll
+                    for (int i = 0; i < HW; i++) {
+                        const int h = warp + i * kWarps;
+                        if (h >= heads) continue;
                         float sum = 0.f;
-                        for (int k = lane; k < kn; k += 32) {
-                            const float2 v = __ldcg((const float2*)(ml + (part(k0 + k) + h) * 2));
-                            const float f = v.y == 0.f ? 0.f : v.x == M ? 1.f : ex2(v.x - M);
+#pragma unroll
+                        for (int r = 0; r < kChunk / 32; r++) {
+                            const int k = lane + 32 * r;
+                            if (k >= kn) continue;
+                            const float2 v = k0 ? __ldcg((const float2*)(ml + (part(k0 + k) + h) * 2)) : own[i][r];
+                            const float f = v.y == 0.f ? 0.f : v.x == M[i] ? 1.f : ex2(v.x - M[i]);
                             wt[h * kChunk + k] = f;
                             sum += f * v.y;
                         }
-                        sum = ax_warp_sum(sum);
-                        if (h < kWarps) L += sum; else L2 += sum;
+                        L[i] += ax_warp_sum(sum);
                     }
                     __syncthreads();
 #pragma unroll
@@ -582,7 +598,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                         }
                     }
                 }
-                if (lane == 0) { if (warp < heads) s_ml[0][warp][1] = L; if (warp + kWarps < heads) s_ml[0][warp + kWarps][1] = L2; }
+                if (lane == 0)
+                    for (int i = 0; i < HW; i++) if (warp + i * kWarps < heads) s_ml[0][warp + i * kWarps][1] = L[i];
                 __syncthreads();
 #pragma unroll
                 for (int e = 0; e < E; e++) {
