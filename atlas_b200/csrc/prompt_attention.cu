@@ -2,7 +2,7 @@
 //
 // 4 · hd flops and one exponential per visible (query, key) pair and head: at hd 128 a tile of 128 × 128 pairs is 1024 clocks of
 // tcgen05.mma and 1024 clocks of the SM's 16 exponentials a clock, so neither may wait for the other.  One prompt of 8192 rows with 32 heads:
-// 586 µs, 938 TFLOP/s = 59 % of the measured matrix rate, at 990 W (the power cap) and 1.6 GHz: a pair of tiles takes 3070 clocks, its
+// 569 µs, 966 TFLOP/s = 60 % of the measured matrix rate, at 990 W (the power cap) and 1.6 GHz: a pair of tiles takes 3070 clocks, its
 // chain being scores → maximum 540 → exponentials 1450 → products and scores of the next tile 1070.
 //   * A CTA works on two query tiles of 128 rows with the same keys: the same rows of two heads that share a KV head, or — where the
 //     heads do not pair up — 256 consecutive rows of one head.

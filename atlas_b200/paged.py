@@ -61,7 +61,17 @@ class DeviceArray:
         return self.ctx.download(self.ptr, self.shape, _NUMPY[self.dtype])
 
     def columns(self, first, shape, strides):
-        """A view that starts `first` elements in, with a shape and strides of its own."""
+        """A view that starts `first` elements in, with a shape and strides of its own; all of it lies within this array."""
+        def reach(shape, strides):
+            if 0 in shape:
+                return 0, -1
+            ends = [(int(n) - 1) * int(s) for n, s in zip(shape, strides)]
+            return sum(e for e in ends if e < 0), sum(e for e in ends if e > 0)
+        if len(shape) != len(strides) or any(n < 0 for n in shape):
+            raise AtlasError("a view needs sizes of zero or more and a stride for each")
+        (lo, hi), (first_here, last_here) = reach(shape, strides), reach(self.shape, self.strides)
+        if hi >= lo and (first + lo < first_here or first + hi > last_here):
+            raise AtlasError(f"a view of elements {first + lo}..{first + hi} leaves an array of elements {first_here}..{last_here}")
         return DeviceArray(self.ctx, self.ptr + first * np.dtype(_NUMPY[self.dtype]).itemsize, shape, self.dtype, strides, base=self)
 
     def __del__(self):

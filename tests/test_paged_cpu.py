@@ -261,3 +261,19 @@ def test_device_array_strides():
     assert a.strides == (32, 8, 1)
     assert a.columns(8, (3, 2, 8), (32, 8, 1)).ptr == P + 32
     assert np.dtype(np.uint16).itemsize * 8 == 16
+
+
+def test_device_array_views_stay_within_their_array():
+    a = arr((3, 4, 8), ab.F32)                                        # elements 0..95
+    assert a.columns(95, (1, 1, 1), (1, 1, 1)).ptr == P + 4 * 95
+    assert a.columns(88, (3, 8), (-40, 1)).ptr == P + 4 * 88          # backwards, 8..95
+    assert a.columns(96, (0, 8), (8, 1)).shape == (0, 8)              # an empty view reaches nothing
+    part = a.columns(8, (3, 2, 8), (32, 8, 1))                        # 0..79 of its own
+    assert part.columns(72, (8,), (1,)).ptr == P + 4 * 80
+    for view, first, shape, strides in [(a, 96, (1,), (1,)), (a, -1, (1,), (1,)), (a, 8, (3, 4, 8), (32, 8, 1)), (a, 79, (3, 8), (-40, 1)),
+                                        (part, 80, (1,), (1,)), (part, 72, (9,), (1,)), (arr((0, 8), ab.F32), 0, (1,), (1,))]:
+        with pytest.raises(ab.AtlasError, match="leaves an array"):
+            view.columns(first, shape, strides)
+    for shape, strides in [((3, 4), (1,)), ((-1, 4), (4, 1))]:
+        with pytest.raises(ab.AtlasError, match="a view needs"):
+            a.columns(0, shape, strides)
