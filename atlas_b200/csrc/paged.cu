@@ -9,6 +9,7 @@
 namespace {
 
 constexpr int kPlanThreads = 256;
+constexpr int kAppendThreads = 128, kReadThreads = 256;
 constexpr int kPlanItems = 512;      // tokens (and pages taken) per CTA
 
 struct PlanArgs {
@@ -173,30 +174,30 @@ __device__ __forceinline__ float max3(float x, float y, float z) {      // NaN i
     float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z)); return d;
 }
 
-// A lane holds sixteen consecutive numbers of one row of K or V; 2 or 4 lanes make a group and find its largest magnitude with
-// shuffles.  scale = bf16(max / 7); the number is x · (1 / scale) rounded half away from zero — the f32 arithmetic of
+// A lane holds thirty-two consecutive numbers of one row of K or V: a group, or half of one whose largest magnitude two lanes
+// find with a shuffle.  scale = bf16(max / 7); the number is x · (1 / scale) rounded half away from zero — the f32 arithmetic of
 // Int4Tensor::quantize with a scale of 16 bits: the numbers are rounded against the scale that is stored, so its own rounding (2^-8 of
 // itself) costs nothing beyond the half step of the number, and no number passes 7 · (1 + 2^-7) before it is rounded: 7 is the largest.
 // A group with a NaN or an infinity gets the scale NaN.
 // Bytes: the rows once, 4.25 or 4.5 bits per number out.  A CTA takes 32 (hd 128) or 64 consecutive rows of one head: as a rule a few whole
-// tiles of the pool.  What bounds it beside the memory is instructions: with run-time shapes and rows found by division 8191 rows × 32
-// heads × 128 took 181 µs, with eight numbers a lane and integer packing 76 µs; now 51 µs.
+// tiles of the pool.  What bounds it beside the memory is instructions (71 % of the issue slots): 8191 rows × 32 heads × 128 in bf16 took
+// 181 µs with run-time shapes and rows found by division, 76 with eight numbers a lane, 50 with sixteen, 39 now (26 at the copy bandwidth).
 template <typename T, int HD, int GS>
-__global__ void __launch_bounds__(256) ax_p4_append_kernel(const RowArgs a) {
-    constexpr int LANES = HD / 16, GL = GS / 16, TOKENS = 256 / LANES;        // lanes per row, lanes per group, rows per CTA
+__global__ void __launch_bounds__(kAppendThreads) ax_p4_append_kernel(const RowArgs a) {
+    constexpr int N = 32, LANES = HD / N, GL = GS / N, TOKENS = kAppendThreads / LANES;        // lanes per row, lanes per group, rows per CTA
     const int li = threadIdx.x % LANES, tok = blockIdx.x * TOKENS + threadIdx.x / LANES, head = blockIdx.y, which = blockIdx.z;
     const AxP4Shape sh = fixed_shape<HD, GS>(a.s);
     const bool live = tok < a.n;
-    float x[16] = {};
+    float x[N] = {};
     float top = 0.f;
     int slot = -1;
     if (live) {
         slot = a.slots[tok];
         const T* src = which ? (const T*)a.v + tok * a.v_tok + head * a.v_head : (const T*)a.k + tok * a.k_tok + head * a.k_head;
-        load8<T>(src + 16 * li, reinterpret_cast<float (&)[8]>(x[0]));
-        load8<T>(src + 16 * li + 8, reinterpret_cast<float (&)[8]>(x[8]));
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
+        for (int i = 0; i < N; i += 8) load8<T>(src + N * li + i, reinterpret_cast<float (&)[8]>(x[i]));
+#pragma unroll
+        for (int i = 0; i < N; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
     }
 #pragma unroll
     for (int d = 1; d < GL; d <<= 1) { const float o = __shfl_xor_sync(AX_FULL, top, d); top = max3(top, o, o); }
@@ -208,19 +209,17 @@ __global__ void __launch_bounds__(256) ax_p4_append_kernel(const RowArgs a) {
     if (sc < 1.17549435e-38f) { sc = 1.0f; sb = 0x3F80; }
     if (odd) { sc = 1.0f; sb = 0x7FC0; }
     const float inv = __frcp_rn(sc);
-    uint32_t half[4];                                                // four numbers each
+    uint32_t half[N / 4];                                            // four numbers each
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        // |y| + (1/2 − 2^-25) + 2^23, the second sum cut off: rounds half away from zero for |y| < 8.  Σ number · 16^j is exact in f32, and so
-        // is the sum with 1.5 · 2^23 + 0x8888, whose low bits are the four nibbles.
-        float w = 0.f;
+    for (int i = 0; i < N / 4; i++) {
+        // y ± (1/2 − 2^-25) cut off: rounds half away from zero for |y| < 8.  Σ (number + 8) · 16^j.
+        int w = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 3; j >= 0; j--) {
             const float y = __fmul_rn(x[4 * i + j], inv);
-            const float m = __fadd_rz(fabsf(y) + 0.49999997f, 8388608.f) - 8388608.f;
-            w = fmaf(copysignf(m, y), (float)(1 << (4 * j)), w);
+            w = w * 16 + __float2int_rz(y + copysignf(0.49999997f, y));
         }
-        half[i] = odd ? 0x8888u : (uint32_t)__float_as_int(w + (12582912.f + 34952.f)) & 0xFFFFu;
+        half[i] = odd ? 0x8888u : (uint32_t)(w + 0x8888) & 0xFFFFu;
     }
     int page, off;
     slot_place(a, slot, page, off);
@@ -229,13 +228,17 @@ __global__ void __launch_bounds__(256) ax_p4_append_kernel(const RowArgs a) {
     const int plane = ax_p4_plane_bytes(sh);
     if (which == 0) {
         uint32_t* kp = reinterpret_cast<uint32_t*>(tile);
-        const uint32_t w0 = half[0] | (half[1] << 16), w1 = half[2] | (half[3] << 16);
-        if (GS == 64) *reinterpret_cast<uint2*>(kp + ax_p4_k_word(sh, r, 16 * li)) = make_uint2(w0, w1);      // one thread's pair of words
-        else { kp[ax_p4_k_word(sh, r, 16 * li)] = w0; kp[ax_p4_k_word(sh, r, 16 * li + 8)] = w1; }
+#pragma unroll
+        for (int i = 0; i < N / 8; i += 2) {
+            const uint32_t w0 = half[2 * i] | (half[2 * i + 1] << 16), w1 = half[2 * i + 2] | (half[2 * i + 3] << 16);
+            uint32_t* at = kp + ax_p4_k_word(sh, r, N * li + 8 * i);
+            if (GS == 64) *reinterpret_cast<uint2*>(at) = make_uint2(w0, w1);                                 // one thread's pair of words
+            else { *at = w0; kp[ax_p4_k_word(sh, r, N * li + 8 * i + 8)] = w1; }
+        }
     } else {
         uint16_t* vp = reinterpret_cast<uint16_t*>(tile + plane);
 #pragma unroll
-        for (int i = 0; i < 4; i++) vp[ax_p4_v_half(sh, r, 16 * li + 4 * i)] = (uint16_t)half[i];
+        for (int i = 0; i < N / 4; i++) vp[ax_p4_v_half(sh, r, N * li + 4 * i)] = (uint16_t)half[i];
     }
     if (li % GL == 0) {
         uint16_t* sp = reinterpret_cast<uint16_t*>(tile + 2 * plane + which * ax_p4_scale_bytes(sh));
@@ -258,8 +261,8 @@ template <> __device__ __forceinline__ void store4<__half>(__half* p, const floa
 // A lane makes four numbers of K and of V, so that a warp's store is one run of bytes (with eight a lane, 32 bytes apart, 8191 rows × 32
 // heads × 128 took 75 µs in f32, now 63 µs: 4.8 TB/s, most of it stores).
 template <typename T, int HD, int GS>
-__global__ void __launch_bounds__(256) ax_p4_read_kernel(const RowArgs a) {
-    constexpr int LANES = HD / 4, TOKENS = 256 / LANES;
+__global__ void __launch_bounds__(kReadThreads) ax_p4_read_kernel(const RowArgs a) {
+    constexpr int LANES = HD / 4, TOKENS = kReadThreads / LANES;
     const int li = threadIdx.x % LANES, tok = blockIdx.x * TOKENS + threadIdx.x / LANES, head = blockIdx.y;
     if (tok >= a.n) return;
     const AxP4Shape sh = fixed_shape<HD, GS>(a.s);
@@ -289,10 +292,10 @@ __global__ void __launch_bounds__(256) ax_p4_read_kernel(const RowArgs a) {
 
 template <typename T, bool READ>
 void launch_rows(const RowArgs& a, cudaStream_t stream) {
-    const int tokens = 256 / (a.s.hd / (READ ? 4 : 16));
+    const int tokens = READ ? kReadThreads / (a.s.hd / 4) : kAppendThreads / (a.s.hd / 32);
     const dim3 grid((unsigned)((a.n + (long long)tokens - 1) / tokens), (unsigned)a.s.n_kv, READ ? 1u : 2u);
-#define AX_ROWS(HD, GS) do { if (READ) ax_p4_read_kernel<T, HD, GS><<<grid, 256, 0, stream>>>(a); \
-                             else ax_p4_append_kernel<T, HD, GS><<<grid, 256, 0, stream>>>(a); } while (0)
+#define AX_ROWS(HD, GS) do { if (READ) ax_p4_read_kernel<T, HD, GS><<<grid, kReadThreads, 0, stream>>>(a); \
+                             else ax_p4_append_kernel<T, HD, GS><<<grid, kAppendThreads, 0, stream>>>(a); } while (0)
     if (a.s.hd == 128) { if (a.s.group == 32) AX_ROWS(128, 32); else AX_ROWS(128, 64); }
     else { if (a.s.group == 32) AX_ROWS(64, 32); else AX_ROWS(64, 64); }
 #undef AX_ROWS
