@@ -88,25 +88,6 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-// two f32 operations in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\t"
-        "mov.b64 {%0, %1}, w;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
 template <int N> __device__ __forceinline__ void lds(uint32_t (&r)[N], const void* p) {
     if constexpr (N == 4) { const uint4 v = *(const uint4*)p; r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
     else if constexpr (N == 2) { const uint2 v = *(const uint2*)p; r[0] = v.x; r[1] = v.y; }
@@ -383,7 +364,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                         for (int nt = 0; nt < 2; nt++) {                       // scales of columns 2t and 2t + 1, NG numbers each
                             const float k0 = gr & 1 ? ax_bf16_hi(ks[u][nt][gr / 2]) : ax_bf16_lo(ks[u][nt][gr / 2]);
                             const float k1 = (NG + gr) & 1 ? ax_bf16_hi(ks[u][nt][(NG + gr) / 2]) : ax_bf16_lo(ks[u][nt][(NG + gr) / 2]);
-                            s[u][nt] = fma2(make_float2(k0, k1), add2(make_float2(d[u][nt][0], d[u][nt][1]), make_float2(d[u][nt][2], d[u][nt][3])), s[u][nt]);
+                            s[u][nt] = ax_fma2(make_float2(k0, k1), ax_add2(make_float2(d[u][nt][0], d[u][nt][1]), make_float2(d[u][nt][2], d[u][nt][3])), s[u][nt]);
                         }
                 }
             }
@@ -398,7 +379,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                         vs[u][nt][gr].x = gr & 1 ? ax_bf16_hi(sw[gr / 2]) : ax_bf16_lo(sw[gr / 2]);
                         vs[u][nt][gr].y = (NG + gr) & 1 ? ax_bf16_hi(sw[(NG + gr) / 2]) : ax_bf16_lo(sw[(NG + gr) / 2]);
                     }
-                    s[u][nt] = mul2(s[u][nt], make_float2(qback, qback));
+                    s[u][nt] = ax_mul2(s[u][nt], make_float2(qback, qback));
                 }
             const int row = info.tile * AX_P4_TILE;
             if (row < seg_lo || row + kUnit * AX_P4_TILE > seg_len || info.ok != 3) {      // rows out of sight have no score and no scale
@@ -428,7 +409,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                     float2 big = vs[u][nt][0];
 #pragma unroll
                     for (int gr = 1; gr < NG; gr++) { big.x = fmaxf(big.x, vs[u][nt][gr].x); big.y = fmaxf(big.y, vs[u][nt][gr].y); }
-                    const float2 z = add2(s[u][nt], make_float2(fmaxf(lg2(big.x), -100.f), fmaxf(lg2(big.y), -100.f)));
+                    const float2 z = ax_add2(s[u][nt], make_float2(fmaxf(lg2(big.x), -100.f), fmaxf(lg2(big.y), -100.f)));
                     top = fmaxf(top, fmaxf(z.x, z.y));
                 }
             top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 1));
@@ -447,9 +428,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             for (int u = 0; u < kUnit; u++)
 #pragma unroll
                 for (int nt = 0; nt < 2; nt++) {                               // scores become probabilities
-                    s[u][nt] = add2(s[u][nt], make_float2(mr, mr));
+                    s[u][nt] = ax_add2(s[u][nt], make_float2(mr, mr));
                     s[u][nt].x = ex2(s[u][nt].x); s[u][nt].y = ex2(s[u][nt].y);
-                    l = add2(l, s[u][nt]);
+                    l = ax_add2(l, s[u][nt]);
                 }
             uint32_t vw[kUnit][2][W];
 #pragma unroll
@@ -464,9 +445,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                     uint32_t hl[4];
 #pragma unroll
                     for (int nt = 0; nt < 2; nt++) {
-                        const float2 y = mul2(s[u][nt], vs[u][nt][gr]);
+                        const float2 y = ax_mul2(s[u][nt], vs[u][nt][gr]);
                         hl[2 * nt] = pack_f16(y.x, y.y);
-                        const float2 r = fma2(unpack_f16(hl[2 * nt]), make_float2(-1.f, -1.f), y);
+                        const float2 r = ax_fma2(unpack_f16(hl[2 * nt]), make_float2(-1.f, -1.f), y);
                         hl[2 * nt + 1] = pack_f16(r.x, r.y);
                     }
                     a[u] = make_uint4(hl[0], hl[1], hl[2], hl[3]);
