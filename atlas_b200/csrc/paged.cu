@@ -9,7 +9,7 @@
 namespace {
 
 constexpr int kPlanThreads = 256;
-constexpr int kAppendThreads = 128, kReadThreads = 256, kReadRows = 2;
+constexpr int kAppendThreads = 64, kReadThreads = 256, kReadRows = 2;
 constexpr int kPlanItems = 512;      // tokens (and pages taken) per CTA
 
 struct PlanArgs {
@@ -179,9 +179,10 @@ __device__ __forceinline__ float max3(float x, float y, float z) {      // NaN i
 // Int4Tensor::quantize with a scale of 16 bits: the numbers are rounded against the scale that is stored, so its own rounding (2^-8 of
 // itself) costs nothing beyond the half step of the number, and no number passes 7 · (1 + 2^-7) before it is rounded: 7 is the largest.
 // A group with a NaN or an infinity gets the scale NaN.
-// Bytes: the rows once, 4.25 or 4.5 bits per number out.  A CTA takes 32 (hd 128) or 64 consecutive rows of one head: as a rule a few whole
-// tiles of the pool.  What bounds it beside the memory is instructions (71 % of the issue slots): 8191 rows × 32 heads × 128 in bf16 took
-// 181 µs with run-time shapes and rows found by division, 76 with eight numbers a lane, 50 with sixteen, 39 now (26 at the copy bandwidth).
+// Bytes: the rows once, 4.25 or 4.5 bits per number out.  A CTA takes 16 (hd 128) or 32 consecutive rows of one head: as a rule a whole
+// tile of the pool or two.  What bounds it beside the memory is instructions (70 % of the issue slots): 8191 rows × 32 heads × 128 in bf16 took
+// 181 µs with run-time shapes and rows found by division, 76 with eight numbers a lane, 50 with sixteen, 39 with thirty-two, 37 with
+// pairs of f32 operations and 64 threads a CTA (256 threads: 40; the copy bandwidth: 26).
 template <typename T, int HD, int GS>
 __global__ void __launch_bounds__(kAppendThreads) ax_p4_append_kernel(const RowArgs a) {
     constexpr int N = 32, LANES = HD / N, GL = GS / N, TOKENS = kAppendThreads / LANES;        // lanes per row, lanes per group, rows per CTA
@@ -215,9 +216,10 @@ __global__ void __launch_bounds__(kAppendThreads) ax_p4_append_kernel(const RowA
         // y ± (1/2 − 2^-25) cut off: rounds half away from zero for |y| < 8.  Σ (number + 8) · 16^j.
         int w = 0;
 #pragma unroll
-        for (int j = 3; j >= 0; j--) {
-            const float y = __fmul_rn(x[4 * i + j], inv);
-            w = w * 16 + __float2int_rz(y + copysignf(0.49999997f, y));
+        for (int j = 2; j >= 0; j -= 2) {
+            float2 y = ax_mul2(make_float2(x[4 * i + j], x[4 * i + j + 1]), make_float2(inv, inv));
+            y = ax_add2(y, make_float2(copysignf(0.49999997f, y.x), copysignf(0.49999997f, y.y)));
+            w = (w * 16 + __float2int_rz(y.y)) * 16 + __float2int_rz(y.x);
         }
         half[i] = odd ? 0x8888u : (uint32_t)(w + 0x8888) & 0xFFFFu;
     }
