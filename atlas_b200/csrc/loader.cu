@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "file_pages.h"
 
 // ── a small JSON reader (objects keep their key order) ───────────────────────────────
 namespace {
@@ -487,7 +488,6 @@ int load_from_files(atlasx_ctx* ctx, const std::vector<std::string>& paths, atla
         if (nr == 0 || nc == 0) continue;                 // this rank keeps nothing of it (padded vocabulary)
         const int up_dtype = d.dtype == ATLASX_BF16 ? ATLASX_BF16 : ATLASX_F32;
         const size_t esz = up_dtype == ATLASX_BF16 ? 2 : 4;
-        const uint8_t* src = st->map + st->data_start + d.off0;
         const void* host = nullptr;
         int on_device = 0;
         if (d.dtype != ATLASX_F16 && nc == cols) {
@@ -508,10 +508,9 @@ int load_from_files(atlasx_ctx* ctx, const std::vector<std::string>& paths, atla
         if (rc) return cleanup(rc);
         // pages of the mapping that a gathered or converted slice touched are not needed again
         if (!on_device) {
-            const long pg = sysconf(_SC_PAGESIZE);
-            const uintptr_t a0 = ((uintptr_t)src + r0 * cols * esz) & ~(uintptr_t)(pg - 1);
-            const uintptr_t a1 = (uintptr_t)src + r1 * cols * esz;
-            if (a1 > a0) madvise((void*)a0, a1 - a0, MADV_DONTNEED);
+            const AxFileRange gone = ax_file_rows(st->data_start + d.off0, d.dtype == ATLASX_F32 ? 4 : 2, cols, r0, r1,
+                                                  (size_t)sysconf(_SC_PAGESIZE), st->map_bytes);
+            if (gone.last > gone.first) madvise((void*)(st->map + gone.first), gone.last - gone.first, MADV_DONTNEED);
         }
         used++;
     }
