@@ -142,6 +142,7 @@ SIGNATURES = {
     "atlasx_pagedkv_append": (ci, [vp, vp, cp]),
     "atlasx_pagedkv_read": (ci, [vp, vp, vp, ci, ci, vp, vp]),
     "atlasx_pagedkv_decode_attention": (ci, [vp, vp, cp]),
+    "atlasx_pagedkv_selftest_wait_expiry": (ci, [vp, vp, cp, C.c_longlong]),
     "atlasx_prompt_attention": (ci, [vp, cp]),
     "atlasx_model_create": (ci, [vp, C.POINTER(ModelConfigC), vp, pvp]),
     "atlasx_model_free": (ci, [vp]),

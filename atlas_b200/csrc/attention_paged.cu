@@ -32,8 +32,8 @@ constexpr int kUnit = 2;                        // tiles that a warp takes at a 
                                                 // take 13 µs so, with two 15.7)
 constexpr int kHeads = 8;                       // query heads of one segment
 constexpr int kChunk = 64;                      // parts of a segment whose weights are in shared memory at a time
-constexpr unsigned long long kWaitNs = 2000000000ull;
-constexpr int kErrWait = 711;
+constexpr unsigned long long kWaitNs = 2000000000ull, kSelftestWaitNs = 20000000ull;
+constexpr int kErrWait = 741;
 
 struct PagedDev {
     AxP4Shape s;
@@ -45,6 +45,8 @@ struct PagedDev {
     float* part_ml;                             // [2 · gridDim][hpt][2]
     float* part_o;                              // [2 · gridDim][hpt][hd]
     int* err;
+    unsigned long long wait_ns;                 // how long a unit's copy may take
+    long long lost;                             // self-test: the unit whose copy is never issued
 };
 
 struct UnitInfo { int seg, tile, ok, pad; };     // segment, first tile, bit u: tile + u is there
@@ -57,13 +59,14 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// bounded: false after two seconds
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    if (mbar_try(bar, parity)) return true;
-    unsigned long long t0 = ax_globaltimer();
-    while (!mbar_try(bar, parity))
-        if (ax_globaltimer() - t0 > kWaitNs) return false;
-    return true;
+// Bounded, and the same answer for all lanes of the warp: one that saw the copy land just as the others gave up would wait for them for good.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned long long ns) {
+    if (__all_sync(AX_FULL, mbar_try(bar, parity))) return true;
+    const unsigned long long t0 = ax_globaltimer();
+    for (;;) {
+        if (__all_sync(AX_FULL, mbar_try(bar, parity))) return true;
+        if (__any_sync(AX_FULL, ax_globaltimer() - t0 > ns)) return false;
+    }
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -103,7 +106,7 @@ __device__ __forceinline__ unsigned tiles_of(int lo, int len) {
     return len > lo ? (unsigned)((len + AX_P4_TILE - 1) / AX_P4_TILE - lo / AX_P4_TILE) : 0u;
 }
 
-template <int HD, int GS>
+template <int HD, int GS, bool LOSE = false>
 __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(const PagedDev dv) {
     constexpr int W = HD / 32;                  // 32-bit words per lane, row block and plane
     constexpr int NG = HD / GS;                 // groups of a row
@@ -176,6 +179,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     const long long X0 = total * c / C, X1 = total * (c + 1) / C;
     const long long x0 = X0 + (X1 - X0) * warp / kWarps, x1 = X0 + (X1 - X0) * (warp + 1) / kWarps;
 
+    // request, segment of the request and unit of the segment of unit y of the whole
+    auto locate = [&](long long y, int& b, int& hh, int& ti) {
+        int lo = 0, hi = batch;                                               // last b with s_pre[b] · nh <= y (skipping requests without rows)
+        while (hi - lo > 1) { const int m = (lo + hi) >> 1; if ((long long)s_pre[m] * dv.nh <= y) lo = m; else hi = m; }
+        const unsigned n = s_pre[lo + 1] - s_pre[lo];
+        const long long rem = y - (long long)s_pre[lo] * dv.nh;
+        if (total <= 0x7FFFFFFFll) { hh = (int)((unsigned)rem / n); ti = (int)((unsigned)rem % n); }
+        else { hh = (int)(rem / n); ti = (int)(rem % n); }
+        b = lo;
+    };
+
     // ── the warp's stream of units: 32 positions are resolved at a time, one per lane, and lane i copies unit i of them ──
     const int count = (int)(x1 - x0);
     const uint8_t* src[kUnit] = {};
@@ -186,13 +200,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             const long long y = x0 + i + lane;
             mine.seg = -1; mine.tile = 0; mine.ok = 0;
             if (y < x1) {
-                int lo = 0, hi = batch;                                       // last b with s_pre[b] · nh <= y (skipping requests without rows)
-                while (hi - lo > 1) { const int m = (lo + hi) >> 1; if ((long long)s_pre[m] * dv.nh <= y) lo = m; else hi = m; }
-                const unsigned n = s_pre[lo + 1] - s_pre[lo];
-                const long long rem = y - (long long)s_pre[lo] * dv.nh;
-                int hh, ti;
-                if (total <= 0x7FFFFFFFll) { hh = (int)((unsigned)rem / n); ti = (int)((unsigned)rem % n); }
-                else { hh = (int)(rem / n); ti = (int)(rem % n); }
+                int lo, hh, ti;
+                locate(y, lo, hh, ti);
                 int first, len; row_range(dv, lo, first, len);
                 mine.seg = lo * dv.nh + hh;
                 mine.tile = first / AX_P4_TILE + us * ti;
@@ -218,7 +227,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             const bool one = mine.ok == 3 && src[1] == src[0] + TILE;          // neighbours in a page
             if (mine.ok) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(mine.ok == 3 ? UNIT : TILE) : "memory");
             else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
-            if (one) copy(0, UNIT);
+            if (LOSE && x0 + i == dv.lost) { }
+            else if (one) copy(0, UNIT);
             else {
                 if (mine.ok & 1) copy(0, TILE);
                 if (mine.ok & 2) copy(1, TILE);
@@ -319,10 +329,19 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         const UnitInfo info = s_info[warp][st];
         // known before the unit is here: a new segment's query comes under its copy
         if (info.seg != seg) { if (seg >= 0) flush(); start(info.seg); }
-        if (!mbar_wait(smem_u32(&s_bar[warp][st]), phase)) {
+        if (!mbar_wait(smem_u32(&s_bar[warp][st]), phase, dv.wait_ns)) {
             if (lane == 0) atomicExch(dv.err, kErrWait);
             for (int y = it; y < count && y < it + kStages; y++)              // what is in flight lands before the CTA goes
-                mbar_wait(smem_u32(&s_bar[warp][y % kStages]), (uint32_t)(y / kStages) & 1u);
+                mbar_wait(smem_u32(&s_bar[warp][y % kStages]), (uint32_t)(y / kStages) & 1u, dv.wait_ns);
+            // The segment that goes on behind the warp's piece is entered all the same, with a sum of zero: every CTA of a segment
+            // has to arrive at its ticket, or the count is ahead in all later launches.
+            int b, hh, ti;
+            locate(x1 - 1, b, hh, ti);
+            const unsigned n = s_pre[b + 1] - s_pre[b];
+            if (b * dv.nh + hh != seg && (long long)s_pre[b] * dv.nh + (long long)(hh + 1) * n > x1) {
+                if (lane == 0) s_seg[warp * 2 + 1] = b * dv.nh + hh;
+                if (lane < kHeads) { s_ml[warp * 2 + 1][lane][0] = -INFINITY; s_ml[warp * 2 + 1][lane][1] = 0.f; }
+            }
             break;
         }
         if (info.ok) {
@@ -601,14 +620,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
 
 constexpr int kMaxGrid = 1024;
 
-template <int HD, int GS>
+template <int HD, int GS, bool LOSE = false>
 int launch(atlasx_ctx* ctx, const PagedDev& dv, int grid, size_t smem) {
     static std::atomic<bool> ready[64] = {};
     if (ctx->device >= 64 || !ready[ctx->device]) {                           // the limit is per device; asking twice does no harm
-        AX_CUDA(cudaFuncSetAttribute(ax_paged_attn_kernel<HD, GS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        AX_CUDA(cudaFuncSetAttribute(ax_paged_attn_kernel<HD, GS, LOSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         if (ctx->device < 64) ready[ctx->device] = true;
     }
-    ax_paged_attn_kernel<HD, GS><<<grid, kWarps * 32, smem, ctx->stream>>>(dv);
+    ax_paged_attn_kernel<HD, GS, LOSE><<<grid, kWarps * 32, smem, ctx->stream>>>(dv);
     AX_CHECK_LAUNCH("ax_paged_attn_kernel");
     return ATLASX_OK;
 }
@@ -623,9 +642,10 @@ size_t ax_paged_attn_workspace_bytes(const atlasx_ctx* ctx, const AxP4Shape& s) 
     return ticket_bytes(grid) + (size_t)2 * grid * kHeads * (s.hd + 2) * 4;
 }
 
-int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPagedAttnArgs& a) {
+int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPagedAttnArgs& a, long long lost) {
     PagedDev dv = {};
     dv.s = kv->s; dv.pool = kv->pool; dv.a = a; dv.err = ctx->dev_error;
+    dv.wait_ns = lost < 0 ? kWaitNs : kSelftestWaitNs; dv.lost = lost;
     dv.group_heads = a.n_heads / kv->s.n_kv;
     dv.head_tiles = (dv.group_heads + kHeads - 1) / kHeads;
     dv.hpt = min(kHeads, dv.group_heads);
@@ -639,6 +659,7 @@ int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPage
     dv.part_o = dv.part_ml + (size_t)2 * grid * kHeads * 2;
     const int tile = ax_p4_tile_bytes(kv->s);
     const size_t smem = (size_t)kWarps * (kStages * kUnit * tile + kv->s.hd / 32 * 2 * 32 * 16 + dv.hpt * kv->s.hd * 4) + (size_t)(a.batch + 1) * 4;
+    if (lost >= 0) return launch<64, 32, true>(ctx, dv, grid, smem);
     if (kv->s.hd == 128) return kv->s.group == 32 ? launch<128, 32>(ctx, dv, grid, smem) : launch<128, 64>(ctx, dv, grid, smem);
     return kv->s.group == 32 ? launch<64, 32>(ctx, dv, grid, smem) : launch<64, 64>(ctx, dv, grid, smem);
 }

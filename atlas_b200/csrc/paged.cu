@@ -458,7 +458,7 @@ extern "C" int atlasx_pagedkv_read(atlasx_ctx* c, const atlasx_pagedkv* kv, cons
     return ATLASX_OK;
 }
 
-extern "C" int atlasx_pagedkv_decode_attention(atlasx_ctx* c, const atlasx_pagedkv* kv, const atlasx_pagedkv_attn_args* p) {
+static int decode_attention(atlasx_ctx* c, const atlasx_pagedkv* kv, const atlasx_pagedkv_attn_args* p, long long lost) {
     AX_ARG(p, "null argument");
     const float* q = p->q;
     float* out = p->out;
@@ -484,5 +484,13 @@ extern "C" int atlasx_pagedkv_decode_attention(atlasx_ctx* c, const atlasx_paged
     AxPagedAttnArgs a;
     a.q = q; a.out = out; a.table = table; a.lens = lens; a.table_width = table_width; a.batch = batch; a.n_heads = n_heads;
     a.window = window; a.scale = scale; a.workspace = workspace ? workspace : kv->workspace;
-    return ax_paged_attn_launch(c, kv, a);
+    return ax_paged_attn_launch(c, kv, a, lost);
+}
+extern "C" int atlasx_pagedkv_decode_attention(atlasx_ctx* c, const atlasx_pagedkv* kv, const atlasx_pagedkv_attn_args* p) {
+    return decode_attention(c, kv, p, -1);
+}
+extern "C" int atlasx_pagedkv_selftest_wait_expiry(atlasx_ctx* c, const atlasx_pagedkv* kv, const atlasx_pagedkv_attn_args* p, long long unit) {
+    AX_ARG(unit >= 0, "the unit must not be negative");
+    AX_ARG(kv && kv->s.hd == 64 && kv->s.group == 32, "the self-test takes head_dim 64 and groups of 32");
+    return decode_attention(c, kv, p, unit);
 }

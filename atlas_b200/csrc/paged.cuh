@@ -43,7 +43,8 @@ struct AxPagedAttnArgs {
     void* workspace;                 // of ax_paged_attn_workspace_bytes()
 };
 size_t ax_paged_attn_workspace_bytes(const atlasx_ctx* ctx, const AxP4Shape& s);
-int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPagedAttnArgs& a);
+// lost >= 0: self-test, the copy of that unit is not issued
+int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPagedAttnArgs& a, long long lost = -1);
 
 // two f32 operations in one instruction
 __device__ __forceinline__ float2 ax_fma2(float2 a, float2 b, float2 c) {

@@ -1,0 +1,47 @@
+"""GPU: the packed serving step where it can go wrong — waits that run out, indices outside the pool, extreme values, lengths and windows —
+against plain implementations in 64 bits.  Helpers and tolerances are those of test_gpu_paged.py unless a test derives its own."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from oracle import orc
+from test_gpu_paged import Cache, bf16, check_decode, decode_by_hand, down, held, prompt_by_hand, prompt_case, rows, up
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ab():
+    import atlas_b200
+    return atlas_b200
+
+
+# ── decode attention: a wait that runs out ───────────────────────────────────────
+@pytest.mark.parametrize("lens,n_kv,nh", [([9000], 1, 4), ([3000, 1, 2999, 64], 2, 16), ([40] * 3000, 2, 2), ([200, 17] * 30, 4, 4)])
+def test_a_decode_call_whose_wait_ran_out_leaves_its_workspace_good(ab, lens, n_kv, nh):
+    """The copy of one unit never comes, at many places of the work: the call ends with an error status, all counters are back at zero, and the
+    next call with the same workspace gives what one with a fresh workspace gives."""
+    from atlas_b200 import _ffi
+    rng = np.random.default_rng(len(lens))
+    c = Cache(ab, rng, lens, n_kv, 64, 32, 16)
+    q = rng.standard_normal((len(lens), nh, 64)).astype(np.float32)
+    want = check_decode(ab, c, nh, 0.125, 0, q=q, workspace=c.kv.workspace())
+    ws = c.kv.workspace()
+    ctx = c.kv.ctx
+    qd, out = up(ab, q, ab.F32), up(ab, q, ab.F32)
+    table, n = ab.DeviceArray.from_host(c.table, ab.I32), ab.DeviceArray.from_host(lens, ab.I32)
+    args = _ffi.PAGED_ATTN.pack(qd.ptr, out.ptr, table.ptr, n.ptr, ws.ptr, 4 * ws.shape[0], nh, c.table.shape[1], len(lens), 0, 0.125)
+    tiles = sum(-(-m // 16) for m in lens) * n_kv
+    units = tiles if tiles <= ctx.sm_count * 3 * 4 else sum(-(-(-(-m // 16)) // 2) for m in lens) * n_kv
+    places = sorted({0, 1, units - 1, units - 2} | set(rng.integers(0, units, 10).tolist()))
+    for unit in places:
+        _ffi.check(_ffi.lib().atlasx_pagedkv_selftest_wait_expiry(ctx.handle, c.kv._h, args, int(unit)))
+        code = C.c_int(0)
+        assert _ffi.lib().atlasx_ctx_poll_device_error(ctx.handle, C.byref(code)) == -5 and code.value == 741
+        assert not ws.download()[:3 * ctx.sm_count].any(), unit
+        assert np.array_equal(check_decode(ab, c, nh, 0.125, 0, q=q, workspace=ws), want), unit
+    # a unit that is not there: nothing is lost
+    _ffi.check(_ffi.lib().atlasx_pagedkv_selftest_wait_expiry(ctx.handle, c.kv._h, args, units))
+    assert ctx.poll_device_error() == 0 and np.array_equal(out.download(), want)

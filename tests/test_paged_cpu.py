@@ -277,3 +277,8 @@ def test_device_array_views_stay_within_their_array():
     for shape, strides in [((3, 4), (1,)), ((-1, 4), (4, 1))]:
         with pytest.raises(ab.AtlasError, match="a view needs"):
             a.columns(0, shape, strides)
+
+
+@pytest.mark.parametrize("unit,text", [(-1, "unit"), (0, "head_dim 64")])
+def test_selftest_refusals(unit, text):
+    refused(_ffi.lib().atlasx_pagedkv_selftest_wait_expiry(None, None, packed(_ffi.PAGED_ATTN, DEC), unit), text)
