@@ -44,7 +44,7 @@ struct PagedDev {
     unsigned* tickets;                          // [gridDim] zero between launches
     float* part_ml;                             // [2 · gridDim][hpt][2]
     float* part_o;                              // [2 · gridDim][hpt][hd]
-    int* err;
+    int *err, *index_err;
     unsigned long long wait_ns;                 // how long a unit's copy may take
     long long lost;                             // self-test: the unit whose copy is never issued
 };
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                     if (page >= 0 && page < dv.s.n_pages) {
                         mine.ok |= 1 << u;
                         src[u] = dv.pool + ax_p4_tile_at(dv.s, page, hh / dv.head_tiles, row % dv.s.page_size);
-                    } else atomicExch(dv.err, AX_DEVERR_PAGE);
+                    } else atomicExch(dv.index_err, AX_DEVERR_PAGE);
                 }
             }
         }
@@ -644,7 +644,7 @@ size_t ax_paged_attn_workspace_bytes(const atlasx_ctx* ctx, const AxP4Shape& s) 
 
 int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPagedAttnArgs& a, long long lost) {
     PagedDev dv = {};
-    dv.s = kv->s; dv.pool = kv->pool; dv.a = a; dv.err = ctx->dev_error;
+    dv.s = kv->s; dv.pool = kv->pool; dv.a = a; dv.err = ctx->dev_error; dv.index_err = ctx->index_error();
     dv.wait_ns = lost < 0 ? kWaitNs : kSelftestWaitNs; dv.lost = lost;
     dv.group_heads = a.n_heads / kv->s.n_kv;
     dv.head_tiles = (dv.group_heads + kHeads - 1) / kHeads;

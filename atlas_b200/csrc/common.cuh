@@ -85,8 +85,10 @@ struct atlasx_ctx {
     void* w_planes = nullptr; size_t w_planes_cap = 0;             // int4 weights of one matrix expanded to bf16 hi | lo planes (token batches)
     // argmax scratch
     float* amax_vals = nullptr; int* amax_idx = nullptr; unsigned* amax_ticket = nullptr; int* amax_out = nullptr;
-    // device error word written by bounded waits
+    // device error words: [0] bounded waits that gave up, which makes results invalid; [1] indices of a caller's array that name nothing,
+    // whose rows are left out.  Only the first stops a model.
     int* dev_error = nullptr;          // device
+    int* index_error() const { return dev_error + 1; }
     int* host_pin = nullptr;           // pinned scratch (ints)
     atlasx_comm* comm = nullptr;
     AxSampleScratch sample;

@@ -43,8 +43,8 @@ extern "C" int atlasx_ctx_create(int device, atlasx_ctx** out) {
     c->sm_count = prop.multiProcessorCount;
     c->smem_optin = prop.sharedMemPerBlockOptin;
     AX_CUDA(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
-    AX_CUDA(cudaMalloc((void**)&c->dev_error, sizeof(int)));
-    AX_CUDA(cudaMemset(c->dev_error, 0, sizeof(int)));
+    AX_CUDA(cudaMalloc((void**)&c->dev_error, 2 * sizeof(int)));
+    AX_CUDA(cudaMemset(c->dev_error, 0, 2 * sizeof(int)));
     AX_CUDA(cudaMallocHost((void**)&c->host_pin, 64 * sizeof(int)));
     const int amax_blocks = 4096;
     AX_CUDA(cudaMalloc((void**)&c->amax_vals, amax_blocks * sizeof(float)));
@@ -113,10 +113,11 @@ extern "C" int atlasx_ctx_set_gemv_impl(atlasx_ctx* c, int impl) {
 }
 extern "C" int atlasx_ctx_poll_device_error(atlasx_ctx* c, int* code_out) {
     AX_ARG(c, "ctx is null");
-    AX_CUDA(cudaMemcpyAsync(c->host_pin, c->dev_error, sizeof(int), cudaMemcpyDeviceToHost, c->stream));
+    AX_CUDA(cudaMemcpyAsync(c->host_pin, c->dev_error, 2 * sizeof(int), cudaMemcpyDeviceToHost, c->stream));
     AX_CUDA(cudaStreamSynchronize(c->stream));
-    const int code = c->host_pin[0];
-    if (code) {
+    const int waited = c->host_pin[0], code = waited ? waited : c->host_pin[1];
+    if (code && !waited) AX_CUDA(cudaMemsetAsync(c->index_error(), 0, sizeof(int), c->stream));
+    if (waited) {                                                      // an index error beside it is reported by the next call
         AX_CUDA(cudaMemsetAsync(c->dev_error, 0, sizeof(int), c->stream));
         // kernels that gave up may have left their arrival counters half counted; they are zero between launches otherwise
         if (c->split_scratch) AX_CUDA(cudaMemsetAsync(c->split_scratch, 0, 16384, c->stream));

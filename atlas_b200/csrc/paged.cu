@@ -434,7 +434,7 @@ extern "C" int atlasx_pagedkv_append(atlasx_ctx* c, atlasx_pagedkv* kv, const at
     RowArgs a = {};
     a.s = kv->s; a.pool = kv->pool; a.k = k; a.v = v;
     a.k_tok = k_token_stride; a.k_head = k_head_stride; a.v_tok = v_token_stride; a.v_head = v_head_stride;
-    a.slots = slots; a.n = n; a.err = c->dev_error;
+    a.slots = slots; a.n = n; a.err = c->index_error();
     a.inv_page = page_inverse(kv->s.page_size);
     launch_rows<false>(dtype, a, c->stream);
     AX_CHECK_LAUNCH("ax_p4_append_kernel");
@@ -451,7 +451,7 @@ extern "C" int atlasx_pagedkv_read(atlasx_ctx* c, const atlasx_pagedkv* kv, cons
     AX_ARG(kv->ctx == c, "the cache belongs to another context");
     AX_ON_DEVICE(c);
     RowArgs a = {};
-    a.s = kv->s; a.pool = kv->pool; a.k_out = k_out; a.v_out = v_out; a.slots = slots; a.n = n; a.err = c->dev_error;
+    a.s = kv->s; a.pool = kv->pool; a.k_out = k_out; a.v_out = v_out; a.slots = slots; a.n = n; a.err = c->index_error();
     a.inv_page = page_inverse(kv->s.page_size);
     launch_rows<true>(dtype, a, c->stream);
     AX_CHECK_LAUNCH("ax_p4_read_kernel");

@@ -5,7 +5,7 @@
 
 #define AX_PAGED_MAX_BATCH 4096
 
-// codes of the device error word beside those of the bounded waits: what an index array holds, not a wait, was wrong
+// codes of the context's second device error word: what an index array holds was wrong
 #define AX_DEVERR_PAGE 801      // a block table names a page outside the pool
 #define AX_DEVERR_SLOT 802      // a slot lies behind the pool
 

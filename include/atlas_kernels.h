@@ -97,7 +97,9 @@ int   atlasx_ctx_sm_count(atlasx_ctx* ctx);
 /* GEMV kernel choice: 0 = automatic (plain loads), 1 = plain 128-bit loads, 2 = bulk-copy (TMA) ring,
  * 3 = as 1 but multi-column products keep the scalar kernel instead of the tensor-core one (A/B comparison) */
 int   atlasx_ctx_set_gemv_impl(atlasx_ctx* ctx, int impl);
-/* nonzero when a device-side bounded wait gave up since the last call (clears it) */
+/* nonzero when a device-side bounded wait gave up since the last call (clears it): ATLASX_ERR_TIMEOUT.  Otherwise nonzero when an index of a
+ * caller's array named nothing (801 a page, 802 a slot of the paged cache; its rows were left out) — clears that, ATLASX_ERR_ARG.  Only the
+ * first makes the calls of a model fail until it is cleared. */
 int   atlasx_ctx_poll_device_error(atlasx_ctx* ctx, int* code_out);
 
 /* GpuBuf / GpuBufBf16 (crates/atlas-tensor/src/lib.rs:178-280): raw device memory */
@@ -229,7 +231,7 @@ int atlasx_pagedkv_free(atlasx_pagedkv* kv);
 size_t atlasx_pagedkv_bytes(int n_pages, int page_size, int n_kv_heads, int head_dim, int group);
 int atlasx_pagedkv_ptrs(atlasx_pagedkv* kv, void** pool_dev, size_t* bytes, size_t* workspace_bytes);
 /* Rows of K and V [n][n_kv_heads][head_dim], f32, bf16 or f16, strides in elements, every row on a 16-byte boundary, into their
- * slots.  A negative slot marks a row that is not there; one behind the pool is left out and raises the device error word
+ * slots.  A negative slot marks a row that is not there; one behind the pool is left out and raises the index error word
  * (atlasx_ctx_poll_device_error).  Slots of one call are distinct. */
 typedef struct {
     const void *k, *v;
@@ -243,7 +245,7 @@ int atlasx_pagedkv_append(atlasx_ctx* ctx, atlasx_pagedkv* kv, const atlasx_page
 int atlasx_pagedkv_read(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const int* slots_dev, int n, int dtype, void* k_out_dev, void* v_out_dev);
 /* One new token per request: q and out [batch][n_heads][head_dim] f32, rows max(0, lens[b] − window) .. lens[b] − 1 of request b
  * (window 0: all) through its block table; lens beyond the table are cut to it, a request of no rows gets zeros.  Rows of a page
- * number outside the pool are left out and raise the device error word.  workspace: NULL for the cache's own, else
+ * number outside the pool are left out and raise the index error word.  workspace: NULL for the cache's own, else
  * workspace_bytes (atlasx_pagedkv_ptrs) zeroed once before its first use; calls that may run at the same time — graphs replayed on
  * different streams — need workspaces of their own. */
 typedef struct {

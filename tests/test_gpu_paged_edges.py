@@ -45,3 +45,36 @@ def test_a_decode_call_whose_wait_ran_out_leaves_its_workspace_good(ab, lens, n_
     # a unit that is not there: nothing is lost
     _ffi.check(_ffi.lib().atlasx_pagedkv_selftest_wait_expiry(ctx.handle, c.kv._h, args, units))
     assert ctx.poll_device_error() == 0 and np.array_equal(out.download(), want)
+
+
+# ── indices that name nothing ────────────────────────────────────────────────────
+def test_bad_slots_and_pages_do_not_stop_a_model(ab):
+    """They are reported by poll_device_error, and the model on the same context goes on."""
+    import helpers
+    w = helpers.synth_weights(helpers.SMALL_SWA, seed=8)
+    m = helpers.cuda_model(dict(helpers.SMALL_SWA), w, helpers.SMALL_SWA_LAYERS, kv_dtype=ab.F32)
+    want = m.forward_one_gpu(7)
+    m.reset()
+    kv = ab.PagedKvCache(2, 16, 1, 64)
+    x = up(ab, np.ones((1, 1, 64)), ab.F32)
+    one = ab.DeviceArray.from_host([1], ab.I32)
+    kv.append(x, x, ab.DeviceArray.from_host([32], ab.I32))
+    assert np.array_equal(m.forward_one_gpu(7), want)
+    with pytest.raises(ab.AtlasError, match="slot"):
+        kv.ctx.poll_device_error()
+    kv.decode_attention(x, up(ab, np.ones((1, 1, 64)), ab.F32), ab.DeviceArray.from_host([[2]], ab.I32), one, 0.1)
+    m.reset()
+    assert np.array_equal(m.forward_one_gpu(7), want)
+    # a wait that ran out is reported first, and does stop the model; the index error beside it is still there afterwards
+    from atlas_b200 import _ffi
+    code = C.c_int(0)
+    _ffi.check(_ffi.lib().atlasx_comm_selftest_wait_expiry(kv.ctx.handle, C.byref(code), 1))
+    with pytest.raises(ab.AtlasError, match="bounded device-side wait"):
+        m.forward_one_gpu(7)
+    with pytest.raises(ab.AtlasError, match="bounded device-side wait"):
+        kv.ctx.poll_device_error()
+    with pytest.raises(ab.AtlasError, match="page outside"):
+        kv.ctx.poll_device_error()
+    assert kv.ctx.poll_device_error() == 0
+    m.reset()
+    assert np.array_equal(m.forward_one_gpu(7), want)
