@@ -207,7 +207,9 @@ __global__ void __launch_bounds__(kAppendThreads) ax_p4_append_kernel(const RowA
     const bool odd = !(top <= 3.402823466e38f);
     uint16_t sb = ax_f32_to_bf16_rne(__fdiv_rn(top, 7.0f));
     float sc = ax_bf16_to_f32(sb);
-    if (sc < 1.17549435e-38f) { sc = 1.0f; sb = 0x3F80; }
+    // Below the smallest normal number every number of the group is zero (against a scale of 1).  What is stored is that smallest
+    // scale: decode attention takes the size of a row's values from its scales, and a row of zeros has none.
+    if (sc < 1.17549435e-38f) { sc = 1.0f; sb = 0x0080; }
     if (odd) { sc = 1.0f; sb = 0x7FC0; }
     const float inv = __frcp_rn(sc);
     uint32_t half[N / 4];                                            // four numbers each

@@ -221,9 +221,10 @@ typedef struct {
 int atlasx_page_plan(atlasx_ctx* ctx, const atlasx_page_plan_args* args);
 
 /* Paged KV cache in four bits: n_pages pages of page_size rows (a multiple of 16, at most 8192), head_dim 64 or 128.  `group` (32 or 64)
- * consecutive numbers of a row of a head share a bf16 scale = bf16(max|x| / 7), 1.0 below the smallest normal number; the number is
- * x · (1 / scale) in f32, rounded half away from zero, −7..7 (Int4Tensor::quantize, crates/atlas-quant/src/lib.rs:113-145, with a
- * 16-bit scale).  A group with a NaN or an infinity reads as NaN.  The layout within a page is the library's own. */
+ * consecutive numbers of a row of a head share a bf16 scale = bf16(max|x| / 7); the number is x · (1 / scale) in f32, rounded half away from
+ * zero, −7..7, and zero for the whole group where the scale is below the smallest normal number (Int4Tensor::quantize,
+ * crates/atlas-quant/src/lib.rs:113-145, with a 16-bit scale).  A group with a NaN or an infinity reads as NaN.  The layout within a page
+ * is the library's own. */
 typedef struct atlasx_pagedkv atlasx_pagedkv;
 int atlasx_pagedkv_create(atlasx_ctx* ctx, int n_pages, int page_size, int n_kv_heads, int head_dim, int group, atlasx_pagedkv** out);
 int atlasx_pagedkv_free(atlasx_pagedkv* kv);

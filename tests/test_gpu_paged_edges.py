@@ -78,3 +78,42 @@ def test_bad_slots_and_pages_do_not_stop_a_model(ab):
     assert kv.ctx.poll_device_error() == 0
     m.reset()
     assert np.array_equal(m.forward_one_gpu(7), want)
+
+
+# ── decode attention: values of very different size ──────────────────────────────
+class Held(Cache):
+    """A cache of given rows: request i has lens[i] rows of its own, one behind the other, in pages of `page`."""
+
+    def __init__(self, ab, lens, k, v, group, page=16):
+        self.ab, self.lens, self.page = ab, lens, page
+        need = [-(-n // page) for n in lens]
+        self.n_pages = sum(need)
+        self.table = np.full((len(lens), max(need)), -1)
+        at = 0
+        for b, m in enumerate(need):
+            self.table[b, :m] = np.arange(at, at + m)
+            at += m
+        full = lambda x: np.concatenate([x, np.zeros((self.n_pages * page - len(x),) + x.shape[1:], x.dtype)])      # noqa: E731
+        k, v = full(np.asarray(k, np.float32)), full(np.asarray(v, np.float32))
+        self.kv = ab.PagedKvCache(self.n_pages, page, k.shape[1], k.shape[2], group=group)
+        self.kv.append(up(ab, k, ab.F32), up(ab, v, ab.F32), ab.DeviceArray.from_host(np.arange(len(k)), ab.I32))
+        self.k, self.v = held(k, group), held(v, group)
+
+
+@pytest.mark.parametrize("hd,group", [(64, 32), (64, 64), (128, 32), (128, 64)])
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-8, 1e-12, 1e-20])
+def test_rows_and_groups_of_zeros_beside_small_values(ab, hd, group, size):
+    """A group of zeros says nothing about the size of the others: V of any size beside zero rows (padding, a first token) and beside a
+    group of zeros is as accurate as without them (the tolerance has no term for them: 7 · scale ≤ 1.01 · max|v| holds for every group
+    that is not zero)."""
+    rng = np.random.default_rng(17)
+    n = 100
+    k, v = rows(rng, n, 2, hd), size * rows(rng, n, 2, hd)
+    v[[0, 5, 40, 41, 99]] = 0
+    v[20:30, :, :group] = 0
+    k[7] = 0
+    c = Held(ab, [n], k, v, group)
+    check_decode(ab, c, 4, 1 / math.sqrt(hd), 0, rng=rng)
+    check_decode(ab, c, 4, 1 / math.sqrt(hd), 3, rng=rng)
+    c = Held(ab, [40], k[:40], 0 * v[:40], group)                          # nothing but zeros
+    assert not check_decode(ab, c, 4, 0.1, 0, rng=rng).any()
