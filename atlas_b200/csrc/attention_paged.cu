@@ -420,6 +420,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                         }
                     }
             }
+            // A probability is at most 2^15 over the smallest scale that counts: 2^95, and 2^31 of them stay below 2^127.  Values under
+            // that scale are exact to 2^-112 instead of to 2^-32 of the largest.
+            constexpr float kSmallest = -80.f;
             float top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < kUnit; u++)
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                     float2 big = vs[u][nt][0];
 #pragma unroll
                     for (int gr = 1; gr < NG; gr++) { big.x = fmaxf(big.x, vs[u][nt][gr].x); big.y = fmaxf(big.y, vs[u][nt][gr].y); }
-                    const float2 z = ax_add2(s[u][nt], make_float2(fmaxf(lg2(big.x), -100.f), fmaxf(lg2(big.y), -100.f)));
+                    const float2 z = ax_add2(s[u][nt], make_float2(fmaxf(lg2(big.x), kSmallest), fmaxf(lg2(big.y), kSmallest)));
                     top = fmaxf(top, fmaxf(z.x, z.y));
                 }
             top = fmaxf(top, __shfl_xor_sync(AX_FULL, top, 1));

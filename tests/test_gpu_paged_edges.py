@@ -117,3 +117,29 @@ def test_rows_and_groups_of_zeros_beside_small_values(ab, hd, group, size):
     check_decode(ab, c, 4, 1 / math.sqrt(hd), 3, rng=rng)
     c = Held(ab, [40], k[:40], 0 * v[:40], group)                          # nothing but zeros
     assert not check_decode(ab, c, 4, 0.1, 0, rng=rng).any()
+
+
+@pytest.mark.parametrize("window", [0, 5_000_000])
+def test_tiny_values_over_many_rows(ab, window):
+    """2^24 rows (2048 times one page of 8192) with V near 1e-30: the sum of the probabilities stays finite.  The softmax over repeated rows is that
+    over the page; a window of w rows sees its last w mod 8192 rows once more than the others.  Tolerance: as for all decode calls, and 2^-112 for values
+    below 2^-80, times 2 for the scale's rounding and the products' sums."""
+    rng = np.random.default_rng(23)
+    page, times = 8192, 2048
+    k, v = rows(rng, page, 1, 64), 1e-30 * rows(rng, page, 1, 64)
+    c = Held(ab, [page], k, v, 32, page)
+    q = rng.standard_normal((1, 2, 64)).astype(np.float32)
+    q[0, 0] = 0                                                              # all rows alike: the largest sum
+    out = up(ab, np.full(q.shape, 7.0), ab.F32)
+    c.kv.decode_attention(up(ab, q, ab.F32), out, ab.DeviceArray.from_host(np.zeros((1, times)), ab.I32),
+                          ab.DeviceArray.from_host([page * times], ab.I32), 0.125, window)
+    n = window or page * times
+    count = np.full(page, n // page)
+    count[page - n % page:] += 1 if n % page else 0
+    for h in range(2):
+        a = c.k[:, 0] @ q[0, h].astype(np.float64) * 0.125
+        p = np.exp(a - a.max()) * count
+        p /= p.sum()
+        e = (2.0 ** -16 + 2.0 ** -18) * 0.125 * (np.abs(c.k[:, 0]) @ np.abs(q[0, h].astype(np.float64))).max()
+        tol = (2 * e + 2.0 ** -12) * (p @ np.abs(c.v[:, 0])) + 2.0 ** -111
+        assert np.all(np.abs(out.download()[0, h] - p @ c.v[:, 0]) <= tol)
