@@ -5,7 +5,10 @@
 #include <stdint.h>
 #include <stddef.h>
 #include <stdio.h>
+#include <functional>
+#include <mutex>
 #include <string>
+#include <vector>
 
 #include "../../include/atlas_kernels.h"
 
@@ -96,6 +99,19 @@ struct atlasx_ctx {
     // at this address — first/last CTA start, first dependency release, last CTA end, first CTA end, last input staged —
     // and the launcher advances the pointer
     unsigned long long* trace_next = nullptr;
+    // objects whose handle was freed while the stream was being captured: freed by the first call after the capture
+    std::mutex deferred_lock;
+    std::vector<std::function<void()>> deferred;
+};
+
+// While the context's stream is being captured nothing may wait for it or free memory: either would end the capture with an error, and a
+// garbage collector frees when it likes.  true: `free_it` is kept for later; false: nothing is captured, go on (what was kept is freed now).
+bool ax_ctx_defer(atlasx_ctx* ctx, std::function<void()> free_it);
+// For the length of a free: memory may go although some other stream is being captured in global mode.
+struct AxRelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    AxRelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~AxRelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
 };
 
 // Timeline stamps of one launch; t is read from %globaltimer (ns).

@@ -84,11 +84,29 @@ extern "C" int atlasx_ctx_create(int device, atlasx_ctx** out) {
     return ATLASX_OK;
 }
 
+bool ax_ctx_defer(atlasx_ctx* c, std::function<void()> free_it) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(c->stream, &st) != cudaSuccess) cudaGetLastError();
+    if (st != cudaStreamCaptureStatusNone) {
+        std::lock_guard<std::mutex> hold(c->deferred_lock);
+        try { if (free_it) c->deferred.push_back(std::move(free_it)); } catch (...) { }      // no memory to keep it in: it stays
+        return true;
+    }
+    std::vector<std::function<void()>> now;
+    {
+        std::lock_guard<std::mutex> hold(c->deferred_lock);
+        now.swap(c->deferred);
+    }
+    for (auto& f : now) f();
+    return false;
+}
+
 void atlasx_comm_destroy(atlasx_ctx* ctx);   // comm.cpp
 
 extern "C" int atlasx_ctx_destroy(atlasx_ctx* c) {
     if (!c) return ATLASX_OK;
     cudaSetDevice(c->device);
+    ax_ctx_defer(c, nullptr);
     cudaStreamSynchronize(c->stream);
     atlasx_comm_destroy(c);
     ax_sample_free_scratch(c);
@@ -101,6 +119,7 @@ extern "C" int atlasx_ctx_destroy(atlasx_ctx* c) {
 }
 extern "C" int atlasx_ctx_sync(atlasx_ctx* c) {
     AX_ARG(c, "ctx is null");
+    ax_ctx_defer(c, nullptr);
     AX_CUDA(cudaStreamSynchronize(c->stream));
     return ATLASX_OK;
 }
@@ -184,12 +203,16 @@ extern "C" int atlasx_malloc(atlasx_ctx* c, size_t bytes, void** out) {
     AX_ARG(c && out, "null argument");
     *out = nullptr;
     if (bytes == 0) return ATLASX_OK;
+    ax_ctx_defer(c, nullptr);
     AX_CUDA(cudaMalloc(out, bytes));
     return ATLASX_OK;
 }
 extern "C" int atlasx_free(atlasx_ctx* c, void* dev) {
     AX_ARG(c, "ctx is null");
-    if (dev) { AX_CUDA(cudaStreamSynchronize(c->stream)); AX_CUDA(cudaFree(dev)); }
+    if (!dev || ax_ctx_defer(c, [c, dev] { atlasx_free(c, dev); })) return ATLASX_OK;
+    AX_CUDA(cudaStreamSynchronize(c->stream));
+    AxRelaxedCapture relaxed;
+    AX_CUDA(cudaFree(dev));
     return ATLASX_OK;
 }
 extern "C" int atlasx_memset(atlasx_ctx* c, void* dev, int value, size_t bytes) {
@@ -345,7 +368,9 @@ extern "C" int atlasx_matrix_wrap(atlasx_ctx* c, int dtype, const void* data, co
 extern "C" int atlasx_matrix_free(atlasx_matrix* m) {
     if (!m) return ATLASX_OK;
     if (m->owned) {
+        if (ax_ctx_defer(m->ctx, [m] { atlasx_matrix_free(m); })) return ATLASX_OK;
         cudaStreamSynchronize(m->ctx->stream);
+        AxRelaxedCapture relaxed;
         cudaFree(m->data_own); cudaFree(m->scales_own);
     }
     delete m;
@@ -476,8 +501,9 @@ extern "C" int atlasx_kvcache_create(atlasx_ctx* c, int max_seq, int n_kv, int h
     return ATLASX_OK;
 }
 extern "C" int atlasx_kvcache_free(atlasx_kvcache* kv) {
-    if (!kv) return ATLASX_OK;
+    if (!kv || ax_ctx_defer(kv->ctx, [kv] { atlasx_kvcache_free(kv); })) return ATLASX_OK;
     cudaStreamSynchronize(kv->ctx->stream);
+    AxRelaxedCapture relaxed;
     cudaFree(kv->k); cudaFree(kv->v);
     delete kv;
     return ATLASX_OK;

@@ -944,8 +944,9 @@ extern "C" int atlasx_model_create(atlasx_ctx* ctx, const atlasx_model_config* c
 }
 
 extern "C" int atlasx_model_free(atlasx_model* m) {
-    if (!m) return ATLASX_OK;
+    if (!m || ax_ctx_defer(m->ctx, [m] { atlasx_model_free(m); })) return ATLASX_OK;
     cudaStreamSynchronize(m->ctx->stream);
+    AxRelaxedCapture relaxed;
     if (m->graph) cudaGraphExecDestroy(m->graph);
     if (m->graph_tok) cudaGraphExecDestroy(m->graph_tok);
     for (Layer& ly : m->layers) if (ly.kv) atlasx_kvcache_free(ly.kv);

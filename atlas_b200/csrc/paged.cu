@@ -402,8 +402,9 @@ extern "C" int atlasx_pagedkv_create(atlasx_ctx* c, int n_pages, int page_size, 
     return ATLASX_OK;
 }
 extern "C" int atlasx_pagedkv_free(atlasx_pagedkv* kv) {
-    if (!kv) return ATLASX_OK;
+    if (!kv || ax_ctx_defer(kv->ctx, [kv] { atlasx_pagedkv_free(kv); })) return ATLASX_OK;
     AX_ON_DEVICE(kv->ctx);
+    AxRelaxedCapture relaxed;
     cudaStreamSynchronize(kv->ctx->stream);
     cudaFree(kv->pool); cudaFree(kv->workspace);
     delete kv;

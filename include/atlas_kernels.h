@@ -103,6 +103,8 @@ int   atlasx_ctx_set_gemv_impl(atlasx_ctx* ctx, int impl);
 int   atlasx_ctx_poll_device_error(atlasx_ctx* ctx, int* code_out);
 
 /* GpuBuf / GpuBufBf16 (crates/atlas-tensor/src/lib.rs:178-280): raw device memory */
+/* While the context's stream is being captured, atlasx_free and the other free calls keep what they are given and free it with the first
+ * call after the capture that allocates, frees or synchronises. */
 int atlasx_malloc(atlasx_ctx* ctx, size_t bytes, void** out_dev);
 int atlasx_free(atlasx_ctx* ctx, void* dev);
 int atlasx_memset(atlasx_ctx* ctx, void* dev, int value, size_t bytes);

@@ -143,3 +143,108 @@ def test_tiny_values_over_many_rows(ab, window):
         e = (2.0 ** -16 + 2.0 ** -18) * 0.125 * (np.abs(c.k[:, 0]) @ np.abs(q[0, h].astype(np.float64))).max()
         tol = (2 * e + 2.0 ** -12) * (p @ np.abs(c.v[:, 0])) + 2.0 ** -111
         assert np.all(np.abs(out.download()[0, h] - p @ c.v[:, 0]) <= tol)
+
+
+# ── capture on the context's stream, with nothing but the driver ─────────────────
+class Graph:
+    """What was called inside `with Graph(ctx)`, replayed on the context's stream or another one (cuStreamBeginCapture: the calls behind
+    cudaStreamBeginCapture and its family)."""
+
+    def __init__(self, ctx, mode=0):
+        self.cu, self.s, self.mode = C.CDLL("libcuda.so.1"), C.c_void_p(ctx.stream), mode      # 0 global, 1 thread-local, 2 relaxed
+        self.exec = C.c_void_p()
+
+    def ok(self, rc):
+        assert rc == 0, "driver error %d" % rc
+
+    def __enter__(self):
+        self.ok(self.cu.cuStreamBeginCapture_v2(self.s, self.mode))
+        return self
+
+    def __exit__(self, kind, *_):
+        g = C.c_void_p()
+        rc = self.cu.cuStreamEndCapture(self.s, C.byref(g))
+        if kind is None:
+            self.ok(rc)
+            self.ok(self.cu.cuGraphInstantiateWithFlags(C.byref(self.exec), g, C.c_ulonglong(0)))
+        if g:
+            self.cu.cuGraphDestroy(g)
+
+    def replay(self, stream=None):
+        self.ok(self.cu.cuGraphLaunch(self.exec, C.c_void_p(stream) if stream else self.s))
+
+    def close(self):
+        if self.exec:
+            self.ok(self.cu.cuGraphExecDestroy(self.exec))
+            self.exec = C.c_void_p()
+
+    def free_bytes(self):
+        a, b = C.c_size_t(), C.c_size_t()
+        self.ok(self.cu.cuMemGetInfo_v2(C.byref(a), C.byref(b)))
+        return a.value
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])
+def test_a_step_is_captured_while_objects_are_freed(ab, mode):
+    """plan → append → decode captured with arrays of this module; arrays, caches, vectors and matrices that nothing refers to any more go
+    while the capture runs.  The capture holds, the graph follows the lengths, and the memory is free afterwards."""
+    rng = np.random.default_rng(61)
+    b, nh, n_kv, hd, page, n_pages, width = 3, 4, 2, 128, 16, 60, 16
+    kv = ab.PagedKvCache(n_pages, page, n_kv, hd)
+    ctx = kv.ctx
+    i32 = lambda x: ab.DeviceArray.from_host(x, ab.I32)                       # noqa: E731
+    order = rng.permutation(n_pages)
+    lens = np.array([100, 16, 47])
+    table_np = np.full((b, width), -1)
+    at = 0
+    for i, n in enumerate(lens):
+        m = -(-n // page)
+        table_np[i, :m] = order[at:at + m]
+        at += m
+    k0, v0 = rows(rng, n_pages * page, n_kv, hd), rows(rng, n_pages * page, n_kv, hd)
+    kv.append(up(ab, k0, ab.F32), up(ab, v0, ab.F32), i32(np.arange(n_pages * page)))
+    kh, vh = held(k0, 32), held(v0, 32)
+    table, free, cached, fresh = i32(table_np), i32(order[at:]), i32(lens), i32([1, 1, 1])
+    cu, now, slots, pos, status = (i32(np.zeros(n)) for n in (b + 1, b, b, b, 3))
+    k, v, q, out = (up(ab, np.zeros((b, h, hd)), ab.F32) for h in (n_kv, n_kv, nh, nh))
+    kn, vn, qn = rows(rng, b, n_kv, hd), rows(rng, b, n_kv, hd), rng.standard_normal((b, nh, hd)).astype(np.float32)
+    for d, x in ((k, kn), (v, vn), (q, qn)):
+        ctx.upload(d.ptr, x)
+    gone = [ab.DeviceArray.empty((1 << 28,), ab.F32), ab.PagedKvCache(4096, 64, 8, 128), ab.GpuVec.zeros(1 << 26),
+            ab.GpuMatrix.upload(np.zeros((512, 512)), 512, 512), ab.GpuKvCache(4096, 8, 128)]
+    # run once outside: kernels are loaded by their first launch
+    ab.page_plan(cached, fresh, free, table, cu, now, slots, pos, status, page_size=page, n_pages=n_pages)
+    kv.append(k, v, slots)
+    kv.decode_attention(q, out, table, now, 0.09)
+    ctx.sync()
+    g = Graph(ctx, mode)
+    before = g.free_bytes()
+    with g:
+        gone.pop()
+        ab.page_plan(cached, fresh, free, table, cu, now, slots, pos, status, page_size=page, n_pages=n_pages)
+        gone.clear()
+        kv.append(k, v, slots)
+        kv.decode_attention(q, out, table, now, 0.09)
+        assert g.free_bytes() < before + (1 << 20)                           # kept
+    for _ in range(3):
+        ctx.upload(out.ptr, np.zeros((b, nh, hd), np.float32))
+        g.replay()
+        got = out.download()
+        assert status.download().tolist()[1:] == [0, 0]
+        sl = slots.download()
+        kh[sl], vh[sl] = held(kn, 32), held(vn, 32)
+        c = Cache.__new__(Cache)
+        c.page, c.table, c.k, c.v = page, table.download(), kh, vh
+        want, tol = decode_by_hand(c, qn, 0.09, 0, (lens + 1).tolist())
+        assert np.all(np.abs(got - want) <= tol)
+        used = int(status.download()[0])
+        ctx.upload(free.ptr, np.roll(free.download(), -used))
+        lens = lens + 1
+        ctx.upload(cached.ptr, lens.astype(np.int32))
+        kn, vn, qn = rows(rng, b, n_kv, hd), rows(rng, b, n_kv, hd), rng.standard_normal((b, nh, hd)).astype(np.float32)
+        for d, x in ((k, kn), (v, vn), (q, qn)):
+            ctx.upload(d.ptr, x)
+    ctx.sync()
+    assert g.free_bytes() > before + (1 << 30)
+    g.close()
+    assert ctx.poll_device_error() == 0
