@@ -355,6 +355,17 @@ extern "C" int atlasx_page_plan(atlasx_ctx* c, const atlasx_page_plan_args* p) {
     AX_ARG(n_tokens <= 0x3FFFFFFF, "too many new rows for one call");
     AX_ARG((free_pages || !n_free) && ((slots && pos) || !n_tokens), "null argument");
     AX_ARG(c, "ctx is null");
+    // CTAs read the inputs while others write: an output over an input (lens over cached, say) would be read half new
+    struct Range {
+        const int* at; long long n;
+        bool meets(const Range& o) const { return n && o.n && at < o.at + o.n && o.at < at + n; }
+    };
+    const Range out[] = { { table, (long long)batch * table_width }, { cu, batch + 1ll }, { lens, batch }, { slots, n_tokens },
+                                                           { pos, n_tokens }, { status, 3 } }, in[] = { { cached, batch }, { fresh, batch }, { free_pages, n_free } };
+    for (const Range& o : out) {
+        for (const Range& i : in) AX_ARG(!o.meets(i), "an output overlaps an input");
+        for (const Range& other : out) AX_ARG(&o == &other || !o.meets(other), "outputs overlap");
+    }
     AX_ON_DEVICE(c);
     PlanArgs a = { cached, fresh, free_pages, batch, n_free, page_size, n_pages, table_width, n_tokens, table, cu, lens, slots, pos, status };
     const int grid = n_tokens ? (n_tokens + kPlanItems - 1) / kPlanItems : 1;      // a page is taken for a new token: never more pages than tokens

@@ -212,7 +212,8 @@ int atlasx_decode_attention_static(void* stream, int kv_dtype, const void* k_dev
  * for new row i of the pack slots[i] = page · page_size + row within the page (−1 where the page is outside the pool) and pos[i],
  * its position in the request; rows from cu[batch] to n_tokens get −1 in both.  status[3]: pages taken, pages missing, requests
  * with lengths that are negative or wider than the table (one more if the new rows are more than n_tokens).  Where either of the
- * last two is not zero nothing is planned: the table stays, cu and lens are 0, slots and pos −1. */
+ * last two is not zero nothing is planned: the table stays, cu and lens are 0, slots and pos −1.  No output may lie over an input
+ * or another output (this step's lens are the next one's cached: two arrays in turn). */
 typedef struct {
     const int *cached, *fresh;                    /* [batch] */
     const int* free_pages;                        /* [n_free] */

@@ -282,3 +282,22 @@ def test_device_array_views_stay_within_their_array():
 @pytest.mark.parametrize("unit,text", [(-1, "unit"), (0, "head_dim 64")])
 def test_selftest_refusals(unit, text):
     refused(_ffi.lib().atlasx_pagedkv_selftest_wait_expiry(None, None, packed(_ffi.PAGED_ATTN, DEC), unit), text)
+
+
+def test_plan_refuses_outputs_that_overlap():
+    """No device is asked: the context is memory of zeros, which a refusal never looks into."""
+    ctx = C.create_string_buffer(1 << 16)
+    q = 1 << 12
+    apart = dict(PLAN, **{n: P + q * i for i, n in enumerate(("cached", "fresh", "free", "table", "cu", "lens", "slots", "pos", "status"))})
+    call = lambda **change: _ffi.lib().atlasx_page_plan(C.addressof(ctx), packed(_ffi.PAGE_PLAN, dict(apart, **change)))      # noqa: E731
+    for out in ("table", "cu", "lens", "slots", "pos", "status"):
+        for other in ("cached", "fresh", "free"):
+            refused(call(**{out: apart[other]}), "overlaps an input")
+        refused(call(**{out: apart["cached"] + 12}), "overlaps an input")                   # the last request's number
+    refused(call(cu=apart["fresh"] - 16), "overlaps an input")                              # five numbers: the last is fresh[0]
+    refused(call(table=apart["fresh"] - 60), "overlaps an input")
+    refused(call(slots=apart["pos"]), "outputs overlap")
+    refused(call(status=apart["table"] + 4 * 15), "outputs overlap")
+    if not ab.cuda_available():                                                             # nothing to refuse: a device is asked for
+        for fine in ({}, dict(fresh=apart["cached"]), dict(cu=apart["fresh"] - 20), dict(lens=apart["cached"] + 16), dict(table=apart["fresh"] - 64)):
+            assert call(**fine) == -2, fine
