@@ -776,7 +776,8 @@ extern "C" int atlasx_prompt_attention(atlasx_ctx* c, const atlasx_prompt_args* 
     AX_ARG(c, "ctx is null");
     AX_ON_DEVICE(c);
     PromptDev dv = {};
-    dv.a = { q, k, v, out, q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head, cu_q, cu_k, batch, n_q, n_k, n_heads, n_kv, hd, window, scale };
+    dv.a = { q, k, v, out, q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head, cu_q, cu_k, batch, n_q, n_k, n_heads, n_kv, hd,
+             window < n_k ? window : 0, scale };                              // no key lies further behind a query, and "position − window" stays within 32 bits
     dv.pair_heads = (n_heads / n_kv) % 2 == 0;
     dv.negate = scale < 0.f;
     dv.wide = (uintptr_t)out % 32 == 0 && (n_q == 1 || o_tok % 16 == 0) && (n_heads == 1 || o_head % 16 == 0);

@@ -248,3 +248,14 @@ def test_a_step_is_captured_while_objects_are_freed(ab, mode):
     assert g.free_bytes() > before + (1 << 30)
     g.close()
     assert ctx.poll_device_error() == 0
+
+
+# ── prompt attention ─────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nh", [2, 3])
+def test_windows_wider_than_the_prompts(ab, hd, nh):
+    """They hide nothing, up to the largest one, with more queries than keys (negative positions) too: bit for bit the result without one."""
+    lq, lk = [300, 20, 9, 150, 140], [170, 3, 0, 150, 400]
+    want = prompt_case(ab, lq, lk, nh, 1, hd, 0, "BF16", np.random.default_rng(71))
+    for window in (400, sum(lk) - 1, sum(lk), 1 << 30, (1 << 31) - 300, (1 << 31) - 1):
+        assert np.array_equal(prompt_case(ab, lq, lk, nh, 1, hd, window, "BF16", np.random.default_rng(71)), want), window
