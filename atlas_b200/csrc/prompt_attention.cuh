@@ -47,7 +47,7 @@ __device__ __forceinline__ void ax_prompt_row(const AxPromptArgs& a, const AxPro
         for (int e = 0; e < N; e++) d += q[e] * ax_to_f32<T>(kp[e]);
         d = ax_warp_sum(d);
         const float mn = fmaxf(m, d);
-        const float c = l == 0.f ? 0.f : expf(m - mn), p = expf(d - mn);
+        const float c = l == 0.f ? 0.f : expf(m - mn), p = d == -INFINITY ? 0.f : expf(d - mn);      // d − mn is NaN while all scores are −inf
         l = l * c + p; m = mn;
 #pragma unroll
         for (int e = 0; e < N; e++) o[e] = o[e] * c + p * ax_to_f32<T>(vp[e]);

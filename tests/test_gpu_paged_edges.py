@@ -259,3 +259,25 @@ def test_windows_wider_than_the_prompts(ab, hd, nh):
     want = prompt_case(ab, lq, lk, nh, 1, hd, 0, "BF16", np.random.default_rng(71))
     for window in (400, sum(lk) - 1, sum(lk), 1 << 30, (1 << 31) - 300, (1 << 31) - 1):
         assert np.array_equal(prompt_case(ab, lq, lk, nh, 1, hd, window, "BF16", np.random.default_rng(71)), want), window
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_score_of_minus_infinity_weighs_nothing_where_a_row_is_taken_again(ab, hd):
+    """Key 0 scores −inf with every query, value 5 has a NaN in column 7: that column is NaN, the others are the softmax over the other keys;
+    query 0 sees nothing but key 0: 0 / 0."""
+    rng = np.random.default_rng(72)
+    n = 150
+    q, k, v = (bf16(rng.standard_normal((n, 1, hd)).astype(np.float32)) for _ in range(3))
+    q[..., 0] = 1.0
+    k[0] = 0
+    want, tol = prompt_by_hand(q[1:], k[1:], v[1:], [0, n - 1], [0, n - 1], 0.1, 0, False)      # key 0 left out
+    k[0, 0, 0] = -np.inf
+    v[5, 0, 7] = np.nan
+    out = ab.DeviceArray.empty((n, 1, hd), ab.BF16)
+    cu = ab.DeviceArray.from_host([0, n], ab.I32)
+    ab.prompt_attention(*(up(ab, t, ab.BF16) for t in (q, k, v)), out, cu, cu, 0.1)
+    got = down(ab, out)
+    assert np.isnan(got[0]).all() and np.isnan(got[5:, 0, 7]).all()
+    fine = np.abs(got[1:] - want) <= tol
+    assert fine[:4].all() and np.delete(fine, 7, axis=2).all()
+    assert ab.Context.default().poll_device_error() == 0
