@@ -584,7 +584,10 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                         }
                     }
                 }
-                const float neg = m == -INFINITY ? 0.f : -m * sc;
+                // Probabilities are rounded to the type of V, half a step of themselves each, because both operands of a product have one type (hi and
+                // lo parts would double the second product); their sum is that of the f32 numbers.  In f16 they are held 2^7 larger (at most 2^15, beside a
+                // largest number of 2^16), so that what is lost of the small ones is below 2^-32 of the reference instead of 2^-25.
+                const float neg = m == -INFINITY ? 0.f : F16 ? fmaf(-m, sc, 7.f) : -m * sc;
                 const float2 sc2 = make_float2(sc, sc), neg2 = make_float2(neg, neg);
                 auto probs = [&](int c0, bool some) {                                    // 32 keys
                     uint32_t p[16];

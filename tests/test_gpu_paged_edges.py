@@ -281,3 +281,20 @@ def test_a_score_of_minus_infinity_weighs_nothing_where_a_row_is_taken_again(ab,
     fine = np.abs(got[1:] - want) <= tol
     assert fine[:4].all() and np.delete(fine, 7, axis=2).all()
     assert ab.Context.default().poll_device_error() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_small_probabilities_in_f16(ab, hd):
+    """One key with a score of 0 and value 0, 2^17 with probabilities of 2^-26 each and value 1: together they are 2^-9 of the row and more than
+    that of the output.  Half a step of an f16 number per probability (they are powers of two: none) and of the output."""
+    n = (1 << 17) + 1
+    q, k, v = np.zeros((1, 1, hd)), np.zeros((n, 1, hd)), np.ones((n, 1, hd))
+    q[..., 0] = 1
+    k[1:, 0, 0] = -26
+    v[0] = 0
+    out = ab.DeviceArray.empty((1, 1, hd), ab.F16)
+    ab.prompt_attention(*(up(ab, t, ab.F16) for t in (q, k, v)), out, ab.DeviceArray.from_host([0, 1], ab.I32), ab.DeviceArray.from_host([0, n], ab.I32),
+                        math.log(2.0))
+    want = 2.0 ** -9 / (1 + 2.0 ** -9)
+    # ln 2 · log2 e in f32 is off by at most 2^-23 of itself, 26 of it as an exponent by 2^-18
+    assert np.all(np.abs(down(ab, out) - want) <= want * (2.0 ** -11 + 2.0 ** -16))
