@@ -18,7 +18,7 @@
 //     own finds sequence and rows in the prefix arrays: nothing depends on host-side lengths, and a captured call follows the arrays.
 //   * A product of 0 and a NaN or infinity in a value row that the query does not see would be NaN: value rows behind the sequence are
 //     zeroed in shared memory, and an output row that is not finite is taken again by ax_prompt_row, which reads visible rows only.
-//   * Every wait is bounded (ten seconds of %globaltimer): on expiry the CTA raises the context's error word, all roles leave, copies
+//   * Every wait is bounded (ten seconds of %globaltimer, in which no row is taken again): on expiry the CTA raises the context's error word, all roles leave, copies
 //     in flight are waited for and tensor memory is released.
 #include <cuda.h>
 #include <atomic>
@@ -37,8 +37,9 @@ constexpr int kProduct = 8, kCopy = 9, kItems = 11;
 constexpr int kSlots = 2;                         // items known ahead
 constexpr int kReaders = 11;                      // arrivals that free an item's slot: eight softmax warps, products, copies, cut
 constexpr int kMaxStages = 6;
-constexpr unsigned long long kWaitNs = 10000000000ull;      // rows that are taken again one by one may hold the others up
-
+// Limit of a wait; the second is for a test that cannot wait that long.  (As an argument of the launch it made the polling loop of waiting warps
+// longer: 24 ragged prompts 285 -> 296 µs.)
+constexpr int kWaitMs = 10000, kTestWaitMs = 10;
 constexpr unsigned long long kAbortNs = 5000000ull;          // after a failure: what is in flight lands within microseconds
 
 struct PromptDev {
@@ -66,18 +67,21 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// Bounded wait.  false: gave up (this thread's deadline passed, or another role raised the abort flag).
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+// Bounded wait.  false: gave up (this thread's deadline passed, or another role raised the abort flag).  flags: [0] abort, [1] warps that take
+// rows again — as long as there are any (each row is a loop over its keys, so it ends) the deadline does not run: a long prompt
+// with a NaN in its first key has minutes of them.
+template <int WAIT_MS> __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* flags, int* err, int code) {
     if (mbar_try(bar, parity)) return true;
     unsigned long long t0 = 0;
     for (;;) {
 #pragma unroll 1
         for (int i = 0; i < 256; i++)                                         // as few instructions as can be: waiting warps share the issue slots
             if (mbar_try(bar, parity)) return true;
-        if (*abort_flag) return false;
+        if (flags[0]) return false;
+        if (flags[1]) t0 = 0;
         const unsigned long long t = ax_globaltimer();
         if (t0 == 0) t0 = t;
-        else if (t - t0 > kWaitNs) { *abort_flag = 1; atomicExch(err, code); return false; }
+        else if (t - t0 > WAIT_MS * 1000000ull) { flags[0] = 1; atomicExch(err, code); return false; }
     }
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -211,7 +215,7 @@ __device__ __forceinline__ Work work_of(const PromptDev& dv, const Item& it) {
     return w;
 }
 
-template <bool F16, int HD>
+template <bool F16, int HD, int WAIT_MS>
 __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                      const __grid_constant__ CUtensorMap map_k,
                                                                      const __grid_constant__ CUtensorMap map_v, const PromptDev dv) {
@@ -224,10 +228,10 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     __shared__ __align__(16) uint4 s_clc;
     __shared__ __align__(16) Item s_item[kSlots];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_issued;
+    __shared__ int s_flags[2], s_issued;
     const int tid = threadIdx.x, warp = __shfl_sync(AX_FULL, tid >> 5, 0), lane = tid & 31;
     const AxPromptArgs& a = dv.a;
-    volatile int* abort_flag = &s_abort;
+    volatile int* flags = s_flags;
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t ring = smem0 + 2 * TILE;
 
@@ -240,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         for (int i = 0; i < NS; i++) { mbar_init(smem_u32(&kv_full[i]), 1); mbar_init(smem_u32(&kv_empty[i]), 1); }
         for (int i = 0; i < kSlots; i++) { mbar_init(smem_u32(&i_full[i]), 1); mbar_init(smem_u32(&i_empty[i]), kReaders); }
         mbar_init(smem_u32(&v_here), 1); mbar_init(smem_u32(&v_cut), 1); mbar_init(smem_u32(&clc_bar), 1);
-        s_abort = 0; s_issued = 0;
+        s_flags[0] = s_flags[1] = 0; s_issued = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -258,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     // the n-th item of this CTA, for every reader in turn; false: no more
     auto item_at = [&](int n, Item& it) {
         const int slot = n % kSlots;
-        if (!mbar_wait(smem_u32(&i_full[slot]), (uint32_t)(n / kSlots) & 1u, abort_flag, dv.err, 731)) return false;
+        if (!mbar_wait<WAIT_MS>(smem_u32(&i_full[slot]), (uint32_t)(n / kSlots) & 1u, flags, dv.err, 731)) return false;
         it = *const_cast<const Item*>(&s_item[slot]);
         return it.lq >= 0;
     };
@@ -316,12 +320,12 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                     at += __shfl_sync(AX_FULL, up, 31);
                 }
                 it.h0 = (int)(block % hx) * (dv.pair_heads ? 2 : 1);
-                if (n >= kSlots) ok = mbar_wait(smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, abort_flag, dv.err, 732);
+                if (n >= kSlots) ok = mbar_wait<WAIT_MS>(smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, flags, dv.err, 732);
                 ok = __all_sync(AX_FULL, ok);
                 if (ok && lane == 0) { s_item[n % kSlots] = it; mbar_arrive(smem_u32(&i_full[n % kSlots])); }
                 n++;
             }
-            bool got = mbar_wait(smem_u32(&clc_bar), clc_phase, abort_flag, dv.err, 733);
+            bool got = mbar_wait<WAIT_MS>(smem_u32(&clc_bar), clc_phase, flags, dv.err, 733);
             if (!__all_sync(AX_FULL, got)) { ok = false; break; }
             clc_phase ^= 1u;
             uint32_t took, next;
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             block = next;
         }
         if (ok) {
-            if (n >= kSlots) ok = mbar_wait(smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, abort_flag, dv.err, 732);
+            if (n >= kSlots) ok = mbar_wait<WAIT_MS>(smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, flags, dv.err, 732);
             if (__all_sync(AX_FULL, ok) && lane == 0) { s_item[n % kSlots].lq = -1; mbar_arrive(smem_u32(&i_full[n % kSlots])); }
         }
         __syncwarp();
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 const Work w = work_of(dv, it);
                 const int kh = w.h0 / (a.n_heads / a.n_kv);
                 auto query = [&](int t) {
-                    ok = mbar_wait(smem_u32(&q_empty[t]), (uint32_t)(nq[t] + 1) & 1u, abort_flag, dv.err, 734);
+                    ok = mbar_wait<WAIT_MS>(smem_u32(&q_empty[t]), (uint32_t)(nq[t] + 1) & 1u, flags, dv.err, 734);
                     if (!ok) return;
                     nq[t]++;
                     const uint32_t bar = smem_u32(&q_full[t]);
@@ -361,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 // The first K tile goes ahead of the queries: their places are free only when the item before has its last scores.
                 const int m = 2 * (w.j1 - w.j0 + 1);
                 for (int i = 0; i < m && ok; i++) {
-                    ok = mbar_wait(smem_u32(&kv_empty[st]), ph, abort_flag, dv.err, 721);
+                    ok = mbar_wait<WAIT_MS>(smem_u32(&kv_empty[st]), ph, flags, dv.err, 721);
                     if (!ok) break;
                     const uint32_t bar = smem_u32(&kv_full[st]);
                     mbar_expect_tx(bar, TILE);
@@ -382,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         // descriptors and columns are uniform values: with a vector register behind each, issuing a product took longer than the product.
         if (elect_one()) {
             bool ok = s_tmem == 0;
-            if (!ok) { *abort_flag = 1; atomicExch(dv.err, 728); }
+            if (!ok) { flags[0] = 1; atomicExch(dv.err, 728); }
             auto qk = [&](int t, int st) {                                    // scores of query tile t with the K tile in stage st
                 const uint32_t k = desc_k(ring) + (uint32_t)st * (TILE >> 4), q = desc_k(smem0) + (uint32_t)t * (TILE >> 4);
                 umma_ss<false>(kS + t * 128, q, k, id_qk);
@@ -401,11 +405,11 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 const Work w = work_of(dv, it);
                 const int n = w.j1 - w.j0 + 1, a0 = w.lo0 - w.j0, z0 = w.on0 ? w.hi0 - w.j0 : -1, a1 = w.lo1 - w.j0, z1 = w.on1 ? w.hi1 - w.j0 : -1;
                 if (n <= 0) continue;
-                ok = mbar_wait(smem_u32(&kv_full[st]), ph, abort_flag, dv.err, 722);
+                ok = mbar_wait<WAIT_MS>(smem_u32(&kv_full[st]), ph, flags, dv.err, 722);
 #pragma unroll
                 for (int t = 0; t < 2; t++)
                     if (ok && (t ? w.on1 : w.on0)) {
-                        ok = mbar_wait(smem_u32(&q_full[t]), pq[t], abort_flag, dv.err, 723);
+                        ok = mbar_wait<WAIT_MS>(smem_u32(&q_full[t]), pq[t], flags, dv.err, 723);
                         pq[t] ^= 1u;
                         if (ok && (t ? a1 : a0) == 0) {
                             qk(t, st);
@@ -417,10 +421,10 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 next();
                 for (int i = 0; i < n && ok; i++) {
                     const int sv = st;
-                    ok = mbar_wait(smem_u32(&kv_full[sv]), ph, abort_flag, dv.err, 722);
+                    ok = mbar_wait<WAIT_MS>(smem_u32(&kv_full[sv]), ph, flags, dv.err, 722);
                     if (ok && i == n - 1 && w.cut) {
                         mbar_arrive(smem_u32(&v_here));
-                        ok = mbar_wait(smem_u32(&v_cut), cuts & 1u, abort_flag, dv.err, 729);
+                        ok = mbar_wait<WAIT_MS>(smem_u32(&v_cut), cuts & 1u, flags, dv.err, 729);
                         cuts++;
                     }
                     if (!ok) break;
@@ -432,11 +436,11 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                         const int at = t ? a1 : a0, zt = t ? z1 : z0;
                         if (ok && i >= at && i <= zt) {
                             // the item before has been read out of the accumulator
-                            if (i == at && items[t] > 0) ok = mbar_wait(smem_u32(&o_free[t]), (uint32_t)(items[t] - 1) & 1u, abort_flag, dv.err, 735);
+                            if (i == at && items[t] > 0) ok = mbar_wait<WAIT_MS>(smem_u32(&o_free[t]), (uint32_t)(items[t] - 1) & 1u, flags, dv.err, 735);
                             if (i == at) items[t]++;
 #pragma unroll
                             for (int part = 0; part < 2; part++) {            // the product starts with the first probabilities
-                                ok = ok && mbar_wait(smem_u32(&p_ready[t][part]), pp[t], abort_flag, dv.err, 724);
+                                ok = ok && mbar_wait<WAIT_MS>(smem_u32(&p_ready[t][part]), pp[t], flags, dv.err, 724);
                                 if (!ok) break;
                                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -447,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                             if (ok) umma_commit(smem_u32(&o_done[t]));
                         }
                         if (ok && i + 1 >= at && i + 1 <= zt) {               // over the scores and probabilities just used
-                            ok = mbar_wait(smem_u32(&kv_full[sk]), ph, abort_flag, dv.err, 722);
+                            ok = mbar_wait<WAIT_MS>(smem_u32(&kv_full[sk]), ph, flags, dv.err, 722);
                             if (ok) {
                                 qk(t, sk);
                                 if (i + 1 == zt) umma_commit(smem_u32(&q_empty[t]));
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             if (w.cut) {
                 const int valid = w.s.lk - w.j1 * kRows;
                 const uint32_t v = ring + (uint32_t)((st + m - 1) % NS) * TILE;
-                ok = mbar_wait(smem_u32(&v_here), cuts & 1u, abort_flag, dv.err, 730);       // told by the thread that saw it arrive
+                ok = mbar_wait<WAIT_MS>(smem_u32(&v_here), cuts & 1u, flags, dv.err, 730);       // told by the thread that saw it arrive
                 ok = __all_sync(AX_FULL, ok);
                 if (!ok) break;
                 cuts++;
@@ -517,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             float m = -INFINITY;
             float2 l0 = make_float2(0.f, 0.f), l1 = l0;
             for (int j = j_lo; j <= j_hi; j++) {
-                ok = mbar_wait(smem_u32(&s_full[t]), ps, abort_flag, dv.err, 725);
+                ok = mbar_wait<WAIT_MS>(smem_u32(&s_full[t]), ps, flags, dv.err, 725);
                 ok = __all_sync(AX_FULL, ok);
                 if (!ok) break;
                 ps ^= 1u;
@@ -570,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                     if (grow) m = top;
                     l0.x *= f; l0.y *= f; l1.x *= f; l1.y *= f;
                     if (started && __any_sync(AX_FULL, moved)) {              // the products of the tile before are in: po is the parity they leave
-                        ok = mbar_wait(smem_u32(&o_done[t]), po ^ 1u, abort_flag, dv.err, 726);
+                        ok = mbar_wait<WAIT_MS>(smem_u32(&o_done[t]), po ^ 1u, flags, dv.err, 726);
                         ok = __all_sync(AX_FULL, ok);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -625,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             // ── output ──
             const bool any = j_hi >= j_lo;
             if (ok && any) {
-                ok = mbar_wait(smem_u32(&o_done[t]), po ^ 1u, abort_flag, dv.err, 727);
+                ok = mbar_wait<WAIT_MS>(smem_u32(&o_done[t]), po ^ 1u, flags, dv.err, 727);
                 ok = __all_sync(AX_FULL, ok);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
@@ -671,10 +675,14 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             const bool sees = key_hi >= 0 && w.s.lk > 0;
             unsigned again = __ballot_sync(AX_FULL, live && (odd != odd || (sees && !(fabsf(m) <= 3.402823466e38f))));
             __syncwarp();
+            if (again) {
+            if (lane == 0) atomicAdd(&s_flags[1], 1);
             while (again) {
                 const int i = __ffs(again) - 1;
                 again &= again - 1;
                 row_again<T, HD>(a, w.s, h, base + (warp & 3) * 32 + i, lane);
+            }
+            if (lane == 0) atomicAdd(&s_flags[1], -1);
             }
         }
     }
@@ -682,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     // ── tail: nothing of this CTA may still be in flight when its shared and tensor memory go away ──
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (s_abort) {
+    if (s_flags[0]) {
         if (tid == 0) {                                                       // copies issued into stages nobody consumed any more
             const int issued = s_issued;
             for (int i = issued > NS ? issued - NS : 0; i < issued; i++) {
@@ -728,12 +736,12 @@ int make_map(CUtensorMap* map, bool f16, const void* data, int rows, int heads, 
     return ATLASX_OK;
 }
 
-template <bool F16, int HD>
+template <bool F16, int HD, int WAIT_MS = kWaitMs>
 int launch(atlasx_ctx* ctx, const PromptDev& dv, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v) {
     constexpr int smem = (2 + (HD == 128 ? 5 : 6)) * (HD / 64) * kBoxBytes + 1024;
     static std::atomic<bool> ready[64] = {};
     if (ctx->device >= 64 || !ready[ctx->device]) {                           // the limit is per device; asking twice does no harm
-        AX_CUDA(cudaFuncSetAttribute(ax_prompt_umma_kernel<F16, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        AX_CUDA(cudaFuncSetAttribute(ax_prompt_umma_kernel<F16, HD, WAIT_MS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         if (ctx->device < 64) ready[ctx->device] = true;
     }
     const int tb = dv.pair_heads ? kRows : 2 * kRows;
@@ -741,7 +749,7 @@ int launch(atlasx_ctx* ctx, const PromptDev& dv, const CUtensorMap& q, const CUt
     const long long tiles = (long long)dv.a.n_q / tb + (dv.a.batch < dv.a.n_q ? dv.a.batch : dv.a.n_q);
     const long long items = tiles * (dv.pair_heads ? dv.a.n_heads / 2 : dv.a.n_heads);
     AX_ARG(items <= 0x7FFFFFFFll, "too many rows and heads for one call");
-    ax_prompt_umma_kernel<F16, HD><<<(unsigned)items, kThreads, smem, ctx->stream>>>(q, k, v, dv);
+    ax_prompt_umma_kernel<F16, HD, WAIT_MS><<<(unsigned)items, kThreads, smem, ctx->stream>>>(q, k, v, dv);
     AX_CHECK_LAUNCH("ax_prompt_umma_kernel");
     return ATLASX_OK;
 }
@@ -794,6 +802,7 @@ extern "C" int atlasx_prompt_attention(atlasx_ctx* c, const atlasx_prompt_args* 
     if (!rc && n_k > 0) rc = make_map(&mv, f16, v, n_k, n_kv, hd, v_tok, v_head);
     if (rc) return rc;
     if (n_k == 0) mk = mv = mq;                                               // never read: no sequence has keys
+    if (c->tune.prompt_short_waits && !f16 && hd == 64) return launch<false, 64, kTestWaitMs>(c, dv, mq, mk, mv);
     if (f16) return hd == 128 ? launch<true, 128>(c, dv, mq, mk, mv) : launch<true, 64>(c, dv, mq, mk, mv);
     return hd == 128 ? launch<false, 128>(c, dv, mq, mk, mv) : launch<false, 64>(c, dv, mq, mk, mv);
 }

@@ -273,7 +273,7 @@ int atlasx_pagedkv_selftest_wait_expiry(atlasx_ctx* ctx, const atlasx_pagedkv* k
  * cu_q[b] .. cu_q[b + 1] − 1 of q and out [n_q][n_heads][head_dim] and rows cu_k[b] .. cu_k[b + 1] − 1 of k and v
  * [n_k][n_kv_heads][head_dim] (1 ≤ batch ≤ 4096, prefix arrays on the device).  Its last query sits at its last key: query i of lq
  * sees keys j ≤ i + lk − lq, with a window only those with i + lk − lq − j < window; a query that sees none gets zeros.  What a
- * query does not see — NaN and infinities too — does not reach it.  Strides in elements, every row on a 16-byte boundary; rows of
+ * query does not see — NaN and infinities too — does not reach it; rows that see them are taken one by one, which is right but slow.  Strides in elements, every row on a 16-byte boundary; rows of
  * out in no sequence are left as they are.  out may not overlap q, k or v. */
 typedef struct {
     const void *q, *k, *v;

@@ -298,3 +298,29 @@ def test_many_small_probabilities_in_f16(ab, hd):
     want = 2.0 ** -9 / (1 + 2.0 ** -9)
     # ln 2 · log2 e in f32 is off by at most 2^-23 of itself, 26 of it as an exponent by 2^-18
     assert np.all(np.abs(down(ab, out) - want) <= want * (2.0 ** -11 + 2.0 ** -16))
+
+
+def test_rows_taken_again_do_not_run_out_the_waits_of_others(ab, monkeypatch):
+    """A NaN in the first key: every row is taken again, an item's rows for longer than a wait may take.  The limit is set low here so that a
+    prompt of 8192 is long enough; with the 10 seconds there are it takes half a million rows."""
+    monkeypatch.setenv("ATLASX_PROMPT_SHORT_WAITS", "1")
+    ctx = ab.Context(0)
+    n, nh, hd = 8192, 5, 64
+    rng = np.random.default_rng(73)
+    q, k, v = (bf16(rng.standard_normal((n, nh, hd)).astype(np.float32)) for _ in range(3))
+    ds = [ab.DeviceArray.from_host(orc.f32_to_bf16_rne(x).reshape(x.shape), ab.BF16, ctx) for x in (q, k, v)]
+    out, cu = ab.DeviceArray.empty((n, nh, hd), ab.BF16, ctx), ab.DeviceArray.from_host([0, n], ab.I32, ctx)
+    ab.prompt_attention(*ds, out, cu, cu, 0.1, ctx=ctx)
+    assert ctx.poll_device_error() == 0
+    some = [0, 1, 127, 128, 3000, 8191]                                     # as in every call, and with no wait expired
+    got = down(ab, out)[some]
+    for i, r in enumerate(some):
+        want, tol = prompt_by_hand(q[r:r + 1], k[:r + 1], v[:r + 1], [0, 1], [0, r + 1], 0.1, 0, False)
+        assert np.all(np.abs(got[i] - want[0]) <= tol[0])
+    k[0] = np.nan
+    ctx.upload(ds[1].ptr, orc.f32_to_bf16_rne(k))
+    ab.prompt_attention(*ds, out, cu, cu, 0.1, ctx=ctx)
+    assert ctx.poll_device_error() == 0
+    assert np.isnan(down(ab, out)).all()
+    del ds, out, cu
+    ctx.close()
