@@ -45,7 +45,6 @@ struct PagedDev {
     float* part_ml;                             // [2 · gridDim][hpt][2]
     float* part_o;                              // [2 · gridDim][hpt][hd]
     int *err, *index_err;
-    unsigned long long wait_ns;                 // how long a unit's copy may take
     long long lost;                             // self-test: the unit whose copy is never issued
 };
 
@@ -113,13 +112,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     constexpr int WG = GS / 32;                 // words per group
     constexpr int PLANE = AX_P4_TILE * HD / 2, SC = AX_P4_TILE * NG * 2, TILE = 2 * (PLANE + SC);
     constexpr int NT = HD / 8;                  // column blocks of the output
+    constexpr unsigned long long kNs = LOSE ? kSelftestWaitNs : kWaitNs;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t s_bar[kWarps][kStages];
     __shared__ __align__(16) UnitInfo s_info[kWarps][kStages];
     __shared__ unsigned s_scan[2][kWarps];
     __shared__ int s_seg[kWarps * 2];
     __shared__ float s_ml[kWarps * 2][kHeads][2];
-    __shared__ int s_last;
+    __shared__ int s_last, s_gave_up;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int batch = dv.a.batch, hpt = dv.hpt;
     // Shared memory: per warp its ring, its query operand, and the output of a first segment that ends within its piece; the output of the
@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
 
     if (tid < kWarps * kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(smem_u32(&s_bar[tid / kStages][tid % kStages])) : "memory");
     if (tid < kWarps * 2) s_seg[tid] = -1;
+    if (tid == 0) s_gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     int us;                                                                   // tiles of a unit: two, or one where that many warps would have none
@@ -323,27 +324,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         }
     };
 
-    int st = 0;
+    int st = 0, it = 0;
     uint32_t phase = 0;
-    for (int it = 0; it < count; it++) {
+    for (; it < count; it++) {
         const UnitInfo info = s_info[warp][st];
         // known before the unit is here: a new segment's query comes under its copy
         if (info.seg != seg) { if (seg >= 0) flush(); start(info.seg); }
-        if (!mbar_wait(smem_u32(&s_bar[warp][st]), phase, dv.wait_ns)) {
-            if (lane == 0) atomicExch(dv.err, kErrWait);
-            for (int y = it; y < count && y < it + kStages; y++)              // what is in flight lands before the CTA goes
-                mbar_wait(smem_u32(&s_bar[warp][y % kStages]), (uint32_t)(y / kStages) & 1u, dv.wait_ns);
-            // The segment that goes on behind the warp's piece is entered all the same, with a sum of zero: every CTA of a segment
-            // has to arrive at its ticket, or the count is ahead in all later launches.
-            int b, hh, ti;
-            locate(x1 - 1, b, hh, ti);
-            const unsigned n = s_pre[b + 1] - s_pre[b];
-            if (b * dv.nh + hh != seg && (long long)s_pre[b] * dv.nh + (long long)(hh + 1) * n > x1) {
-                if (lane == 0) s_seg[warp * 2 + 1] = b * dv.nh + hh;
-                if (lane < kHeads) { s_ml[warp * 2 + 1][lane][0] = -INFINITY; s_ml[warp * 2 + 1][lane][1] = 0.f; }
-            }
-            break;
-        }
+        if (!mbar_wait(smem_u32(&s_bar[warp][st]), phase, kNs)) break;
         if (info.ok) {
             // Both tiles side by side: their chains — scores, softmax, products — are each other's cover.  (One tile at a time left 54 % of the
             // issue slots and 41 % of the busiest pipe in use.)
@@ -493,9 +480,31 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         __syncwarp();
         if (++st == kStages) { st = 0; phase ^= 1u; }
     }
+    if (it < count) {                                                          // gave up
+        if (lane == 0) { atomicExch(dv.err, kErrWait); s_gave_up = 1; }
+        for (int y = it; y < count && y < it + kStages; y++)                  // what is in flight lands before the CTA goes
+            mbar_wait(smem_u32(&s_bar[warp][y % kStages]), (uint32_t)(y / kStages) & 1u, kNs);
+    }
     __syncwarp();                                                              // the ring is read by all lanes before the last output goes over it
     if (seg >= 0) flush();
     __syncthreads();
+    if (s_gave_up) {
+        // The segment that goes on in the next CTA is entered all the same, with a sum of zero: every CTA of a segment has to arrive at
+        // its ticket, or the count is ahead in all later launches.  (The one that began in a CTA before is the first that a warp takes.)
+        if (tid == 0) {
+            int b, hh, ti;
+            locate(X1 - 1, b, hh, ti);
+            const int last = b * dv.nh + hh;
+            const unsigned n = s_pre[b + 1] - s_pre[b];
+            bool entered = (long long)s_pre[b] * dv.nh + (long long)(hh + 1) * n <= X1;
+            for (int i = 0; i < kWarps * 2; i++) entered = entered || s_seg[i] == last;
+            if (!entered) {
+                s_seg[kWarps * 2 - 1] = last;                                 // free: the last warp enters nothing else there
+                for (int h = 0; h < kHeads; h++) { s_ml[kWarps * 2 - 1][h][0] = -INFINITY; s_ml[kWarps * 2 - 1][h][1] = 0.f; }
+            }
+        }
+        __syncthreads();
+    }
 
     // ── segments that no warp holds alone ──
     for (int i = 0; i < kWarps * 2;) {
@@ -648,7 +657,7 @@ size_t ax_paged_attn_workspace_bytes(const atlasx_ctx* ctx, const AxP4Shape& s) 
 int ax_paged_attn_launch(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const AxPagedAttnArgs& a, long long lost) {
     PagedDev dv = {};
     dv.s = kv->s; dv.pool = kv->pool; dv.a = a; dv.err = ctx->dev_error; dv.index_err = ctx->index_error();
-    dv.wait_ns = lost < 0 ? kWaitNs : kSelftestWaitNs; dv.lost = lost;
+    dv.lost = lost;
     dv.group_heads = a.n_heads / kv->s.n_kv;
     dv.head_tiles = (dv.group_heads + kHeads - 1) / kHeads;
     dv.hpt = min(kHeads, dv.group_heads);
