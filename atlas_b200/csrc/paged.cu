@@ -440,8 +440,9 @@ extern "C" int atlasx_pagedkv_append(atlasx_ctx* c, atlasx_pagedkv* kv, const at
     if (n == 0) return ATLASX_OK;
     AX_ARG(k && v && slots, "null argument");
     const long long step = 16 / elem_bytes(dtype);
-    AX_ARG(((uintptr_t)k | (uintptr_t)v) % 16 == 0 && k_token_stride % step == 0 && k_head_stride % step == 0 &&
-           v_token_stride % step == 0 && v_head_stride % step == 0, "rows must start on 16-byte boundaries");
+    // a stride that is never taken may be anything: of one row, of one head
+    const long long token_strides = n > 1 ? k_token_stride | v_token_stride : 0, head_strides = !kv || kv->s.n_kv > 1 ? k_head_stride | v_head_stride : 0;
+    AX_ARG(((uintptr_t)k | (uintptr_t)v) % 16 == 0 && (token_strides | head_strides) % step == 0, "rows must start on 16-byte boundaries");
     AX_ARG(c && kv, "ctx or cache is null");
     AX_ARG(kv->ctx == c, "the cache belongs to another context");
     AX_ON_DEVICE(c);

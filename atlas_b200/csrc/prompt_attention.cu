@@ -726,8 +726,7 @@ int make_map(CUtensorMap* map, bool f16, const void* data, int rows, int heads, 
     EncodeTiledFn fn = encode_fn();
     if (!fn) return atlasx_fail(ATLASX_ERR_CUDA, "the driver does not export cuTensorMapEncodeTiled");
     const cuuint64_t dims[3] = { (cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows };
-    // a stride that is never used may be anything the caller had; the map wants a multiple of 16 above zero
-    const cuuint64_t strides[2] = { (cuuint64_t)(heads > 1 ? head : hd) * 2, (cuuint64_t)(rows > 1 ? tok : (long long)heads * hd) * 2 };
+    const cuuint64_t strides[2] = { (cuuint64_t)head * 2, (cuuint64_t)tok * 2 };
     const cuuint32_t box[3] = { 64, 1, kRows }, step[3] = { 1, 1, 1 };
     const CUresult r = fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(data), dims, strides,
                           box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -760,8 +759,8 @@ extern "C" int atlasx_prompt_attention(atlasx_ctx* c, const atlasx_prompt_args* 
     AX_ARG(p, "null argument");
     const void *q = p->q, *k = p->k, *v = p->v;
     void* out = p->out;
-    const long long q_tok = p->q_token_stride, q_head = p->q_head_stride, k_tok = p->k_token_stride, k_head = p->k_head_stride,
-                    v_tok = p->v_token_stride, v_head = p->v_head_stride, o_tok = p->out_token_stride, o_head = p->out_head_stride;
+    long long q_tok = p->q_token_stride, q_head = p->q_head_stride, k_tok = p->k_token_stride, k_head = p->k_head_stride,
+              v_tok = p->v_token_stride, v_head = p->v_head_stride, o_tok = p->out_token_stride, o_head = p->out_head_stride;
     const int *cu_q = p->cu_q, *cu_k = p->cu_k, dtype = p->dtype, batch = p->batch, n_q = p->n_q, n_k = p->n_k, n_heads = p->n_heads,
               n_kv = p->n_kv_heads, hd = p->head_dim, window = p->window;
     const float scale = p->scale;
@@ -775,13 +774,19 @@ extern "C" int atlasx_prompt_attention(atlasx_ctx* c, const atlasx_prompt_args* 
     AX_ARG(window >= 0, "window must be non-negative");
     AX_ARG(scale - scale == 0.f, "scale must be finite");
     if (n_q == 0) return ATLASX_OK;
+    // a stride that is never taken may be anything the caller has: of one row, of one head
+    if (n_q == 1) q_tok = o_tok = (long long)n_heads * hd;
+    if (n_k <= 1) k_tok = v_tok = (long long)n_kv * hd;
+    if (n_heads == 1) q_head = o_head = hd;
+    if (n_kv == 1 || n_k == 0) k_head = v_head = hd;
     AX_ARG(q && out && cu_q && cu_k && ((k && v) || n_k == 0), "null argument");
     AX_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 == 0 &&
            (q_tok | q_head | k_tok | k_head | v_tok | v_head | o_tok | o_head) % 8 == 0, "rows must start on 16-byte boundaries");
     AX_ARG(q_tok >= 0 && q_head >= 0 && k_tok >= 0 && k_head >= 0 && v_tok >= 0 && v_head >= 0, "strides must not be negative");
-    AX_ARG((q_head > 0 || n_heads == 1) && ((k_head > 0 && v_head > 0) || n_kv == 1 || n_k == 0) &&
-           (q_tok > 0 || n_q == 1) && ((k_tok > 0 && v_tok > 0) || n_k <= 1), "strides must not be zero");
-    AX_ARG((o_head >= hd || n_heads == 1) && (o_tok >= hd || n_q == 1), "rows of out overlap");
+    AX_ARG(q_head > 0 && k_head > 0 && v_head > 0 && q_tok > 0 && k_tok > 0 && v_tok > 0, "strides must not be zero");
+    // all heads of a row before the next row, or all rows of a head before the next head
+    AX_ARG(o_head >= hd && o_tok >= hd && o_tok < (1ll << 38) && o_head < (1ll << 38) &&
+           (n_q == 1 || n_heads == 1 || o_tok >= (n_heads - 1) * o_head + hd || o_tok <= (o_head - hd) / (n_q - 1)), "rows of out overlap");
     AX_ARG(q_tok < (1ll << 38) && q_head < (1ll << 38) && k_tok < (1ll << 38) && k_head < (1ll << 38) && v_tok < (1ll << 38) && v_head < (1ll << 38),
            "strides must be below 2^38");
     AX_ARG(c, "ctx is null");
@@ -791,7 +796,7 @@ extern "C" int atlasx_prompt_attention(atlasx_ctx* c, const atlasx_prompt_args* 
              window < n_k ? window : 0, scale };                              // no key lies further behind a query, and "position − window" stays within 32 bits
     dv.pair_heads = (n_heads / n_kv) % 2 == 0;
     dv.negate = scale < 0.f;
-    dv.wide = (uintptr_t)out % 32 == 0 && (n_q == 1 || o_tok % 16 == 0) && (n_heads == 1 || o_head % 16 == 0);
+    dv.wide = (uintptr_t)out % 32 == 0 && o_tok % 16 == 0 && o_head % 16 == 0;
     // a hidden key's score is −inf · sc: a scale of zero must not make it NaN.  Scores below 2^126 / 1e37 of it are still all alike.
     dv.sc = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-37f);
     dv.err = c->dev_error;

@@ -235,8 +235,8 @@ int atlasx_pagedkv_free(atlasx_pagedkv* kv);
 size_t atlasx_pagedkv_bytes(int n_pages, int page_size, int n_kv_heads, int head_dim, int group);
 int atlasx_pagedkv_ptrs(atlasx_pagedkv* kv, void** pool_dev, size_t* bytes, size_t* workspace_bytes);
 /* Rows of K and V [n][n_kv_heads][head_dim], f32, bf16 or f16, strides in elements, every row on a 16-byte boundary, into their
- * slots.  A negative slot marks a row that is not there; one behind the pool is left out and raises the index error word
- * (atlasx_ctx_poll_device_error).  Slots of one call are distinct. */
+ * slots (the strides of a single row or head may be anything).  A negative slot marks a row that is not there; one behind the pool is left
+ * out and raises the index error word (atlasx_ctx_poll_device_error).  Slots of one call are distinct. */
 typedef struct {
     const void *k, *v;
     const int* slots;                             /* [n] */
@@ -273,8 +273,9 @@ int atlasx_pagedkv_selftest_wait_expiry(atlasx_ctx* ctx, const atlasx_pagedkv* k
  * cu_q[b] .. cu_q[b + 1] − 1 of q and out [n_q][n_heads][head_dim] and rows cu_k[b] .. cu_k[b + 1] − 1 of k and v
  * [n_k][n_kv_heads][head_dim] (1 ≤ batch ≤ 4096, prefix arrays on the device).  Its last query sits at its last key: query i of lq
  * sees keys j ≤ i + lk − lq, with a window only those with i + lk − lq − j < window; a query that sees none gets zeros.  What a
- * query does not see — NaN and infinities too — does not reach it; rows that see them are taken one by one, which is right but slow.  Strides in elements, every row on a 16-byte boundary; rows of
- * out in no sequence are left as they are.  out may not overlap q, k or v. */
+ * query does not see — NaN and infinities too — does not reach it; rows that see them are taken one by one, which is right but slow.
+ * Strides in elements, every row on a 16-byte boundary (the strides of a single row or head may be anything), out in [row][head] or
+ * [head][row] order; rows of out in no sequence are left as they are.  out may not overlap q, k or v. */
 typedef struct {
     const void *q, *k, *v;
     void* out;

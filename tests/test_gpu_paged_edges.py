@@ -324,3 +324,32 @@ def test_rows_taken_again_do_not_run_out_the_waits_of_others(ab, monkeypatch):
     assert np.isnan(down(ab, out)).all()
     del ds, out, cu
     ctx.close()
+
+
+# ── single rows and heads with strides of their own ──────────────────────────────
+def test_a_single_row_and_a_single_head_of_odd_buffers(ab):
+    rng = np.random.default_rng(74)
+    hd = 64
+    buf = bf16(rng.standard_normal(1000).astype(np.float32))
+    b = up(ab, buf, ab.BF16)
+    row = lambda at, h: buf[at:at + h * hd].reshape(1, h, hd)                # noqa: E731
+    q, k, v = b.columns(8, (1, 2, hd), (333, hd, 1)), b.columns(200, (1, 1, hd), (77, 5, 1)), b.columns(304, (1, 1, hd), (1, 3, 1))
+    out = up(ab, np.full((1, 2, hd), 7.0), ab.BF16)
+    cu = ab.DeviceArray.from_host([0, 1], ab.I32)
+    ab.prompt_attention(q, k, v, out.columns(0, (1, 2, hd), (31, hd, 1)), cu, cu, 0.1)
+    assert np.array_equal(down(ab, out), np.repeat(row(304, 1), 2, axis=1))            # one key: its value
+    kv = ab.PagedKvCache(1, 16, 1, hd)
+    slot = ab.DeviceArray.from_host([3], ab.I32)
+    kv.append(k, v, slot)
+    ko, vo = ab.DeviceArray.empty((1, 1, hd), ab.F32), ab.DeviceArray.empty((1, 1, hd), ab.F32)
+    kv.read(slot, ko, vo)
+    assert np.array_equal(ko.download(), held(row(200, 1), 32).astype(np.float32)) and np.array_equal(vo.download(), held(row(304, 1), 32).astype(np.float32))
+    # many rows of one head: only the head stride is free
+    n = 7
+    k = b.columns(16, (n, 1, hd), (72, 1, 1))
+    sd = ab.DeviceArray.from_host(np.arange(n), ab.I32)
+    kv.append(k, k, sd)
+    ko, vo = ab.DeviceArray.empty((n, 1, hd), ab.F32), ab.DeviceArray.empty((n, 1, hd), ab.F32)
+    kv.read(sd, ko, vo)
+    want = np.stack([buf[16 + 72 * i:16 + 72 * i + hd] for i in range(n)]).reshape(n, 1, hd)
+    assert np.array_equal(ko.download(), held(want, 32).astype(np.float32))

@@ -301,3 +301,19 @@ def test_plan_refuses_outputs_that_overlap():
     if not ab.cuda_available():                                                             # nothing to refuse: a device is asked for
         for fine in ({}, dict(fresh=apart["cached"]), dict(cu=apart["fresh"] - 20), dict(lens=apart["cached"] + 16), dict(table=apart["fresh"] - 64)):
             assert call(**fine) == -2, fine
+
+
+def test_strides_that_are_never_taken_may_be_anything():
+    """Of a single row, of a single head.  Nothing is refused: a device is asked for, or the context is missed."""
+    for change in (dict(n=1, kt=129, vt=1), dict(n=1, kt=0, vt=-3)):
+        refused(_ffi.lib().atlasx_pagedkv_append(None, None, packed(_ffi.PAGED_ROWS, dict(ROWS, **change))), "ctx or cache is null")
+    for change in (dict(n_q=1, qt=1, ot=3), dict(n_q=1, qt=0, ot=-8), dict(n_k=1, kt=0, vt=5), dict(n_k=0, k=None, v=None, kt=0, vt=1, kh=0, vh=-3),
+                   dict(n_heads=1, n_kv=1, qh=0, kh=3, vh=-1, oh=7)):
+        refused(_ffi.lib().atlasx_prompt_attention(None, packed(_ffi.PROMPT, dict(PROMPT, **change))), "ctx is null")
+
+
+@pytest.mark.parametrize("ot,oh,fine", [(512, 128, True), (128, 1280, True), (496, 128, False), (384, 128, False), (128, 1272, False), (256, 128, False), (128, 128, False),
+                                        (1 << 40, 1 << 40, False)])
+def test_rows_of_out_must_not_meet(ot, oh, fine):
+    """Ten rows of four heads of 128."""
+    refused(_ffi.lib().atlasx_prompt_attention(None, packed(_ffi.PROMPT, dict(PROMPT, ot=ot, oh=oh))), "ctx is null" if fine else "overlap")
