@@ -169,9 +169,10 @@ def _contiguous(view, name):
     return view
 
 
-def _device(ctx, x):
-    """Device of the call: the context's, or — before there is one — the first array's."""
-    return ctx.device if ctx is not None else (x.ctx.device if type(x) is DeviceArray else 0)
+def _device(ctx):
+    """Device of the call: the context's, or that of the default context (device 0), which may not exist yet."""
+    ctx = ctx or Context._default
+    return ctx.device if ctx is not None else 0
 
 
 def _whole(x, name, limit=0x7FFFFFFF):
@@ -184,7 +185,7 @@ def _whole(x, name, limit=0x7FFFFFFF):
 def page_plan(cached, fresh, free_pages, table, cu, lens, slots, pos, status, page_size, n_pages, ctx=None):
     """Block tables, slots and positions of a step from request lengths: see atlasx_page_plan.  int32 device arrays: cached, fresh,
     lens [batch]; free_pages [any]; table [batch, width], extended in place; cu [batch + 1]; slots, pos [rows]; status [3]."""
-    dev = _device(ctx, cached)
+    dev = _device(ctx)
     p_cached = _ints(cached, "cached", None, dev)
     b = _length(cached)
     p_slots = _ints(slots, "slots", None, dev)
@@ -263,7 +264,7 @@ class PagedKvCache:
 def prompt_attention(q, k, v, out, cu_q, cu_k, scale=None, window_size=0, ctx=None):
     """Causal attention of packed prompts: q, out [rows, n_heads, head_dim], k, v [key rows, n_kv_heads, head_dim], bf16 or f16; sequence
     b owns rows cu_q[b]..cu_q[b + 1] of q and cu_k[b]..cu_k[b + 1] of k and v, its last query at its last key.  scale None: 1/√head_dim."""
-    dev, types = _device(ctx, q), (BF16, F16)
+    dev, types = _device(ctx), (BF16, F16)
     qp, n, qt, qh, dt, nh, hd = _rows(q, "q", types, dev)
     kp, m, kt, kh, dk, nk, _ = _rows(k, "k", types, dev, None, hd)
     vp, mv, vt, vh, dv, _, _ = _rows(v, "v", types, dev, nk, hd)

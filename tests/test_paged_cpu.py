@@ -317,3 +317,14 @@ def test_strides_that_are_never_taken_may_be_anything():
 def test_rows_of_out_must_not_meet(ot, oh, fine):
     """Ten rows of four heads of 128."""
     refused(_ffi.lib().atlasx_prompt_attention(None, packed(_ffi.PROMPT, dict(PROMPT, ot=ot, oh=oh))), "ctx is null" if fine else "overlap")
+
+
+def test_arrays_of_another_device_are_refused_without_a_context():
+    """The default context, on device 0, takes the call: arrays that are all on device 1 do not move it there."""
+    one = lambda shape, dtype: arr(shape, dtype, device=1)                    # noqa: E731
+    b = one((4,), ab.I32)
+    with pytest.raises(ab.AtlasError, match="cached is not on device 0"):
+        ab.page_plan(b, b, b, one((4, 3), ab.I32), one((5,), ab.I32), b, b, b, one((3,), ab.I32), page_size=16, n_pages=4)
+    q, cu = one((5, 4, 64), ab.BF16), one((3,), ab.I32)
+    with pytest.raises(ab.AtlasError, match="q is not on device 0"):
+        ab.prompt_attention(q, q, q, q, cu, cu)
