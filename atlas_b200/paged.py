@@ -205,6 +205,8 @@ class PagedKvCache:
         self.ctx = ctx or Context.default()
         self._h = None
         h = C.c_void_p()
+        for n, name in ((n_pages, "n_pages"), (page_size, "page_size"), (n_kv_heads, "n_kv_heads"), (head_dim, "head_dim"), (group, "group")):
+            _whole(n, name)
         check(_ffi.lib().atlasx_pagedkv_create(self.ctx.handle, n_pages, page_size, n_kv_heads, head_dim, group, C.byref(h)))
         self._h = h
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim, self.group = n_pages, page_size, n_kv_heads, head_dim, group

@@ -328,3 +328,14 @@ def test_arrays_of_another_device_are_refused_without_a_context():
     q, cu = one((5, 4, 64), ab.BF16), one((3,), ab.I32)
     with pytest.raises(ab.AtlasError, match="q is not on device 0"):
         ab.prompt_attention(q, q, q, q, cu, cu)
+
+
+@pytest.mark.parametrize("place", range(5))
+def test_a_cache_of_more_than_a_c_int_is_refused(place):
+    """Not cut to its low 32 bits."""
+    shape = [4, 16, 1, 128, 32]
+    with pytest.raises(ab.AtlasError, match="ctx is null"):
+        ab.PagedKvCache(*shape, ctx=FakeContext())
+    shape[place] += 1 << 32
+    with pytest.raises(ab.AtlasError, match="out of range"):
+        ab.PagedKvCache(*shape, ctx=FakeContext())
