@@ -153,7 +153,7 @@ template <> __device__ __forceinline__ void load8<__half>(const __half* p, float
 
 struct RowArgs {
     AxP4Shape s;
-    unsigned long long inv_page;  // ceil(2^36 / (page_size / 16)): slot / page_size without a division
+    unsigned long long inv_page;  // ax_p4_page_inverse
     uint8_t* pool;
     const void *k, *v;            // append: [token][head][hd], token and head strides in elements
     long long k_tok, k_head, v_tok, v_head;
@@ -163,9 +163,9 @@ struct RowArgs {
     int* err;
 };
 
-// A slot's page and row within it.  slot / 16 < 2^27 and page_size / 16 ≤ 2^9, so the rounded-up reciprocal with 36 bits is exact.
+// a slot's page and row within it
 __device__ __forceinline__ void slot_place(const RowArgs& a, int slot, int& page, int& off) {
-    page = (int)(((unsigned long long)(unsigned)(slot >> 4) * a.inv_page) >> 36);
+    page = ax_p4_page_of(slot, a.inv_page);
     off = slot - page * a.s.page_size;
 }
 template <int HD, int GS> __device__ __forceinline__ AxP4Shape fixed_shape(const AxP4Shape& s) { return AxP4Shape{ s.n_pages, s.page_size, s.n_kv, HD, GS }; }
@@ -215,12 +215,12 @@ __global__ void __launch_bounds__(kAppendThreads) ax_p4_append_kernel(const RowA
     uint32_t half[N / 4];                                            // four numbers each
 #pragma unroll
     for (int i = 0; i < N / 4; i++) {
-        // y ± (1/2 − 2^-25) cut off: rounds half away from zero for |y| < 8.  Σ (number + 8) · 16^j.
+        // Σ (number + 8) · 16^j
         int w = 0;
 #pragma unroll
         for (int j = 2; j >= 0; j -= 2) {
             float2 y = ax_mul2(make_float2(x[4 * i + j], x[4 * i + j + 1]), make_float2(inv, inv));
-            y = ax_add2(y, make_float2(copysignf(0.49999997f, y.x), copysignf(0.49999997f, y.y)));
+            y = ax_add2(y, make_float2(ax_p4_half(y.x), ax_p4_half(y.y)));
             w = (w * 16 + __float2int_rz(y.y)) * 16 + __float2int_rz(y.x);
         }
         half[i] = odd ? 0x8888u : (uint32_t)(w + 0x8888) & 0xFFFFu;
@@ -334,10 +334,6 @@ void launch_rows(int dtype, const RowArgs& a, cudaStream_t stream) {
     else launch_rows<__half, READ>(a, stream);
 }
 
-unsigned long long page_inverse(int page_size) {
-    const unsigned long long d = (unsigned long long)page_size / AX_P4_TILE;
-    return ((1ull << 36) + d - 1) / d;
-}
 int elem_bytes(int dtype) { return dtype == ATLASX_F32 ? 4 : 2; }
 
 }  // namespace
@@ -450,7 +446,7 @@ extern "C" int atlasx_pagedkv_append(atlasx_ctx* c, atlasx_pagedkv* kv, const at
     a.s = kv->s; a.pool = kv->pool; a.k = k; a.v = v;
     a.k_tok = k_token_stride; a.k_head = k_head_stride; a.v_tok = v_token_stride; a.v_head = v_head_stride;
     a.slots = slots; a.n = n; a.err = c->index_error();
-    a.inv_page = page_inverse(kv->s.page_size);
+    a.inv_page = ax_p4_page_inverse(kv->s.page_size);
     launch_rows<false>(dtype, a, c->stream);
     AX_CHECK_LAUNCH("ax_p4_append_kernel");
     return ATLASX_OK;
@@ -467,7 +463,7 @@ extern "C" int atlasx_pagedkv_read(atlasx_ctx* c, const atlasx_pagedkv* kv, cons
     AX_ON_DEVICE(c);
     RowArgs a = {};
     a.s = kv->s; a.pool = kv->pool; a.k_out = k_out; a.v_out = v_out; a.slots = slots; a.n = n; a.err = c->index_error();
-    a.inv_page = page_inverse(kv->s.page_size);
+    a.inv_page = ax_p4_page_inverse(kv->s.page_size);
     launch_rows<true>(dtype, a, c->stream);
     AX_CHECK_LAUNCH("ax_p4_read_kernel");
     return ATLASX_OK;

@@ -14,6 +14,7 @@
 //      8·nt + 4 + t in its high half (the k pair 2t, 2t + 1 of the product), column g owning GS / 8 consecutive numbers of a group.
 // A nibble is the number plus eight.
 #pragma once
+#include <math.h>
 #include <stdint.h>
 #include <stddef.h>
 #ifdef __CUDACC__
@@ -53,3 +54,12 @@ AX_HD int ax_p4_v_half(const AxP4Shape& s, int r, int d4) {
 }
 // scale (within the K or V scales) of group gr of row r
 AX_HD int ax_p4_scale(const AxP4Shape& s, int r, int gr) { return ax_p4_col(r) * ax_p4_groups(s) + gr; }
+// What is added to a scaled value |y| < 8 before it is cut off to a whole number: rounds half away from zero (1/2 − 2^-25, so that the number
+// below 1/2 stays below 1).
+AX_HD float ax_p4_half(float y) { return copysignf(0.49999997f, y); }
+// slot / page_size without a division: (slot / 16) · ceil(2^36 / (page_size / 16)) >> 36.  slot / 16 < 2^27 and page_size / 16 ≤ 2^9, so it is exact.
+AX_HD unsigned long long ax_p4_page_inverse(int page_size) {
+    const unsigned long long d = (unsigned long long)page_size / AX_P4_TILE;
+    return ((1ull << 36) + d - 1) / d;
+}
+AX_HD int ax_p4_page_of(int slot, unsigned long long inverse) { return (int)(((unsigned long long)(unsigned)(slot >> 4) * inverse) >> 36); }

@@ -353,3 +353,71 @@ def test_a_single_row_and_a_single_head_of_odd_buffers(ab):
     kv.read(sd, ko, vo)
     want = np.stack([buf[16 + 72 * i:16 + 72 * i + hd] for i in range(n)]).reshape(n, 1, hd)
     assert np.array_equal(ko.download(), held(want, 32).astype(np.float32))
+
+
+def test_values_next_to_halves_are_rounded_away_from_zero(ab):
+    """A scale of 1 (a 7 in every group) and values next to every half and whole number, both signs."""
+    f = np.float32
+    y = [c for k in range(7) for c in (f(k), f(k + 0.5))]
+    y = y + [np.nextafter(c, f(-9)) for c in y] + [np.nextafter(c, f(9)) for c in y]
+    y = np.array(y + [-c for c in y], np.float32)
+    x = np.zeros((-(-len(y) // 31), 1, 64), np.float32)
+    for i, c in enumerate(y):
+        x[i // 31, 0, 1 + i % 31] = c
+    x[..., 0] = x[..., 32] = 7
+    n = len(x)
+    kv = ab.PagedKvCache(1, 16, 1, 64)
+    sd = ab.DeviceArray.from_host(np.arange(n), ab.I32)
+    kv.append(up(ab, x, ab.F32), up(ab, x, ab.F32), sd)
+    ko, vo = ab.DeviceArray.empty((n, 1, 64), ab.F32), ab.DeviceArray.empty((n, 1, 64), ab.F32)
+    kv.read(sd, ko, vo)
+    want = np.copysign(np.floor(np.abs(x.astype(np.float64)) + 0.5), x)
+    assert np.array_equal(ko.download(), want) and np.array_equal(vo.download(), want)
+
+
+# ── decode attention: how accurate its parts are ─────────────────────────────────
+@pytest.mark.parametrize("hd,group", [(64, 32), (64, 64), (128, 32), (128, 64)])
+def test_a_single_cached_row_comes_back_to_21_bits(ab, hd, group):
+    """One row: the output is that row.  p · scale is rounded to f32 (2^-24), split into f16 parts (2^-22 of itself; the lo part's own smallest half step
+    is 2^-25 where the row's largest p · scale is 2^7), the two products are added, divided by p (2^-24 each): |Δo| ≤ 2^-21·|v| +
+    2^-32·1.01·max|v|.  Parts of eight bits would leave 2^-17."""
+    rng = np.random.default_rng(81)
+    b = 500
+    k, v = rows(rng, b, 1, hd), rows(rng, b, 1, hd) * np.exp2(rng.integers(-30, 31, (b, 1, 1)))
+    c = Held(ab, [1] * b, np.repeat(k, 16, 0), np.repeat(v, 16, 0), group)      # a page each
+    q = rng.standard_normal((b, 2, hd)).astype(np.float32)
+    out = up(ab, 0 * q, ab.F32)
+    c.kv.decode_attention(up(ab, q, ab.F32), out, ab.DeviceArray.from_host(np.arange(b).reshape(b, 1), ab.I32), ab.DeviceArray.from_host([1] * b, ab.I32), 0.1)
+    want = np.repeat(c.v[::16], 2, 1)
+    tol = 2.0 ** -21 * np.abs(want) + 2.0 ** -32 * 1.01 * np.abs(want).max(2, keepdims=True)
+    err = np.abs(out.download() - want)
+    assert np.all(err <= tol), float((err / tol).max())
+
+
+@pytest.mark.parametrize("hd,group", [(64, 32), (64, 64), (128, 32), (128, 64)])
+def test_scores_are_good_to_20_bits(ab, hd, group):
+    """Two rows with values 7u and −7u: the output is 7u·tanh((s1 − s2) / 2).  Queries have one number, so a score is one product: scale · log2 e
+    is rounded twice, its product with the query once, the query's parts are good to 2^-22, the scale of K, the power of two's way back and the
+    difference from the reference round once more: at most 2^-22 + 6·2^-24 < 2^-21 of |s|, and of the reference, which is within 22 of the
+    larger s in log2 units (15 and the 7 below): 2^-24 · (|s| + 22).  exp2 is good to 2^-22.  |Δo| ≤ 7u · (½ · (|s1| + |s2|) · 2^-20 + 2^-19); parts of
+    eight bits would leave 2^-17·|s|."""
+    rng = np.random.default_rng(82)
+    b, nh = 700, 4
+    k = rows(rng, 2 * b, 1, hd)
+    v = np.ones((2 * b, 1, hd), np.float32)
+    v[1::2] = -1
+    k16, v16 = np.zeros((16 * b, 1, hd), np.float32), np.zeros((16 * b, 1, hd), np.float32)
+    for j in range(2):
+        k16[j::16], v16[j::16] = k[j::2], v[j::2]
+    c = Held(ab, [2] * b, k16, v16, group)
+    q = np.zeros((b, nh, hd), np.float32)
+    at = rng.integers(0, hd, (b, nh))
+    np.put_along_axis(q, at[..., None], rng.uniform(1, 8, (b, nh, 1)).astype(np.float32), 2)
+    out = up(ab, 0 * q, ab.F32)
+    c.kv.decode_attention(up(ab, q, ab.F32), out, ab.DeviceArray.from_host(np.arange(b).reshape(b, 1), ab.I32), ab.DeviceArray.from_host([2] * b, ab.I32), 0.7)
+    s = [np.einsum("bhd,bd->bh", q.astype(np.float64), c.k[j::16, 0]) * float(np.float32(0.7)) for j in range(2)]
+    unit = c.v[0, 0, 0]
+    want = unit * np.tanh((s[0] - s[1]) / 2)
+    tol = unit * (0.5 * (np.abs(s[0]) + np.abs(s[1])) * 2.0 ** -20 + 2.0 ** -19)
+    err = np.abs(out.download() - want[..., None]).max(2)
+    assert np.all(err <= tol), float((err / tol).max())

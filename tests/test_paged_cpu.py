@@ -339,3 +339,49 @@ def test_a_cache_of_more_than_a_c_int_is_refused(place):
     shape[place] += 1 << 32
     with pytest.raises(ab.AtlasError, match="out of range"):
         ab.PagedKvCache(*shape, ctx=FakeContext())
+
+
+# ── the kernels' own arithmetic ──────────────────────────────────────────────────
+@pytest.fixture(scope="module")
+def arith(tmp_path_factory):
+    """Rounding and slot arithmetic as the kernels have them (csrc/paged_index.h), compiled for the host."""
+    d = tmp_path_factory.mktemp("arith")
+    (d / "shim.cpp").write_text('#include "paged_index.h"\nextern "C" {\n'
+                                'int number(float y) { volatile float s = y + ax_p4_half(y); return (int)s; }\n'
+                                'unsigned long long inverse(int p) { return ax_p4_page_inverse(p); }\n'
+                                'int page_of(int slot, unsigned long long inv) { return ax_p4_page_of(slot, inv); }\n}\n')
+    so = str(d / "shim.so")
+    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-I", os.path.join(ROOT, "atlas_b200", "csrc"), str(d / "shim.cpp"), "-o", so], check=True)
+    L = C.CDLL(so)
+    L.number.argtypes, L.inverse.restype, L.page_of.argtypes = [C.c_float], C.c_ulonglong, [C.c_int, C.c_ulonglong]
+    return L
+
+
+def test_the_kernels_round_half_away_from_zero(arith):
+    """Next to every half and whole number below 8, on both sides of zero."""
+    f = np.float32
+    for k in range(8):
+        for c in (f(k), f(k + 0.5)):
+            y = c
+            for _ in range(4):
+                y = np.nextafter(y, f(-1))
+            for _ in range(9):
+                if abs(y) < 7.5:
+                    want = int(np.copysign(np.floor(abs(np.float64(y)) + 0.5), y))
+                    assert arith.number(float(y)) == want and arith.number(float(-y)) == -want, y
+                y = np.nextafter(y, f(100))
+    for y in (1e-45, 1e-38, 1e-20, 0.0):
+        assert arith.number(y) == arith.number(-y) == 0
+
+
+def test_the_kernels_find_a_slots_page(arith):
+    for p in range(16, 8193, 16):
+        inv = arith.inverse(p)
+        top = (1 << 31) - 1
+        n = top // p
+        for page in {0, 1, 2, n // 3, n // 2, n - 2, n - 1}:
+            for off in (0, 1, 15, 16, p - 1):
+                slot = page * p + off
+                if 0 <= slot <= top and off < p:
+                    assert arith.page_of(slot, inv) == page, (p, slot)
+        assert arith.page_of(top, inv) == top // p
