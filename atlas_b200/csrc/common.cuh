@@ -77,7 +77,8 @@ struct atlasx_ctx {
         int mail_reduce = -1;          // ATLASX_MAIL_REDUCE: mailbox parts summed 0 = by every consumer CTA, 1 = by a kernel of their own,
                                        // 2 = by the first CTAs of the consumer (default, −1)
         int tp_select = 1;             // ATLASX_TP_SELECT=0: greedy selection always over all-gathered logits
-        int prompt_short_waits = 0;    // ATLASX_PROMPT_SHORT_WAITS=1: waits inside the packed prompt attention (bf16, heads of 64) end after 10 ms, not 10 s
+        int prompt_short_waits = 0;    // ATLASX_PROMPT_SHORT_WAITS=1: waits inside the packed prompt attention (bf16, heads of 64) end after 10 ms, not 10 s; 2: and one
+                                       // copy is never issued, so that they do end
         int step_trace = 0;            // ATLASX_STEP_TRACE=1: timeline stamps in the captured step
         int comm_timeout_ms = 30000;   // ATLASX_COMM_TIMEOUT_MS: host deadline for a tensor-parallel step to complete
     } tune;

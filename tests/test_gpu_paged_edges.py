@@ -421,3 +421,37 @@ def test_scores_are_good_to_20_bits(ab, hd, group):
     tol = unit * (0.5 * (np.abs(s[0]) + np.abs(s[1])) * 2.0 ** -20 + 2.0 ** -19)
     err = np.abs(out.download() - want[..., None]).max(2)
     assert np.all(err <= tol), float((err / tol).max())
+
+
+@pytest.mark.parametrize("n,nh,n_kv", [(300, 1, 1), (700, 4, 2), (5000, 16, 8)])
+def test_a_prompt_call_whose_wait_ran_out_leaves_everything_usable(ab, monkeypatch, n, nh, n_kv):
+    """The copy of one K tile never comes.  The call ends with an error status, the other items' rows are right, and the next call on the
+    same context (tensor memory and all) is too."""
+    ctx_of = lambda v: (monkeypatch.setenv("ATLASX_PROMPT_SHORT_WAITS", v), ab.Context(0))[1]      # noqa: E731
+    rng = np.random.default_rng(91)
+    hd = 64
+    q, k, v = (bf16(rng.standard_normal((n, h, hd)).astype(np.float32)) for h in (nh, n_kv, n_kv))
+    results = []
+    for mode in ("2", "1"):
+        ctx = ctx_of(mode)
+        ds = [ab.DeviceArray.from_host(orc.f32_to_bf16_rne(x).reshape(x.shape), ab.BF16, ctx) for x in (q, k, v)]
+        out, cu = ab.DeviceArray.from_host(np.zeros((n, nh, hd)), ab.BF16, ctx), ab.DeviceArray.from_host([0, n], ab.I32, ctx)
+        for _ in range(2):
+            ab.prompt_attention(*ds, out, cu, cu, 0.1, ctx=ctx)
+            if mode == "2":
+                code = C.c_int(0)
+                from atlas_b200 import _ffi
+                assert _ffi.lib().atlasx_ctx_poll_device_error(ctx.handle, C.byref(code)) == -5 and 721 <= code.value <= 735
+            else:
+                assert ctx.poll_device_error() == 0
+        results.append(down(ab, out))
+        del ds, out, cu
+        ctx.close()
+    broken, fine = results
+    some = [0, 1, 127, 255, n - 1]
+    for r in some:
+        want, tol = prompt_by_hand(q[r:r + 1], k[:r + 1], v[:r + 1], [0, 1], [0, r + 1], 0.1, 0, False)
+        assert np.all(np.abs(fine[r] - want[0]) <= tol[0])
+    # an item is 256 rows of a head or 128 of two: the lost one, and those that its CTA had taken over, were not written
+    same = (broken == fine).all(2)
+    assert (same | (broken == 0).all(2)).all() and not same.all()
