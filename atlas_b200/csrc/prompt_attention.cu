@@ -17,7 +17,8 @@
 //     first scores of the next item run under the end of the one before (a CTA per item spent 5 to 7 µs starting and ending).  A warp of its
 //     own finds sequence and rows in the prefix arrays: nothing depends on host-side lengths, and a captured call follows the arrays.
 //   * A product of 0 and a NaN or infinity in a value row that the query does not see would be NaN: value rows behind the sequence are
-//     zeroed in shared memory, and an output row that is not finite is taken again by ax_prompt_row, which reads visible rows only.
+//     zeroed in shared memory, and an output row that is not finite (though its scores are numbers) is taken again by ax_prompt_row, which
+//     reads visible rows only.
 //   * Every wait is bounded (ten seconds of %globaltimer, in which no row is taken again): on expiry the CTA raises the context's error word, all roles leave, copies
 //     in flight are waited for and tensor memory is released.
 #include <cuda.h>
@@ -70,7 +71,7 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 }
 // Bounded wait.  false: gave up (this thread's deadline passed, or another role raised the abort flag).  flags: [0] abort, [1] warps that take
 // rows again — as long as there are any (each row is a loop over its keys, so it ends) the deadline does not run: a long prompt
-// with a NaN in its first key has minutes of them.
+// with a NaN in its first value has minutes of them.
 template <int WAIT_MS> __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* flags, int* err, int code) {
     if (mbar_try(bar, parity)) return true;
     unsigned long long t0 = 0;
@@ -567,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 for (int c = 8; c < 120; c += 2) mx[(c >> 1) & 7] = max3(mx[(c >> 1) & 7], x[c], x[c + 1]);
                 const float top = max3(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], x[120])),
                                        max3(x[121], x[122], x[123]), max3(max3(x[124], x[125], x[126]), x[127], x[127]));
-                if (top != top) m = top;                                      // the row is taken again
+                if (top != top) m = top;                                      // a visible score is NaN: so is every probability from here on
                 const bool grow = top > m && (m == -INFINITY || (top - m) * sc > 8.f);
                 const bool started = j > j_lo;
                 if (__any_sync(AX_FULL, grow)) {
@@ -675,7 +676,8 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 }
             }
             const bool sees = key_hi >= 0 && w.s.lk > 0;
-            unsigned again = __ballot_sync(AX_FULL, live && (odd != odd || (sees && !(fabsf(m) <= 3.402823466e38f))));
+            // a visible score that is NaN makes the row NaN, as it is already
+            unsigned again = __ballot_sync(AX_FULL, live && m == m && (odd != odd || (sees && !(fabsf(m) <= 3.402823466e38f))));
             __syncwarp();
             if (again) {
             if (lane == 0) atomicAdd(&s_flags[1], 1);

@@ -301,7 +301,7 @@ def test_many_small_probabilities_in_f16(ab, hd):
 
 
 def test_rows_taken_again_do_not_run_out_the_waits_of_others(ab, monkeypatch):
-    """A NaN in the first key: every row is taken again, an item's rows for longer than a wait may take.  The limit is set low here so that a
+    """A NaN in the first value: every row is taken again, an item's rows for longer than a wait may take.  The limit is set low here so that a
     prompt of 8192 is long enough; with the 10 seconds there are it takes half a million rows."""
     monkeypatch.setenv("ATLASX_PROMPT_SHORT_WAITS", "1")
     ctx = ab.Context(0)
@@ -317,8 +317,8 @@ def test_rows_taken_again_do_not_run_out_the_waits_of_others(ab, monkeypatch):
     for i, r in enumerate(some):
         want, tol = prompt_by_hand(q[r:r + 1], k[:r + 1], v[:r + 1], [0, 1], [0, r + 1], 0.1, 0, False)
         assert np.all(np.abs(got[i] - want[0]) <= tol[0])
-    k[0] = np.nan
-    ctx.upload(ds[1].ptr, orc.f32_to_bf16_rne(k))
+    v[0] = np.nan
+    ctx.upload(ds[2].ptr, orc.f32_to_bf16_rne(v))
     ab.prompt_attention(*ds, out, cu, cu, 0.1, ctx=ctx)
     assert ctx.poll_device_error() == 0
     assert np.isnan(down(ab, out)).all()
@@ -455,3 +455,54 @@ def test_a_prompt_call_whose_wait_ran_out_leaves_everything_usable(ab, monkeypat
     # an item is 256 rows of a head or 128 of two: the lost one, and those that its CTA had taken over, were not written
     same = (broken == fine).all(2)
     assert (same | (broken == 0).all(2)).all() and not same.all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("where", ["q", "k"])
+def test_a_nan_score_makes_its_rows_nan_and_no_others(ab, hd, where):
+    """In a query: that row of that head.  In a key: the rows that see it, within the window and their sequence, of all heads that share it."""
+    rng = np.random.default_rng(92)
+    lens, nh, window = [200, 300], 4, 70
+    n = sum(lens)
+    q, k, v = (bf16(rng.standard_normal((n, h, hd)).astype(np.float32)) for h in (nh, 2, 2))
+    cu = np.array([0, 200, 500])
+    want, tol = prompt_by_hand(q, k, v, cu, cu, 0.1, window, False)
+    nan = np.zeros((n, nh), bool)
+    if where == "q":
+        q[250, 2, 5] = np.nan
+        nan[250, 2] = True
+    else:
+        k[260, 1, 5] = np.nan
+        nan[260:330, 2:] = True
+    out = up(ab, np.full(q.shape, 7.0), ab.BF16)
+    c = ab.DeviceArray.from_host(cu, ab.I32)
+    ab.prompt_attention(*(up(ab, t, ab.BF16) for t in (q, k, v)), out, c, c, 0.1, window)
+    got = down(ab, out)
+    assert np.isnan(got[nan]).all()
+    assert np.all(np.abs(got - want)[~nan] <= tol[~nan])
+
+
+def test_a_nan_in_an_early_key_of_a_long_prompt(ab):
+    """Nothing but NaN, written as fast as anything else: row by row, 40 000 rows of 8 heads would take many seconds."""
+    torch = pytest.importorskip("torch")
+    n, nh, hd = 40000, 8, 64
+    rng = np.random.default_rng(93)
+    x = bf16(rng.standard_normal((n, nh, hd)).astype(np.float32))
+    qd, vd = up(ab, x, ab.BF16), up(ab, x, ab.BF16)
+    kd = [up(ab, x, ab.BF16), None]
+    x[3] = np.nan
+    kd[1] = up(ab, x, ab.BF16)
+    out, cu = ab.DeviceArray.empty((n, nh, hd), ab.BF16), ab.DeviceArray.from_host([0, n], ab.I32)
+    ctx = ab.Context.default()
+    s = torch.cuda.ExternalStream(ctx.stream)
+    ms = []
+    for k in kd + kd:
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record(s)
+        ab.prompt_attention(qd, k, vd, out, cu, cu, 0.1)
+        b.record(s)
+        ctx.sync()
+        ms.append(a.elapsed_time(b))
+    got = down(ab, out)
+    assert np.isnan(got[3:]).all() and np.isfinite(got[:3]).all()
+    assert ms[3] < 3 * ms[2], ms
