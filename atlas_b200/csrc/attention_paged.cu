@@ -51,23 +51,15 @@ struct PagedDev {
 struct UnitInfo { int seg, tile, ok, pad; };     // segment, first tile, bit u: tile + u is there
 
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
 // Bounded, and the same answer for all lanes of the warp: one that saw the copy land just as the others gave up would wait for them for good.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned long long ns) {
-    if (__all_sync(AX_FULL, mbar_try(bar, parity))) return true;
+    if (__all_sync(AX_FULL, ax_mbar_try(bar, parity))) return true;
     const unsigned long long t0 = ax_globaltimer();
     for (;;) {
-        if (__all_sync(AX_FULL, mbar_try(bar, parity))) return true;
+        if (__all_sync(AX_FULL, ax_mbar_try(bar, parity))) return true;
         if (__any_sync(AX_FULL, ax_globaltimer() - t0 > ns)) return false;
     }
 }
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {         // round to nearest
     uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r;
@@ -131,7 +123,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     auto s_o = [&](int slot) { return reinterpret_cast<float*>(smem + (slot >> 1) * own + (slot & 1 ? 0 : RING + QBYTES)); };
     unsigned* s_pre = reinterpret_cast<unsigned*>(smem + kWarps * own);
 
-    if (tid < kWarps * kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(smem_u32(&s_bar[tid / kStages][tid % kStages])) : "memory");
+    if (tid < kWarps * kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(ax_smem_u32(&s_bar[tid / kStages][tid % kStages])) : "memory");
     if (tid < kWarps * 2) s_seg[tid] = -1;
     if (tid == 0) s_gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -219,11 +211,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             }
         }
         if (lane == (i & 31)) {
-            const uint32_t bar = smem_u32(&s_bar[warp][st]);
+            const uint32_t bar = ax_smem_u32(&s_bar[warp][st]);
             s_info[warp][st] = mine;
             auto copy = [&](int u, uint32_t bytes) {
                 asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                             :: "r"(smem_u32(ring + st * UNIT + u * TILE)), "l"(src[u]), "r"(bytes), "r"(bar) : "memory");
+                             :: "r"(ax_smem_u32(ring + st * UNIT + u * TILE)), "l"(src[u]), "r"(bytes), "r"(bar) : "memory");
             };
             const bool one = mine.ok == 3 && src[1] == src[0] + TILE;          // neighbours in a page
             if (mine.ok) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(mine.ok == 3 ? UNIT : TILE) : "memory");
@@ -330,7 +322,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
         const UnitInfo info = s_info[warp][st];
         // known before the unit is here: a new segment's query comes under its copy
         if (info.seg != seg) { if (seg >= 0) flush(); start(info.seg); }
-        if (!mbar_wait(smem_u32(&s_bar[warp][st]), phase, kNs)) break;
+        if (!mbar_wait(ax_smem_u32(&s_bar[warp][st]), phase, kNs)) break;
         if (info.ok) {
             // Both tiles side by side: their chains — scores, softmax, products — are each other's cover.  (One tile at a time left 54 % of the
             // issue slots and 41 % of the busiest pipe in use.)
@@ -426,7 +418,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             // The reference is moved only where a p · scale would pass 2^15; then the largest becomes 2^7, so what is lost of the small
             // ones (half a step of f16's subnormals, 2^-25) is at most 2^-32 of the largest.
             if (__any_sync(AX_FULL, top > m + 15.f)) {
-                const float mn = fmaxf(m, top - 7.f), f = m == -INFINITY ? 0.f : ex2(m - mn);
+                const float mn = fmaxf(m, top - 7.f), f = m == -INFINITY ? 0.f : ax_ex2(m - mn);
                 l.x *= f; l.y *= f;
 #pragma unroll
                 for (int i = 0; i < NT; i++) { o[i][0] *= f; o[i][1] *= f; o[i][2] *= f; o[i][3] *= f; }
@@ -438,7 +430,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
 #pragma unroll
                 for (int nt = 0; nt < 2; nt++) {                               // scores become probabilities
                     s[u][nt] = ax_add2(s[u][nt], make_float2(mr, mr));
-                    s[u][nt].x = ex2(s[u][nt].x); s[u][nt].y = ex2(s[u][nt].y);
+                    s[u][nt].x = ax_ex2(s[u][nt].x); s[u][nt].y = ax_ex2(s[u][nt].y);
                     l = ax_add2(l, s[u][nt]);
                 }
             uint32_t vw[kUnit][2][W];
@@ -483,7 +475,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
     if (it < count) {                                                          // gave up
         if (lane == 0) { atomicExch(dv.err, kErrWait); s_gave_up = 1; }
         for (int y = it; y < count && y < it + kStages; y++)                  // what is in flight lands before the CTA goes
-            mbar_wait(smem_u32(&s_bar[warp][y % kStages]), (uint32_t)(y / kStages) & 1u, kNs);
+            mbar_wait(ax_smem_u32(&s_bar[warp][y % kStages]), (uint32_t)(y / kStages) & 1u, kNs);
     }
     __syncwarp();                                                              // the ring is read by all lanes before the last output goes over it
     if (seg >= 0) flush();
@@ -526,7 +518,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
             float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int k = i; k < j; k++)
                 if (s_seg[k] == sg && s_ml[k][h][1] != 0.f) {
-                    const float f = s_ml[k][h][0] == M ? 1.f : ex2(s_ml[k][h][0] - M);
+                    const float f = s_ml[k][h][0] == M ? 1.f : ax_ex2(s_ml[k][h][0] - M);
                     const float4 v = *(const float4*)(s_o(k) + h * HD + d);
                     L = fmaf(f, s_ml[k][h][1], L);
                     A.x = fmaf(f, v.x, A.x); A.y = fmaf(f, v.y, A.y); A.z = fmaf(f, v.z, A.z); A.w = fmaf(f, v.w, A.w);
@@ -591,7 +583,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) ax_paged_attn_kernel(
                             const int k = lane + 32 * r;
                             if (k >= kn) continue;
                             const float2 v = k0 ? __ldcg((const float2*)(ml + (part(k0 + k) + h) * 2)) : own[i][r];
-                            const float f = v.y == 0.f ? 0.f : v.x == M[i] ? 1.f : ex2(v.x - M[i]);
+                            const float f = v.y == 0.f ? 0.f : v.x == M[i] ? 1.f : ax_ex2(v.x - M[i]);
                             wt[h * kChunk + k] = f;
                             sum += f * v.y;
                         }

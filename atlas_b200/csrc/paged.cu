@@ -170,10 +170,6 @@ __device__ __forceinline__ void slot_place(const RowArgs& a, int slot, int& page
 }
 template <int HD, int GS> __device__ __forceinline__ AxP4Shape fixed_shape(const AxP4Shape& s) { return AxP4Shape{ s.n_pages, s.page_size, s.n_kv, HD, GS }; }
 
-__device__ __forceinline__ float max3(float x, float y, float z) {      // NaN if one is
-    float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z)); return d;
-}
-
 // A lane holds thirty-two consecutive numbers of one row of K or V: a group, or half of one whose largest magnitude two lanes
 // find with a shuffle.  scale = bf16(max / 7); the number is x · (1 / scale) rounded half away from zero — the f32 arithmetic of
 // Int4Tensor::quantize with a scale of 16 bits: the numbers are rounded against the scale that is stored, so its own rounding (2^-8 of
@@ -198,10 +194,10 @@ __global__ void __launch_bounds__(kAppendThreads) ax_p4_append_kernel(const RowA
 #pragma unroll
         for (int i = 0; i < N; i += 8) load8<T>(src + N * li + i, reinterpret_cast<float (&)[8]>(x[i]));
 #pragma unroll
-        for (int i = 0; i < N; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
+        for (int i = 0; i < N; i += 2) top = ax_max3(top, fabsf(x[i]), fabsf(x[i + 1]));
     }
 #pragma unroll
-    for (int d = 1; d < GL; d <<= 1) { const float o = __shfl_xor_sync(AX_FULL, top, d); top = max3(top, o, o); }
+    for (int d = 1; d < GL; d <<= 1) { const float o = __shfl_xor_sync(AX_FULL, top, d); top = ax_max3(top, o, o); }
     if (!live || slot < 0) return;                                   // a negative slot marks an absent row
     if (slot >= sh.n_pages * sh.page_size) { if (li == 0) atomicExch(a.err, AX_DEVERR_SLOT); return; }
     const bool odd = !(top <= 3.402823466e38f);

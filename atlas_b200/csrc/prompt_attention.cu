@@ -53,7 +53,6 @@ struct PromptDev {
     int* err;
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
 }
@@ -63,22 +62,16 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
 // Bounded wait.  false: gave up (this thread's deadline passed, or another role raised the abort flag).  flags: [0] abort, [1] warps that take
 // rows again — as long as there are any (each row is a loop over its keys, so it ends) the deadline does not run: a long prompt
 // with a NaN in its first value has minutes of them.
 template <int WAIT_MS> __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* flags, int* err, int code) {
-    if (mbar_try(bar, parity)) return true;
+    if (ax_mbar_try(bar, parity)) return true;
     unsigned long long t0 = 0;
     for (;;) {
 #pragma unroll 1
         for (int i = 0; i < 256; i++)                                         // as few instructions as can be: waiting warps share the issue slots
-            if (mbar_try(bar, parity)) return true;
+            if (ax_mbar_try(bar, parity)) return true;
         if (flags[0]) return false;
         if (flags[1]) t0 = 0;
         const unsigned long long t = ax_globaltimer();
@@ -159,21 +152,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 #undef AX_I
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\t"
-        "mov.b64 {%0, %1}, w;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-// largest of three; NaN if one is
-__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 template <bool F16> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     uint32_t r;
     if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -234,18 +212,18 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     const int tid = threadIdx.x, warp = __shfl_sync(AX_FULL, tid >> 5, 0), lane = tid & 31;
     const AxPromptArgs& a = dv.a;
     volatile int* flags = s_flags;
-    const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t smem0 = (ax_smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t ring = smem0 + 2 * TILE;
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(smem_u32(&q_full[i]), 1); mbar_init(smem_u32(&q_empty[i]), 1); mbar_init(smem_u32(&s_full[i]), 1);
-            mbar_init(smem_u32(&o_done[i]), 1); mbar_init(smem_u32(&o_free[i]), kRows);
-            for (int b = 0; b < 2; b++) mbar_init(smem_u32(&p_ready[i][b]), kRows);
+            mbar_init(ax_smem_u32(&q_full[i]), 1); mbar_init(ax_smem_u32(&q_empty[i]), 1); mbar_init(ax_smem_u32(&s_full[i]), 1);
+            mbar_init(ax_smem_u32(&o_done[i]), 1); mbar_init(ax_smem_u32(&o_free[i]), kRows);
+            for (int b = 0; b < 2; b++) mbar_init(ax_smem_u32(&p_ready[i][b]), kRows);
         }
-        for (int i = 0; i < NS; i++) { mbar_init(smem_u32(&kv_full[i]), 1); mbar_init(smem_u32(&kv_empty[i]), 1); }
-        for (int i = 0; i < kSlots; i++) { mbar_init(smem_u32(&i_full[i]), 1); mbar_init(smem_u32(&i_empty[i]), kReaders); }
-        mbar_init(smem_u32(&v_here), 1); mbar_init(smem_u32(&v_cut), 1); mbar_init(smem_u32(&clc_bar), 1);
+        for (int i = 0; i < NS; i++) { mbar_init(ax_smem_u32(&kv_full[i]), 1); mbar_init(ax_smem_u32(&kv_empty[i]), 1); }
+        for (int i = 0; i < kSlots; i++) { mbar_init(ax_smem_u32(&i_full[i]), 1); mbar_init(ax_smem_u32(&i_empty[i]), kReaders); }
+        mbar_init(ax_smem_u32(&v_here), 1); mbar_init(ax_smem_u32(&v_cut), 1); mbar_init(ax_smem_u32(&clc_bar), 1);
         s_flags[0] = s_flags[1] = 0; s_issued = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -254,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         for (const CUtensorMap* map : { &map_q, &map_k, &map_v }) asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory");
     }
     if (warp == kProduct) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(ax_smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -264,11 +242,11 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
     // the n-th item of this CTA, for every reader in turn; false: no more
     auto item_at = [&](int n, Item& it) {
         const int slot = n % kSlots;
-        if (!mbar_wait<WAIT_MS>(smem_u32(&i_full[slot]), (uint32_t)(n / kSlots) & 1u, flags, dv.err, 731)) return false;
+        if (!mbar_wait<WAIT_MS>(ax_smem_u32(&i_full[slot]), (uint32_t)(n / kSlots) & 1u, flags, dv.err, 731)) return false;
         it = *const_cast<const Item*>(&s_item[slot]);
         return it.lq >= 0;
     };
-    auto item_read = [&](int n) { mbar_arrive(smem_u32(&i_empty[n % kSlots])); };
+    auto item_read = [&](int n) { mbar_arrive(ax_smem_u32(&i_empty[n % kSlots])); };
 
     // 384 threads start with 168 registers each (64512 in all); a row of scores is 128 of them.  256 · 208 + 128 · 80 = 63488.
     if (warp >= kProduct) {
@@ -291,9 +269,9 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
         while (ok && more) {
             // ask for the next CTA's place while this one's item is looked up
             if (lane == 0) {
-                mbar_expect_tx(smem_u32(&clc_bar), 16);
+                mbar_expect_tx(ax_smem_u32(&clc_bar), 16);
                 asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
-                             :: "r"(smem_u32(&s_clc)), "r"(smem_u32(&clc_bar)) : "memory");
+                             :: "r"(ax_smem_u32(&s_clc)), "r"(ax_smem_u32(&clc_bar)) : "memory");
             }
             __syncwarp();
             const long long x = all - 1 - block / hx;
@@ -322,27 +300,27 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                     at += __shfl_sync(AX_FULL, up, 31);
                 }
                 it.h0 = (int)(block % hx) * (dv.pair_heads ? 2 : 1);
-                if (n >= kSlots) ok = mbar_wait<WAIT_MS>(smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, flags, dv.err, 732);
+                if (n >= kSlots) ok = mbar_wait<WAIT_MS>(ax_smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, flags, dv.err, 732);
                 ok = __all_sync(AX_FULL, ok);
-                if (ok && lane == 0) { s_item[n % kSlots] = it; mbar_arrive(smem_u32(&i_full[n % kSlots])); }
+                if (ok && lane == 0) { s_item[n % kSlots] = it; mbar_arrive(ax_smem_u32(&i_full[n % kSlots])); }
                 n++;
             }
-            bool got = mbar_wait<WAIT_MS>(smem_u32(&clc_bar), clc_phase, flags, dv.err, 733);
+            bool got = mbar_wait<WAIT_MS>(ax_smem_u32(&clc_bar), clc_phase, flags, dv.err, 733);
             if (!__all_sync(AX_FULL, got)) { ok = false; break; }
             clc_phase ^= 1u;
             uint32_t took, next;
             asm volatile("{\n\t.reg .b128 r;\n\t.reg .pred p;\n\tld.shared.b128 r, [%2];\n\t"
                          "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
                          "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
-                         : "=r"(took), "=r"(next) : "r"(smem_u32(&s_clc)) : "memory");
+                         : "=r"(took), "=r"(next) : "r"(ax_smem_u32(&s_clc)) : "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // read before the next answer is written
             __syncwarp();
             more = took != 0;
             block = next;
         }
         if (ok) {
-            if (n >= kSlots) ok = mbar_wait<WAIT_MS>(smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, flags, dv.err, 732);
-            if (__all_sync(AX_FULL, ok) && lane == 0) { s_item[n % kSlots].lq = -1; mbar_arrive(smem_u32(&i_full[n % kSlots])); }
+            if (n >= kSlots) ok = mbar_wait<WAIT_MS>(ax_smem_u32(&i_empty[n % kSlots]), (uint32_t)(n / kSlots - 1) & 1u, flags, dv.err, 732);
+            if (__all_sync(AX_FULL, ok) && lane == 0) { s_item[n % kSlots].lq = -1; mbar_arrive(ax_smem_u32(&i_full[n % kSlots])); }
         }
         __syncwarp();
     } else if (warp == kCopy) {
@@ -356,10 +334,10 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 const Work w = work_of(dv, it);
                 const int kh = w.h0 / (a.n_heads / a.n_kv);
                 auto query = [&](int t) {
-                    ok = mbar_wait<WAIT_MS>(smem_u32(&q_empty[t]), (uint32_t)(nq[t] + 1) & 1u, flags, dv.err, 734);
+                    ok = mbar_wait<WAIT_MS>(ax_smem_u32(&q_empty[t]), (uint32_t)(nq[t] + 1) & 1u, flags, dv.err, 734);
                     if (!ok) return;
                     nq[t]++;
-                    const uint32_t bar = smem_u32(&q_full[t]);
+                    const uint32_t bar = ax_smem_u32(&q_full[t]);
                     mbar_expect_tx(bar, TILE);
                     for (int b = 0; b < BOXES; b++)
                         tma_load_3d(smem0 + t * TILE + b * kBoxBytes, &map_q, b * 64, dv.pair_heads ? w.h0 + t : w.h0, w.s.q0 + (t ? w.base1 : w.base0), bar);
@@ -367,9 +345,9 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 // The first K tile goes ahead of the queries: their places are free only when the item before has its last scores.
                 const int m = 2 * (w.j1 - w.j0 + 1);
                 for (int i = 0; i < m && ok; i++) {
-                    ok = mbar_wait<WAIT_MS>(smem_u32(&kv_empty[st]), ph, flags, dv.err, 721);
+                    ok = mbar_wait<WAIT_MS>(ax_smem_u32(&kv_empty[st]), ph, flags, dv.err, 721);
                     if (!ok) break;
-                    const uint32_t bar = smem_u32(&kv_full[st]);
+                    const uint32_t bar = ax_smem_u32(&kv_full[st]);
                     mbar_expect_tx(bar, TILE);
                     const CUtensorMap* map = i & 1 ? &map_v : &map_k;
                     const bool lost = WAIT_MS == kTestWaitMs && dv.lose && blockIdx.x == 0 && n == 0 && i == 2;
@@ -396,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
 #pragma unroll
                 for (int i = 1; i < HD / 16; i++)
                     umma_ss<true>(kS + t * 128, q + (i / 4) * (kBoxBytes >> 4) + (i % 4) * 2, k + (i / 4) * (kBoxBytes >> 4) + (i % 4) * 2, id_qk);
-                umma_commit(smem_u32(&s_full[t]));
+                umma_commit(ax_smem_u32(&s_full[t]));
             };
             int st = 0;                                                       // stages are taken in turn; ph: parity of their phase
             uint32_t ph = 0, pq[2] = { 0, 0 }, pp[2] = { 0, 0 }, cuts = 0;    // parities of a tile's queries and probabilities, of the cuts
@@ -408,26 +386,26 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 const Work w = work_of(dv, it);
                 const int n = w.j1 - w.j0 + 1, a0 = w.lo0 - w.j0, z0 = w.on0 ? w.hi0 - w.j0 : -1, a1 = w.lo1 - w.j0, z1 = w.on1 ? w.hi1 - w.j0 : -1;
                 if (n <= 0) continue;
-                ok = mbar_wait<WAIT_MS>(smem_u32(&kv_full[st]), ph, flags, dv.err, 722);
+                ok = mbar_wait<WAIT_MS>(ax_smem_u32(&kv_full[st]), ph, flags, dv.err, 722);
 #pragma unroll
                 for (int t = 0; t < 2; t++)
                     if (ok && (t ? w.on1 : w.on0)) {
-                        ok = mbar_wait<WAIT_MS>(smem_u32(&q_full[t]), pq[t], flags, dv.err, 723);
+                        ok = mbar_wait<WAIT_MS>(ax_smem_u32(&q_full[t]), pq[t], flags, dv.err, 723);
                         pq[t] ^= 1u;
                         if (ok && (t ? a1 : a0) == 0) {
                             qk(t, st);
-                            if ((t ? z1 : z0) == 0) umma_commit(smem_u32(&q_empty[t]));
+                            if ((t ? z1 : z0) == 0) umma_commit(ax_smem_u32(&q_empty[t]));
                         }
                     }
                 if (!ok) break;
-                umma_commit(smem_u32(&kv_empty[st]));
+                umma_commit(ax_smem_u32(&kv_empty[st]));
                 next();
                 for (int i = 0; i < n && ok; i++) {
                     const int sv = st;
-                    ok = mbar_wait<WAIT_MS>(smem_u32(&kv_full[sv]), ph, flags, dv.err, 722);
+                    ok = mbar_wait<WAIT_MS>(ax_smem_u32(&kv_full[sv]), ph, flags, dv.err, 722);
                     if (ok && i == n - 1 && w.cut) {
-                        mbar_arrive(smem_u32(&v_here));
-                        ok = mbar_wait<WAIT_MS>(smem_u32(&v_cut), cuts & 1u, flags, dv.err, 729);
+                        mbar_arrive(ax_smem_u32(&v_here));
+                        ok = mbar_wait<WAIT_MS>(ax_smem_u32(&v_cut), cuts & 1u, flags, dv.err, 729);
                         cuts++;
                     }
                     if (!ok) break;
@@ -439,11 +417,11 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                         const int at = t ? a1 : a0, zt = t ? z1 : z0;
                         if (ok && i >= at && i <= zt) {
                             // the item before has been read out of the accumulator
-                            if (i == at && items[t] > 0) ok = mbar_wait<WAIT_MS>(smem_u32(&o_free[t]), (uint32_t)(items[t] - 1) & 1u, flags, dv.err, 735);
+                            if (i == at && items[t] > 0) ok = mbar_wait<WAIT_MS>(ax_smem_u32(&o_free[t]), (uint32_t)(items[t] - 1) & 1u, flags, dv.err, 735);
                             if (i == at) items[t]++;
 #pragma unroll
                             for (int part = 0; part < 2; part++) {            // the product starts with the first probabilities
-                                ok = ok && mbar_wait<WAIT_MS>(smem_u32(&p_ready[t][part]), pp[t], flags, dv.err, 724);
+                                ok = ok && mbar_wait<WAIT_MS>(ax_smem_u32(&p_ready[t][part]), pp[t], flags, dv.err, 724);
                                 if (!ok) break;
                                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -451,19 +429,19 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                                     umma_ts(kO + t * HD, kS + t * 128 + c * 8, vd + c * (2048 >> 4), id_pv, c ? 1u : (uint32_t)(i != at));
                             }
                             pp[t] ^= 1u;
-                            if (ok) umma_commit(smem_u32(&o_done[t]));
+                            if (ok) umma_commit(ax_smem_u32(&o_done[t]));
                         }
                         if (ok && i + 1 >= at && i + 1 <= zt) {               // over the scores and probabilities just used
-                            ok = mbar_wait<WAIT_MS>(smem_u32(&kv_full[sk]), ph, flags, dv.err, 722);
+                            ok = mbar_wait<WAIT_MS>(ax_smem_u32(&kv_full[sk]), ph, flags, dv.err, 722);
                             if (ok) {
                                 qk(t, sk);
-                                if (i + 1 == zt) umma_commit(smem_u32(&q_empty[t]));
+                                if (i + 1 == zt) umma_commit(ax_smem_u32(&q_empty[t]));
                             }
                         }
                     }
                     if (!ok) break;
-                    umma_commit(smem_u32(&kv_empty[sv]));
-                    if (i + 1 < n) { umma_commit(smem_u32(&kv_empty[sk])); next(); }
+                    umma_commit(ax_smem_u32(&kv_empty[sv]));
+                    if (i + 1 < n) { umma_commit(ax_smem_u32(&kv_empty[sk])); next(); }
                 }
             }
         }
@@ -485,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             if (w.cut) {
                 const int valid = w.s.lk - w.j1 * kRows;
                 const uint32_t v = ring + (uint32_t)((st + m - 1) % NS) * TILE;
-                ok = mbar_wait<WAIT_MS>(smem_u32(&v_here), cuts & 1u, flags, dv.err, 730);       // told by the thread that saw it arrive
+                ok = mbar_wait<WAIT_MS>(ax_smem_u32(&v_here), cuts & 1u, flags, dv.err, 730);       // told by the thread that saw it arrive
                 ok = __all_sync(AX_FULL, ok);
                 if (!ok) break;
                 cuts++;
@@ -495,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(v + b * kBoxBytes + at), "r"(0) : "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&v_cut));
+                if (lane == 0) mbar_arrive(ax_smem_u32(&v_cut));
             }
             st = (st + m) % NS;
         }
@@ -524,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             float m = -INFINITY;
             float2 l0 = make_float2(0.f, 0.f), l1 = l0;
             for (int j = j_lo; j <= j_hi; j++) {
-                ok = mbar_wait<WAIT_MS>(smem_u32(&s_full[t]), ps, flags, dv.err, 725);
+                ok = mbar_wait<WAIT_MS>(ax_smem_u32(&s_full[t]), ps, flags, dv.err, 725);
                 ok = __all_sync(AX_FULL, ok);
                 if (!ok) break;
                 ps ^= 1u;
@@ -565,19 +543,19 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
 #pragma unroll
                 for (int c = 0; c < 8; c++) mx[c] = x[c];
 #pragma unroll
-                for (int c = 8; c < 120; c += 2) mx[(c >> 1) & 7] = max3(mx[(c >> 1) & 7], x[c], x[c + 1]);
-                const float top = max3(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], x[120])),
-                                       max3(x[121], x[122], x[123]), max3(max3(x[124], x[125], x[126]), x[127], x[127]));
+                for (int c = 8; c < 120; c += 2) mx[(c >> 1) & 7] = ax_max3(mx[(c >> 1) & 7], x[c], x[c + 1]);
+                const float top = ax_max3(ax_max3(ax_max3(mx[0], mx[1], mx[2]), ax_max3(mx[3], mx[4], mx[5]), ax_max3(mx[6], mx[7], x[120])),
+                                       ax_max3(x[121], x[122], x[123]), ax_max3(ax_max3(x[124], x[125], x[126]), x[127], x[127]));
                 if (top != top) m = top;                                      // a visible score is NaN: so is every probability from here on
                 const bool grow = top > m && (m == -INFINITY || (top - m) * sc > 8.f);
                 const bool started = j > j_lo;
                 if (__any_sync(AX_FULL, grow)) {
                     const bool moved = grow && m != -INFINITY;                // a row that has seen nothing has sums and outputs of zero
-                    const float f = moved ? ex2((m - top) * sc) : 1.f;
+                    const float f = moved ? ax_ex2((m - top) * sc) : 1.f;
                     if (grow) m = top;
                     l0.x *= f; l0.y *= f; l1.x *= f; l1.y *= f;
                     if (started && __any_sync(AX_FULL, moved)) {              // the products of the tile before are in: po is the parity they leave
-                        ok = mbar_wait<WAIT_MS>(smem_u32(&o_done[t]), po ^ 1u, flags, dv.err, 726);
+                        ok = mbar_wait<WAIT_MS>(ax_smem_u32(&o_done[t]), po ^ 1u, flags, dv.err, 726);
                         ok = __all_sync(AX_FULL, ok);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -604,9 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                     } else
 #pragma unroll
                     for (int c = 0; c < 16; c++) {
-                        float2 y = fma2(make_float2(x[c0 + 2 * c], x[c0 + 2 * c + 1]), sc2, neg2);
-                        y.x = ex2(y.x); y.y = ex2(y.y);
-                        if (c & 1) l1 = add2(l1, y); else l0 = add2(l0, y);
+                        float2 y = ax_fma2(make_float2(x[c0 + 2 * c], x[c0 + 2 * c + 1]), sc2, neg2);
+                        y.x = ax_ex2(y.x); y.y = ax_ex2(y.y);
+                        if (c & 1) l1 = ax_add2(l1, y); else l0 = ax_add2(l0, y);
                         p[c] = pack<F16>(y.x, y.y);
                     }
                     tmem_st16(ts + c0 / 2, p);
@@ -614,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                 auto hand_over = [&](int part) {
                     tmem_wait_st();
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    mbar_arrive(smem_u32(&p_ready[t][part]));
+                    mbar_arrive(ax_smem_u32(&p_ready[t][part]));
                 };
                 if (hidden) {
                     probs(0, true); probs(32, true);
@@ -632,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             // ── output ──
             const bool any = j_hi >= j_lo;
             if (ok && any) {
-                ok = mbar_wait<WAIT_MS>(smem_u32(&o_done[t]), po ^ 1u, flags, dv.err, 727);
+                ok = mbar_wait<WAIT_MS>(ax_smem_u32(&o_done[t]), po ^ 1u, flags, dv.err, 727);
                 ok = __all_sync(AX_FULL, ok);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
@@ -649,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
                     tmem_ld32(to + c, o);
                     if (c + 32 == HD) {                                       // the accumulator may take the next item's products
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        mbar_arrive(smem_u32(&o_free[t]));
+                        mbar_arrive(ax_smem_u32(&o_free[t]));
                     }
                 } else {
 #pragma unroll
@@ -699,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1) ax_prompt_umma_kernel(const __gri
             const int issued = s_issued;
             for (int i = issued > NS ? issued - NS : 0; i < issued; i++) {
                 const unsigned long long t0 = ax_globaltimer();
-                while (!mbar_try(smem_u32(&kv_full[i % NS]), (uint32_t)(i / NS) & 1u) && ax_globaltimer() - t0 < kAbortNs) { }
+                while (!ax_mbar_try(ax_smem_u32(&kv_full[i % NS]), (uint32_t)(i / NS) & 1u) && ax_globaltimer() - t0 < kAbortNs) { }
             }
         }
         if (tid == 32) {                                                      // queries, products and an answer asked for before the failure: time to land
