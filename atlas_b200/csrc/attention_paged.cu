@@ -10,7 +10,9 @@
 //     hi parts, rows 8..15 the lo parts of the same f32 values, so one instruction gives both and the sum of two accumulators
 //     is good to 2^-22 of each value (bf16 halves left 4e-6 of the output, 2^-16 of each value).  The score accumulators are
 //     already the operand layout of the second product.  f16 has little range, so a head's query is brought to 2^14 by a power
-//     of two, and the softmax reference follows the largest p · scale of V instead of the largest p.
+//     of two, and the softmax reference follows the largest p · scale of V instead of the largest p: what a group of V holds is exact to 2^-32 of
+//     the row's largest p · |v|, whatever the size of V is (groups of zeros are stored with the smallest scale; with scales of V
+//     above 2^90 rows whose weight is below 2^-133 of the scale are lost, their p being below the range of f32).
 //   * A nibble u (the number plus eight) becomes an f16 number by mask-and-or and one exact operation: 1024 + u − 1032, or, four
 //     bits up, (1024 + 16u) / 16 − 72: nine instructions for eight numbers.  (A masked nibble of K as the f16 subnormal it
 //     is, with −8 · Σq as the accumulators' start, takes 62.5 µs instead of 64.9 for 12 windowed requests and 118 instead of 120 for

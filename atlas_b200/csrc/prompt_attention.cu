@@ -3,7 +3,10 @@
 // 4 · hd flops and one exponential per visible (query, key) pair and head: at hd 128 a tile of 128 × 128 pairs is 1024 clocks of
 // tcgen05.mma and 1024 clocks of the SM's 16 exponentials a clock, so neither may wait for the other.  One prompt of 8192 rows with 32 heads:
 // 569 µs, 966 TFLOP/s = 60 % of the measured matrix rate, at 990 W (the power cap) and 1.6 GHz: a pair of tiles takes 3070 clocks, its
-// chain being scores → maximum 540 → exponentials 1450 → products and scores of the next tile 1070.
+// chain being scores → maximum 540 → exponentials 1450 → products and scores of the next tile 1070.  228 pairs an SM are seven eighths of
+// the time; the rest is the seven items an SM beside their pairs, 13 to 17 thousand clocks each — both tiles of a CTA come to their end at once,
+// and nothing feeds the tensor core while they are read out, stored and the next item is taken.  Of 24 ragged prompts (91 pairs and 13 items
+// an SM) that is two fifths.
 //   * A CTA works on two query tiles of 128 rows with the same keys: the same rows of two heads that share a KV head, or — where the
 //     heads do not pair up — 256 consecutive rows of one head.
 //   * S = Q·Kᵀ (f32) and O (128 × hd f32) live in tensor memory; the probabilities go back over the scores as 16-bit numbers and are
@@ -13,14 +16,14 @@
 //   * While the softmax of one query tile runs, the tensor core has the other's products.
 //   * K and V tiles of 128 keys come by tiled bulk copies through one ring of shared-memory stages: K0 V0 K1 V1 …
 //   * An item is one pair of query tiles; there is a CTA for each, late (long) row tiles of all heads first.  A CTA that runs takes over the
-//     items of CTAs that have not started (clusterlaunchcontrol: the hardware hands them out, no counter in memory): its copies and
-//     first scores of the next item run under the end of the one before (a CTA per item spent 5 to 7 µs starting and ending).  A warp of its
+//     items of CTAs that have not started (clusterlaunchcontrol: the hardware hands them out, no counter in memory): its copies for
+//     the next item run under the end of the one before (a CTA per item spent 5 to 7 µs starting and ending).  A warp of its
 //     own finds sequence and rows in the prefix arrays: nothing depends on host-side lengths, and a captured call follows the arrays.
 //   * A product of 0 and a NaN or infinity in a value row that the query does not see would be NaN: value rows behind the sequence are
 //     zeroed in shared memory, and an output row that is not finite (though its scores are numbers) is taken again by ax_prompt_row, which
 //     reads visible rows only.
-//   * Every wait is bounded (ten seconds of %globaltimer, in which no row is taken again): on expiry the CTA raises the context's error word, all roles leave, copies
-//     in flight are waited for and tensor memory is released.
+//   * Every wait is bounded (ten seconds of %globaltimer, in which no row is taken again): on expiry the CTA raises the context's error word,
+//     all roles leave, copies in flight are waited for and tensor memory is released.
 #include <cuda.h>
 #include <atomic>
 #include <type_traits>

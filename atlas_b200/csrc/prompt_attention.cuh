@@ -1,4 +1,4 @@
-// prompt_attention.cuh — arguments of the packed prompt attention and the row-by-row form every variant can fall back on.
+// prompt_attention.cuh — arguments of the packed prompt attention and the form of a single row, for rows that are taken again.
 #pragma once
 #include "paged.cuh"
 

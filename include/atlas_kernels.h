@@ -80,7 +80,7 @@ void atlas_quantize_int4(const float* input, uint8_t* output, float* scale, int 
 #define ATLASX_ERR_STATE    (-6)
 
 enum atlasx_dtype { ATLASX_F32 = 0, ATLASX_BF16 = 1, ATLASX_INT8 = 2, ATLASX_INT4 = 3,
-                    ATLASX_F16 = 4 /* a file dtype only: converted to f32 while loading */ };
+                    ATLASX_F16 = 4 /* in files (converted to f32 while loading) and as rows of the packed serving calls */ };
 #define ATLASX_AUTO (-1)      /* weight_format for the loaders: bf16 when the file's linear weights are BF16, else f32 */
 
 /* message of the last failing atlasx_* call on this thread ("" if none) */
