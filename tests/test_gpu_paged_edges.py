@@ -506,3 +506,57 @@ def test_a_nan_in_an_early_key_of_a_long_prompt(ab):
     got = down(ab, out)
     assert np.isnan(got[3:]).all() and np.isfinite(got[:3]).all()
     assert ms[3] < 3 * ms[2], ms
+
+
+# ── offsets that pass 32 bits ────────────────────────────────────────────────────
+def test_a_cache_of_more_than_4_gib(ab):
+    """65 536 pages of 64 rows and 8 heads (4.8 GB): rows in the first and the last pages, through append, read and decode attention."""
+    rng = np.random.default_rng(95)
+    n_pages, page, n_kv, hd = 65536, 64, 8, 128
+    kv = ab.PagedKvCache(n_pages, page, n_kv, hd)
+    assert kv.bytes > 1 << 32
+    pages = np.array([n_pages - 1, 0, n_pages - 2, 1, 59652, 59653])          # byte 2^32 lies in page 58 254
+    n = len(pages) * page
+    k, v = rows(rng, n, n_kv, hd), rows(rng, n, n_kv, hd)
+    slots = (pages[:, None] * page + np.arange(page)).ravel()
+    sd = ab.DeviceArray.from_host(slots, ab.I32)
+    kv.append(up(ab, k, ab.F32), up(ab, v, ab.F32), sd)
+    ko, vo = ab.DeviceArray.empty((n, n_kv, hd), ab.F32), ab.DeviceArray.empty((n, n_kv, hd), ab.F32)
+    kv.read(sd, ko, vo)
+    assert np.array_equal(ko.download(), held(k, 32).astype(np.float32)) and np.array_equal(vo.download(), held(v, 32).astype(np.float32))
+    c = Cache.__new__(Cache)
+    c.page, c.table, c.k, c.v = page, np.arange(6).reshape(1, 6), held(k, 32), held(v, 32)
+    q = rng.standard_normal((1, 16, hd)).astype(np.float32)
+    out = up(ab, 0 * q, ab.F32)
+    kv.decode_attention(up(ab, q, ab.F32), out, ab.DeviceArray.from_host(pages.reshape(1, 6), ab.I32), ab.DeviceArray.from_host([n - 5], ab.I32), 0.09)
+    want, tol = decode_by_hand(c, q, 0.09, 0, [n - 5])
+    assert np.all(np.abs(out.download() - want) <= tol)
+    assert kv.ctx.poll_device_error() == 0
+
+
+@pytest.mark.parametrize("hd,nh", [(128, 32), (64, 33)])
+def test_prompt_rows_behind_2_31_elements(ab, hd, nh):
+    """A sequence at the end of buffers of 2^31 and more elements each; the rows before it belong to no sequence."""
+    rng = np.random.default_rng(96)
+    n, m = (1 << 31) // (nh * hd) + 400, 300
+    ctx = ab.Context.default()
+    x = [bf16(rng.standard_normal((m, nh, hd)).astype(np.float32)) for _ in range(3)]
+    big = [ab.DeviceArray.empty((n, nh, hd), ab.BF16) for _ in range(4)]
+    first = n - m
+    at = 2 * first * nh * hd
+    assert first * nh * hd > 1 << 31
+    for d, y in zip(big, x):
+        ctx.upload(d.ptr + at, orc.f32_to_bf16_rne(y))
+    cu = ab.DeviceArray.from_host([first, n], ab.I32)
+    ab.prompt_attention(*big, cu, cu, 0.1)
+    got = orc.bf16_to_f32(ctx.download(big[3].ptr + at, (m * nh * hd,), np.uint16)).reshape(m, nh, hd)
+    want, tol = prompt_by_hand(*x, [0, m], [0, m], 0.1, 0, False)
+    assert np.all(np.abs(got - want) <= tol)
+    # and the row form there
+    x[2][0] = np.nan
+    ctx.upload(big[2].ptr + at, orc.f32_to_bf16_rne(x[2]))
+    ab.prompt_attention(*big, cu, cu, 0.1, window_size=m - 1)
+    got = orc.bf16_to_f32(ctx.download(big[3].ptr + at, (m * nh * hd,), np.uint16)).reshape(m, nh, hd)
+    assert np.isnan(got[:m - 1]).all() and np.all(np.abs(got[m - 1] - prompt_by_hand(x[0][m - 1:], x[1][1:], x[2][1:], [0, 1], [0, m - 1], 0.1, 0, False)[0][0])
+                                                  <= prompt_by_hand(x[0][m - 1:], x[1][1:], x[2][1:], [0, 1], [0, m - 1], 0.1, 0, False)[1][0])
+    assert ctx.poll_device_error() == 0
