@@ -262,9 +262,10 @@ typedef struct {
     float scale;
 } atlasx_pagedkv_attn_args;
 int atlasx_pagedkv_decode_attention(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const atlasx_pagedkv_attn_args* args);
-/* Self-test of an expired wait (head_dim 64, groups of 32): the same call, but the copy of one unit (two tiles of 16 rows of a KV head, counted
- * over all requests and KV heads) is never issued.  Its warp gives up after 20 ms, the error word is raised (code 741) and the rows
- * that it had still to see are missing from the outputs; the workspace stays good for the calls that follow. */
+/* Self-test of an expired wait (head_dim 64, groups of 32): the same call, but the copy of one unit (two tiles of 16 rows of a KV head — one
+ * where there are not two for every warp — counted over all requests and KV heads) is never issued.  Its warp gives up after 20 ms, the
+ * error word is raised (code 741) and the rows that it had still to see are missing from the outputs; the workspace stays good for the
+ * calls that follow. */
 int atlasx_pagedkv_selftest_wait_expiry(atlasx_ctx* ctx, const atlasx_pagedkv* kv, const atlasx_pagedkv_attn_args* args, long long unit);
 
 /* Causal attention of whole packed prompts, bf16 or f16 in and out; head_dim 64 or 128.  Scores, their maxima and sums and the outputs are f32
